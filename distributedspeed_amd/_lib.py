@@ -77,8 +77,14 @@ class DsxFlatPlan(_c.Structure):
                 ("scaler", DsxScalerConfig), ("group_end", _c.c_int64 * 16)]
 
 
+class DsxMatrix(_c.Structure):
+    _fields_ = [("in_", _P), ("out", _P), ("ld_in", _c.c_int64), ("ld_out", _c.c_int64), ("rows", _c.c_int64),
+                ("cols", _c.c_int64)]
+
+
 for _s, _n in ((DsxState, 64), (DsxScalerConfig, 32), (DsxAdamwHyper, 56), (DsxStepScalars, 64),
-               (DsxTensorRef, 56), (DsxChunk, 24), (DsxGroupsDev, 1112), (DsxFlatPlan, 248)):
+               (DsxTensorRef, 56), (DsxChunk, 24), (DsxGroupsDev, 1112), (DsxFlatPlan, 248),
+               (DsxMatrix, 48)):
     assert _c.sizeof(_s) == _n, (_s.__name__, _c.sizeof(_s))
 
 # name -> (restype, argtypes); every symbol include/dsx.h declares.
@@ -128,6 +134,8 @@ SIGNATURES = {
                                        _c.c_int, _c.c_int, _P, DsxScalerConfig, _P, _P, _c.c_int32, _P, _P]),
     "dsx_zero_step_multi": (_c.c_int, [_P, _P, _c.c_int64, _c.c_int64, _c.c_int, _c.c_int, _P, DsxScalerConfig, _P,
                                        _P, _c.c_int32, _P, _P]),
+    "dsx_orthogonalize_workspace": (_c.c_int64, [_P, _c.c_int32]),
+    "dsx_orthogonalize": (_c.c_int, [_P, _c.c_int32, _c.c_int, _c.c_int32, _P, _c.c_double, _P, _c.c_int64, _P]),
 }
 
 _lib: ctypes.CDLL | None = None

@@ -3,8 +3,9 @@
     python -m distributedspeed_amd.build
 
 The flags that matter for correctness:
-  -ffp-contract=off   no implicit fused multiply-adds: each operation rounds
-                      where torch's kernels round (explicit fmaf only)
+  -ffp-contract=off   (the optimizer step) no implicit fused multiply-adds:
+                      each operation rounds where torch's kernels round
+                      (explicit fmaf only)
   -Xclang -target-feature -Xclang -packed-fp32-ops
                       no packed fp32 instructions (v_pk_*_f32)
 and for speed:
@@ -23,13 +24,22 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
-SRC = os.path.join(HERE, "csrc", "dsx_step.hip")
+CSRC = os.path.join(HERE, "csrc")
 INCLUDE = os.path.join(ROOT, "include")
 OUT = os.path.join(HERE, "libdsx.so")
 ARCH = os.environ.get("DSX_OFFLOAD_ARCH", "gfx950")
+
+# source -> its own flags. The optimizer step rounds where torch rounds; the
+# block and Muon kernels have no such partner and may contract.
+SOURCES = {
+    "dsx_step.hip": ["-ffp-contract=off"],
+    "dsx_muon.hip": [],
+}
 
 
 def hipcc() -> str:
@@ -39,26 +49,33 @@ def hipcc() -> str:
     raise RuntimeError("hipcc not found")
 
 
-def command(out: str = OUT, extra: list[str] | None = None) -> list[str]:
-    return [hipcc(), f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", "-shared",
-            "-ffp-contract=off", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
+def command(source: str, out: str, extra: list[str] | None = None) -> list[str]:
+    """The compile command of one source to an object file."""
+    return [hipcc(), f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", "-c", *SOURCES[source],
+            "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
             "-mllvm", "-amdgpu-kernarg-preload-count=16",
             "-Wall", "-Wno-unused-function",
-            f"-I{INCLUDE}", SRC, "-o", out] + list(extra or [])
+            f"-I{INCLUDE}", f"-I{CSRC}", os.path.join(CSRC, source), "-o", out] + list(extra or [])
 
 
-def build(out: str = OUT, verbose: bool = False) -> str:
-    cmd = command(out)
-    tmp = out + ".tmp"
-    cmd[cmd.index(out)] = tmp
+def _run(cmd: list[str]) -> list[str]:
     res = subprocess.run(cmd, capture_output=True, text=True)
     # hipcc's host pass warns that it does not know the packed-fp32 feature: harmless.
     noise = [ln for ln in (res.stderr or "").splitlines() if "packed-fp32-ops" not in ln and ln.strip()]
     if res.returncode != 0:
         raise RuntimeError("hipcc failed:\n" + "\n".join(noise))
+    return noise
+
+
+def build(out: str = OUT, verbose: bool = False) -> str:
+    with tempfile.TemporaryDirectory(prefix="dsx_build_") as tmp:
+        objects = {src: os.path.join(tmp, src + ".o") for src in SOURCES}
+        with ThreadPoolExecutor(max_workers=min(4, len(SOURCES))) as pool:
+            noise = [ln for got in pool.map(lambda src: _run(command(src, objects[src])), SOURCES) for ln in got]
+        _run([hipcc(), f"--offload-arch={ARCH}", "-fPIC", "-shared", *objects.values(), "-o", out + ".tmp"])
     if verbose and noise:
         print("\n".join(noise), file=sys.stderr)
-    os.replace(tmp, out)
+    os.replace(out + ".tmp", out)
     return out
 
 

@@ -1,0 +1,621 @@
+// dsx_muon.hip -- Newton-Schulz orthogonalisation of matrices, and the Muon
+// step around it (see include/dsx.h).
+//
+// For each matrix G (R x C, s = min(R, C)):
+//   X0 = G / (|G|_F + eps);   for each step with its coefficients (a, b, c):
+//   A = X X^T (or X^T X where R > C; s x s),  B = b A + c A A,
+//   X <- a X + B X (or a X + X B).
+// A and B are symmetric: only the tiles on and above the diagonal are
+// computed, each written at both places. A step is three launches for a whole
+// list of matrices; every launch finds its matrix and tile from a table in
+// the kernel's arguments.
+//
+// Numbers. The iterates are fp16 with fp32 sums: entries of X, A and B are
+// bounded by their spectral norms (about 1.2, 1.5 and 2.9 with Muon's
+// coefficients), so range is no concern and fp16's 11 bits leave 8 times less
+// rounding error than bf16 (against 64 bits, 1024 x 1024: 1.1e-3 and 8.8e-3).
+// All three are stored times kScale, which keeps the small entries of large
+// matrices (1e-6 for A) in fp16's normal range. X0 is scaled by a power of two
+// alone, so a 16-bit input is not rounded at all; the rest of 1 / |G|, the
+// factor r in (1/2, 1], is folded into the first step's sums:
+//   A = X0~ X0~^T / (kScale r)^2,  X1 = (a X0~ + B X0~) / (r kScale).
+
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include <new>
+#include <type_traits>
+
+#include "dsx.h"
+#include "dsx_gemm.h"
+#include "dsx_internal.h"
+
+namespace {
+
+using namespace dsxg;
+using dsxi::as_stream;
+using dsxi::ceil_div;
+using dsxi::fail;
+using dsxi::launch_status;
+using dsxi::round_up;
+
+constexpr float kScale = 4096.0f;
+constexpr int kMats = 24;        // matrices of one launch (the table is a kernel argument)
+constexpr int kMaxParts = 512;   // norm partials per matrix
+constexpr int kNormTile = 64;    // the norm and cast kernels' square tile
+
+struct Mat {
+  const void* in;
+  void*  out;
+  float* momentum;
+  float* master;
+  int64_t ld_in, ld_out;
+  int64_t x[2], a, b;  // offsets in the workspace, in 16-bit elements
+  int32_t rows, cols, rows8, cols8;
+  int32_t tile0;       // first tile of this matrix in the launch at hand
+  int32_t part0, parts;
+  float   lr;          // Muon: the step size of this matrix
+};
+struct Table {
+  Mat m[kMats];
+  int32_t n;
+};
+static_assert(sizeof(Table) <= 3584, "the table travels in the kernel arguments");
+
+struct Info {
+  float p;      // X0~ = G p, a power of two
+  float inv_r;  // 1 / r
+  int32_t bad;  // the norm is not finite
+  int32_t reserved;
+};
+
+struct MuonArgs {
+  const float* grad_scale;  // grads are divided by this (NULL: 1)
+  int32_t* skip;            // any matrix's norm not finite
+  float momentum, decay;
+  int32_t nesterov;
+};
+
+__device__ inline int find(const Table& t, int tile) {
+  int i = 0;
+  while (i + 1 < t.n && tile >= t.m[i + 1].tile0) i++;
+  return i;
+}
+
+template <int DT>
+__device__ inline void load4(const void* p, int64_t at, bool vec, int left, float* v) {
+  if (DT == DSX_F32) {
+    const float* q = (const float*)p + at;
+    if (vec && left >= 4) {
+      const f4v w = *(const f4v*)q;
+      for (int e = 0; e < 4; e++) v[e] = w[e];
+    } else {
+      for (int e = 0; e < 4; e++) v[e] = e < left ? q[e] : 0.0f;
+    }
+  } else {
+    using T = typename std::conditional<DT == DSX_F16, F16, BF16>::type;
+    const short* q = (const short*)p + at;
+    if (vec && left >= 4) {
+      const s4v w = *(const s4v*)q;
+      for (int e = 0; e < 4; e++) v[e] = T::widen(w[e]);
+    } else {
+      for (int e = 0; e < 4; e++) v[e] = e < left ? T::widen(q[e]) : 0.0f;
+    }
+  }
+}
+
+// The matrix that is orthogonalised, four values of a row: the input itself,
+// or Muon's update (buf = mu buf + (1 - mu) g; u = mu buf + (1 - mu) g with
+// Nesterov's correction, else buf).
+template <int DT, bool MUON>
+__device__ inline void update4(const Mat& m, const MuonArgs& ma, float inv, int r, int c, bool vec, float* u,
+                               float* buf) {
+  const int left = m.cols - c;
+  load4<DT>(m.in, r * m.ld_in + c, vec, left, u);
+  if (MUON) {
+    load4<DSX_F32>(m.momentum, (int64_t)r * m.cols + c, (m.cols & 3) == 0, left, buf);
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const float g = u[e] * inv;
+      buf[e] = fmaf(ma.momentum, buf[e], (1.0f - ma.momentum) * g);
+      u[e] = ma.nesterov ? fmaf(ma.momentum, buf[e], (1.0f - ma.momentum) * g) : buf[e];
+    }
+  }
+}
+
+__device__ inline float inverse_scale(const MuonArgs& ma) { return ma.grad_scale ? 1.0f / *ma.grad_scale : 1.0f; }
+
+// Sums of squares: `parts` blocks per matrix, each over every parts-th tile;
+// squares and sums in fp64 (an fp32 input's squares may leave fp32's range).
+template <int DT, bool MUON>
+__global__ __launch_bounds__(256) void k_sumsq(Table t, double* __restrict__ partials, MuonArgs ma) {
+  const int i = find(t, blockIdx.x);
+  const Mat& m = t.m[i];
+  const int part = blockIdx.x - m.tile0, tid = threadIdx.x;
+  const int tc = (m.cols + kNormTile - 1) / kNormTile, tiles = tc * ((m.rows + kNormTile - 1) / kNormTile);
+  const bool vec = (m.ld_in & 3) == 0 && ((uintptr_t)m.in & (DT == DSX_F32 ? 15 : 7)) == 0;
+  const float inv = MUON ? inverse_scale(ma) : 1.0f;
+  if (MUON && ma.skip && blockIdx.x == 0 && part == 0 && tid == 0 && m.part0 == 0) *ma.skip = 0;
+  double sum = 0;
+  for (int tile = part; tile < tiles; tile += m.parts) {
+    const int r0 = tile / tc * kNormTile + (tid >> 4), c = tile % tc * kNormTile + (tid & 15) * 4;
+    if (c >= m.cols) continue;
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      const int r = r0 + 16 * k;
+      if (r >= m.rows) break;
+      float u[4], buf[4];
+      update4<DT, MUON>(m, ma, inv, r, c, vec, u, buf);
+#pragma unroll
+      for (int e = 0; e < 4; e++) sum += (double)u[e] * u[e];
+    }
+  }
+  __shared__ double part_sum[4];
+  for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
+  if ((tid & 63) == 0) part_sum[tid >> 6] = sum;
+  __syncthreads();
+  if (tid == 0) partials[m.part0 + part] = part_sum[0] + part_sum[1] + part_sum[2] + part_sum[3];
+}
+
+// One block per matrix: its norm, the power of two and the rest of 1 / norm.
+__global__ __launch_bounds__(64) void k_norms(Table t, const double* __restrict__ partials, Info* __restrict__ info,
+                                              double eps, int32_t* skip) {
+  const Mat& m = t.m[blockIdx.x];
+  double sum = 0;
+  for (int k = threadIdx.x; k < m.parts; k += 64) sum += partials[m.part0 + k];
+  for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
+  if (threadIdx.x) return;
+  Info f = {0.0f, 1.0f, 0, 0};
+  if (isfinite(sum)) {
+    const double inv = (double)kScale / (sqrt(sum) + eps);
+    int e;
+    frexp(inv, &e);  // inv in [2^(e-1), 2^e)
+    f.p = (float)ldexp(1.0, e - 1);
+    f.inv_r = (float)(inv / ldexp(1.0, e - 1));
+  } else {
+    f.bad = 1;
+    if (skip) atomicOr(skip, 1);
+  }
+  info[blockIdx.x] = f;
+}
+
+// X0~ = fp16(G p), zero beyond the matrix; all NaN where the norm is not finite
+// (every entry of the exact result is). Muon: the momentum buffer is written
+// here, once the step is known not to be skipped.
+template <int DT, bool MUON>
+__global__ __launch_bounds__(256) void k_cast(Table t, short* __restrict__ ws, const Info* __restrict__ info,
+                                              MuonArgs ma) {
+  const int i = find(t, blockIdx.x);
+  const Mat& m = t.m[i];
+  const int tile = blockIdx.x - m.tile0, tid = threadIdx.x;
+  const int tc = (m.cols8 + kNormTile - 1) / kNormTile;
+  const int r0 = tile / tc * kNormTile + (tid >> 4), c = tile % tc * kNormTile + (tid & 15) * 4;
+  if (c >= m.cols8 || (MUON && *ma.skip)) return;
+  const bool vec = (m.ld_in & 3) == 0 && ((uintptr_t)m.in & (DT == DSX_F32 ? 15 : 7)) == 0;
+  const float inv = MUON ? inverse_scale(ma) : 1.0f;
+  const Info f = info[i];
+#pragma unroll
+  for (int k = 0; k < 4; k++) {
+    const int r = r0 + 16 * k;
+    if (r >= m.rows8) break;
+    float u[4] = {0, 0, 0, 0}, buf[4];
+    if (r < m.rows && c < m.cols) {
+      update4<DT, MUON>(m, ma, inv, r, c, vec, u, buf);
+      if (MUON)
+        for (int e = 0; e < 4; e++)
+          if (c + e < m.cols) m.momentum[(int64_t)r * m.cols + c + e] = buf[e];
+      if (f.bad)
+        for (int e = 0; e < 4; e++) u[e] = __builtin_nanf("");
+    }
+    s4v o;
+#pragma unroll
+    for (int e = 0; e < 4; e++) o[e] = F16::round(f.bad ? u[e] : (c + e < m.cols ? u[e] * f.p : 0.0f));
+    *(s4v*)(ws + m.x[0] + (int64_t)r * m.cols8 + c) = o;
+  }
+}
+
+__device__ inline void triangle(int t, int* i, int* j) {
+  int q = (int)((sqrtf(8.0f * t + 1.0f) - 1.0f) * 0.5f);
+  while (q * (q + 1) / 2 > t) q--;
+  while ((q + 1) * (q + 2) / 2 <= t) q++;
+  *j = q;
+  *i = t - q * (q + 1) / 2;
+}
+
+// A symmetric product's tile, written at (m, n) and, off the diagonal, at (n, m).
+// GRAM: A = X X^T (wide) or X^T X (TALL) from the current X; else B = b A + c A A.
+template <class G, bool GRAM, bool TALL>
+__global__ __launch_bounds__(G::THREADS) void k_symmetric(Table t, short* __restrict__ ws,
+                                                          const Info* __restrict__ info, int cur, int first, float b,
+                                                          float c, const int32_t* skip) {
+  __shared__ __attribute__((aligned(1024))) char lds[G::kLds];
+  if (skip && *skip) return;
+  const int bid = xcd_order(blockIdx.x, gridDim.x);
+  const int i = find(t, bid);
+  const Mat& m = t.m[i];
+  const int s = min(m.rows8, m.cols8);
+  int ti, tj;
+  triangle(bid - m.tile0, &ti, &tj);
+  G g;
+  g.init();
+  const short* src = ws + (GRAM ? m.x[cur] : m.a);
+  const Operand o{src, GRAM ? m.cols8 : s, s};
+  g.run(lds, o, o, o, ti * G::TM, tj * G::TN, GRAM ? max(m.rows8, m.cols8) : s);
+  const float inv_r = first ? info[i].inv_r : 1.0f;
+  const float k = GRAM ? inv_r * inv_r * (1.0f / kScale) : c * (1.0f / kScale);
+  short* dst = ws + (GRAM ? m.a : m.b);
+#pragma unroll
+  for (int x = 0; x < G::MF; x++) {
+    const int r = ti * G::TM + g.row_of(x);
+    if (r >= s) continue;
+#pragma unroll
+    for (int y = 0; y < G::NF; y++) {
+      const int q = tj * G::TN + g.col_of(y);
+      if (q >= s) continue;  // s is a multiple of 8: four columns are inside or outside together
+      s4v w;
+      if (GRAM) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) w[e] = F16::round(k * g.acc[x][y][e]);
+      } else {
+        const s4v a = *(const s4v*)(src + (int64_t)r * s + q);
+#pragma unroll
+        for (int e = 0; e < 4; e++) w[e] = F16::round(fmaf(k, g.acc[x][y][e], b * F16::widen(a[e])));
+      }
+      *(s4v*)(dst + (int64_t)r * s + q) = w;
+      if (ti != tj)
+#pragma unroll
+        for (int e = 0; e < 4; e++) dst[(int64_t)(q + e) * s + r] = w[e];
+    }
+  }
+}
+
+// X <- (a X + B X) / r, or with X B where TALL. LAST: the result itself, to the
+// output in bf16 (OUT 0) or as Muon's parameter update (fp32 master and 16-bit
+// copy of OUT's type, 0 for none).
+template <class G, bool TALL, bool LAST, bool MUON>
+__global__ __launch_bounds__(G::THREADS) void k_apply(Table t, short* __restrict__ ws, const Info* __restrict__ info,
+                                                      int cur, int first, float a, MuonArgs ma, int out_dt) {
+  __shared__ __attribute__((aligned(1024))) char lds[G::kLds];
+  if (MUON && *ma.skip) return;
+  const int bid = xcd_order(blockIdx.x, gridDim.x);
+  const int i = find(t, bid);
+  const Mat& m = t.m[i];
+  const int s = min(m.rows8, m.cols8);
+  const int mt = (m.rows8 + G::TM - 1) / G::TM, nt = (m.cols8 + G::TN - 1) / G::TN;
+  int ti, tj;
+  band_order(bid - m.tile0, mt, nt, 8, &ti, &tj);
+  const short* x = ws + m.x[cur];
+  const Operand ox{x, m.cols8, TALL ? m.rows8 : m.cols8}, ob{ws + m.b, s, s};
+  G g;
+  g.init();
+  if (TALL)
+    g.run(lds, ox, ob, ob, ti * G::TM, tj * G::TN, s);
+  else
+    g.run(lds, ob, ox, ox, ti * G::TM, tj * G::TN, s);
+  const float inv_r = first ? info[i].inv_r : 1.0f;
+#pragma unroll
+  for (int p = 0; p < G::MF; p++) {
+    const int r = ti * G::TM + g.row_of(p);
+    if (r >= (LAST ? m.rows : m.rows8)) continue;
+#pragma unroll
+    for (int q = 0; q < G::NF; q++) {
+      const int c = tj * G::TN + g.col_of(q);
+      if (c >= (LAST ? m.cols : m.cols8)) continue;
+      const s4v old = *(const s4v*)(x + (int64_t)r * m.cols8 + c);
+      float v[4];
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+        v[e] = fmaf(a, F16::widen(old[e]), g.acc[p][q][e] * (1.0f / kScale)) * inv_r;
+      if (!LAST) {
+        s4v w;
+#pragma unroll
+        for (int e = 0; e < 4; e++) w[e] = F16::round(v[e]);
+        *(s4v*)(ws + m.x[cur ^ 1] + (int64_t)r * m.cols8 + c) = w;
+      } else if (!MUON) {
+        short* o = (short*)m.out + r * m.ld_out + c;
+        s4v w;
+#pragma unroll
+        for (int e = 0; e < 4; e++) w[e] = BF16::round(v[e] * (1.0f / kScale));
+        if (c + 4 <= m.cols && ((uintptr_t)o & 7) == 0)
+          *(s4v*)o = w;
+        else
+          for (int e = 0; e < 4; e++)
+            if (c + e < m.cols) o[e] = w[e];
+      } else {
+        float* w = m.master + (int64_t)r * m.cols + c;
+        short* o = (short*)m.out + r * m.ld_out + c;
+        for (int e = 0; e < 4; e++) {
+          if (c + e >= m.cols) break;
+          const float n = fmaf(-m.lr * (1.0f / kScale), v[e], w[e] * ma.decay);
+          w[e] = n;
+          if (out_dt) o[e] = out_dt == DSX_F16 ? F16::round(n) : BF16::round(n);
+        }
+      }
+    }
+  }
+}
+
+// ---- host ------------------------------------------------------------------
+
+template <bool RA, bool RB>
+using Big = Gemm<F16, 256, 256, 2, 4, RA, RB, true>;
+template <bool RA, bool RB>
+using Small = Gemm<F16, 128, 128, 2, 2, RA, RB, true>;
+
+struct Source {  // one matrix of the caller's list
+  const void* in;
+  void* out;
+  float* momentum;
+  float* master;
+  int64_t ld_in, ld_out;
+  int32_t rows, cols;
+  float lr;
+};
+
+int64_t halves_of(int32_t rows, int32_t cols) {
+  const int64_t r = round_up(rows, 8), c = round_up(cols, 8), s = r < c ? r : c;
+  return 2 * round_up(r * c, 128) + 2 * round_up(s * s, 128);
+}
+int32_t parts_of(int32_t rows, int32_t cols) {
+  const int64_t tiles = ceil_div(rows, kNormTile) * ceil_div(cols, kNormTile);
+  const int64_t p = ceil_div(tiles, 4);
+  return (int32_t)(p < 1 ? 1 : p > kMaxParts ? kMaxParts : p);
+}
+
+// The list in runs of at most kMats matrices of one orientation.
+struct Plan {
+  int64_t info_bytes = 0, partial_bytes = 0, halves = 0;
+};
+
+// Orders the list by orientation (wide first) and lays out the workspace:
+// skip flag, norm records, partials, then the fp16 matrices of the largest run.
+template <class F>
+Plan each_run(const Source* src, int32_t count, F&& f) {
+  Plan plan;
+  int64_t part0 = 0;
+  int32_t index = 0;
+  for (int tall = 0; tall < 2; tall++) {
+    Table t{};
+    int64_t at = 0;
+    auto flush = [&]() {
+      if (t.n) f(t, tall != 0, index - t.n);
+      if (at > plan.halves) plan.halves = at;
+      t.n = 0;
+      at = 0;
+    };
+    for (int32_t k = 0; k < count; k++) {
+      const Source& q = src[k];
+      if (q.rows <= 0 || q.cols <= 0 || (q.rows > q.cols) != (tall != 0)) continue;
+      Mat& m = t.m[t.n++];
+      m = Mat{};
+      m.in = q.in;
+      m.out = q.out;
+      m.momentum = q.momentum;
+      m.master = q.master;
+      m.ld_in = q.ld_in;
+      m.ld_out = q.ld_out;
+      m.rows = q.rows;
+      m.cols = q.cols;
+      m.rows8 = (int32_t)round_up(q.rows, 8);
+      m.cols8 = (int32_t)round_up(q.cols, 8);
+      m.lr = q.lr;
+      const int64_t s = m.rows8 < m.cols8 ? m.rows8 : m.cols8;
+      m.x[0] = at;
+      m.x[1] = m.x[0] + round_up((int64_t)m.rows8 * m.cols8, 128);
+      m.a = m.x[1] + round_up((int64_t)m.rows8 * m.cols8, 128);
+      m.b = m.a + round_up(s * s, 128);
+      at = m.b + round_up(s * s, 128);
+      m.parts = parts_of(q.rows, q.cols);
+      m.part0 = (int32_t)part0;
+      part0 += m.parts;
+      index++;
+      if (t.n == kMats) flush();
+    }
+    flush();
+  }
+  plan.info_bytes = 256 + round_up((int64_t)index * (int64_t)sizeof(Info), 256);
+  plan.partial_bytes = round_up(part0 * 8, 256);
+  return plan;
+}
+
+// Sets the launch's first tile of each matrix; returns the tile count.
+template <class F>
+int64_t tiles_of(Table& t, F&& per) {
+  int64_t n = 0;
+  for (int i = 0; i < t.n; i++) {
+    t.m[i].tile0 = (int32_t)n;
+    n += per(t.m[i]);
+  }
+  return n;
+}
+
+int cu_count() {
+  static const int n = [] {
+    int dev = 0, v = 0;
+    if (hipGetDevice(&dev) != hipSuccess ||
+        hipDeviceGetAttribute(&v, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || v <= 0)
+      v = 256;
+    return v;
+  }();
+  return n;
+}
+
+template <class G, bool GRAM, bool TALL>
+void launch_symmetric(Table& t, short* ws, const Info* info, int cur, int first, float b, float c, const int32_t* skip,
+                      hipStream_t s) {
+  const int64_t n = tiles_of(t, [](const Mat& m) {
+    const int64_t k = ceil_div(m.rows8 < m.cols8 ? m.rows8 : m.cols8, G::TM);
+    return k * (k + 1) / 2;
+  });
+  k_symmetric<G, GRAM, TALL><<<dim3((unsigned)n), G::THREADS, 0, s>>>(t, ws, info, cur, first, b, c, skip);
+}
+
+template <class G, bool TALL, bool MUON>
+void launch_apply(Table& t, short* ws, const Info* info, int cur, int first, bool last, float a, const MuonArgs& ma,
+                  int out_dt, hipStream_t s) {
+  const int64_t n =
+      tiles_of(t, [](const Mat& m) { return ceil_div(m.rows8, G::TM) * ceil_div(m.cols8, G::TN); });
+  if (last)
+    k_apply<G, TALL, true, MUON><<<dim3((unsigned)n), G::THREADS, 0, s>>>(t, ws, info, cur, first, a, ma, out_dt);
+  else
+    k_apply<G, TALL, false, false><<<dim3((unsigned)n), G::THREADS, 0, s>>>(t, ws, info, cur, first, a, ma, out_dt);
+}
+
+// 256-tiles where they fill the CUs at least twice over, else 128-tiles.
+bool use_big(const Table& t, bool triangle) {
+  int64_t n = 0;
+  for (int i = 0; i < t.n; i++) {
+    const Mat& m = t.m[i];
+    const int64_t k = ceil_div(m.rows8 < m.cols8 ? m.rows8 : m.cols8, 256);
+    n += triangle ? k * (k + 1) / 2 : ceil_div(m.rows8, 256) * ceil_div(m.cols8, 256);
+  }
+  return n >= 2 * cu_count();
+}
+
+template <bool MUON>
+void iterate(Table& t, bool tall, short* ws, const Info* info, int steps, const double* coef, const MuonArgs& ma,
+             int out_dt, hipStream_t s) {
+  const bool big_sym = use_big(t, true), big_app = use_big(t, false);
+  const int32_t* skip = MUON ? ma.skip : nullptr;
+  for (int k = 0; k < steps; k++) {
+    const float a = (float)coef[3 * k], b = (float)coef[3 * k + 1], c = (float)coef[3 * k + 2];
+    const int cur = k & 1, first = k == 0, last = k == steps - 1;
+#define DSX_SYM(G, GRAM, TALL) launch_symmetric<G, GRAM, TALL>(t, ws, info, cur, first, b, c, skip, s)
+    using BR = Big<true, true>;
+    using SR = Small<true, true>;
+    using BC = Big<false, false>;
+    using SC = Small<false, false>;
+    using BX = Big<true, false>;
+    using SX = Small<true, false>;
+    if (tall) {
+      if (big_sym) DSX_SYM(BC, true, true); else DSX_SYM(SC, true, true);
+    } else {
+      if (big_sym) DSX_SYM(BR, true, false); else DSX_SYM(SR, true, false);
+    }
+    if (big_sym) DSX_SYM(BR, false, false); else DSX_SYM(SR, false, false);
+#undef DSX_SYM
+    if (tall) {
+      if (big_app) launch_apply<BR, true, MUON>(t, ws, info, cur, first, last, a, ma, out_dt, s);
+      else launch_apply<SR, true, MUON>(t, ws, info, cur, first, last, a, ma, out_dt, s);
+    } else {
+      if (big_app) launch_apply<BX, false, MUON>(t, ws, info, cur, first, last, a, ma, out_dt, s);
+      else launch_apply<SX, false, MUON>(t, ws, info, cur, first, last, a, ma, out_dt, s);
+    }
+  }
+}
+
+template <int DT, bool MUON>
+int drive(const Source* src, int32_t count, int steps, const double* coef, double eps, MuonArgs ma, int out_dt,
+          char* base, int64_t bytes, const char* what, hipStream_t s) {
+  const Plan plan = each_run(src, count, [](Table&, bool, int) {});
+  const int64_t need = plan.info_bytes + plan.partial_bytes + 2 * plan.halves;
+  if (bytes < need)
+    return fail(DSX_EINVAL, "%s: the workspace has %lld bytes, %lld are needed", what, (long long)bytes,
+                (long long)need);
+  int32_t* skip = (int32_t*)base;
+  Info* info = (Info*)(base + 256);
+  double* partials = (double*)(base + plan.info_bytes);
+  short* ws = (short*)(base + plan.info_bytes + plan.partial_bytes);
+  ma.skip = MUON ? skip : nullptr;
+  auto sums = [&](Table& t, bool, int) {
+    const int64_t n = tiles_of(t, [](const Mat& m) { return (int64_t)m.parts; });
+    k_sumsq<DT, MUON><<<dim3((unsigned)n), 256, 0, s>>>(t, partials, ma);
+  };
+  auto norms = [&](Table& t, bool, int at) { k_norms<<<t.n, 64, 0, s>>>(t, partials, info + at, eps, ma.skip); };
+  auto rest = [&](Table& t, bool tall, int at) {
+    const int64_t n = tiles_of(t, [](const Mat& m) {
+      return ceil_div(m.rows8, kNormTile) * ceil_div(m.cols8, kNormTile);
+    });
+    k_cast<DT, MUON><<<dim3((unsigned)n), 256, 0, s>>>(t, ws, info + at, ma);
+    iterate<MUON>(t, tall, ws, info + at, steps, coef, ma, out_dt, s);
+  };
+  each_run(src, count, sums);
+  each_run(src, count, norms);
+  each_run(src, count, rest);
+  return launch_status(what);
+}
+
+int check_common(const char* what, int32_t count, int steps, const double* coef, double eps, const void* ws) {
+  if (count < 0) return fail(DSX_EINVAL, "%s: count must be >= 0", what);
+  if (steps < 1 || steps > 64) return fail(DSX_EINVAL, "%s: steps must be in [1, 64]", what);
+  if (!coef) return fail(DSX_EINVAL, "%s: coefficients is NULL", what);
+  for (int k = 0; k < 3 * steps; k++)
+    if (!isfinite(coef[k])) return fail(DSX_EINVAL, "%s: coefficients must be finite", what);
+  if (!(eps >= 1e-20 && eps <= 1.0)) return fail(DSX_EINVAL, "%s: eps must be in [1e-20, 1]", what);
+  if (!ws || ((uintptr_t)ws & 255)) return fail(DSX_EINVAL, "%s: the workspace must be 256-byte aligned", what);
+  return DSX_OK;
+}
+
+int check_shape(const char* what, int32_t k, int64_t rows, int64_t cols) {
+  if (rows < 0 || cols < 0 || rows > DSX_MATRIX_MAX_DIM || cols > DSX_MATRIX_MAX_DIM)
+    return fail(DSX_EINVAL, "%s: matrix %d is %lld x %lld: dimensions must be in [0, %d]", what, (int)k,
+                (long long)rows, (long long)cols, DSX_MATRIX_MAX_DIM);
+  return DSX_OK;
+}
+
+constexpr int32_t kMaxList = 4096;
+
+}  // namespace
+
+extern "C" {
+
+int64_t dsx_orthogonalize_workspace(const DsxMatrix* mats, int32_t count) {
+  if (count < 0 || count > kMaxList || (count && !mats))
+    return fail(-1, "dsx_orthogonalize_workspace: bad list");
+  Source* src = new (std::nothrow) Source[count ? count : 1];
+  if (!src) return fail(-1, "dsx_orthogonalize_workspace: out of memory");
+  for (int32_t k = 0; k < count; k++) {
+    if (check_shape("dsx_orthogonalize_workspace", k, mats[k].rows, mats[k].cols)) {
+      delete[] src;
+      return -1;
+    }
+    src[k] = Source{};
+    src[k].rows = (int32_t)mats[k].rows;
+    src[k].cols = (int32_t)mats[k].cols;
+  }
+  const Plan plan = each_run(src, count, [](Table&, bool, int) {});
+  delete[] src;
+  return plan.info_bytes + plan.partial_bytes + 2 * plan.halves;
+}
+
+int dsx_orthogonalize(const DsxMatrix* mats, int32_t count, int dtype, int32_t steps, const double* coefficients,
+                      double eps, void* workspace, int64_t workspace_bytes, void* stream) {
+  const char* what = "dsx_orthogonalize";
+  if (count > kMaxList) return fail(DSX_EINVAL, "%s: at most %d matrices", what, kMaxList);
+  if (int rc = check_common(what, count, steps, coefficients, eps, workspace)) return rc;
+  if (count && !mats) return fail(DSX_EINVAL, "%s: mats is NULL", what);
+  if (dtype != DSX_F32 && !dsxi::is16(dtype)) return fail(DSX_EINVAL, "%s: bad dtype %d", what, dtype);
+  Source* src = new (std::nothrow) Source[count ? count : 1];
+  if (!src) return fail(DSX_EINVAL, "%s: out of memory", what);
+  int rc = DSX_OK;
+  const uintptr_t unit = dtype == DSX_F32 ? 3 : 1;
+  for (int32_t k = 0; k < count && !rc; k++) {
+    const DsxMatrix& q = mats[k];
+    rc = check_shape(what, k, q.rows, q.cols);
+    if (rc || !q.rows || !q.cols) {
+      src[k] = Source{};
+      continue;
+    }
+    if (!q.in || !q.out || ((uintptr_t)q.in & unit) || ((uintptr_t)q.out & 1))
+      rc = fail(DSX_EINVAL, "%s: matrix %d has a NULL or misaligned pointer", what, (int)k);
+    else if (q.ld_in < q.cols || q.ld_out < q.cols)
+      rc = fail(DSX_EINVAL, "%s: matrix %d has a row stride below its columns", what, (int)k);
+    src[k] = Source{q.in, q.out, nullptr, nullptr, q.ld_in, q.ld_out, (int32_t)q.rows, (int32_t)q.cols, 0.0f};
+  }
+  if (!rc) {
+    const MuonArgs ma{};
+    char* base = (char*)workspace;
+    hipStream_t s = as_stream(stream);
+    if (dtype == DSX_F32)
+      rc = drive<DSX_F32, false>(src, count, steps, coefficients, eps, ma, DSX_BF16, base, workspace_bytes, what, s);
+    else if (dtype == DSX_F16)
+      rc = drive<DSX_F16, false>(src, count, steps, coefficients, eps, ma, DSX_BF16, base, workspace_bytes, what, s);
+    else
+      rc = drive<DSX_BF16, false>(src, count, steps, coefficients, eps, ma, DSX_BF16, base, workspace_bytes, what, s);
+  }
+  delete[] src;
+  return rc;
+}
+
+}  // extern "C"

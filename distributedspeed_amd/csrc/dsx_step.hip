@@ -30,6 +30,7 @@
 #include <type_traits>
 
 #include "dsx.h"
+#include "dsx_internal.h"
 
 static_assert(sizeof(DsxState) == 64, "DsxState layout");
 static_assert(sizeof(DsxScalerConfig) == 32, "DsxScalerConfig layout");
@@ -52,14 +53,11 @@ static __device__ __align__(256) unsigned char scratch[DSX_NOALLOC_SCRATCH_BYTES
 
 namespace {
 
-constexpr int kBlock = 256;
-constexpr int kWaves = kBlock / 64;
-
-typedef float    f4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u2 __attribute__((ext_vector_type(2)));
-typedef uint32_t u4 __attribute__((ext_vector_type(4)));
-
 thread_local char g_err[512];
+
+}  // namespace
+
+namespace dsxi {
 
 int fail(int code, const char* fmt, ...) {
   va_list ap;
@@ -75,6 +73,20 @@ int launch_status(const char* what) {
     return fail((int)e, "%s: launch failed: %s", what, hipGetErrorString(e));
   return DSX_OK;
 }
+
+}  // namespace dsxi
+
+namespace {
+
+constexpr int kBlock = 256;
+constexpr int kWaves = kBlock / 64;
+
+typedef float    f4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+
+using dsxi::fail;
+using dsxi::launch_status;
 
 __host__ __device__ inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 bool is16(int dt) { return dt == DSX_F16 || dt == DSX_BF16; }

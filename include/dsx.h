@@ -91,6 +91,9 @@ extern "C" {
 #define DSX_NOALLOC_MAX_PARTIALS 8192
 #define DSX_NOALLOC_SCRATCH_BYTES (8 * DSX_NOALLOC_MAX_PARTIALS + 256)
 
+/* upper bound on a matrix dimension of the Muon and block entry points */
+#define DSX_MATRIX_MAX_DIM (1 << 20)
+
 /* Device-resident optimizer + loss-scaler state (64 bytes). Write it with
  * dsx_state_init, or copy back one the library wrote (a checkpoint). A
  * caller that fills one itself must zero clip_once_coef, clip_once,
@@ -590,6 +593,40 @@ int dsx_zero_step_lists(const DsxTensorRef* tensors, const DsxChunk* chunks,
                         DsxState* state, DsxScalerConfig scaler,
                         const DsxGroupsDev* groups, double* partials,
                         int32_t nparts, DsxStepScalars* out, void* stream);
+
+/* ---- Muon: orthogonalisation by Newton-Schulz products ---------------- */
+
+/* One matrix of a list (a host array): rows x cols, row-major with row
+ * strides ld_in and ld_out in elements. */
+typedef struct DsxMatrix {
+  const void* in;
+  void*       out;
+  int64_t     ld_in;
+  int64_t     ld_out;
+  int64_t     rows;
+  int64_t     cols;
+} DsxMatrix;
+
+/* Bytes of device scratch dsx_orthogonalize needs for the list (the shapes
+ * alone are read); -1 with dsx_last_error for a bad list. Host only. */
+int64_t dsx_orthogonalize_workspace(const DsxMatrix* mats /* host */,
+                                    int32_t count);
+
+/* out = the Newton-Schulz iterate of in, for each matrix of the list:
+ *   X0 = G / (|G|_F + eps); then for each of `steps` triples (a, b, c) of
+ *   `coefficients` (host):  A = X X^T,  X = a X + (b A + c A A) X
+ * (the transposed products where rows > cols: the result is the same).
+ * in is of `dtype` (DSX_F32, DSX_F16 or DSX_BF16), out is bf16. A zero matrix
+ * gives zeros; a matrix with a non-finite element gives NaN throughout. The
+ * iterates are held in fp16 with fp32 sums: the coefficients must keep every
+ * singular value below 4 and every one of b A + c A A below 16 in magnitude
+ * (Muon's 3.4445, -4.7750, 2.0315 stay below 1.3 and 2.9). Matrices with no
+ * element are skipped. steps in [1, 64], eps in [1e-20, 1]; `workspace` is
+ * 256-byte aligned device memory. No counterpart in the reference. */
+int dsx_orthogonalize(const DsxMatrix* mats /* host */, int32_t count,
+                      int dtype, int32_t steps,
+                      const double* coefficients /* host */, double eps,
+                      void* workspace, int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
