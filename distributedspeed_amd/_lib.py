@@ -82,9 +82,16 @@ class DsxMatrix(_c.Structure):
                 ("cols", _c.c_int64)]
 
 
+class DsxFfn(_c.Structure):
+    _fields_ = [("x", _P), ("w_gate", _P), ("w_up", _P), ("w_down", _P)] + \
+               [(k, _c.c_int64) for k in ("ld_x", "ld_gate", "ld_up", "ld_down", "tokens", "width", "inner")] + \
+               [(k, _c.c_int32) for k in ("dtype", "activation", "keep", "reserved")] + \
+               [("saved", _P), ("workspace", _P), ("workspace_bytes", _c.c_int64)]
+
+
 for _s, _n in ((DsxState, 64), (DsxScalerConfig, 32), (DsxAdamwHyper, 56), (DsxStepScalars, 64),
                (DsxTensorRef, 56), (DsxChunk, 24), (DsxGroupsDev, 1112), (DsxFlatPlan, 248),
-               (DsxMatrix, 48)):
+               (DsxMatrix, 48), (DsxFfn, 128)):
     assert _c.sizeof(_s) == _n, (_s.__name__, _c.sizeof(_s))
 
 # name -> (restype, argtypes); every symbol include/dsx.h declares.
@@ -136,6 +143,10 @@ SIGNATURES = {
                                        _P, _c.c_int32, _P, _P]),
     "dsx_orthogonalize_workspace": (_c.c_int64, [_P, _c.c_int32]),
     "dsx_orthogonalize": (_c.c_int, [_P, _c.c_int32, _c.c_int, _c.c_int32, _P, _c.c_double, _P, _c.c_int64, _P]),
+    "dsx_ffn_saved_bytes": (_c.c_int64, [_c.c_int64, _c.c_int64, _c.c_int32]),
+    "dsx_ffn_workspace_bytes": (_c.c_int64, [_P, _c.c_int32]),
+    "dsx_ffn_forward": (_c.c_int, [_P, _P, _c.c_int64, _P]),
+    "dsx_ffn_backward": (_c.c_int, [_P, _P, _c.c_int64, _P, _c.c_int64, _P, _P, _P, _P]),
 }
 
 _lib: ctypes.CDLL | None = None

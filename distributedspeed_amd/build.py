@@ -39,6 +39,7 @@ ARCH = os.environ.get("DSX_OFFLOAD_ARCH", "gfx950")
 SOURCES = {
     "dsx_step.hip": ["-ffp-contract=off"],
     "dsx_muon.hip": [],
+    "dsx_ffn.hip": [],
 }
 
 

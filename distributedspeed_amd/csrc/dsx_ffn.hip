@@ -1,0 +1,603 @@
+// dsx_ffn.hip -- the gated feed-forward block and its gradients (see
+// include/dsx.h).
+//
+//   g = x Wg^T, u = x Wu^T, h = act(g) u, y = h Wd^T      (M tokens, D wide, F inner)
+//   dh = dy Wd, dg = dh u act'(g), du = dh act(g)
+//   dx = dg Wg + du Wu, dWg = dg^T x, dWu = du^T x, dWd = dy^T h
+//
+// Forward is two launches: the first computes both projections in one tile
+// (half its columns from Wg, half from Wu, so a lane holds g and u of the same
+// element) and writes h; the second is the product with Wd. Backward is three:
+// dh with the gradients of g and u as its epilogue, dx as one sum over 2F, and
+// the three weight gradients as one launch.
+//
+// What the backward's epilogue needs of the forward is not g and u but the two
+// factors u act'(g) and act(g), from the fp32 sums: dg and du are then products
+// with no activation to evaluate. A factor is kept as the upper 24 bits of its
+// fp32 value (16 bits and 8 bits in separate planes): kept in bf16 they would
+// add a rounding to both gradients as large as the one of dg and du to 16
+// bits, which the matrix instruction's types do demand. h, dg and du are
+// rounded to the inputs' type once.
+//
+// With few tokens there are fewer tiles than CUs while the weights' bytes
+// bound the time: the sum over k is split over blocks, each writing fp32
+// partial sums, and a second launch adds them in order and applies the
+// epilogue.
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <type_traits>
+
+#include "dsx.h"
+#include "dsx_gemm.h"
+#include "dsx_internal.h"
+
+namespace {
+
+using namespace dsxg;
+using dsxi::as_stream;
+using dsxi::ceil_div;
+using dsxi::fail;
+using dsxi::launch_status;
+using dsxi::round_up;
+
+// ---- activations -----------------------------------------------------------
+
+struct ActValue {
+  float f, d;  // value and derivative
+};
+
+__device__ inline ActValue activate(int act, float g) {
+  ActValue r;
+  if (act == DSX_ACT_SILU) {
+    const float s = 1.0f / (1.0f + __expf(-g));
+    r.f = g * s;
+    r.d = s * (1.0f + g * (1.0f - s));
+  } else if (act == DSX_ACT_GELU) {
+    const float phi = 0.5f * (1.0f + erff(g * 0.70710678118654752f));
+    r.f = g * phi;
+    r.d = phi + g * 0.39894228040143268f * __expf(-0.5f * g * g);
+  } else if (act == DSX_ACT_GELU_TANH) {
+    const float k = 0.79788456080286536f, c = 0.044715f;
+    const float t = tanhf(k * (g + c * g * g * g));
+    r.f = 0.5f * g * (1.0f + t);
+    r.d = 0.5f * (1.0f + t) + 0.5f * g * (1.0f - t * t) * k * (1.0f + 3.0f * c * g * g);
+  } else {
+    r.f = g > 0.0f ? g : (g != g ? g : 0.0f);
+    r.d = g > 0.0f ? 1.0f : 0.0f;
+  }
+  return r;
+}
+
+// ---- what the forward keeps ------------------------------------------------
+
+// Planes of [tokens][ldf]: h (16 bit), then the upper 16 and the next 8 bits
+// of the two factors.
+struct Saved {
+  short* h;
+  uint16_t* p_hi;
+  uint16_t* q_hi;
+  uint8_t* p_lo;
+  uint8_t* q_lo;
+  int64_t ld;
+};
+
+typedef uint16_t u16x4 __attribute__((ext_vector_type(4)));
+typedef uint8_t  u8x4 __attribute__((ext_vector_type(4)));
+
+// fp32 rounded to its upper 24 bits (nearest; NaN and inf stay what they are).
+__device__ inline uint32_t top24(float v) {
+  uint32_t b = __builtin_bit_cast(uint32_t, v);
+  if ((b & 0x7F800000u) != 0x7F800000u) b += 0x80u;
+  else if (b & 0x007FFFFFu) b |= 0x00400000u;  // a NaN whose low bits alone say so
+  return b;
+}
+__device__ inline void put24(uint16_t* hi, uint8_t* lo, int64_t at, const float* v) {
+  u16x4 a;
+  u8x4 b;
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    const uint32_t w = top24(v[e]);
+    a[e] = (uint16_t)(w >> 16);
+    b[e] = (uint8_t)(w >> 8);
+  }
+  *(u16x4*)(hi + at) = a;
+  *(u8x4*)(lo + at) = b;
+}
+__device__ inline void get24(const uint16_t* hi, const uint8_t* lo, int64_t at, float* v) {
+  const u16x4 a = *(const u16x4*)(hi + at);
+  const u8x4 b = *(const u8x4*)(lo + at);
+#pragma unroll
+  for (int e = 0; e < 4; e++) v[e] = __builtin_bit_cast(float, ((uint32_t)a[e] << 16) | ((uint32_t)b[e] << 8));
+}
+
+// ---- epilogues: four columns of a row --------------------------------------
+
+template <class T>
+struct Store {  // C in the inputs' type
+  static constexpr bool kPair = false;
+  short* c;
+  int64_t ld;
+  __device__ inline void operator()(int m, int n, int N, const f4v& v, const f4v&) const {
+    short* o = c + m * ld + n;
+    s4v w;
+#pragma unroll
+    for (int e = 0; e < 4; e++) w[e] = T::round(v[e]);
+    if (n + 4 <= N && ((uintptr_t)o & 7) == 0)
+      *(s4v*)o = w;
+    else
+      for (int e = 0; e < 4; e++)
+        if (n + e < N) o[e] = w[e];
+  }
+};
+
+template <class T>
+struct Up {  // h and the factors from g and u
+  static constexpr bool kPair = true;
+  Saved s;
+  int act, keep;
+  __device__ inline void operator()(int m, int n, int, const f4v& g, const f4v& u) const {
+    const int64_t at = m * s.ld + n;
+    s4v w;
+    float p[4], q[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const ActValue a = activate(act, g[e]);
+      w[e] = T::round(a.f * u[e]);
+      p[e] = u[e] * a.d;
+      q[e] = a.f;
+    }
+    *(s4v*)(s.h + at) = w;
+    if (keep) {
+      put24(s.p_hi, s.p_lo, at, p);
+      put24(s.q_hi, s.q_lo, at, q);
+    }
+  }
+};
+
+template <class T>
+struct Factors {  // dg and du from dh
+  static constexpr bool kPair = false;
+  Saved s;
+  short* dg;
+  short* du;
+  __device__ inline void operator()(int m, int n, int, const f4v& v, const f4v&) const {
+    const int64_t at = m * s.ld + n;
+    float p[4], q[4];
+    get24(s.p_hi, s.p_lo, at, p);
+    get24(s.q_hi, s.q_lo, at, q);
+    s4v a, b;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      a[e] = T::round(v[e] * p[e]);
+      b[e] = T::round(v[e] * q[e]);
+    }
+    *(s4v*)(dg + at) = a;
+    *(s4v*)(du + at) = b;
+  }
+};
+
+// ---- one product: C = sum over segments of A_s B_s^T ------------------------
+
+struct Product {
+  Operand a[2], b[2];  // b[1] is the second half tile's operand for a pair, else segment 1's
+  int k;               // of each segment
+  int segments;
+  int m, n;
+  int mt, nt;
+  int splits, per;     // K tiles per split, over all segments
+  float* part;         // fp32 partial sums [split][m][ldp] where splits > 1 (a pair: u at ldp / 2)
+  int64_t ldp;
+};
+
+__device__ inline Operand at_k(Operand o, bool row, int k) {
+  o.p += row ? k : k * o.ld;
+  return o;
+}
+
+template <class G, bool RA, bool RB, class E>
+__global__ __launch_bounds__(G::THREADS) void k_product(Product p, E e) {
+  __shared__ __attribute__((aligned(1024))) char lds[G::kLds];
+  constexpr int TN = E::kPair ? G::TN / 2 : G::TN;
+  const int tiles = p.mt * p.nt;
+  const int bid = xcd_order(blockIdx.x, gridDim.x);
+  const int split = bid / tiles;
+  int ti, tj;
+  band_order(bid - split * tiles, p.mt, p.nt, 8, &ti, &tj);
+  G g;
+  g.init();
+  const int kt = (p.k + kBK - 1) / kBK;
+  const int lo = split * p.per, hi = min(lo + p.per, kt * p.segments);
+  for (int s = 0; s < p.segments; s++) {
+    const int k0 = max(lo - s * kt, 0) * kBK, k1 = min(min(hi - s * kt, kt) * kBK, p.k);
+    if (k0 >= k1) continue;
+    const Operand a = at_k(p.a[s], RA, k0);
+    const Operand b = at_k(E::kPair ? p.b[0] : p.b[s], RB, k0);
+    const Operand b1 = E::kPair ? at_k(p.b[1], RB, k0) : b;
+    g.run(lds, a, b, b1, ti * G::TM, tj * TN, k1 - k0);
+  }
+  constexpr int NF = E::kPair ? G::NF / 2 : G::NF;
+#pragma unroll
+  for (int i = 0; i < G::MF; i++) {
+    const int m = ti * G::TM + g.row_of(i);
+    if (m >= p.m) continue;
+#pragma unroll
+    for (int j = 0; j < NF; j++) {
+      const int n = tj * TN + (E::kPair ? g.half_col(j) : g.col_of(j));
+      if (n >= p.n) continue;
+      const f4v v = g.acc[i][j], w = E::kPair ? g.acc[i][(j + NF) % G::NF] : v;
+      if (p.splits > 1) {
+        float* o = p.part + ((int64_t)split * p.m + m) * p.ldp + n;
+        *(f4v*)o = v;
+        if (E::kPair) *(f4v*)(o + p.ldp / 2) = w;
+      } else {
+        e(m, n, p.n, v, w);
+      }
+    }
+  }
+}
+
+// Adds the splits' partial sums in order and applies the epilogue.
+template <class E>
+__global__ __launch_bounds__(256) void k_join(const float* __restrict__ part, int m, int n, int64_t ldp, int splits,
+                                              E e) {
+  const int c = (blockIdx.x * 256 + threadIdx.x) * 4, r = blockIdx.y;
+  if (c >= n) return;
+  f4v v = {0, 0, 0, 0}, w = {0, 0, 0, 0};
+  const float* q = part + r * ldp + c;
+  for (int s = 0; s < splits; s++, q += m * ldp) {
+    v += *(const f4v*)q;
+    if (E::kPair) w += *(const f4v*)(q + ldp / 2);
+  }
+  e(r, c, n, v, w);
+}
+
+// ---- the weight gradients: up to three products over the tokens ------------
+
+struct WeightGrad {
+  Operand a, b;
+  short* out;
+  int m, n, tile0, nt;
+};
+struct WeightGrads {
+  WeightGrad w[3];
+  int count, tokens;
+};
+
+template <class G, class T>
+__global__ __launch_bounds__(G::THREADS) void k_weight_grads(WeightGrads t) {
+  __shared__ __attribute__((aligned(1024))) char lds[G::kLds];
+  const int bid = xcd_order(blockIdx.x, gridDim.x);
+  int i = 0;
+  while (i + 1 < t.count && bid >= t.w[i + 1].tile0) i++;
+  const WeightGrad& q = t.w[i];
+  int ti, tj;
+  band_order(bid - q.tile0, (q.m + G::TM - 1) / G::TM, q.nt, 8, &ti, &tj);
+  G g;
+  g.init();
+  g.run(lds, q.a, q.b, q.b, ti * G::TM, tj * G::TN, t.tokens);
+  const Store<T> e{q.out, q.n};
+#pragma unroll
+  for (int x = 0; x < G::MF; x++) {
+    const int m = ti * G::TM + g.row_of(x);
+    if (m >= q.m) continue;
+#pragma unroll
+    for (int y = 0; y < G::NF; y++) {
+      const int n = tj * G::TN + g.col_of(y);
+      if (n < q.n) e(m, n, q.n, g.acc[x][y], g.acc[x][y]);
+    }
+  }
+}
+
+// ---- host ------------------------------------------------------------------
+
+int cu_count() {
+  static const int n = [] {
+    int dev = 0, v = 0;
+    if (hipGetDevice(&dev) != hipSuccess ||
+        hipDeviceGetAttribute(&v, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || v <= 0)
+      v = 256;
+    return v;
+  }();
+  return n;
+}
+
+// Tile rows and splits of a product of m x n over kt K tiles.
+struct Shape {
+  int tm, tn, splits, per;
+};
+
+Shape shape_of(int64_t m, int64_t n, int64_t kt, bool pair, bool direct) {
+  const int cus = 256;  // the split count fixes the order of sums: by sizes alone, the same on any card
+  Shape s{};
+  const int64_t cols = pair ? 2 * n : n;
+  if (!direct) {
+    s.tm = m <= 32 ? 32 : 128;
+    s.tn = 128;
+  } else if (m <= 64) {
+    s.tm = m <= 16 ? 16 : m <= 32 ? 32 : 64;
+    s.tn = 128;
+  } else {
+    const bool big = ceil_div(m, 256) * ceil_div(cols, 256) >= 2 * cus;
+    s.tm = s.tn = big ? 256 : 128;
+  }
+  const int64_t tiles = ceil_div(m, s.tm) * ceil_div(cols, s.tn);
+  const int64_t want = s.tm <= 64 ? 4 * cus : 2 * cus;  // blocks that a CU holds at once, over all CUs
+  int64_t splits = tiles >= want / 2 ? 1 : ceil_div(want, tiles);
+  if (splits > kt / 2) splits = kt / 2;  // two K tiles each at least
+  if (splits < 1) splits = 1;
+  s.per = (int)ceil_div(kt, splits);
+  s.splits = (int)ceil_div(kt, s.per);
+  return s;
+}
+
+int64_t ld_inner(int64_t inner) { return round_up(inner, 8); }
+
+int64_t part_bytes(int64_t m, int64_t n, const Shape& s, bool pair) {
+  return s.splits > 1 ? s.splits * m * round_up(n, 8) * (pair ? 2 : 1) * 4 : 0;
+}
+
+template <class T, bool RA, bool RB, class E>
+void launch_product(Product p, const Shape& s, bool direct, float* part, const E& e, hipStream_t st) {
+  constexpr bool PAIR = E::kPair;
+  const int64_t cols = PAIR ? 2 * (int64_t)p.n : p.n;
+  p.mt = (int)ceil_div(p.m, s.tm);
+  p.nt = (int)ceil_div(cols, s.tn);
+  p.splits = s.splits;
+  p.per = s.per;
+  p.part = part;
+  p.ldp = round_up(p.n, 8) * (PAIR ? 2 : 1);
+  const dim3 grid((unsigned)(p.mt * p.nt * p.splits));
+#define DSX_RUN(TM, TN, WM, WN, DIRECT)                              \
+  do {                                                               \
+    using G = Gemm<T, TM, TN, WM, WN, RA, RB, DIRECT, PAIR>;         \
+    k_product<G, RA, RB, E><<<grid, G::THREADS, 0, st>>>(p, e);      \
+  } while (0)
+  if (direct) {
+    if (s.tm == 16) DSX_RUN(16, 128, 1, 4, true);
+    else if (s.tm == 32) DSX_RUN(32, 128, 1, 4, true);
+    else if (s.tm == 64) DSX_RUN(64, 128, 1, 4, true);
+    else if (s.tm == 128) DSX_RUN(128, 128, 2, 2, true);
+    else DSX_RUN(256, 256, 2, 4, true);
+  } else {
+    if (s.tm == 32) DSX_RUN(32, 128, 1, 4, false);
+    else DSX_RUN(128, 128, 2, 2, false);
+  }
+#undef DSX_RUN
+  if (p.splits > 1)
+    k_join<E><<<dim3((unsigned)ceil_div(p.n, 1024), (unsigned)p.m), 256, 0, st>>>(part, p.m, p.n, p.ldp, p.splits, e);
+}
+
+// The direct loads' demands of one operand (rows or columns of `contiguous`
+// elements at a stride of ld).
+bool direct_ok(const void* p, int64_t ld, int64_t contiguous) {
+  return ((uintptr_t)p & 15) == 0 && ld % 8 == 0 && contiguous % 8 == 0 && ld <= (1 << 22);
+}
+
+struct Sizes {
+  int64_t m, d, f, ldf;
+  int kd, kf;  // K tiles over D and over F
+};
+Sizes sizes_of(const DsxFfn& q) {
+  Sizes z{q.tokens, q.width, q.inner, ld_inner(q.inner), 0, 0};
+  z.kd = (int)ceil_div(z.d, kBK);
+  z.kf = (int)ceil_div(z.f, kBK);
+  return z;
+}
+
+Saved saved_of(const DsxFfn& q) {
+  const int64_t ld = ld_inner(q.inner), n = q.tokens * ld;
+  Saved s{};
+  char* p = (char*)q.saved;
+  s.ld = ld;
+  s.h = (short*)p;
+  s.p_hi = (uint16_t*)(p + 2 * n);
+  s.q_hi = (uint16_t*)(p + 4 * n);
+  s.p_lo = (uint8_t*)(p + 6 * n);
+  s.q_lo = (uint8_t*)(p + 7 * n);
+  return s;
+}
+
+struct Direct {
+  bool up, down, dh, dx, dw;
+};
+Direct direct_of(const DsxFfn& q, const void* dy, int64_t ld_dy) {
+  const bool x = direct_ok(q.x, q.ld_x, q.width), wg = direct_ok(q.w_gate, q.ld_gate, q.width),
+             wu = direct_ok(q.w_up, q.ld_up, q.width), wd = direct_ok(q.w_down, q.ld_down, q.inner),
+             y = dy && direct_ok(dy, ld_dy, q.width), f = q.inner % 8 == 0;
+  Direct d{};
+  d.up = x && wg && wu;
+  d.down = wd && f;
+  d.dh = y && wd;
+  d.dx = wg && wu && f;
+  d.dw = x && y && f;
+  return d;
+}
+
+int64_t workspace_of(const DsxFfn& q, bool backward) {
+  const Sizes z = sizes_of(q);
+  // both load forms, so that the size does not hang on addresses
+  int64_t part = 0;
+  for (int direct = 0; direct < 2; direct++) {
+    int64_t b[4] = {part_bytes(z.m, z.f, shape_of(z.m, z.f, z.kd, true, direct), true),
+                    part_bytes(z.m, z.d, shape_of(z.m, z.d, z.kf, false, direct), false), 0, 0};
+    if (backward) {
+      b[2] = part_bytes(z.m, z.f, shape_of(z.m, z.f, z.kd, false, direct), false);
+      b[3] = part_bytes(z.m, z.d, shape_of(z.m, z.d, 2 * z.kf, false, direct), false);
+      b[0] = b[1] = 0;
+    }
+    for (int64_t v : b)
+      if (v > part) part = v;
+  }
+  return round_up(part, 256) + (backward ? 2 * round_up(z.m * z.ldf * 2, 256) : 0) + 256;
+}
+
+template <class T>
+int forward(const DsxFfn& q, void* y, int64_t ld_y, hipStream_t st) {
+  const Sizes z = sizes_of(q);
+  const Direct dir = direct_of(q, nullptr, 0);
+  const Saved s = saved_of(q);
+  float* part = (float*)q.workspace;
+  Product p{};
+  p.a[0] = {(const short*)q.x, q.ld_x, (int)z.m};
+  p.b[0] = {(const short*)q.w_gate, q.ld_gate, (int)z.f};
+  p.b[1] = {(const short*)q.w_up, q.ld_up, (int)z.f};
+  p.k = (int)z.d;
+  p.segments = 1;
+  p.m = (int)z.m;
+  p.n = (int)z.f;
+  launch_product<T, true, true>(p, shape_of(z.m, z.f, z.kd, true, dir.up), dir.up, part,
+                                Up<T>{s, q.activation, q.keep}, st);
+  Product r{};
+  r.a[0] = {s.h, s.ld, (int)z.m};
+  r.b[0] = {(const short*)q.w_down, q.ld_down, (int)z.d};
+  r.k = (int)z.f;
+  r.segments = 1;
+  r.m = (int)z.m;
+  r.n = (int)z.d;
+  launch_product<T, true, true>(r, shape_of(z.m, z.d, z.kf, false, dir.down), dir.down, part,
+                                Store<T>{(short*)y, ld_y}, st);
+  return launch_status("dsx_ffn_forward");
+}
+
+template <class T, bool DIRECT>
+void launch_weight_grads(WeightGrads& w, hipStream_t st) {
+  int64_t big = 0;
+  for (int i = 0; i < w.count; i++) big += ceil_div(w.w[i].m, 256) * ceil_div(w.w[i].n, 256);
+  const int tile = DIRECT && big >= 2 * cu_count() && w.tokens >= 512 ? 256 : 128;
+  int64_t n = 0;
+  for (int i = 0; i < w.count; i++) {
+    w.w[i].tile0 = (int)n;
+    w.w[i].nt = (int)ceil_div(w.w[i].n, tile);
+    n += ceil_div(w.w[i].m, tile) * w.w[i].nt;
+  }
+  if (!n) return;
+  if constexpr (DIRECT) {
+    if (tile == 256) {
+      using G = Gemm<T, 256, 256, 2, 4, false, false, true>;
+      k_weight_grads<G, T><<<dim3((unsigned)n), G::THREADS, 0, st>>>(w);
+      return;
+    }
+  }
+  using G = Gemm<T, 128, 128, 2, 2, false, false, DIRECT>;
+  k_weight_grads<G, T><<<dim3((unsigned)n), G::THREADS, 0, st>>>(w);
+}
+
+template <class T>
+int backward(const DsxFfn& q, const void* dy, int64_t ld_dy, void* dx, int64_t ld_dx, void* dw_gate, void* dw_up,
+             void* dw_down, hipStream_t st) {
+  const Sizes z = sizes_of(q);
+  const Direct dir = direct_of(q, dy, ld_dy);
+  const Saved s = saved_of(q);
+  const int64_t plane = round_up(z.m * z.ldf * 2, 256);
+  short* dg = (short*)q.workspace;
+  short* du = (short*)((char*)q.workspace + plane);
+  float* part = (float*)((char*)q.workspace + 2 * plane);
+  const int m = (int)z.m;
+  if (dx || dw_gate || dw_up) {
+    Product p{};
+    p.a[0] = {(const short*)dy, ld_dy, m};
+    p.b[0] = {(const short*)q.w_down, q.ld_down, (int)z.f};
+    p.k = (int)z.d;
+    p.segments = 1;
+    p.m = m;
+    p.n = (int)z.f;
+    launch_product<T, true, false>(p, shape_of(z.m, z.f, z.kd, false, dir.dh), dir.dh, part, Factors<T>{s, dg, du},
+                                   st);
+  }
+  if (dx) {
+    Product r{};
+    r.a[0] = {dg, z.ldf, m};
+    r.a[1] = {du, z.ldf, m};
+    r.b[0] = {(const short*)q.w_gate, q.ld_gate, (int)z.d};
+    r.b[1] = {(const short*)q.w_up, q.ld_up, (int)z.d};
+    r.k = (int)z.f;
+    r.segments = 2;
+    r.m = m;
+    r.n = (int)z.d;
+    launch_product<T, true, false>(r, shape_of(z.m, z.d, 2 * z.kf, false, dir.dx), dir.dx, part,
+                                   Store<T>{(short*)dx, ld_dx}, st);
+  }
+  WeightGrads w{};
+  w.tokens = m;
+  const Operand x{(const short*)q.x, q.ld_x, (int)z.d}, oy{(const short*)dy, ld_dy, (int)z.d};
+  const Operand og{dg, z.ldf, (int)z.f}, ou{du, z.ldf, (int)z.f}, oh{s.h, s.ld, (int)z.f};
+  if (dw_gate) w.w[w.count++] = {og, x, (short*)dw_gate, (int)z.f, (int)z.d, 0, 0};
+  if (dw_up) w.w[w.count++] = {ou, x, (short*)dw_up, (int)z.f, (int)z.d, 0, 0};
+  if (dw_down) w.w[w.count++] = {oy, oh, (short*)dw_down, (int)z.d, (int)z.f, 0, 0};
+  if (dir.dw)
+    launch_weight_grads<T, true>(w, st);
+  else
+    launch_weight_grads<T, false>(w, st);
+  return launch_status("dsx_ffn_backward");
+}
+
+int check_sizes(const char* what, const DsxFfn* q) {
+  if (!q) return fail(DSX_EINVAL, "%s: the block is NULL", what);
+  if (q->tokens < 0 || q->tokens > DSX_MATRIX_MAX_DIM || q->width < 1 || q->width > DSX_MATRIX_MAX_DIM ||
+      q->inner < 1 || q->inner > DSX_MATRIX_MAX_DIM)
+    return fail(DSX_EINVAL, "%s: tokens in [0, %d], width and inner in [1, %d]", what, DSX_MATRIX_MAX_DIM,
+                DSX_MATRIX_MAX_DIM);
+  if (!dsxi::is16(q->dtype)) return fail(DSX_EINVAL, "%s: dtype must be DSX_F16 or DSX_BF16", what);
+  if (q->activation < DSX_ACT_SILU || q->activation > DSX_ACT_RELU)
+    return fail(DSX_EINVAL, "%s: bad activation %d", what, q->activation);
+  return DSX_OK;
+}
+
+int check_block(const char* what, const DsxFfn* q, bool backward) {
+  if (int rc = check_sizes(what, q)) return rc;
+  if (!q->tokens) return DSX_OK;
+  if (!q->x || !q->w_gate || !q->w_up || !q->w_down || !q->saved || !q->workspace)
+    return fail(DSX_EINVAL, "%s: NULL pointer", what);
+  if ((((uintptr_t)q->x | (uintptr_t)q->w_gate | (uintptr_t)q->w_up | (uintptr_t)q->w_down) & 1) ||
+      (((uintptr_t)q->saved | (uintptr_t)q->workspace) & 255))
+    return fail(DSX_EINVAL, "%s: misaligned pointer", what);
+  if (q->ld_x < q->width || q->ld_gate < q->width || q->ld_up < q->width || q->ld_down < q->inner)
+    return fail(DSX_EINVAL, "%s: a row stride is below the row's length", what);
+  if (q->workspace_bytes < workspace_of(*q, backward))
+    return fail(DSX_EINVAL, "%s: the workspace has %lld bytes, %lld are needed", what, (long long)q->workspace_bytes,
+                (long long)workspace_of(*q, backward));
+  return DSX_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t dsx_ffn_saved_bytes(int64_t tokens, int64_t inner, int32_t keep) {
+  if (tokens < 0 || inner < 1 || tokens > DSX_MATRIX_MAX_DIM || inner > DSX_MATRIX_MAX_DIM)
+    return fail(-1, "dsx_ffn_saved_bytes: sizes out of range");
+  return tokens * ld_inner(inner) * (keep ? 8 : 2);
+}
+
+int64_t dsx_ffn_workspace_bytes(const DsxFfn* block, int32_t backward) {
+  if (check_sizes("dsx_ffn_workspace_bytes", block)) return -1;
+  return workspace_of(*block, backward != 0);
+}
+
+int dsx_ffn_forward(const DsxFfn* block, void* y, int64_t ld_y, void* stream) {
+  const char* what = "dsx_ffn_forward";
+  if (int rc = check_block(what, block, false)) return rc;
+  if (!block->tokens) return DSX_OK;
+  if (!y || ((uintptr_t)y & 1) || ld_y < block->width) return fail(DSX_EINVAL, "%s: bad output", what);
+  hipStream_t s = as_stream(stream);
+  return block->dtype == DSX_F16 ? forward<F16>(*block, y, ld_y, s) : forward<BF16>(*block, y, ld_y, s);
+}
+
+int dsx_ffn_backward(const DsxFfn* block, const void* dy, int64_t ld_dy, void* dx, int64_t ld_dx, void* dw_gate,
+                     void* dw_up, void* dw_down, void* stream) {
+  const char* what = "dsx_ffn_backward";
+  if (int rc = check_block(what, block, true)) return rc;
+  if (!block->keep) return fail(DSX_EINVAL, "%s: the forward kept nothing (keep is 0)", what);
+  if (!block->tokens) return DSX_OK;
+  if (!dy || ((uintptr_t)dy & 1) || ld_dy < block->width) return fail(DSX_EINVAL, "%s: bad output gradient", what);
+  if (dx && (((uintptr_t)dx & 1) || ld_dx < block->width)) return fail(DSX_EINVAL, "%s: bad input gradient", what);
+  if (((uintptr_t)dw_gate | (uintptr_t)dw_up | (uintptr_t)dw_down) & 1)
+    return fail(DSX_EINVAL, "%s: misaligned weight gradient", what);
+  hipStream_t s = as_stream(stream);
+  return block->dtype == DSX_F16 ? backward<F16>(*block, dy, ld_dy, dx, ld_dx, dw_gate, dw_up, dw_down, s)
+                                 : backward<BF16>(*block, dy, ld_dy, dx, ld_dx, dw_gate, dw_up, dw_down, s);
+}
+
+}  // extern "C"

@@ -80,11 +80,14 @@ static __device__ inline void band_order(int t, int mt, int nt, int band, int* t
 
 template <int ROWS, bool ROW, int THREADS>
 struct Stage {
-  static constexpr int kInstr = ROWS * kBK / 8 / THREADS;  // 16-byte chunks per thread
+  static constexpr int kChunks = ROWS * kBK / 8;
+  static constexpr int kInstr = (kChunks + THREADS - 1) / THREADS;  // 16-byte chunks per thread
+  static constexpr bool kPart = kChunks % THREADS != 0;             // the last waves have none
   static constexpr int kBytes = ROWS * kBK * 2;
   static constexpr int kPerRow = ROW ? kBK / 8 : ROWS / 8;  // chunks in one stored row
   static constexpr bool kRow = ROW;
-  static_assert(ROWS * kBK / 8 % THREADS == 0, "whole chunks per thread");
+  static_assert(kChunks % THREADS == 0 || kChunks < THREADS, "whole loads");
+  static_assert(kChunks % 64 == 0, "whole waves");
 
   // Swizzle of a stored row: row tiles permute their 8 chunks by the row pair;
   // col tiles permute 32-byte pairs of chunks by the k rows that one
@@ -205,8 +208,14 @@ struct Gemm {
     }
   }
 
+  // Whether this thread's wave loads a part of a tile smaller than the block.
+  template <class S>
+  __device__ inline bool has() const {
+    return !S::kPart || __builtin_amdgcn_readfirstlane(tid >> 6) < S::kChunks / 64;
+  }
   template <class S>
   __device__ inline void load_direct(char* dst, const short* p, const uint32_t* off) {
+    if (!has<S>()) return;
 #pragma unroll
     for (int j = 0; j < S::kInstr; j++) {
       const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -227,6 +236,7 @@ struct Gemm {
   // Zeros where the last tile holds no k.
   template <class S>
   __device__ inline void zero_tail(char* dst, bool row, int kleft) {
+    if (!has<S>()) return;
 #pragma unroll
     for (int j = 0; j < S::kInstr; j++) {
       int r, c;
@@ -236,6 +246,7 @@ struct Gemm {
   }
   template <class S>
   __device__ inline void load_regs(s8v* v, const short* p, int64_t ld, int ileft, int kleft) {
+    if (!has<S>()) return;
 #pragma unroll
     for (int j = 0; j < S::kInstr; j++) {
       int r, c;
@@ -245,6 +256,7 @@ struct Gemm {
   }
   template <class S>
   __device__ inline void store_regs(char* dst, const s8v* v) {
+    if (!has<S>()) return;
 #pragma unroll
     for (int j = 0; j < S::kInstr; j++) *(s8v*)(dst + (j * THREADS + tid) * 16) = v[j];
   }

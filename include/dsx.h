@@ -628,6 +628,61 @@ int dsx_orthogonalize(const DsxMatrix* mats /* host */, int32_t count,
                       const double* coefficients /* host */, double eps,
                       void* workspace, int64_t workspace_bytes, void* stream);
 
+/* ---- the gated feed-forward block ------------------------------------- */
+
+/* activations */
+#define DSX_ACT_SILU      0 /* g / (1 + exp(-g))                             */
+#define DSX_ACT_GELU      1 /* g Phi(g), by erf                              */
+#define DSX_ACT_GELU_TANH 2 /* its tanh form                                 */
+#define DSX_ACT_RELU      3
+
+/* The block over `tokens` rows (a host struct): x is [tokens][width], w_gate
+ * and w_up [inner][width], w_down [width][inner], all of `dtype` (DSX_F16 or
+ * DSX_BF16), row-major with row strides in elements. `saved` is device memory
+ * of dsx_ffn_saved_bytes: the forward writes h = act(g) u there and, with
+ * keep, what the backward needs; the backward reads it. Both it and
+ * `workspace` are 256-byte aligned. */
+typedef struct DsxFfn {
+  const void* x;
+  const void* w_gate;
+  const void* w_up;
+  const void* w_down;
+  int64_t     ld_x;
+  int64_t     ld_gate;
+  int64_t     ld_up;
+  int64_t     ld_down;
+  int64_t     tokens;
+  int64_t     width;
+  int64_t     inner;
+  int32_t     dtype;
+  int32_t     activation;
+  int32_t     keep;
+  int32_t     reserved;
+  void*       saved;
+  void*       workspace;
+  int64_t     workspace_bytes;
+} DsxFfn;
+
+/* Bytes of `saved` and of `workspace` (host only; the addresses in `block`
+ * are not read); -1 with dsx_last_error for sizes out of range. */
+int64_t dsx_ffn_saved_bytes(int64_t tokens, int64_t inner, int32_t keep);
+int64_t dsx_ffn_workspace_bytes(const DsxFfn* block /* host */,
+                                int32_t backward);
+
+/* y = (act(x w_gate^T) * (x w_up^T)) w_down^T, y [tokens][width] with row
+ * stride ld_y. fp32 sums; h is rounded to `dtype`. No counterpart in the
+ * reference. */
+int dsx_ffn_forward(const DsxFfn* block /* host */, void* y, int64_t ld_y,
+                    void* stream);
+
+/* The gradients for dy [tokens][width]: dx (row stride ld_dx) and the weights'
+ * (contiguous, of the weights' shapes), all of `dtype`, written, not added to.
+ * Any of the four may be NULL and is then not computed. With no token nothing
+ * is written. `block` as the forward had it, with keep nonzero. */
+int dsx_ffn_backward(const DsxFfn* block /* host */, const void* dy,
+                     int64_t ld_dy, void* dx, int64_t ld_dx, void* dw_gate,
+                     void* dw_up, void* dw_down, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
