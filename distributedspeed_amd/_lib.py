@@ -89,9 +89,16 @@ class DsxFfn(_c.Structure):
                [("saved", _P), ("workspace", _P), ("workspace_bytes", _c.c_int64)]
 
 
+class DsxNorm(_c.Structure):
+    _fields_ = [("residual", _P), ("branch", _P), ("post_weight", _P), ("gate", _P), ("next_weight", _P)] + \
+               [(k, _c.c_int64) for k in ("ld_residual", "ld_branch", "rows", "width", "gate_rows")] + \
+               [("dtype", _c.c_int32), ("branch_scale", _c.c_float), ("residual_scale", _c.c_float),
+                ("eps", _c.c_float), ("rstd", _P)]
+
+
 for _s, _n in ((DsxState, 64), (DsxScalerConfig, 32), (DsxAdamwHyper, 56), (DsxStepScalars, 64),
                (DsxTensorRef, 56), (DsxChunk, 24), (DsxGroupsDev, 1112), (DsxFlatPlan, 248),
-               (DsxMatrix, 48), (DsxFfn, 128)):
+               (DsxMatrix, 48), (DsxFfn, 128), (DsxNorm, 104)):
     assert _c.sizeof(_s) == _n, (_s.__name__, _c.sizeof(_s))
 
 # name -> (restype, argtypes); every symbol include/dsx.h declares.
@@ -147,6 +154,9 @@ SIGNATURES = {
     "dsx_ffn_workspace_bytes": (_c.c_int64, [_P, _c.c_int32]),
     "dsx_ffn_forward": (_c.c_int, [_P, _P, _c.c_int64, _P]),
     "dsx_ffn_backward": (_c.c_int, [_P, _P, _c.c_int64, _P, _c.c_int64, _P, _P, _P, _P]),
+    "dsx_norm_workspace_bytes": (_c.c_int64, [_P]),
+    "dsx_norm_forward": (_c.c_int, [_P, _P, _P, _P]),
+    "dsx_norm_backward": (_c.c_int, [_P, _P, _c.c_int64, _P, _c.c_int64, _P, _P, _P, _P, _P, _P, _c.c_int64, _P]),
 }
 
 _lib: ctypes.CDLL | None = None

@@ -1,6 +1,8 @@
 """A gated feed-forward block as differentiable GPU operators.
 
     gated_ffn(x, w_gate, w_up, w_down)            (act(x Wg^T) * (x Wu^T)) Wd^T
+    gated_residual_norm(residual, branch, ...)    the norms before and after it,
+                                                  with its gate and residual
 
 Both directions run the library's own kernels on the current stream, without a
 host synchronisation; the gradients work with torch.autograd and so with the
@@ -13,7 +15,7 @@ import ctypes
 import torch
 
 from . import _lib, ops
-from ._lib import DsxFfn
+from ._lib import DsxFfn, DsxNorm
 
 ACTIVATIONS = {"silu": 0, "gelu": 1, "gelu_tanh": 2, "relu": 3}
 
@@ -126,3 +128,125 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     else:
         y, _ = _forward(*(_rows(t.detach()) for t in (flat, w_gate, w_up, w_down)), act, False)
     return y.view(x.shape) if x.dim() != 2 else y
+
+
+class _GatedResidualNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, residual, branch, post_weight, gate, next_weight, scales):
+        keep = any(ctx.needs_input_grad[:5])
+        residual = _rows(residual)
+        branch = None if branch is None else _rows(branch)
+        post_weight, gate, next_weight = (None if t is None else t.contiguous()
+                                          for t in (post_weight, gate, next_weight))
+        hidden, normed, rstd = _norm_forward(residual, branch, post_weight, gate, next_weight, scales, keep)
+        ctx.set_materialize_grads(False)
+        if keep:
+            ctx.save_for_backward(residual, branch, post_weight, gate, next_weight, rstd)
+            ctx.scales = scales
+        return hidden, normed
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_hidden, d_normed):
+        *inputs, rstd = ctx.saved_tensors
+        residual, dev = inputs[0], inputs[0].device
+        if d_hidden is None and d_normed is None:
+            return (None,) * 6
+        d_hidden, d_normed = (None if t is None else _rows(t) for t in (d_hidden, d_normed))
+        make = torch.empty if residual.shape[0] else torch.zeros  # with no row the vectors' gradients are zero
+        grads = [make(t.shape, dtype=t.dtype, device=dev) if t is not None and need else None
+                 for t, need in zip(inputs, ctx.needs_input_grad)]
+        q = _describe_norm(*inputs, ctx.scales, rstd)
+        with torch.cuda.device(dev):
+            work = _scratch(_lib.load().dsx_norm_workspace_bytes(ctypes.byref(q)), dev)
+            _lib.call("dsx_norm_backward", ctypes.byref(q), ops._ptr(d_hidden), 0 if d_hidden is None else _ld(d_hidden),
+                      ops._ptr(d_normed), 0 if d_normed is None else _ld(d_normed), *(ops._ptr(g) for g in grads),
+                      ops._ptr(work), work.numel(), ops.stream_of(dev))
+        return (*grads, None)
+
+
+def _describe_norm(residual, branch, post_weight, gate, next_weight, scales, rstd) -> DsxNorm:
+    at = [None if t is None else t.data_ptr() for t in (residual, branch, post_weight, gate, next_weight)]
+    rows, d = residual.shape
+    gate_rows = 0 if gate is None else gate.numel() // d
+    return DsxNorm(*at, _ld(residual), 0 if branch is None else _ld(branch), rows, d, gate_rows,
+                   ops.grad_code(residual.dtype), *scales, None if rstd is None else rstd.data_ptr())
+
+
+def _norm_forward(residual, branch, post_weight, gate, next_weight, scales, keep: bool):
+    dev = residual.device
+    hidden = torch.empty(residual.shape, dtype=residual.dtype, device=dev)
+    normed = None if next_weight is None else torch.empty_like(hidden)
+    rstd = torch.empty(2, residual.shape[0], dtype=torch.float32, device=dev) if keep else None
+    q = _describe_norm(residual, branch, post_weight, gate, next_weight, scales, rstd)
+    with torch.cuda.device(dev):
+        _lib.call("dsx_norm_forward", ctypes.byref(q), ops._ptr(hidden), ops._ptr(normed), ops.stream_of(dev))
+    return hidden, normed, rstd
+
+
+def gated_residual_norm(residual: torch.Tensor, branch: torch.Tensor | None = None, *,
+                        post_weight: torch.Tensor | None = None, gate: torch.Tensor | None = None,
+                        next_weight: torch.Tensor | None = None, branch_scale: float = 1.0,
+                        residual_scale: float = 1.0, eps: float = 1e-6
+                        ) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """(hidden, normed) around a block whose output is `branch`:
+
+        z      = rms(branch) * post_weight        (branch, without post_weight)
+        hidden = residual_scale * residual + branch_scale * gate * z
+        normed = rms(hidden) * next_weight        (None, without next_weight)
+
+    with rms(v) = v / sqrt(mean(v^2) + eps) over the last dimension. Without a
+    branch it is the norm before a first block. residual and branch are
+    [..., width], the weights [width]; gate is [width] (a value a channel) or
+    [samples, width], whose i-th row serves the i-th of `samples` equal runs of
+    rows. All tensors are of one type (fp32, fp16 or bf16) on one GPU. The
+    arithmetic is fp32 and rounded once; normed is taken from hidden before its
+    rounding. Rows may be strided.
+
+    Differentiable once in all five tensors; the backward computes hidden again
+    from the inputs and keeps 8 bytes a row beside them."""
+    if not isinstance(residual, torch.Tensor):
+        raise TypeError("residual must be a tensor")
+    dev = ops._device(residual)
+    ops.grad_code(residual.dtype)
+    if residual.dim() < 1 or residual.shape[-1] < 1:
+        raise ValueError(f"residual must be [..., width] with a width of at least 1, got {tuple(residual.shape)}")
+    d = residual.shape[-1]
+    rows = residual.numel() // d
+    if branch is None and (post_weight is not None or gate is not None):
+        raise ValueError("post_weight and gate belong to a branch, and there is none")
+    for name, t in (("branch", branch), ("post_weight", post_weight), ("gate", gate), ("next_weight", next_weight)):
+        if t is None:
+            continue
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be a tensor or None")
+        if t.device != dev:
+            raise ValueError(f"{name} is on {t.device}, expected {dev}")
+        if t.dtype != residual.dtype:
+            raise TypeError(f"{name} must be {residual.dtype}, got {t.dtype}")
+    if branch is not None and branch.shape != residual.shape:
+        raise ValueError(f"branch must be {list(residual.shape)}, got {list(branch.shape)}")
+    for name, t in (("post_weight", post_weight), ("next_weight", next_weight)):
+        if t is not None and tuple(t.shape) != (d,):
+            raise ValueError(f"{name} must be [{d}], got {list(t.shape)}")
+    if gate is not None:
+        if gate.dim() not in (1, 2) or gate.shape[-1] != d or gate.numel() == 0:
+            raise ValueError(f"gate must be [{d}] or [samples, {d}], got {list(gate.shape)}")
+        if gate.dim() == 2 and rows % gate.shape[0]:
+            raise ValueError(f"gate has {gate.shape[0]} rows, which do not divide the {rows} rows")
+    if not eps >= 0:
+        raise ValueError(f"eps must be >= 0, got {eps}")
+    scales = (float(branch_scale), float(residual_scale), float(eps))
+    flat = residual if residual.dim() == 2 else residual.reshape(-1, d)
+    flat_branch = branch if branch is None or branch.dim() == 2 else branch.reshape(-1, d)
+    inputs = (flat, flat_branch, post_weight, gate, next_weight)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in inputs):
+        hidden, normed = _GatedResidualNorm.apply(*inputs, scales)
+    else:
+        vectors = (None if t is None else t.detach().contiguous() for t in inputs[2:])
+        hidden, normed, _ = _norm_forward(_rows(flat.detach()), None if branch is None else _rows(flat_branch.detach()),
+                                          *vectors, scales, False)
+    if residual.dim() != 2:
+        hidden = hidden.view(residual.shape)
+        normed = None if normed is None else normed.view(residual.shape)
+    return hidden, normed

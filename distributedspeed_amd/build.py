@@ -40,6 +40,7 @@ SOURCES = {
     "dsx_step.hip": ["-ffp-contract=off"],
     "dsx_muon.hip": [],
     "dsx_ffn.hip": [],
+    "dsx_norm.hip": [],
 }
 
 

@@ -683,6 +683,58 @@ int dsx_ffn_backward(const DsxFfn* block /* host */, const void* dy,
                      int64_t ld_dy, void* dx, int64_t ld_dx, void* dw_gate,
                      void* dw_up, void* dw_down, void* stream);
 
+/* ---- norms around a block, with its gate and residual ----------------- */
+
+/* upper bound on the rows of a norm call */
+#define DSX_NORM_MAX_ROWS (1 << 28)
+
+/* The inputs (a host struct of device pointers, all of `dtype`: DSX_F32,
+ * DSX_F16 or DSX_BF16): residual and branch [rows][width] with row strides in
+ * elements, post_weight and next_weight [width], gate [gate_rows][width], whose
+ * row i serves the i-th of gate_rows equal runs of rows. branch, post_weight,
+ * gate and next_weight may be NULL. rstd is fp32 [2][rows]: written by the
+ * forward (unless NULL), read by the backward. */
+typedef struct DsxNorm {
+  const void* residual;
+  const void* branch;
+  const void* post_weight;
+  const void* gate;
+  const void* next_weight;
+  int64_t     ld_residual;
+  int64_t     ld_branch;
+  int64_t     rows;
+  int64_t     width;
+  int64_t     gate_rows;
+  int32_t     dtype;
+  float       branch_scale;
+  float       residual_scale;
+  float       eps;
+  float*      rstd;
+} DsxNorm;
+
+/* Bytes of device scratch the backward needs (the sizes, dtype and whether
+ * pointers are NULL are read); -1 with dsx_last_error. Host only. */
+int64_t dsx_norm_workspace_bytes(const DsxNorm* args /* host */);
+
+/* z = rms(branch) post_weight (branch without post_weight),
+ * hidden = residual_scale residual + branch_scale gate z,
+ * normed = rms(hidden) next_weight (not written without next_weight);
+ * rms(v) = v / sqrt(mean(v^2) + eps). fp32 throughout, rounded once; normed is
+ * of the unrounded hidden. Outputs are contiguous. No counterpart in the
+ * reference. */
+int dsx_norm_forward(const DsxNorm* args /* host */, void* hidden,
+                     void* normed, void* stream);
+
+/* The gradients of the inputs, each contiguous and of `dtype`, or NULL where
+ * not wanted, for d_hidden and d_normed (row strides ld_dh and ld_dn; NULL:
+ * zero). Column sums are added in an order set by the sizes alone. With no row
+ * nothing is written. */
+int dsx_norm_backward(const DsxNorm* args /* host */, const void* d_hidden,
+                      int64_t ld_dh, const void* d_normed, int64_t ld_dn,
+                      void* d_residual, void* d_branch, void* d_post_weight,
+                      void* d_gate, void* d_next_weight, void* workspace,
+                      int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
