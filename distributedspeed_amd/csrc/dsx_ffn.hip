@@ -83,8 +83,8 @@ struct Saved {
   int64_t ld;
 };
 
-typedef uint16_t u16x4 __attribute__((ext_vector_type(4)));
-typedef uint8_t  u8x4 __attribute__((ext_vector_type(4)));
+typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
+typedef uint8_t  u8x8 __attribute__((ext_vector_type(8)));
 
 // fp32 rounded to its upper 24 bits (nearest; NaN and inf stay what they are).
 __device__ inline uint32_t top24(float v) {
@@ -94,40 +94,46 @@ __device__ inline uint32_t top24(float v) {
   return b;
 }
 __device__ inline void put24(uint16_t* hi, uint8_t* lo, int64_t at, const float* v) {
-  u16x4 a;
-  u8x4 b;
+  u16x8 a;
+  u8x8 b;
 #pragma unroll
-  for (int e = 0; e < 4; e++) {
+  for (int e = 0; e < 8; e++) {
     const uint32_t w = top24(v[e]);
     a[e] = (uint16_t)(w >> 16);
     b[e] = (uint8_t)(w >> 8);
   }
-  *(u16x4*)(hi + at) = a;
-  *(u8x4*)(lo + at) = b;
+  *(u16x8*)(hi + at) = a;
+  *(u8x8*)(lo + at) = b;
 }
 __device__ inline void get24(const uint16_t* hi, const uint8_t* lo, int64_t at, float* v) {
-  const u16x4 a = *(const u16x4*)(hi + at);
-  const u8x4 b = *(const u8x4*)(lo + at);
+  const u16x8 a = *(const u16x8*)(hi + at);
+  const u8x8 b = *(const u8x8*)(lo + at);
 #pragma unroll
-  for (int e = 0; e < 4; e++) v[e] = __builtin_bit_cast(float, ((uint32_t)a[e] << 16) | ((uint32_t)b[e] << 8));
+  for (int e = 0; e < 8; e++) v[e] = __builtin_bit_cast(float, ((uint32_t)a[e] << 16) | ((uint32_t)b[e] << 8));
 }
 
-// ---- epilogues: four columns of a row --------------------------------------
+// ---- epilogues: eight columns of a row (n is a multiple of 8, below N) ------
+
+template <class T>
+__device__ inline s8v round8(const float* v) {
+  s8v w;
+#pragma unroll
+  for (int e = 0; e < 8; e++) w[e] = T::round(v[e]);
+  return w;
+}
 
 template <class T>
 struct Store {  // C in the inputs' type
   static constexpr bool kPair = false;
   short* c;
   int64_t ld;
-  __device__ inline void operator()(int m, int n, int N, const f4v& v, const f4v&) const {
+  __device__ inline void operator()(int m, int n, int N, const float* v, const float*) const {
     short* o = c + m * ld + n;
-    s4v w;
-#pragma unroll
-    for (int e = 0; e < 4; e++) w[e] = T::round(v[e]);
-    if (n + 4 <= N && ((uintptr_t)o & 7) == 0)
-      *(s4v*)o = w;
+    const s8v w = round8<T>(v);
+    if (n + 8 <= N)
+      *(s8u*)o = w;
     else
-      for (int e = 0; e < 4; e++)
+      for (int e = 0; e < 8; e++)
         if (n + e < N) o[e] = w[e];
   }
 };
@@ -137,18 +143,17 @@ struct Up {  // h and the factors from g and u
   static constexpr bool kPair = true;
   Saved s;
   int act, keep;
-  __device__ inline void operator()(int m, int n, int, const f4v& g, const f4v& u) const {
+  __device__ inline void operator()(int m, int n, int, const float* g, const float* u) const {
     const int64_t at = m * s.ld + n;
-    s4v w;
-    float p[4], q[4];
+    float h[8], p[8], q[8];
 #pragma unroll
-    for (int e = 0; e < 4; e++) {
+    for (int e = 0; e < 8; e++) {
       const ActValue a = activate(act, g[e]);
-      w[e] = T::round(a.f * u[e]);
+      h[e] = a.f * u[e];
       p[e] = u[e] * a.d;
       q[e] = a.f;
     }
-    *(s4v*)(s.h + at) = w;
+    *(s8v*)(s.h + at) = round8<T>(h);
     if (keep) {
       put24(s.p_hi, s.p_lo, at, p);
       put24(s.q_hi, s.q_lo, at, q);
@@ -162,19 +167,18 @@ struct Factors {  // dg and du from dh
   Saved s;
   short* dg;
   short* du;
-  __device__ inline void operator()(int m, int n, int, const f4v& v, const f4v&) const {
+  __device__ inline void operator()(int m, int n, int, const float* v, const float*) const {
     const int64_t at = m * s.ld + n;
-    float p[4], q[4];
+    float p[8], q[8];
     get24(s.p_hi, s.p_lo, at, p);
     get24(s.q_hi, s.q_lo, at, q);
-    s4v a, b;
 #pragma unroll
-    for (int e = 0; e < 4; e++) {
-      a[e] = T::round(v[e] * p[e]);
-      b[e] = T::round(v[e] * q[e]);
+    for (int e = 0; e < 8; e++) {
+      p[e] *= v[e];
+      q[e] *= v[e];
     }
-    *(s4v*)(dg + at) = a;
-    *(s4v*)(du + at) = b;
+    *(s8v*)(dg + at) = round8<T>(p);
+    *(s8v*)(du + at) = round8<T>(q);
   }
 };
 
@@ -196,8 +200,13 @@ __device__ inline Operand at_k(Operand o, bool row, int k) {
   return o;
 }
 
+__device__ inline void put8(float* p, const float* v) {
+  *(f4v*)p = f4v{v[0], v[1], v[2], v[3]};
+  *(f4v*)(p + 4) = f4v{v[4], v[5], v[6], v[7]};
+}
+
 template <class G, bool RA, bool RB, class E>
-__global__ __launch_bounds__(G::THREADS) void k_product(Product p, E e) {
+__global__ DSX_TILE_KERNEL(G) void k_product(Product p, E e) {
   __shared__ __attribute__((aligned(1024))) char lds[G::kLds];
   constexpr int TN = E::kPair ? G::TN / 2 : G::TN;
   const int tiles = p.mt * p.nt;
@@ -217,38 +226,52 @@ __global__ __launch_bounds__(G::THREADS) void k_product(Product p, E e) {
     const Operand b1 = E::kPair ? at_k(p.b[1], RB, k0) : b;
     g.run(lds, a, b, b1, ti * G::TM, tj * TN, k1 - k0);
   }
-  constexpr int NF = E::kPair ? G::NF / 2 : G::NF;
-#pragma unroll
-  for (int i = 0; i < G::MF; i++) {
-    const int m = ti * G::TM + g.row_of(i);
-    if (m >= p.m) continue;
-#pragma unroll
-    for (int j = 0; j < NF; j++) {
-      const int n = tj * TN + (E::kPair ? g.half_col(j) : g.col_of(j));
-      if (n >= p.n) continue;
-      const f4v v = g.acc[i][j], w = E::kPair ? g.acc[i][(j + NF) % G::NF] : v;
-      if (p.splits > 1) {
-        float* o = p.part + ((int64_t)split * p.m + m) * p.ldp + n;
-        *(f4v*)o = v;
-        if (E::kPair) *(f4v*)(o + p.ldp / 2) = w;
-      } else {
-        e(m, n, p.n, v, w);
-      }
+  g.emit(lds, [&](int r, int c, const float* v, const float* w) {
+    const int m = ti * G::TM + r, n = tj * TN + c;
+    if (m >= p.m || n >= p.n) return;
+    if (p.splits > 1) {
+      float* o = p.part + ((int64_t)split * p.m + m) * p.ldp + n;
+      put8(o, v);
+      if (E::kPair) put8(o + p.ldp / 2, w);
+    } else {
+      e(m, n, p.n, v, w);
     }
-  }
+  });
 }
 
-// Adds the splits' partial sums in order and applies the epilogue.
+// Adds the splits' partial sums in order and applies the epilogue: a block
+// takes 32 runs of eight columns of a row, eight threads a run, each adding
+// every eighth split.
 template <class E>
 __global__ __launch_bounds__(256) void k_join(const float* __restrict__ part, int m, int n, int64_t ldp, int splits,
                                               E e) {
-  const int c = (blockIdx.x * 256 + threadIdx.x) * 4, r = blockIdx.y;
-  if (c >= n) return;
-  f4v v = {0, 0, 0, 0}, w = {0, 0, 0, 0};
-  const float* q = part + r * ldp + c;
-  for (int s = 0; s < splits; s++, q += m * ldp) {
-    v += *(const f4v*)q;
-    if (E::kPair) w += *(const f4v*)(q + ldp / 2);
+  __shared__ __attribute__((aligned(16))) float sums[8][32][E::kPair ? 16 : 8];
+  const int i = threadIdx.x & 31, q = threadIdx.x >> 5, c = (blockIdx.x * 32 + i) * 8, r = blockIdx.y;
+  if (c < n) {
+    f4v v[4] = {};
+    const float* at = part + ((int64_t)q * m + r) * ldp + c;
+#pragma unroll 4
+    for (int s = q; s < splits; s += 8, at += 8 * m * ldp) {
+      v[0] += *(const f4v*)at;
+      v[1] += *(const f4v*)(at + 4);
+      if (E::kPair) {
+        v[2] += *(const f4v*)(at + ldp / 2);
+        v[3] += *(const f4v*)(at + ldp / 2 + 4);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < (E::kPair ? 4 : 2); k++) *(f4v*)&sums[q][i][4 * k] = v[k];
+  }
+  __syncthreads();
+  if (q || c >= n) return;
+  float v[8], w[8];
+#pragma unroll
+  for (int k = 0; k < 8; k++) {
+    v[k] = w[k] = 0.0f;
+    for (int s = 0; s < 8; s++) {
+      v[k] += sums[s][i][k];
+      if (E::kPair) w[k] += sums[s][i][8 + (k & 7)];
+    }
   }
   e(r, c, n, v, w);
 }
@@ -266,7 +289,7 @@ struct WeightGrads {
 };
 
 template <class G, class T>
-__global__ __launch_bounds__(G::THREADS) void k_weight_grads(WeightGrads t) {
+__global__ DSX_TILE_KERNEL(G) void k_weight_grads(WeightGrads t) {
   __shared__ __attribute__((aligned(1024))) char lds[G::kLds];
   const int bid = xcd_order(blockIdx.x, gridDim.x);
   int i = 0;
@@ -278,35 +301,27 @@ __global__ __launch_bounds__(G::THREADS) void k_weight_grads(WeightGrads t) {
   g.init();
   g.run(lds, q.a, q.b, q.b, ti * G::TM, tj * G::TN, t.tokens);
   const Store<T> e{q.out, q.n};
-#pragma unroll
-  for (int x = 0; x < G::MF; x++) {
-    const int m = ti * G::TM + g.row_of(x);
-    if (m >= q.m) continue;
-#pragma unroll
-    for (int y = 0; y < G::NF; y++) {
-      const int n = tj * G::TN + g.col_of(y);
-      if (n < q.n) e(m, n, q.n, g.acc[x][y], g.acc[x][y]);
-    }
-  }
+  g.emit(lds, [&](int r, int c, const float* v, const float*) {
+    const int m = ti * G::TM + r, n = tj * G::TN + c;
+    if (m < q.m && n < q.n) e(m, n, q.n, v, v);
+  });
 }
 
 // ---- host ------------------------------------------------------------------
-
-int cu_count() {
-  static const int n = [] {
-    int dev = 0, v = 0;
-    if (hipGetDevice(&dev) != hipSuccess ||
-        hipDeviceGetAttribute(&v, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || v <= 0)
-      v = 256;
-    return v;
-  }();
-  return n;
-}
 
 // Tile rows and splits of a product of m x n over kt K tiles.
 struct Shape {
   int tm, tn, splits, per;
 };
+
+// 256- or 128-tiles for m x n: a CU runs one block of the first at a time or
+// two of the second, whose products take 1.2 times as long for the same area
+// (1100 and 900 TFLOP/s at 4096^3), so the rounds decide.
+int square_tile(int64_t m, int64_t n, int64_t cus) {
+  const int64_t big = ceil_div(ceil_div(m, 256) * ceil_div(n, 256), cus) * 10;
+  const int64_t small = ceil_div(ceil_div(m, 128) * ceil_div(n, 128), 2 * cus) * 6;
+  return big <= small ? 256 : 128;
+}
 
 Shape shape_of(int64_t m, int64_t n, int64_t kt, bool pair, bool direct) {
   const int cus = 256;  // the split count fixes the order of sums: by sizes alone, the same on any card
@@ -319,8 +334,7 @@ Shape shape_of(int64_t m, int64_t n, int64_t kt, bool pair, bool direct) {
     s.tm = m <= 16 ? 16 : m <= 32 ? 32 : 64;
     s.tn = 128;
   } else {
-    const bool big = ceil_div(m, 256) * ceil_div(cols, 256) >= 2 * cus;
-    s.tm = s.tn = big ? 256 : 128;
+    s.tm = s.tn = square_tile(m, cols, cus);
   }
   const int64_t tiles = ceil_div(m, s.tm) * ceil_div(cols, s.tn);
   const int64_t want = s.tm <= 64 ? 4 * cus : 2 * cus;  // blocks that a CU holds at once, over all CUs
@@ -366,7 +380,7 @@ void launch_product(Product p, const Shape& s, bool direct, float* part, const E
   }
 #undef DSX_RUN
   if (p.splits > 1)
-    k_join<E><<<dim3((unsigned)ceil_div(p.n, 1024), (unsigned)p.m), 256, 0, st>>>(part, p.m, p.n, p.ldp, p.splits, e);
+    k_join<E><<<dim3((unsigned)ceil_div(p.n, 256), (unsigned)p.m), 256, 0, st>>>(part, p.m, p.n, p.ldp, p.splits, e);
 }
 
 // The direct loads' demands of one operand (rows or columns of `contiguous`
@@ -463,9 +477,12 @@ int forward(const DsxFfn& q, void* y, int64_t ld_y, hipStream_t st) {
 
 template <class T, bool DIRECT>
 void launch_weight_grads(WeightGrads& w, hipStream_t st) {
-  int64_t big = 0;
-  for (int i = 0; i < w.count; i++) big += ceil_div(w.w[i].m, 256) * ceil_div(w.w[i].n, 256);
-  const int tile = DIRECT && big >= 2 * cu_count() && w.tokens >= 512 ? 256 : 128;
+  int64_t big = 0, small = 0;  // square_tile's rule over the three
+  for (int i = 0; i < w.count; i++) {
+    big += ceil_div(w.w[i].m, 256) * ceil_div(w.w[i].n, 256);
+    small += ceil_div(w.w[i].m, 128) * ceil_div(w.w[i].n, 128);
+  }
+  const int tile = DIRECT && ceil_div(big, 256) * 10 <= ceil_div(small, 512) * 6 ? 256 : 128;
   int64_t n = 0;
   for (int i = 0; i < w.count; i++) {
     w.w[i].tile0 = (int)n;

@@ -54,6 +54,13 @@ struct BF16 {
 
 constexpr int kBK = 64;
 
+// A kernel of tile G. Two waves a SIMD for the square tiles, which is what
+// their shared memory allows: left to itself the compiler aims at more, puts
+// the sums into the accumulation registers and moves them back and forth
+// within the loop (128-tiles, 4096 x 14336 x 4096: 990 and 1144 TFLOP/s).
+#define DSX_TILE_KERNEL(G) \
+  __launch_bounds__(G::THREADS) __attribute__((amdgpu_waves_per_eu(G::kWavesPerSimd, G::kWavesPerSimd)))
+
 // One operand of one K segment: `rows` is its extent along i, `k` along k.
 struct Operand {
   const short* p;
@@ -86,6 +93,7 @@ struct Stage {
   static constexpr int kBytes = ROWS * kBK * 2;
   static constexpr int kPerRow = ROW ? kBK / 8 : ROWS / 8;  // chunks in one stored row
   static constexpr bool kRow = ROW;
+  static constexpr int kGroupMask = ROWS % 256 == 0 ? 15 : ROWS % 128 == 0 ? 7 : 3;  // stays within ROWS / 16 pairs
   static_assert(kChunks % THREADS == 0 || kChunks < THREADS, "whole loads");
   static_assert(kChunks % 64 == 0, "whole waves");
 
@@ -95,7 +103,7 @@ struct Stage {
   static __device__ inline int chunk_of(int r, int slot) {
     if (ROW) return slot ^ ((r >> 1) & 7);
     const int g = (r & 3) + 4 * ((r >> 3) & 3);
-    return (((slot >> 1) ^ (g & (ROWS / 16 - 1))) << 1) | (slot & 1);
+    return (((slot >> 1) ^ (g & kGroupMask)) << 1) | (slot & 1);
   }
   // The stored row and the chunk of the thread's j-th load.
   static __device__ inline void place(int j, int tid, int* r, int* c) {
@@ -144,6 +152,8 @@ struct Gemm {
   static constexpr int NB = SPLIT ? 2 : 1;
   static constexpr int kTile = SA::kBytes + NB * SB::kBytes;
   static constexpr int kLds = 2 * kTile;
+  static constexpr int kWavesFit = 163840 / kLds * (WM * WN) / 4;
+  static constexpr int kWavesPerSimd = kWavesFit < 4 ? kWavesFit : 4;
 
   f4v acc[MF][NF];
   int tid, lane, wm, wn;
@@ -160,13 +170,65 @@ struct Gemm {
       for (int j = 0; j < NF; j++) acc[i][j] = f4v{0, 0, 0, 0};
   }
 
-  // Row of C within the tile that this lane's fragment (mf) holds, and the
-  // first of the four consecutive columns of fragment nf.
-  __device__ inline int row_of(int mf) const { return wm * WTM + mf * 16 + (lane & 15); }
-  __device__ inline int col_of(int nf) const { return wn * WTN + nf * 16 + (lane >> 4) * 4; }
-  // SPLIT: the column within a half tile; fragments nf < NF/2 are the first
-  // operand's, the others the second's at the same columns.
-  __device__ inline int half_col(int nf) const { return wn * (WTN / 2) + nf * 16 + (lane >> 4) * 4; }
+  // Hands out C, eight consecutive columns at a time: f(row, col, v, w), both
+  // within the tile (within a half tile, v of the first operand and w of the
+  // second, for SPLIT). A fragment holds four columns of a row in a lane, 32
+  // bytes of 16-bit output a row and instruction; by way of a strip of 16 rows
+  // in the wave's own part of shared memory (the tiles' place, free by now) the
+  // lanes of a row write 128 bytes together.
+  // t(col, row0, v) gets the same strip by columns where TRANSPOSED: 16
+  // consecutive rows of one column.
+  static constexpr int kStripLd = WTN + 4;  // floats: 16 rows fall on different banks
+  template <bool TRANSPOSED, class F, class U>
+  __device__ inline void emit(char* lds, F&& f, U&& t) {
+    static_assert(WM * WN * 16 * kStripLd * 4 <= kLds, "the strips fit the tiles' place");
+    float* strip = (float*)lds + (wm * WN + wn) * 16 * kStripLd;
+    constexpr int COLS = SPLIT ? WTN / 2 : WTN, PER = COLS / 8;
+#pragma unroll
+    for (int i = 0; i < MF; i++) {
+#pragma unroll
+      for (int j = 0; j < NF; j++) *(f4v*)(strip + (lane & 15) * kStripLd + j * 16 + (lane >> 4) * 4) = acc[i][j];
+      wave_sync();
+#pragma unroll
+      for (int p0 = 0; p0 < 16 * PER; p0 += 64) {
+        const int p = p0 + lane, r = p / PER, c = p % PER * 8;
+        if (16 * PER % 64 && p >= 16 * PER) break;
+        float v[8], w[8];
+        get8(strip + r * kStripLd + c, v);
+        if (SPLIT) get8(strip + r * kStripLd + COLS + c, w);
+        f(wm * WTM + i * 16 + r, wn * COLS + c, v, w);
+      }
+      if (TRANSPOSED)
+#pragma unroll
+        for (int c0 = 0; c0 < WTN; c0 += 64) {
+          const int c = c0 + lane;
+          if (WTN % 64 && c >= WTN) break;
+          float v[16];
+#pragma unroll
+          for (int r = 0; r < 16; r++) v[r] = strip[r * kStripLd + c];
+          t(wn * WTN + c, wm * WTM + i * 16, v);
+        }
+      wave_sync();
+    }
+  }
+  template <class F>
+  __device__ inline void emit(char* lds, F&& f) {
+    emit<false>(lds, f, [](int, int, const float*) {});
+  }
+  static __device__ inline void get8(const float* p, float* v) {
+    const f4v a = *(const f4v*)p, b = *(const f4v*)(p + 4);
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      v[e] = a[e];
+      v[e + 4] = b[e];
+    }
+  }
+  // Orders a wave's own LDS accesses across its lanes.
+  static __device__ inline void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  }
 
   template <class S>
   static __device__ inline s8v frag(const char* tile, int i0, int kk, int lane) {
@@ -176,7 +238,7 @@ struct Gemm {
     }
     constexpr int rb = S::kPerRow * 16;  // bytes of a stored row
     const int k = kk * 32 + (lane >> 4) * 8 + ((lane & 15) >> 2);
-    const int g = ((k & 3) + 4 * ((k >> 3) & 3)) & (S::kPerRow / 2 - 1);
+    const int g = ((k & 3) + 4 * ((k >> 3) & 3)) & S::kGroupMask;
     const char* q = tile + k * rb + (((i0 >> 4) ^ g) << 5) + (lane & 3) * 8;
     typedef __attribute__((address_space(3))) s4v* lp;
     const s4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)q);
@@ -184,27 +246,40 @@ struct Gemm {
     return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
   }
 
-  __device__ inline void compute(const char* tile) {
-    const char* ta = tile;
+  struct Frags {
+    s8v a[MF], b[NF];
+  };
+  // The fragments of half a K tile (32 of its 64 k).
+  __device__ inline void read(Frags& f, const char* tile, int kk) const {
     const char* tb = tile + SA::kBytes;
 #pragma unroll
-    for (int kk = 0; kk < 2; kk++) {
-      s8v a[MF], b[NF];
+    for (int j = 0; j < NF; j++) {
+      if (SPLIT)
+        f.b[j] = frag<SB>(tb + (j < NF / 2 ? 0 : SB::kBytes), wn * (WTN / 2) + (j % (NF / 2)) * 16, kk, lane);
+      else
+        f.b[j] = frag<SB>(tb, wn * WTN + j * 16, kk, lane);
+    }
 #pragma unroll
-      for (int j = 0; j < NF; j++) {
-        if (SPLIT)
-          b[j] = frag<SB>(tb + (j < NF / 2 ? 0 : SB::kBytes), wn * (WTN / 2) + (j % (NF / 2)) * 16, kk, lane);
-        else
-          b[j] = frag<SB>(tb, wn * WTN + j * 16, kk, lane);
-      }
+    for (int i = 0; i < MF; i++) f.a[i] = frag<SA>(tile, wm * WTM + i * 16, kk, lane);
+  }
+  // B's fragment first: D's lane is then the row of C and its four values are
+  // consecutive columns.
+  __device__ inline void multiply(const Frags& f) {
 #pragma unroll
-      for (int i = 0; i < MF; i++) a[i] = frag<SA>(ta, wm * WTM + i * 16, kk, lane);
-      // B's fragment first: D's lane is then the row of C and its four values
-      // are consecutive columns.
+    for (int i = 0; i < MF; i++)
 #pragma unroll
-      for (int i = 0; i < MF; i++)
+      for (int j = 0; j < NF; j++) acc[i][j] = T::mfma(f.b[j], f.a[i], acc[i][j]);
+  }
+  // Reads of one half tile spread over the products of the other. Measured on
+  // 4096 x 14336 x 4096: row operands 1252 -> 1278 TFLOP/s; with a col operand
+  // it is the slower order (1125 -> 1021), so those keep the compiler's.
+  static __device__ inline void interleave() {
+    if (!(RA && RB)) return;
+    constexpr int reads = MF + NF, per = MF * NF / reads > 0 ? MF * NF / reads : 1;
 #pragma unroll
-        for (int j = 0; j < NF; j++) acc[i][j] = T::mfma(b[j], a[i], acc[i][j]);
+    for (int i = 0; i < reads; i++) {
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);   // an LDS read
+      __builtin_amdgcn_sched_group_barrier(0x008, per, 0);  // matrix instructions
     }
   }
 
@@ -286,25 +361,49 @@ struct Gemm {
         pb += sb;
         pb1 += sb1;
       };
+      Frags f0, f1;
       set(K);
       load(lds);
-      for (int t = 0; t < nt; t++) {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();
+      if (nt > 1) {
+        if (K - kBK < kBK) set(K - kBK);
+        load(lds + kTile);
+      }
+      auto tail = [&](int t) {
+        const int left = K - t * kBK;
+        if (left >= kBK) return;
         char* cur = lds + (t & 1) * kTile;
+        zero_tail<SA>(cur, RA, left);
+        zero_tail<SB>(cur + SA::kBytes, RB, left);
+        if (SPLIT) zero_tail<SB>(cur + SA::kBytes + SB::kBytes, RB, left);
+        __syncthreads();
+      };
+      if (nt == 1) tail(0);
+      read(f0, lds, 0);
+      for (int t = 0; t + 1 < nt; t++) {
+        char* cur = lds + (t & 1) * kTile;
+        char* nxt = lds + ((t + 1) & 1) * kTile;
+        read(f1, cur, 1);
+        multiply(f0);
+        interleave();
+        // all of this tile is in registers, all of the next in shared memory
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
-        if (t + 1 < nt) {
-          const int left = K - (t + 1) * kBK;
+        if (t + 2 < nt) {
+          const int left = K - (t + 2) * kBK;
           if (left < kBK) set(left);
-          load(lds + ((t + 1) & 1) * kTile);
-        } else if (K - t * kBK < kBK) {
-          const int left = K - t * kBK;
-          zero_tail<SA>(cur, RA, left);
-          zero_tail<SB>(cur + SA::kBytes, RB, left);
-          if (SPLIT) zero_tail<SB>(cur + SA::kBytes + SB::kBytes, RB, left);
-          __syncthreads();
+          load(cur);
+        } else {
+          tail(t + 1);
         }
-        compute(cur);
+        read(f0, nxt, 0);
+        multiply(f1);
+        interleave();
       }
+      read(f1, lds + ((nt - 1) & 1) * kTile, 1);
+      multiply(f0);
+      multiply(f1);
     } else {
       s8v va[SA::kInstr], vb[SB::kInstr], vb1[SPLIT ? SB::kInstr : 1];
       auto load = [&](int left) {
@@ -325,7 +424,12 @@ struct Gemm {
       for (int t = 0; t < nt; t++) {
         __syncthreads();
         if (t + 1 < nt) load(K - (t + 1) * kBK);
-        compute(lds + (t & 1) * kTile);
+        Frags f;
+#pragma unroll
+        for (int kk = 0; kk < 2; kk++) {
+          read(f, lds + (t & 1) * kTile, kk);
+          multiply(f);
+        }
         if (t + 1 < nt) store(lds + ((t + 1) & 1) * kTile);
       }
     }

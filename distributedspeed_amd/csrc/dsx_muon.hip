@@ -226,7 +226,7 @@ __device__ inline void triangle(int t, int* i, int* j) {
 // A symmetric product's tile, written at (m, n) and, off the diagonal, at (n, m).
 // GRAM: A = X X^T (wide) or X^T X (TALL) from the current X; else B = b A + c A A.
 template <class G, bool GRAM, bool TALL>
-__global__ __launch_bounds__(G::THREADS) void k_symmetric(Table t, short* __restrict__ ws,
+__global__ DSX_TILE_KERNEL(G) void k_symmetric(Table t, short* __restrict__ ws,
                                                           const Info* __restrict__ info, int cur, int first, float b,
                                                           float c, const int32_t* skip) {
   __shared__ __attribute__((aligned(1024))) char lds[G::kLds];
@@ -245,36 +245,38 @@ __global__ __launch_bounds__(G::THREADS) void k_symmetric(Table t, short* __rest
   const float inv_r = first ? info[i].inv_r : 1.0f;
   const float k = GRAM ? inv_r * inv_r * (1.0f / kScale) : c * (1.0f / kScale);
   short* dst = ws + (GRAM ? m.a : m.b);
+  // eight values, at q (a multiple of 8, as s is) of row r
+  auto put = [&](int r, int q, const float* v) {
+    if (r >= s || q >= s) return;
+    const int64_t at = (int64_t)r * s + q;
+    s8v w;
+    if (GRAM) {
 #pragma unroll
-  for (int x = 0; x < G::MF; x++) {
-    const int r = ti * G::TM + g.row_of(x);
-    if (r >= s) continue;
+      for (int e = 0; e < 8; e++) w[e] = F16::round(k * v[e]);
+    } else {
+      const s8v a = *(const s8v*)(src + at);
 #pragma unroll
-    for (int y = 0; y < G::NF; y++) {
-      const int q = tj * G::TN + g.col_of(y);
-      if (q >= s) continue;  // s is a multiple of 8: four columns are inside or outside together
-      s4v w;
-      if (GRAM) {
-#pragma unroll
-        for (int e = 0; e < 4; e++) w[e] = F16::round(k * g.acc[x][y][e]);
-      } else {
-        const s4v a = *(const s4v*)(src + (int64_t)r * s + q);
-#pragma unroll
-        for (int e = 0; e < 4; e++) w[e] = F16::round(fmaf(k, g.acc[x][y][e], b * F16::widen(a[e])));
-      }
-      *(s4v*)(dst + (int64_t)r * s + q) = w;
-      if (ti != tj)
-#pragma unroll
-        for (int e = 0; e < 4; e++) dst[(int64_t)(q + e) * s + r] = w[e];
+      for (int e = 0; e < 8; e++) w[e] = F16::round(fmaf(k, v[e], b * F16::widen(a[e])));
     }
-  }
+    *(s8v*)(dst + at) = w;
+  };
+  const int r0 = ti * G::TM, c0 = tj * G::TN;
+  if (ti == tj)
+    g.emit(lds, [&](int r, int q, const float* v, const float*) { put(r0 + r, c0 + q, v); });
+  else
+    g.template emit<true>(
+        lds, [&](int r, int q, const float* v, const float*) { put(r0 + r, c0 + q, v); },
+        [&](int q, int r, const float* v) {
+          put(c0 + q, r0 + r, v);
+          put(c0 + q, r0 + r + 8, v + 8);
+        });
 }
 
 // X <- (a X + B X) / r, or with X B where TALL. LAST: the result itself, to the
 // output in bf16 (OUT 0) or as Muon's parameter update (fp32 master and 16-bit
 // copy of OUT's type, 0 for none).
 template <class G, bool TALL, bool LAST, bool MUON>
-__global__ __launch_bounds__(G::THREADS) void k_apply(Table t, short* __restrict__ ws, const Info* __restrict__ info,
+__global__ DSX_TILE_KERNEL(G) void k_apply(Table t, short* __restrict__ ws, const Info* __restrict__ info,
                                                       int cur, int first, float a, MuonArgs ma, int out_dt) {
   __shared__ __attribute__((aligned(1024))) char lds[G::kLds];
   if (MUON && *ma.skip) return;
@@ -294,52 +296,50 @@ __global__ __launch_bounds__(G::THREADS) void k_apply(Table t, short* __restrict
   else
     g.run(lds, ob, ox, ox, ti * G::TM, tj * G::TN, s);
   const float inv_r = first ? info[i].inv_r : 1.0f;
+  g.emit(lds, [&](int r, int c, const float* sum, const float*) {
+    r += ti * G::TM;
+    c += tj * G::TN;
+    if (r >= (LAST ? m.rows : m.rows8) || c >= (LAST ? m.cols : m.cols8)) return;
+    const s8v old = *(const s8v*)(x + (int64_t)r * m.cols8 + c);
+    float v[8];
 #pragma unroll
-  for (int p = 0; p < G::MF; p++) {
-    const int r = ti * G::TM + g.row_of(p);
-    if (r >= (LAST ? m.rows : m.rows8)) continue;
+    for (int e = 0; e < 8; e++) v[e] = fmaf(a, F16::widen(old[e]), sum[e] * (1.0f / kScale)) * inv_r;
+    if (!LAST) {
+      s8v w;
 #pragma unroll
-    for (int q = 0; q < G::NF; q++) {
-      const int c = tj * G::TN + g.col_of(q);
-      if (c >= (LAST ? m.cols : m.cols8)) continue;
-      const s4v old = *(const s4v*)(x + (int64_t)r * m.cols8 + c);
-      float v[4];
+      for (int e = 0; e < 8; e++) w[e] = F16::round(v[e]);
+      *(s8v*)(ws + m.x[cur ^ 1] + (int64_t)r * m.cols8 + c) = w;
+      return;
+    }
+    short* o = (short*)m.out + r * m.ld_out + c;
+    const int left = m.cols - c;
+    if (!MUON) {
+      s8v w;
 #pragma unroll
-      for (int e = 0; e < 4; e++)
-        v[e] = fmaf(a, F16::widen(old[e]), g.acc[p][q][e] * (1.0f / kScale)) * inv_r;
-      if (!LAST) {
-        s4v w;
-#pragma unroll
-        for (int e = 0; e < 4; e++) w[e] = F16::round(v[e]);
-        *(s4v*)(ws + m.x[cur ^ 1] + (int64_t)r * m.cols8 + c) = w;
-      } else if (!MUON) {
-        short* o = (short*)m.out + r * m.ld_out + c;
-        s4v w;
-#pragma unroll
-        for (int e = 0; e < 4; e++) w[e] = BF16::round(v[e] * (1.0f / kScale));
-        if (c + 4 <= m.cols && ((uintptr_t)o & 7) == 0)
-          *(s4v*)o = w;
-        else
-          for (int e = 0; e < 4; e++)
-            if (c + e < m.cols) o[e] = w[e];
-      } else {
-        float* w = m.master + (int64_t)r * m.cols + c;
-        short* o = (short*)m.out + r * m.ld_out + c;
-        for (int e = 0; e < 4; e++) {
-          if (c + e >= m.cols) break;
-          const float n = fmaf(-m.lr * (1.0f / kScale), v[e], w[e] * ma.decay);
-          w[e] = n;
-          if (out_dt) o[e] = out_dt == DSX_F16 ? F16::round(n) : BF16::round(n);
-        }
+      for (int e = 0; e < 8; e++) w[e] = BF16::round(v[e] * (1.0f / kScale));
+      if (left >= 8)
+        *(s8u*)o = w;
+      else
+        for (int e = 0; e < 8; e++)
+          if (e < left) o[e] = w[e];
+    } else {
+      float* w = m.master + (int64_t)r * m.cols + c;
+      for (int e = 0; e < 8; e++) {
+        if (e >= left) break;
+        const float n = fmaf(-m.lr * (1.0f / kScale), v[e], w[e] * ma.decay);
+        w[e] = n;
+        if (out_dt) o[e] = out_dt == DSX_F16 ? F16::round(n) : BF16::round(n);
       }
     }
-  }
+  });
 }
 
 // ---- host ------------------------------------------------------------------
 
 template <bool RA, bool RB>
 using Big = Gemm<F16, 256, 256, 2, 4, RA, RB, true>;
+template <bool RA, bool RB>
+using Mid = Gemm<F16, 192, 192, 2, 4, RA, RB, true>;
 template <bool RA, bool RB>
 using Small = Gemm<F16, 128, 128, 2, 2, RA, RB, true>;
 
@@ -430,17 +430,6 @@ int64_t tiles_of(Table& t, F&& per) {
   return n;
 }
 
-int cu_count() {
-  static const int n = [] {
-    int dev = 0, v = 0;
-    if (hipGetDevice(&dev) != hipSuccess ||
-        hipDeviceGetAttribute(&v, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || v <= 0)
-      v = 256;
-    return v;
-  }();
-  return n;
-}
-
 template <class G, bool GRAM, bool TALL>
 void launch_symmetric(Table& t, short* ws, const Info* info, int cur, int first, float b, float c, const int32_t* skip,
                       hipStream_t s) {
@@ -462,46 +451,54 @@ void launch_apply(Table& t, short* ws, const Info* info, int cur, int first, boo
     k_apply<G, TALL, false, false><<<dim3((unsigned)n), G::THREADS, 0, s>>>(t, ws, info, cur, first, a, ma, out_dt);
 }
 
-// 256-tiles where they fill the CUs at least twice over, else 128-tiles.
-bool use_big(const Table& t, bool triangle) {
-  int64_t n = 0;
-  for (int i = 0; i < t.n; i++) {
-    const Mat& m = t.m[i];
-    const int64_t k = ceil_div(m.rows8 < m.cols8 ? m.rows8 : m.cols8, 256);
-    n += triangle ? k * (k + 1) / 2 : ceil_div(m.rows8, 256) * ceil_div(m.cols8, 256);
+// The square tile of a launch: a CU runs one block of 256 or 192 at a time or
+// two of 128, whose products take 1.2 times as long for the same area; the
+// whole rounds over the CUs decide. (The Gram matrix of 4096 x 14336: 136, 253
+// and 528 tiles, of which only the 192s fill the chip once and no more.)
+int tile_of(const Table& t, bool triangle) {
+  const int64_t size[3] = {256, 192, 128}, slots[3] = {256, 256, 512}, cost[3] = {65536 * 10, 36864 * 10, 32768 * 12};
+  int best = 0;
+  int64_t least = INT64_MAX;
+  for (int k = 0; k < 3; k++) {
+    int64_t n = 0;
+    for (int i = 0; i < t.n; i++) {
+      const Mat& m = t.m[i];
+      const int64_t a = ceil_div(m.rows8, size[k]), b = ceil_div(m.cols8, size[k]), q = a < b ? a : b;
+      n += triangle ? q * (q + 1) / 2 : a * b;
+    }
+    const int64_t c = ceil_div(n, slots[k]) * cost[k];
+    if (c < least) {
+      least = c;
+      best = k;
+    }
   }
-  return n >= 2 * cu_count();
+  return (int)size[best];
 }
 
 template <bool MUON>
 void iterate(Table& t, bool tall, short* ws, const Info* info, int steps, const double* coef, const MuonArgs& ma,
              int out_dt, hipStream_t s) {
-  const bool big_sym = use_big(t, true), big_app = use_big(t, false);
+  const int sym = tile_of(t, true), app = tile_of(t, false);
   const int32_t* skip = MUON ? ma.skip : nullptr;
   for (int k = 0; k < steps; k++) {
     const float a = (float)coef[3 * k], b = (float)coef[3 * k + 1], c = (float)coef[3 * k + 2];
     const int cur = k & 1, first = k == 0, last = k == steps - 1;
-#define DSX_SYM(G, GRAM, TALL) launch_symmetric<G, GRAM, TALL>(t, ws, info, cur, first, b, c, skip, s)
-    using BR = Big<true, true>;
-    using SR = Small<true, true>;
-    using BC = Big<false, false>;
-    using SC = Small<false, false>;
-    using BX = Big<true, false>;
-    using SX = Small<true, false>;
+#define DSX_BY_TILE(TILE, F, RA, RB, ...)                                      \
+  do {                                                                         \
+    if (TILE == 256) F<Big<RA, RB>, __VA_ARGS__;                               \
+    else if (TILE == 192) F<Mid<RA, RB>, __VA_ARGS__;                          \
+    else F<Small<RA, RB>, __VA_ARGS__;                                         \
+  } while (0)
     if (tall) {
-      if (big_sym) DSX_SYM(BC, true, true); else DSX_SYM(SC, true, true);
+      DSX_BY_TILE(sym, launch_symmetric, false, false, true, true>(t, ws, info, cur, first, b, c, skip, s));
+      DSX_BY_TILE(sym, launch_symmetric, true, true, false, false>(t, ws, info, cur, first, b, c, skip, s));
+      DSX_BY_TILE(app, launch_apply, true, true, true, MUON>(t, ws, info, cur, first, last, a, ma, out_dt, s));
     } else {
-      if (big_sym) DSX_SYM(BR, true, false); else DSX_SYM(SR, true, false);
+      DSX_BY_TILE(sym, launch_symmetric, true, true, true, false>(t, ws, info, cur, first, b, c, skip, s));
+      DSX_BY_TILE(sym, launch_symmetric, true, true, false, false>(t, ws, info, cur, first, b, c, skip, s));
+      DSX_BY_TILE(app, launch_apply, true, false, false, MUON>(t, ws, info, cur, first, last, a, ma, out_dt, s));
     }
-    if (big_sym) DSX_SYM(BR, false, false); else DSX_SYM(SR, false, false);
-#undef DSX_SYM
-    if (tall) {
-      if (big_app) launch_apply<BR, true, MUON>(t, ws, info, cur, first, last, a, ma, out_dt, s);
-      else launch_apply<SR, true, MUON>(t, ws, info, cur, first, last, a, ma, out_dt, s);
-    } else {
-      if (big_app) launch_apply<BX, false, MUON>(t, ws, info, cur, first, last, a, ma, out_dt, s);
-      else launch_apply<SX, false, MUON>(t, ws, info, cur, first, last, a, ma, out_dt, s);
-    }
+#undef DSX_BY_TILE
   }
 }
 

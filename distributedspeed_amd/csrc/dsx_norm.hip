@@ -319,26 +319,36 @@ __global__ __launch_bounds__(W) void k_backward(Args a, Grads g) {
   if (g.dw2) Elem<DSX_F32>::store(g.part, 2 * plane + at, left, s2);
 }
 
-// out[sample][col] = sum over the sample's `count` partial rows, in order:
-// 64 columns a block, four runs of rows added one after another.
+// The partial rows of up to three vectors, added in order: for each, out[sample]
+// [col] = the sum over that sample's rows. A block takes 32 columns; its eight
+// runs of rows are added one after another.
+struct Columns {
+  const float* part[3];
+  void* out[3];
+  int count[3];    // partial rows per sample
+  int samples[3];
+  int n;
+};
 template <int DT>
-__global__ __launch_bounds__(256) void k_columns(const float* __restrict__ part, int count, int width,
-                                                 void* __restrict__ out) {
-  __shared__ float run[4][64];
-  const int c = blockIdx.x * 64 + (threadIdx.x & 63), q = threadIdx.x >> 6;
-  const float* p = part + (int64_t)blockIdx.y * count * width;
+__global__ __launch_bounds__(256) void k_columns(Columns t, int width) {
+  __shared__ float run[8][32];
+  int sample = blockIdx.y, v = 0;
+  while (v + 1 < t.n && sample >= t.samples[v]) sample -= t.samples[v++];
+  const int count = t.count[v], i = threadIdx.x & 31, q = threadIdx.x >> 5, c = blockIdx.x * 32 + i;
+  const float* p = t.part[v] + (int64_t)sample * count * width + c;
   float s = 0;
   if (c < width) {
-    const int lo = count * q / 4, hi = count * (q + 1) / 4;
+    const int hi = (int)((int64_t)count * (q + 1) / 8);
 #pragma unroll 8
-    for (int k = lo; k < hi; k++) s += p[(int64_t)k * width + c];
+    for (int k = (int)((int64_t)count * q / 8); k < hi; k++) s += p[(int64_t)k * width];
   }
-  run[q][threadIdx.x & 63] = s;
+  run[q][i] = s;
   __syncthreads();
-  if (q == 0 && c < width) {
-    const int i = threadIdx.x;
-    Elem<DT>::put(out, (int64_t)blockIdx.y * width + c, (run[0][i] + run[1][i]) + (run[2][i] + run[3][i]));
-  }
+  if (q || c >= width) return;
+  s = 0;
+#pragma unroll
+  for (int k = 0; k < 8; k++) s += run[k][i];
+  Elem<DT>::put(t.out[v], (int64_t)sample * width + c, s);
 }
 
 // ---- rows wider than 8192 ---------------------------------------------------
@@ -530,12 +540,20 @@ void backward(const Args& a, Grads g, float* means, int samples, hipStream_t s) 
       default: k_backward<DT, 1024><<<grid, 1024, 0, s>>>(a, g); break;
     }
   }
-  const unsigned blocks = (unsigned)ceil_div(a.width, 64);
   const int64_t plane = (int64_t)g.units * a.width;
-  if (g.dw1) k_columns<DT><<<dim3(blocks, 1), 256, 0, s>>>(g.part, g.units, a.width, g.dw1);
-  if (g.dgate && g.slices > 1)
-    k_columns<DT><<<dim3(blocks, (unsigned)samples), 256, 0, s>>>(g.part + plane, g.slices, a.width, g.dgate);
-  if (g.dw2) k_columns<DT><<<dim3(blocks, 1), 256, 0, s>>>(g.part + 2 * plane, g.units, a.width, g.dw2);
+  Columns t{};
+  int total = 0;
+  auto add = [&](void* out, int which, int count, int n) {
+    t.part[t.n] = g.part + which * plane;
+    t.out[t.n] = out;
+    t.count[t.n] = count;
+    t.samples[t.n++] = n;
+    total += n;
+  };
+  if (g.dw1) add(g.dw1, 0, g.units, 1);
+  if (g.dw2) add(g.dw2, 2, g.units, 1);
+  if (g.dgate && g.slices > 1) add(g.dgate, 1, g.slices, samples);
+  if (t.n) k_columns<DT><<<dim3((unsigned)ceil_div(a.width, 32), (unsigned)total), 256, 0, s>>>(t, a.width);
 }
 
 bool off(const void* p, int dtype) { return p && ((uintptr_t)p & (dtype == DSX_F32 ? 3 : 1)); }
@@ -547,8 +565,8 @@ int check(const char* what, const DsxNorm* q) {
     return fail(DSX_EINVAL, "%s: rows in [0, %d], width in [1, %d]", what, DSX_NORM_MAX_ROWS, DSX_MATRIX_MAX_DIM);
   if (!q->branch && (q->post_weight || q->gate))
     return fail(DSX_EINVAL, "%s: a weight or gate of a branch that is NULL", what);
-  if (q->gate && (q->gate_rows < 1 || q->gate_rows > 65535 || (q->rows && q->rows % q->gate_rows)))
-    return fail(DSX_EINVAL, "%s: gate_rows must divide rows and lie in [1, 65535]", what);
+  if (q->gate && (q->gate_rows < 1 || q->gate_rows > 65533 || (q->rows && q->rows % q->gate_rows)))
+    return fail(DSX_EINVAL, "%s: gate_rows must divide rows and lie in [1, 65533]", what);
   if (!(q->eps >= 0.0f)) return fail(DSX_EINVAL, "%s: eps must be >= 0", what);
   return DSX_OK;
 }
