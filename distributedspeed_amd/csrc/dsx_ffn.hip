@@ -314,17 +314,19 @@ struct Shape {
   int tm, tn, splits, per;
 };
 
-// 256- or 128-tiles for m x n: a CU runs one block of the first at a time or
-// two of the second, whose products take 1.2 times as long for the same area
-// (1100 and 900 TFLOP/s at 4096^3), so the rounds decide.
-int square_tile(int64_t m, int64_t n, int64_t cus) {
-  const int64_t big = ceil_div(ceil_div(m, 256) * ceil_div(n, 256), cus) * 10;
-  const int64_t small = ceil_div(ceil_div(m, 128) * ceil_div(n, 128), 2 * cus) * 6;
+// 256- or 128-tiles, for n256 and n128 of them: a CU runs one block of the
+// first at a time or two of the second, whose products take 1.2 times as long
+// for the same area (a lone block of 128 on a CU: 1.4 times); the rounds over
+// the CUs decide. (By sizes alone, as the split count: the same on any card.)
+constexpr int kCus = 256;
+int square_tile(int64_t n256, int64_t n128) {
+  const int64_t rest = n128 % (2 * kCus);
+  const int64_t big = ceil_div(n256, kCus) * 4 * 10;
+  const int64_t small = n128 / (2 * kCus) * 24 + (rest > kCus ? 24 : rest ? 14 : 0);
   return big <= small ? 256 : 128;
 }
 
 Shape shape_of(int64_t m, int64_t n, int64_t kt, bool pair, bool direct) {
-  const int cus = 256;  // the split count fixes the order of sums: by sizes alone, the same on any card
   Shape s{};
   const int64_t cols = pair ? 2 * n : n;
   if (!direct) {
@@ -334,10 +336,10 @@ Shape shape_of(int64_t m, int64_t n, int64_t kt, bool pair, bool direct) {
     s.tm = m <= 16 ? 16 : m <= 32 ? 32 : 64;
     s.tn = 128;
   } else {
-    s.tm = s.tn = square_tile(m, cols, cus);
+    s.tm = s.tn = square_tile(ceil_div(m, 256) * ceil_div(cols, 256), ceil_div(m, 128) * ceil_div(cols, 128));
   }
   const int64_t tiles = ceil_div(m, s.tm) * ceil_div(cols, s.tn);
-  const int64_t want = s.tm <= 64 ? 4 * cus : 2 * cus;  // blocks that a CU holds at once, over all CUs
+  const int64_t want = s.tm <= 64 ? 4 * kCus : 2 * kCus;  // blocks that a CU holds at once, over all CUs
   int64_t splits = tiles >= want / 2 ? 1 : ceil_div(want, tiles);
   if (splits > kt / 2) splits = kt / 2;  // two K tiles each at least
   if (splits < 1) splits = 1;
@@ -482,7 +484,7 @@ void launch_weight_grads(WeightGrads& w, hipStream_t st) {
     big += ceil_div(w.w[i].m, 256) * ceil_div(w.w[i].n, 256);
     small += ceil_div(w.w[i].m, 128) * ceil_div(w.w[i].n, 128);
   }
-  const int tile = DIRECT && ceil_div(big, 256) * 10 <= ceil_div(small, 512) * 6 ? 256 : 128;
+  const int tile = DIRECT ? square_tile(big, small) : 128;
   int64_t n = 0;
   for (int i = 0; i < w.count; i++) {
     w.w[i].tile0 = (int)n;

@@ -139,6 +139,16 @@ struct Stage {
   }
 };
 
+// The transposing LDS read. `restrict` carries alias information to the
+// instruction: without any, the compiler waits for every direct load in flight
+// before each such read (tile t + 1's loads before tile t is multiplied),
+// although the loads fill the other tile and are waited for at the barrier.
+// Measured with a col operand, 8192^3: XXXX TFLOP/s.
+typedef __attribute__((address_space(3))) s4v LdsBlock;
+static __device__ inline s4v read_transposed(LdsBlock* __restrict__ p) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16(p);
+}
+
 // The product tile. NT = threads, WM x WN waves of (TM/WM) x (TN/WN).
 // SPLIT: B's tile is two half tiles from two operands (the gate and the up
 // projection), and a wave's columns are half of one and half of the other.
@@ -240,9 +250,7 @@ struct Gemm {
     const int k = kk * 32 + (lane >> 4) * 8 + ((lane & 15) >> 2);
     const int g = ((k & 3) + 4 * ((k >> 3) & 3)) & S::kGroupMask;
     const char* q = tile + k * rb + (((i0 >> 4) ^ g) << 5) + (lane & 3) * 8;
-    typedef __attribute__((address_space(3))) s4v* lp;
-    const s4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)q);
-    const s4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(q + 4 * rb));
+    const s4v lo = read_transposed((LdsBlock*)q), hi = read_transposed((LdsBlock*)(q + 4 * rb));
     return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
   }
 
@@ -270,12 +278,12 @@ struct Gemm {
 #pragma unroll
       for (int j = 0; j < NF; j++) acc[i][j] = T::mfma(f.b[j], f.a[i], acc[i][j]);
   }
-  // Reads of one half tile spread over the products of the other. Measured on
-  // 4096 x 14336 x 4096: row operands 1252 -> 1278 TFLOP/s; with a col operand
-  // it is the slower order (1125 -> 1021), so those keep the compiler's.
+  // Reads of one half tile spread over the products of the other, so that
+  // neither unit waits for a burst of the other's (256-tiles, 8192^3, operands
+  // row/row, row/col and col/col: 1318, 1294 and 1277 TFLOP/s in the compiler's
+  // order, 1316, 1320 and 1332 in this one).
   static __device__ inline void interleave() {
-    if (!(RA && RB)) return;
-    constexpr int reads = MF + NF, per = MF * NF / reads > 0 ? MF * NF / reads : 1;
+    constexpr int reads = MF * (RA ? 1 : 2) + NF * (RB ? 1 : 2), per = MF * NF / reads > 0 ? MF * NF / reads : 1;
 #pragma unroll
     for (int i = 0; i < reads; i++) {
       __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);   // an LDS read

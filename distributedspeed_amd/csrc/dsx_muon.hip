@@ -451,12 +451,13 @@ void launch_apply(Table& t, short* ws, const Info* info, int cur, int first, boo
     k_apply<G, TALL, false, false><<<dim3((unsigned)n), G::THREADS, 0, s>>>(t, ws, info, cur, first, a, ma, out_dt);
 }
 
-// The square tile of a launch: a CU runs one block of 256 or 192 at a time or
-// two of 128, whose products take 1.2 times as long for the same area; the
-// whole rounds over the CUs decide. (The Gram matrix of 4096 x 14336: 136, 253
-// and 528 tiles, of which only the 192s fill the chip once and no more.)
+// The square tile of a launch. A CU runs one block of 256 or 192 at a time, or
+// two of 128, whose products take 1.2 times as long for the same area (a lone
+// block of 128 on a CU: 1.4 times); the rounds over the CUs decide. (The Gram
+// matrix of 4096 x 14336: 136, 253 and 528 tiles, of which only the 192s fill
+// the chip once and no more: 370, 327 and 520 us.)
 int tile_of(const Table& t, bool triangle) {
-  const int64_t size[3] = {256, 192, 128}, slots[3] = {256, 256, 512}, cost[3] = {65536 * 10, 36864 * 10, 32768 * 12};
+  const int64_t cus = 256, size[3] = {256, 192, 128};
   int best = 0;
   int64_t least = INT64_MAX;
   for (int k = 0; k < 3; k++) {
@@ -466,9 +467,15 @@ int tile_of(const Table& t, bool triangle) {
       const int64_t a = ceil_div(m.rows8, size[k]), b = ceil_div(m.cols8, size[k]), q = a < b ? a : b;
       n += triangle ? q * (q + 1) / 2 : a * b;
     }
-    const int64_t c = ceil_div(n, slots[k]) * cost[k];
-    if (c < least) {
-      least = c;
+    int64_t cost;
+    if (size[k] > 128) {
+      cost = ceil_div(n, cus) * size[k] * size[k] * 10;
+    } else {
+      const int64_t rest = n % (2 * cus);
+      cost = (n / (2 * cus) * 24 + (rest > cus ? 24 : rest ? 14 : 0)) * 128 * 128;
+    }
+    if (cost < least) {
+      least = cost;
       best = k;
     }
   }
