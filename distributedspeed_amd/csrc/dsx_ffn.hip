@@ -105,11 +105,15 @@ __device__ inline void put24(uint16_t* hi, uint8_t* lo, int64_t at, const float*
   *(u16x8*)(hi + at) = a;
   *(u8x8*)(lo + at) = b;
 }
-__device__ inline void get24(const uint16_t* hi, const uint8_t* lo, int64_t at, float* v) {
-  const u16x8 a = *(const u16x8*)(hi + at);
-  const u8x8 b = *(const u8x8*)(lo + at);
-#pragma unroll
-  for (int e = 0; e < 8; e++) v[e] = __builtin_bit_cast(float, ((uint32_t)a[e] << 16) | ((uint32_t)b[e] << 8));
+struct Raw24 {
+  u16x8 hi;
+  u8x8 lo;
+};
+__device__ inline Raw24 get24(const uint16_t* hi, const uint8_t* lo, int64_t at) {
+  return {*(const u16x8*)(hi + at), *(const u8x8*)(lo + at)};
+}
+__device__ inline float widen24(const Raw24& r, int e) {
+  return __builtin_bit_cast(float, ((uint32_t)r.hi[e] << 16) | ((uint32_t)r.lo[e] << 8));
 }
 
 // ---- epilogues: eight columns of a row (n is a multiple of 8, below N) ------
@@ -125,9 +129,11 @@ __device__ inline s8v round8(const float* v) {
 template <class T>
 struct Store {  // C in the inputs' type
   static constexpr bool kPair = false;
+  typedef Nothing Raw;
   short* c;
   int64_t ld;
-  __device__ inline void operator()(int m, int n, int N, const float* v, const float*) const {
+  __device__ inline Raw load(int, int) const { return {}; }
+  __device__ inline void operator()(int m, int n, int N, const float* v, const float*, const Raw&) const {
     short* o = c + m * ld + n;
     const s8v w = round8<T>(v);
     if (n + 8 <= N)
@@ -141,9 +147,11 @@ struct Store {  // C in the inputs' type
 template <class T>
 struct Up {  // h and the factors from g and u
   static constexpr bool kPair = true;
+  typedef Nothing Raw;
   Saved s;
   int act, keep;
-  __device__ inline void operator()(int m, int n, int, const float* g, const float* u) const {
+  __device__ inline Raw load(int, int) const { return {}; }
+  __device__ inline void operator()(int m, int n, int, const float* g, const float* u, const Raw&) const {
     const int64_t at = m * s.ld + n;
     float h[8], p[8], q[8];
 #pragma unroll
@@ -164,18 +172,25 @@ struct Up {  // h and the factors from g and u
 template <class T>
 struct Factors {  // dg and du from dh
   static constexpr bool kPair = false;
+  struct Raw {
+    Raw24 p, q;
+  };
   Saved s;
   short* dg;
   short* du;
-  __device__ inline void operator()(int m, int n, int, const float* v, const float*) const {
+  int rows, cols;
+  __device__ inline Raw load(int m, int n) const {
+    if (m >= rows || n >= cols) return {};
+    const int64_t at = m * s.ld + n;
+    return {get24(s.p_hi, s.p_lo, at), get24(s.q_hi, s.q_lo, at)};
+  }
+  __device__ inline void operator()(int m, int n, int, const float* v, const float*, const Raw& r) const {
     const int64_t at = m * s.ld + n;
     float p[8], q[8];
-    get24(s.p_hi, s.p_lo, at, p);
-    get24(s.q_hi, s.q_lo, at, q);
 #pragma unroll
     for (int e = 0; e < 8; e++) {
-      p[e] *= v[e];
-      q[e] *= v[e];
+      p[e] = widen24(r.p, e) * v[e];
+      q[e] = widen24(r.q, e) * v[e];
     }
     *(s8v*)(dg + at) = round8<T>(p);
     *(s8v*)(du + at) = round8<T>(q);
@@ -200,11 +215,6 @@ __device__ inline Operand at_k(Operand o, bool row, int k) {
   return o;
 }
 
-__device__ inline void put8(float* p, const float* v) {
-  *(f4v*)p = f4v{v[0], v[1], v[2], v[3]};
-  *(f4v*)(p + 4) = f4v{v[4], v[5], v[6], v[7]};
-}
-
 template <class G, bool RA, bool RB, class E>
 __global__ DSX_TILE_KERNEL(G) void k_product(Product p, E e) {
   __shared__ __attribute__((aligned(1024))) char lds[G::kLds];
@@ -226,17 +236,20 @@ __global__ DSX_TILE_KERNEL(G) void k_product(Product p, E e) {
     const Operand b1 = E::kPair ? at_k(p.b[1], RB, k0) : b;
     g.run(lds, a, b, b1, ti * G::TM, tj * TN, k1 - k0);
   }
-  g.emit(lds, [&](int r, int c, const float* v, const float* w) {
-    const int m = ti * G::TM + r, n = tj * TN + c;
-    if (m >= p.m || n >= p.n) return;
-    if (p.splits > 1) {
-      float* o = p.part + ((int64_t)split * p.m + m) * p.ldp + n;
-      put8(o, v);
-      if (E::kPair) put8(o + p.ldp / 2, w);
-    } else {
-      e(m, n, p.n, v, w);
-    }
-  });
+  g.template emit<false>(
+      lds, [&](int r, int c) { return p.splits > 1 ? typename E::Raw{} : e.load(ti * G::TM + r, tj * TN + c); },
+      [&](int r, int c, float* v, float* w, const typename E::Raw& raw) {
+        const int m = ti * G::TM + r, n = tj * TN + c;
+        if (m >= p.m || n >= p.n) return;
+        if (p.splits > 1) {
+          float* o = p.part + ((int64_t)split * p.m + m) * p.ldp + n;
+          G::put8(o, v);
+          if (E::kPair) G::put8(o + p.ldp / 2, w);
+        } else {
+          e(m, n, p.n, v, w, raw);
+        }
+      },
+      [](int, int, const float*) {});
 }
 
 // Adds the splits' partial sums in order and applies the epilogue: a block
@@ -273,7 +286,7 @@ __global__ __launch_bounds__(256) void k_join(const float* __restrict__ part, in
       if (E::kPair) w[k] += sums[s][i][8 + (k & 7)];
     }
   }
-  e(r, c, n, v, w);
+  e(r, c, n, v, w, e.load(r, c));
 }
 
 // ---- the weight gradients: up to three products over the tokens ------------
@@ -301,10 +314,13 @@ __global__ DSX_TILE_KERNEL(G) void k_weight_grads(WeightGrads t) {
   g.init();
   g.run(lds, q.a, q.b, q.b, ti * G::TM, tj * G::TN, t.tokens);
   const Store<T> e{q.out, q.n};
-  g.emit(lds, [&](int r, int c, const float* v, const float*) {
-    const int m = ti * G::TM + r, n = tj * G::TN + c;
-    if (m < q.m && n < q.n) e(m, n, q.n, v, v);
-  });
+  g.template emit<false>(
+      lds, [](int, int) { return Nothing{}; },
+      [&](int r, int c, float* v, float* w, const Nothing& none) {
+        const int m = ti * G::TM + r, n = tj * G::TN + c;
+        if (m < q.m && n < q.n) e(m, n, q.n, v, w, none);
+      },
+      [](int, int, const float*) {});
 }
 
 // ---- host ------------------------------------------------------------------
@@ -374,11 +390,11 @@ void launch_product(Product p, const Shape& s, bool direct, float* part, const E
     if (s.tm == 16) DSX_RUN(16, 128, 1, 4, true);
     else if (s.tm == 32) DSX_RUN(32, 128, 1, 4, true);
     else if (s.tm == 64) DSX_RUN(64, 128, 1, 4, true);
-    else if (s.tm == 128) DSX_RUN(128, 128, 2, 2, true);
+    else if (s.tm == 128) DSX_RUN(128, 128, 2, 4, true);
     else DSX_RUN(256, 256, 2, 4, true);
   } else {
     if (s.tm == 32) DSX_RUN(32, 128, 1, 4, false);
-    else DSX_RUN(128, 128, 2, 2, false);
+    else DSX_RUN(128, 128, 2, 4, false);
   }
 #undef DSX_RUN
   if (p.splits > 1)
@@ -499,7 +515,7 @@ void launch_weight_grads(WeightGrads& w, hipStream_t st) {
       return;
     }
   }
-  using G = Gemm<T, 128, 128, 2, 2, false, false, DIRECT>;
+  using G = Gemm<T, 128, 128, 2, 4, false, false, DIRECT>;
   k_weight_grads<G, T><<<dim3((unsigned)n), G::THREADS, 0, st>>>(w);
 }
 
@@ -522,7 +538,7 @@ int backward(const DsxFfn& q, const void* dy, int64_t ld_dy, void* dx, int64_t l
     p.segments = 1;
     p.m = m;
     p.n = (int)z.f;
-    launch_product<T, true, false>(p, shape_of(z.m, z.f, z.kd, false, dir.dh), dir.dh, part, Factors<T>{s, dg, du},
+    launch_product<T, true, false>(p, shape_of(z.m, z.f, z.kd, false, dir.dh), dir.dh, part, Factors<T>{s, dg, du, m, (int)z.f},
                                    st);
   }
   if (dx) {

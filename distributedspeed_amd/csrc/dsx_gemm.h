@@ -9,7 +9,7 @@
 // registers by the transposing LDS read (16 lanes read a 4 x 16 block, each
 // lane gets one column of it).
 //
-// A block walks K in tiles of 64, two tiles in shared memory: while the waves
+// A block walks K in tiles of 64, two of them in shared memory: while the waves
 // multiply one, the other is filled by 16-byte loads that go straight to
 // shared memory (no registers, no LDS store instructions). A tile is kept in
 // 16-byte chunks at permuted places, so that the 16 lanes of a fragment read
@@ -53,6 +53,8 @@ struct BF16 {
 };
 
 constexpr int kBK = 64;
+
+struct Nothing {};  // of an epilogue that reads nothing
 
 // A kernel of tile G. Two waves a SIMD for the square tiles, which is what
 // their shared memory allows: left to itself the compiler aims at more, puts
@@ -180,50 +182,72 @@ struct Gemm {
       for (int j = 0; j < NF; j++) acc[i][j] = f4v{0, 0, 0, 0};
   }
 
-  // Hands out C, eight consecutive columns at a time: f(row, col, v, w), both
-  // within the tile (within a half tile, v of the first operand and w of the
-  // second, for SPLIT). A fragment holds four columns of a row in a lane, 32
+  // Hands out C, eight consecutive columns at a time: f(row, col, v, w, raw),
+  // both within the tile (within a half tile, v of the first operand and w of
+  // the second, for SPLIT). A fragment holds four columns of a row in a lane, 32
   // bytes of 16-bit output a row and instruction; by way of a strip of 16 rows
   // in the wave's own part of shared memory (the tiles' place, free by now) the
-  // lanes of a row write 128 bytes together.
-  // t(col, row0, v) gets the same strip by columns where TRANSPOSED: 16
-  // consecutive rows of one column.
+  // lanes of a row write 128 bytes together. raw is what pre(row, col) loaded
+  // for the same place, two strips ahead.
+  // Where COLUMNS, f's v (which it may change) is handed out again by columns:
+  // t(col, row0, v), 16 consecutive rows of one column.
   static constexpr int kStripLd = WTN + 4;  // floats: 16 rows fall on different banks
-  template <bool TRANSPOSED, class F, class U>
-  __device__ inline void emit(char* lds, F&& f, U&& t) {
+  template <bool COLUMNS, class P, class F, class U>
+  __device__ inline void emit(char* lds, P&& pre, F&& f, U&& t) {
     static_assert(WM * WN * 16 * kStripLd * 4 <= kLds, "the strips fit the tiles' place");
+    static_assert(!(COLUMNS && SPLIT), "one operand");
     float* strip = (float*)lds + (wm * WN + wn) * 16 * kStripLd;
-    constexpr int COLS = SPLIT ? WTN / 2 : WTN, PER = COLS / 8;
+    constexpr int COLS = SPLIT ? WTN / 2 : WTN, PER = COLS / 8, PASSES = (16 * PER + 63) / 64, AHEAD = 2;
+    decltype(pre(0, 0)) raw[AHEAD + 1][PASSES];
+    auto at = [&](int q, int* r, int* c) {
+      const int p = q * 64 + lane;
+      *r = p / PER;
+      *c = p % PER * 8;
+      return 16 * PER % 64 == 0 || p < 16 * PER;
+    };
+    auto fetch = [&](int i) {
+#pragma unroll
+      for (int q = 0; q < PASSES; q++) {
+        int r, c;
+        if (at(q, &r, &c)) raw[i % (AHEAD + 1)][q] = pre(wm * WTM + i * 16 + r, wn * COLS + c);
+      }
+    };
+#pragma unroll
+    for (int i = 0; i < AHEAD && i < MF; i++) fetch(i);
 #pragma unroll
     for (int i = 0; i < MF; i++) {
+      if (i + AHEAD < MF) fetch(i + AHEAD);
 #pragma unroll
       for (int j = 0; j < NF; j++) *(f4v*)(strip + (lane & 15) * kStripLd + j * 16 + (lane >> 4) * 4) = acc[i][j];
       wave_sync();
 #pragma unroll
-      for (int p0 = 0; p0 < 16 * PER; p0 += 64) {
-        const int p = p0 + lane, r = p / PER, c = p % PER * 8;
-        if (16 * PER % 64 && p >= 16 * PER) break;
+      for (int q = 0; q < PASSES; q++) {
+        int r, c;
+        if (!at(q, &r, &c)) continue;
         float v[8], w[8];
         get8(strip + r * kStripLd + c, v);
         if (SPLIT) get8(strip + r * kStripLd + COLS + c, w);
-        f(wm * WTM + i * 16 + r, wn * COLS + c, v, w);
+        f(wm * WTM + i * 16 + r, wn * COLS + c, v, w, raw[i % (AHEAD + 1)][q]);
+        if (COLUMNS) put8(strip + r * kStripLd + c, v);
       }
-      if (TRANSPOSED)
+      wave_sync();
+      if (COLUMNS) {
 #pragma unroll
         for (int c0 = 0; c0 < WTN; c0 += 64) {
           const int c = c0 + lane;
-          if (WTN % 64 && c >= WTN) break;
+          if (WTN % 64 && c >= WTN) continue;
           float v[16];
 #pragma unroll
           for (int r = 0; r < 16; r++) v[r] = strip[r * kStripLd + c];
           t(wn * WTN + c, wm * WTM + i * 16, v);
         }
-      wave_sync();
+        wave_sync();
+      }
     }
   }
-  template <class F>
-  __device__ inline void emit(char* lds, F&& f) {
-    emit<false>(lds, f, [](int, int, const float*) {});
+  static __device__ inline void put8(float* p, const float* v) {
+    *(f4v*)p = f4v{v[0], v[1], v[2], v[3]};
+    *(f4v*)(p + 4) = f4v{v[4], v[5], v[6], v[7]};
   }
   static __device__ inline void get8(const float* p, float* v) {
     const f4v a = *(const f4v*)p, b = *(const f4v*)(p + 4);
@@ -254,6 +278,12 @@ struct Gemm {
     return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
   }
 
+  // A barrier once this wave's direct loads have landed and its LDS reads are done.
+  static __device__ inline void sync_loads() {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  }
   struct Frags {
     s8v a[MF], b[NF];
   };
@@ -372,8 +402,7 @@ struct Gemm {
       Frags f0, f1;
       set(K);
       load(lds);
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      __syncthreads();
+      sync_loads();
       if (nt > 1) {
         if (K - kBK < kBK) set(K - kBK);
         load(lds + kTile);
@@ -395,9 +424,7 @@ struct Gemm {
         read(f1, cur, 1);
         multiply(f0);
         interleave();
-        // all of this tile is in registers, all of the next in shared memory
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
+        sync_loads();  // all of this tile is in registers, all of the next in shared memory
         if (t + 2 < nt) {
           const int left = K - (t + 2) * kBK;
           if (left < kBK) set(left);

@@ -1,14 +1,14 @@
 // dsx_muon.hip -- Newton-Schulz orthogonalisation of matrices, and the Muon
 // step around it (see include/dsx.h).
 //
-// For each matrix G (R x C, s = min(R, C)):
+// For each matrix G (s x l with s <= l; a matrix with more rows than columns is
+// transposed on the way in and out, the result being the same):
 //   X0 = G / (|G|_F + eps);   for each step with its coefficients (a, b, c):
-//   A = X X^T (or X^T X where R > C; s x s),  B = b A + c A A,
-//   X <- a X + B X (or a X + X B).
+//   A = X X^T (s x s),  B = b A + c A A,  X <- a X + B X.
 // A and B are symmetric: only the tiles on and above the diagonal are
 // computed, each written at both places. A step is three launches for a whole
-// list of matrices; every launch finds its matrix and tile from a table in
-// the kernel's arguments.
+// list of matrices of any shapes; every launch finds its matrix and tile from a
+// table in the kernel's arguments.
 //
 // Numbers. The iterates are fp16 with fp32 sums: entries of X, A and B are
 // bounded by their spectral norms (about 1.2, 1.5 and 2.9 with Muon's
@@ -42,7 +42,7 @@ using dsxi::round_up;
 
 constexpr float kScale = 4096.0f;
 constexpr int kMats = 24;        // matrices of one launch (the table is a kernel argument)
-constexpr int kMaxParts = 512;   // norm partials per matrix
+constexpr int kMaxParts = 2048;  // norm partials per matrix
 constexpr int kNormTile = 64;    // the norm and cast kernels' square tile
 
 struct Mat {
@@ -51,17 +51,19 @@ struct Mat {
   float* momentum;
   float* master;
   int64_t ld_in, ld_out;
-  int64_t x[2], a, b;  // offsets in the workspace, in 16-bit elements
-  int32_t rows, cols, rows8, cols8;
-  int32_t tile0;       // first tile of this matrix in the launch at hand
+  int64_t x[2], a, b;   // offsets in the workspace, in 16-bit elements
+  int32_t rows, cols;   // of the caller's matrix
+  int32_t s, l;         // of X: its sides rounded up to multiples of 8, s <= l
+  int32_t tall;         // X is the matrix transposed
   int32_t part0, parts;
-  float   lr;          // Muon: the step size of this matrix
+  float   lr;           // Muon: the step size of this matrix
 };
 struct Table {
+  int32_t tile0[kMats];  // first tile of each matrix in the launch at hand
+  int32_t n, reserved;
   Mat m[kMats];
-  int32_t n;
 };
-static_assert(sizeof(Table) <= 3584, "the table travels in the kernel arguments");
+static_assert(sizeof(Table) <= 3840, "the table travels in the kernel arguments");
 
 struct Info {
   float p;      // X0~ = G p, a power of two
@@ -77,10 +79,11 @@ struct MuonArgs {
   int32_t nesterov;
 };
 
+// The matrix that a block's tile belongs to: all first tiles are read at once.
 __device__ inline int find(const Table& t, int tile) {
-  int i = 0;
-  while (i + 1 < t.n && tile >= t.m[i + 1].tile0) i++;
-  return i;
+  const int i = threadIdx.x & 63;
+  const bool begun = i < t.n && tile >= t.tile0[i < kMats ? i : 0];
+  return __popcll(__ballot(begun)) - 1;
 }
 
 template <int DT>
@@ -132,7 +135,7 @@ template <int DT, bool MUON>
 __global__ __launch_bounds__(256) void k_sumsq(Table t, double* __restrict__ partials, MuonArgs ma) {
   const int i = find(t, blockIdx.x);
   const Mat& m = t.m[i];
-  const int part = blockIdx.x - m.tile0, tid = threadIdx.x;
+  const int part = blockIdx.x - t.tile0[i], tid = threadIdx.x;
   const int tc = (m.cols + kNormTile - 1) / kNormTile, tiles = tc * ((m.rows + kNormTile - 1) / kNormTile);
   const bool vec = (m.ld_in & 3) == 0 && ((uintptr_t)m.in & (DT == DSX_F32 ? 15 : 7)) == 0;
   const float inv = MUON ? inverse_scale(ma) : 1.0f;
@@ -158,14 +161,8 @@ __global__ __launch_bounds__(256) void k_sumsq(Table t, double* __restrict__ par
   if (tid == 0) partials[m.part0 + part] = part_sum[0] + part_sum[1] + part_sum[2] + part_sum[3];
 }
 
-// One block per matrix: its norm, the power of two and the rest of 1 / norm.
-__global__ __launch_bounds__(64) void k_norms(Table t, const double* __restrict__ partials, Info* __restrict__ info,
-                                              double eps, int32_t* skip) {
-  const Mat& m = t.m[blockIdx.x];
-  double sum = 0;
-  for (int k = threadIdx.x; k < m.parts; k += 64) sum += partials[m.part0 + k];
-  for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
-  if (threadIdx.x) return;
+// From the sum of squares: the power of two and the rest of 1 / norm.
+__device__ inline Info info_of(double sum, double eps) {
   Info f = {0.0f, 1.0f, 0, 0};
   if (isfinite(sum)) {
     const double inv = (double)kScale / (sqrt(sum) + eps);
@@ -175,43 +172,73 @@ __global__ __launch_bounds__(64) void k_norms(Table t, const double* __restrict_
     f.inv_r = (float)(inv / ldexp(1.0, e - 1));
   } else {
     f.bad = 1;
-    if (skip) atomicOr(skip, 1);
   }
-  info[blockIdx.x] = f;
+  return f;
+}
+
+// A wave's sum of a matrix's partials, in an order set by their count.
+__device__ inline double total(const double* __restrict__ p, int parts) {
+  double sum = 0;
+#pragma unroll 4
+  for (int k = threadIdx.x & 63; k < parts; k += 64) sum += p[k];
+  for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
+  return sum;
+}
+
+// Muon: whether any matrix's norm is not finite, before anything is written.
+__global__ __launch_bounds__(64) void k_norms(Table t, const double* __restrict__ partials, double eps,
+                                              int32_t* skip) {
+  const Mat& m = t.m[blockIdx.x];
+  const Info f = info_of(total(partials + m.part0, m.parts), eps);
+  if (threadIdx.x == 0 && f.bad) atomicOr(skip, 1);
 }
 
 // X0~ = fp16(G p), zero beyond the matrix; all NaN where the norm is not finite
 // (every entry of the exact result is). Muon: the momentum buffer is written
 // here, once the step is known not to be skipped.
 template <int DT, bool MUON>
-__global__ __launch_bounds__(256) void k_cast(Table t, short* __restrict__ ws, const Info* __restrict__ info,
-                                              MuonArgs ma) {
+__global__ __launch_bounds__(256) void k_cast(Table t, short* __restrict__ ws, const double* __restrict__ partials,
+                                              Info* __restrict__ info, double eps, MuonArgs ma) {
+  __shared__ short turn[kNormTile][kNormTile + 4];
+  if (MUON && *ma.skip) return;
   const int i = find(t, blockIdx.x);
   const Mat& m = t.m[i];
-  const int tile = blockIdx.x - m.tile0, tid = threadIdx.x;
-  const int tc = (m.cols8 + kNormTile - 1) / kNormTile;
-  const int r0 = tile / tc * kNormTile + (tid >> 4), c = tile % tc * kNormTile + (tid & 15) * 4;
-  if (c >= m.cols8 || (MUON && *ma.skip)) return;
+  const int tile = blockIdx.x - t.tile0[i], tid = threadIdx.x;
+  const Info f = info_of(total(partials + m.part0, m.parts), eps);
+  if (tile == 0 && tid == 0) info[i] = f;
+  const int tc = (m.l + kNormTile - 1) / kNormTile;  // X's tile, and where it lies in the matrix
+  const int xr = tile / tc * kNormTile, xc = tile % tc * kNormTile;
+  const int r0 = (m.tall ? xc : xr) + (tid >> 4), c = (m.tall ? xr : xc) + (tid & 15) * 4;
   const bool vec = (m.ld_in & 3) == 0 && ((uintptr_t)m.in & (DT == DSX_F32 ? 15 : 7)) == 0;
   const float inv = MUON ? inverse_scale(ma) : 1.0f;
-  const Info f = info[i];
 #pragma unroll
   for (int k = 0; k < 4; k++) {
     const int r = r0 + 16 * k;
-    if (r >= m.rows8) break;
     float u[4] = {0, 0, 0, 0}, buf[4];
     if (r < m.rows && c < m.cols) {
       update4<DT, MUON>(m, ma, inv, r, c, vec, u, buf);
       if (MUON)
         for (int e = 0; e < 4; e++)
           if (c + e < m.cols) m.momentum[(int64_t)r * m.cols + c + e] = buf[e];
-      if (f.bad)
-        for (int e = 0; e < 4; e++) u[e] = __builtin_nanf("");
+      for (int e = 0; e < 4; e++) u[e] = f.bad ? __builtin_nanf("") : c + e < m.cols ? u[e] * f.p : 0.0f;
     }
     s4v o;
 #pragma unroll
-    for (int e = 0; e < 4; e++) o[e] = F16::round(f.bad ? u[e] : (c + e < m.cols ? u[e] * f.p : 0.0f));
-    *(s4v*)(ws + m.x[0] + (int64_t)r * m.cols8 + c) = o;
+    for (int e = 0; e < 4; e++) o[e] = F16::round(u[e]);
+    if (!m.tall) {
+      if (r < m.s && c < m.l) *(s4v*)(ws + m.x[0] + (int64_t)r * m.l + c) = o;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; e++) turn[(tid & 15) * 4 + e][(tid >> 4) + 16 * k] = o[e];
+    }
+  }
+  if (!m.tall) return;
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < 4; k++) {
+    const int r = xr + (tid >> 4) + 16 * k, q = xc + (tid & 15) * 4;
+    if (r < m.s && q < m.l)
+      *(s4v*)(ws + m.x[0] + (int64_t)r * m.l + q) = *(const s4v*)&turn[(tid >> 4) + 16 * k][(tid & 15) * 4];
   }
 }
 
@@ -224,124 +251,170 @@ __device__ inline void triangle(int t, int* i, int* j) {
 }
 
 // A symmetric product's tile, written at (m, n) and, off the diagonal, at (n, m).
-// GRAM: A = X X^T (wide) or X^T X (TALL) from the current X; else B = b A + c A A.
-template <class G, bool GRAM, bool TALL>
-__global__ DSX_TILE_KERNEL(G) void k_symmetric(Table t, short* __restrict__ ws,
-                                                          const Info* __restrict__ info, int cur, int first, float b,
-                                                          float c, const int32_t* skip) {
+// GRAM: A = X X^T of the current X; else B = b A + c A A.
+template <class G, bool GRAM>
+__global__ DSX_TILE_KERNEL(G) void k_symmetric(Table t, short* __restrict__ ws, const Info* __restrict__ info, int cur,
+                                               int first, float b, float c, const int32_t* skip) {
   __shared__ __attribute__((aligned(1024))) char lds[G::kLds];
   if (skip && *skip) return;
   const int bid = xcd_order(blockIdx.x, gridDim.x);
   const int i = find(t, bid);
   const Mat& m = t.m[i];
-  const int s = min(m.rows8, m.cols8);
+  const int s = m.s;
   int ti, tj;
-  triangle(bid - m.tile0, &ti, &tj);
+  triangle(bid - t.tile0[i], &ti, &tj);
   G g;
   g.init();
-  const short* src = ws + (GRAM ? m.x[cur] : m.a);
-  const Operand o{src, GRAM ? m.cols8 : s, s};
-  g.run(lds, o, o, o, ti * G::TM, tj * G::TN, GRAM ? max(m.rows8, m.cols8) : s);
   const float inv_r = first ? info[i].inv_r : 1.0f;
+  const short* src = ws + (GRAM ? m.x[cur] : m.a);
+  const Operand o{src, GRAM ? m.l : s, s};
+  const int r0 = ti * G::TM, c0 = tj * G::TN;
+  g.run(lds, o, o, o, r0, c0, GRAM ? m.l : s);
   const float k = GRAM ? inv_r * inv_r * (1.0f / kScale) : c * (1.0f / kScale);
   short* dst = ws + (GRAM ? m.a : m.b);
-  // eight values, at q (a multiple of 8, as s is) of row r
-  auto put = [&](int r, int q, const float* v) {
-    if (r >= s || q >= s) return;
-    const int64_t at = (int64_t)r * s + q;
-    s8v w;
-    if (GRAM) {
-#pragma unroll
-      for (int e = 0; e < 8; e++) w[e] = F16::round(k * v[e]);
-    } else {
-      const s8v a = *(const s8v*)(src + at);
-#pragma unroll
-      for (int e = 0; e < 8; e++) w[e] = F16::round(fmaf(k, v[e], b * F16::widen(a[e])));
-    }
-    *(s8v*)(dst + at) = w;
+  auto pre = [&](int r, int q) {  // s is a multiple of 8: eight values are inside or outside together
+    r += r0;
+    q += c0;
+    return GRAM || r >= s || q >= s ? s8v{} : *(const s8v*)(src + (int64_t)r * s + q);
   };
-  const int r0 = ti * G::TM, c0 = tj * G::TN;
+  auto put = [&](int r, int q, float* v, float*, const s8v& a) {
+    s8v w;
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      v[e] = GRAM ? k * v[e] : fmaf(k, v[e], b * F16::widen(a[e]));
+      w[e] = F16::round(v[e]);
+    }
+    r += r0;
+    q += c0;
+    if (r < s && q < s) *(s8v*)(dst + (int64_t)r * s + q) = w;
+  };
+  auto mirror = [&](int q, int r, const float* v) {
+    r += r0;
+    q += c0;
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      s8v w;
+#pragma unroll
+      for (int e = 0; e < 8; e++) w[e] = F16::round(v[8 * h + e]);
+      if (q < s && r + 8 * h < s) *(s8v*)(dst + (int64_t)q * s + r + 8 * h) = w;
+    }
+  };
   if (ti == tj)
-    g.emit(lds, [&](int r, int q, const float* v, const float*) { put(r0 + r, c0 + q, v); });
+    g.template emit<false>(lds, pre, put, mirror);
   else
-    g.template emit<true>(
-        lds, [&](int r, int q, const float* v, const float*) { put(r0 + r, c0 + q, v); },
-        [&](int q, int r, const float* v) {
-          put(c0 + q, r0 + r, v);
-          put(c0 + q, r0 + r + 8, v + 8);
-        });
+    g.template emit<true>(lds, pre, put, mirror);
 }
 
-// X <- (a X + B X) / r, or with X B where TALL. LAST: the result itself, to the
-// output in bf16 (OUT 0) or as Muon's parameter update (fp32 master and 16-bit
-// copy of OUT's type, 0 for none).
-template <class G, bool TALL, bool LAST, bool MUON>
-__global__ DSX_TILE_KERNEL(G) void k_apply(Table t, short* __restrict__ ws, const Info* __restrict__ info,
-                                                      int cur, int first, float a, MuonArgs ma, int out_dt) {
+// Muon's update of `n` <= 16 parameters: w = w decay - lr O (v holds kScale O).
+template <int N>
+__device__ inline void step_params(const Mat& m, const MuonArgs& ma, int out_dt, int64_t r, int c, const float* v) {
+  float* w = m.master + r * m.cols + c;
+  short* o = (short*)m.out + r * m.ld_out + c;
+#pragma unroll
+  for (int e = 0; e < N; e++) {
+    if (c + e >= m.cols) break;
+    const float n = fmaf(-m.lr * (1.0f / kScale), v[e], w[e] * ma.decay);
+    w[e] = n;
+    if (out_dt) o[e] = out_dt == DSX_F16 ? F16::round(n) : BF16::round(n);
+  }
+}
+// N values of a row of the result in bf16 (v holds kScale O).
+template <int N>
+__device__ inline void store_row(const Mat& m, int64_t r, int c, const float* v) {
+  short* o = (short*)m.out + r * m.ld_out + c;
+#pragma unroll
+  for (int h = 0; h < N; h += 8) {
+    s8v w;
+#pragma unroll
+    for (int e = 0; e < 8; e++) w[e] = BF16::round(v[h + e] * (1.0f / kScale));
+    if (c + h + 8 <= m.cols)
+      *(s8u*)(o + h) = w;
+    else
+      for (int e = 0; e < 8; e++)
+        if (c + h + e < m.cols) o[h + e] = w[e];
+  }
+}
+
+// X <- (a X + B X) / r. LAST: the result itself, transposed back where the
+// matrix was, to the output in bf16 or as Muon's parameter update (fp32 master
+// and 16-bit copy of out_dt, 0 for none).
+template <class G, bool LAST, bool MUON>
+__global__ DSX_TILE_KERNEL(G) void k_apply(Table t, short* __restrict__ ws, const Info* __restrict__ info, int cur,
+                                           int first, float a, MuonArgs ma, int out_dt) {
   __shared__ __attribute__((aligned(1024))) char lds[G::kLds];
   if (MUON && *ma.skip) return;
   const int bid = xcd_order(blockIdx.x, gridDim.x);
   const int i = find(t, bid);
   const Mat& m = t.m[i];
-  const int s = min(m.rows8, m.cols8);
-  const int mt = (m.rows8 + G::TM - 1) / G::TM, nt = (m.cols8 + G::TN - 1) / G::TN;
+  const int s = m.s, l = m.l;
   int ti, tj;
-  band_order(bid - m.tile0, mt, nt, 8, &ti, &tj);
+  band_order(bid - t.tile0[i], (s + G::TM - 1) / G::TM, (l + G::TN - 1) / G::TN, 8, &ti, &tj);
+  const float inv_r = first ? info[i].inv_r : 1.0f;
   const short* x = ws + m.x[cur];
-  const Operand ox{x, m.cols8, TALL ? m.rows8 : m.cols8}, ob{ws + m.b, s, s};
+  short* y = ws + m.x[cur ^ 1];
+  const Operand ob{ws + m.b, s, s}, ox{x, l, l};
+  const int r0 = ti * G::TM, c0 = tj * G::TN;
   G g;
   g.init();
-  if (TALL)
-    g.run(lds, ox, ob, ob, ti * G::TM, tj * G::TN, s);
-  else
-    g.run(lds, ob, ox, ox, ti * G::TM, tj * G::TN, s);
-  const float inv_r = first ? info[i].inv_r : 1.0f;
-  g.emit(lds, [&](int r, int c, const float* sum, const float*) {
-    r += ti * G::TM;
-    c += tj * G::TN;
-    if (r >= (LAST ? m.rows : m.rows8) || c >= (LAST ? m.cols : m.cols8)) return;
-    const s8v old = *(const s8v*)(x + (int64_t)r * m.cols8 + c);
-    float v[8];
+  g.run(lds, ob, ox, ox, r0, c0, s);
+  auto pre = [&](int r, int c) {
+    r += r0;
+    c += c0;
+    return r >= s || c >= l ? s8v{} : *(const s8v*)(x + (int64_t)r * l + c);
+  };
+  auto value = [&](float* v, const s8v& old) {
 #pragma unroll
-    for (int e = 0; e < 8; e++) v[e] = fmaf(a, F16::widen(old[e]), sum[e] * (1.0f / kScale)) * inv_r;
-    if (!LAST) {
-      s8v w;
+    for (int e = 0; e < 8; e++) v[e] = fmaf(a, F16::widen(old[e]), v[e] * (1.0f / kScale)) * inv_r;
+  };
+  auto none = [](int, int, const float*) {};
+  if (!LAST) {
+    g.template emit<false>(
+        lds, pre,
+        [&](int r, int c, float* v, float*, const s8v& old) {
+          value(v, old);
+          s8v w;
 #pragma unroll
-      for (int e = 0; e < 8; e++) w[e] = F16::round(v[e]);
-      *(s8v*)(ws + m.x[cur ^ 1] + (int64_t)r * m.cols8 + c) = w;
-      return;
-    }
-    short* o = (short*)m.out + r * m.ld_out + c;
-    const int left = m.cols - c;
-    if (!MUON) {
-      s8v w;
-#pragma unroll
-      for (int e = 0; e < 8; e++) w[e] = BF16::round(v[e] * (1.0f / kScale));
-      if (left >= 8)
-        *(s8u*)o = w;
-      else
-        for (int e = 0; e < 8; e++)
-          if (e < left) o[e] = w[e];
-    } else {
-      float* w = m.master + (int64_t)r * m.cols + c;
-      for (int e = 0; e < 8; e++) {
-        if (e >= left) break;
-        const float n = fmaf(-m.lr * (1.0f / kScale), v[e], w[e] * ma.decay);
-        w[e] = n;
-        if (out_dt) o[e] = out_dt == DSX_F16 ? F16::round(n) : BF16::round(n);
-      }
-    }
-  });
+          for (int e = 0; e < 8; e++) w[e] = F16::round(v[e]);
+          r += r0;
+          c += c0;
+          if (r < s && c < l) *(s8v*)(y + (int64_t)r * l + c) = w;
+        },
+        none);
+  } else if (!m.tall) {
+    g.template emit<false>(
+        lds, pre,
+        [&](int r, int c, float* v, float*, const s8v& old) {
+          value(v, old);
+          r += r0;
+          c += c0;
+          if (r >= m.rows || c >= m.cols) return;
+          if (MUON) step_params<8>(m, ma, out_dt, r, c, v);
+          else store_row<8>(m, r, c, v);
+        },
+        none);
+  } else {
+    g.template emit<true>(
+        lds, pre, [&](int, int, float* v, float*, const s8v& old) { value(v, old); },
+        [&](int r, int c, const float* v) {  // a column of X is a row of the matrix
+          r += c0;
+          c += r0;
+          if (r >= m.rows || c >= m.cols) return;
+          if (MUON) step_params<16>(m, ma, out_dt, r, c, v);
+          else store_row<16>(m, r, c, v);
+        });
+  }
 }
 
 // ---- host ------------------------------------------------------------------
 
-template <bool RA, bool RB>
-using Big = Gemm<F16, 256, 256, 2, 4, RA, RB, true>;
-template <bool RA, bool RB>
-using Mid = Gemm<F16, 192, 192, 2, 4, RA, RB, true>;
-template <bool RA, bool RB>
-using Small = Gemm<F16, 128, 128, 2, 2, RA, RB, true>;
+template <bool RB>
+using Big = Gemm<F16, 256, 256, 2, 4, true, RB, true>;
+template <bool RB>
+using Mid = Gemm<F16, 192, 192, 2, 4, true, RB, true>;
+template <bool RB>
+using Small = Gemm<F16, 128, 128, 2, 4, true, RB, true>;
+template <bool RB>
+using Tiny = Gemm<F16, 64, 64, 2, 2, true, RB, true>;
 
 struct Source {  // one matrix of the caller's list
   const void* in;
@@ -353,67 +426,61 @@ struct Source {  // one matrix of the caller's list
   float lr;
 };
 
-int64_t halves_of(int32_t rows, int32_t cols) {
-  const int64_t r = round_up(rows, 8), c = round_up(cols, 8), s = r < c ? r : c;
-  return 2 * round_up(r * c, 128) + 2 * round_up(s * s, 128);
-}
 int32_t parts_of(int32_t rows, int32_t cols) {
   const int64_t tiles = ceil_div(rows, kNormTile) * ceil_div(cols, kNormTile);
   const int64_t p = ceil_div(tiles, 4);
   return (int32_t)(p < 1 ? 1 : p > kMaxParts ? kMaxParts : p);
 }
 
-// The list in runs of at most kMats matrices of one orientation.
 struct Plan {
   int64_t info_bytes = 0, partial_bytes = 0, halves = 0;
 };
 
-// Orders the list by orientation (wide first) and lays out the workspace:
-// skip flag, norm records, partials, then the fp16 matrices of the largest run.
+// The list in runs of at most kMats matrices, f(table, index of the first).
+// The workspace: skip flag, norm records, partials, then the fp16 matrices of
+// the largest run.
 template <class F>
 Plan each_run(const Source* src, int32_t count, F&& f) {
   Plan plan;
-  int64_t part0 = 0;
+  Table t{};
+  int64_t part0 = 0, at = 0;
   int32_t index = 0;
-  for (int tall = 0; tall < 2; tall++) {
-    Table t{};
-    int64_t at = 0;
-    auto flush = [&]() {
-      if (t.n) f(t, tall != 0, index - t.n);
-      if (at > plan.halves) plan.halves = at;
-      t.n = 0;
-      at = 0;
-    };
-    for (int32_t k = 0; k < count; k++) {
-      const Source& q = src[k];
-      if (q.rows <= 0 || q.cols <= 0 || (q.rows > q.cols) != (tall != 0)) continue;
-      Mat& m = t.m[t.n++];
-      m = Mat{};
-      m.in = q.in;
-      m.out = q.out;
-      m.momentum = q.momentum;
-      m.master = q.master;
-      m.ld_in = q.ld_in;
-      m.ld_out = q.ld_out;
-      m.rows = q.rows;
-      m.cols = q.cols;
-      m.rows8 = (int32_t)round_up(q.rows, 8);
-      m.cols8 = (int32_t)round_up(q.cols, 8);
-      m.lr = q.lr;
-      const int64_t s = m.rows8 < m.cols8 ? m.rows8 : m.cols8;
-      m.x[0] = at;
-      m.x[1] = m.x[0] + round_up((int64_t)m.rows8 * m.cols8, 128);
-      m.a = m.x[1] + round_up((int64_t)m.rows8 * m.cols8, 128);
-      m.b = m.a + round_up(s * s, 128);
-      at = m.b + round_up(s * s, 128);
-      m.parts = parts_of(q.rows, q.cols);
-      m.part0 = (int32_t)part0;
-      part0 += m.parts;
-      index++;
-      if (t.n == kMats) flush();
-    }
-    flush();
+  auto flush = [&]() {
+    if (t.n) f(t, index - t.n);
+    if (at > plan.halves) plan.halves = at;
+    t.n = 0;
+    at = 0;
+  };
+  for (int32_t k = 0; k < count; k++) {
+    const Source& q = src[k];
+    if (q.rows <= 0 || q.cols <= 0) continue;
+    Mat& m = t.m[t.n++];
+    m = Mat{};
+    m.in = q.in;
+    m.out = q.out;
+    m.momentum = q.momentum;
+    m.master = q.master;
+    m.ld_in = q.ld_in;
+    m.ld_out = q.ld_out;
+    m.rows = q.rows;
+    m.cols = q.cols;
+    m.tall = q.rows > q.cols;
+    m.s = (int32_t)round_up(m.tall ? q.cols : q.rows, 8);
+    m.l = (int32_t)round_up(m.tall ? q.rows : q.cols, 8);
+    m.lr = q.lr;
+    const int64_t x = round_up((int64_t)m.s * m.l, 128), sq = round_up((int64_t)m.s * m.s, 128);
+    m.x[0] = at;
+    m.x[1] = at + x;
+    m.a = at + 2 * x;
+    m.b = m.a + sq;
+    at = m.b + sq;
+    m.parts = parts_of(q.rows, q.cols);
+    m.part0 = (int32_t)part0;
+    part0 += m.parts;
+    index++;
+    if (t.n == kMats) flush();
   }
+  flush();
   plan.info_bytes = 256 + round_up((int64_t)index * (int64_t)sizeof(Info), 256);
   plan.partial_bytes = round_up(part0 * 8, 256);
   return plan;
@@ -424,31 +491,30 @@ template <class F>
 int64_t tiles_of(Table& t, F&& per) {
   int64_t n = 0;
   for (int i = 0; i < t.n; i++) {
-    t.m[i].tile0 = (int32_t)n;
+    t.tile0[i] = (int32_t)n;
     n += per(t.m[i]);
   }
   return n;
 }
 
-template <class G, bool GRAM, bool TALL>
+template <class G, bool GRAM>
 void launch_symmetric(Table& t, short* ws, const Info* info, int cur, int first, float b, float c, const int32_t* skip,
                       hipStream_t s) {
   const int64_t n = tiles_of(t, [](const Mat& m) {
-    const int64_t k = ceil_div(m.rows8 < m.cols8 ? m.rows8 : m.cols8, G::TM);
+    const int64_t k = ceil_div(m.s, G::TM);
     return k * (k + 1) / 2;
   });
-  k_symmetric<G, GRAM, TALL><<<dim3((unsigned)n), G::THREADS, 0, s>>>(t, ws, info, cur, first, b, c, skip);
+  k_symmetric<G, GRAM><<<dim3((unsigned)n), G::THREADS, 0, s>>>(t, ws, info, cur, first, b, c, skip);
 }
 
-template <class G, bool TALL, bool MUON>
+template <class G, bool MUON>
 void launch_apply(Table& t, short* ws, const Info* info, int cur, int first, bool last, float a, const MuonArgs& ma,
                   int out_dt, hipStream_t s) {
-  const int64_t n =
-      tiles_of(t, [](const Mat& m) { return ceil_div(m.rows8, G::TM) * ceil_div(m.cols8, G::TN); });
+  const int64_t n = tiles_of(t, [](const Mat& m) { return ceil_div(m.s, G::TM) * ceil_div(m.l, G::TN); });
   if (last)
-    k_apply<G, TALL, true, MUON><<<dim3((unsigned)n), G::THREADS, 0, s>>>(t, ws, info, cur, first, a, ma, out_dt);
+    k_apply<G, true, MUON><<<dim3((unsigned)n), G::THREADS, 0, s>>>(t, ws, info, cur, first, a, ma, out_dt);
   else
-    k_apply<G, TALL, false, false><<<dim3((unsigned)n), G::THREADS, 0, s>>>(t, ws, info, cur, first, a, ma, out_dt);
+    k_apply<G, false, false><<<dim3((unsigned)n), G::THREADS, 0, s>>>(t, ws, info, cur, first, a, ma, out_dt);
 }
 
 // The square tile of a launch. A CU runs one block of 256 or 192 at a time, or
@@ -457,19 +523,21 @@ void launch_apply(Table& t, short* ws, const Info* info, int cur, int first, boo
 // matrix of 4096 x 14336: 136, 253 and 528 tiles, of which only the 192s fill
 // the chip once and no more: 370, 327 and 520 us.)
 int tile_of(const Table& t, bool triangle) {
+#ifdef FORCE_TILE
+  return FORCE_TILE;
+#endif
   const int64_t cus = 256, size[3] = {256, 192, 128};
   int best = 0;
   int64_t least = INT64_MAX;
   for (int k = 0; k < 3; k++) {
     int64_t n = 0;
     for (int i = 0; i < t.n; i++) {
-      const Mat& m = t.m[i];
-      const int64_t a = ceil_div(m.rows8, size[k]), b = ceil_div(m.cols8, size[k]), q = a < b ? a : b;
-      n += triangle ? q * (q + 1) / 2 : a * b;
+      const int64_t a = ceil_div(t.m[i].s, size[k]), b = ceil_div(t.m[i].l, size[k]);
+      n += triangle ? a * (a + 1) / 2 : a * b;
     }
     int64_t cost;
     if (size[k] > 128) {
-      cost = ceil_div(n, cus) * size[k] * size[k] * 10;
+      cost = ceil_div(n, cus) * size[k] * size[k] * (size[k] == 256 ? 10 : 12);
     } else {
       const int64_t rest = n % (2 * cus);
       cost = (n / (2 * cus) * 24 + (rest > cus ? 24 : rest ? 14 : 0)) * 128 * 128;
@@ -483,28 +551,23 @@ int tile_of(const Table& t, bool triangle) {
 }
 
 template <bool MUON>
-void iterate(Table& t, bool tall, short* ws, const Info* info, int steps, const double* coef, const MuonArgs& ma,
-             int out_dt, hipStream_t s) {
+void iterate(Table& t, short* ws, const Info* info, int steps, const double* coef, const MuonArgs& ma, int out_dt,
+             hipStream_t s) {
   const int sym = tile_of(t, true), app = tile_of(t, false);
   const int32_t* skip = MUON ? ma.skip : nullptr;
   for (int k = 0; k < steps; k++) {
     const float a = (float)coef[3 * k], b = (float)coef[3 * k + 1], c = (float)coef[3 * k + 2];
     const int cur = k & 1, first = k == 0, last = k == steps - 1;
-#define DSX_BY_TILE(TILE, F, RA, RB, ...)                                      \
-  do {                                                                         \
-    if (TILE == 256) F<Big<RA, RB>, __VA_ARGS__;                               \
-    else if (TILE == 192) F<Mid<RA, RB>, __VA_ARGS__;                          \
-    else F<Small<RA, RB>, __VA_ARGS__;                                         \
+#define DSX_BY_TILE(TILE, F, RB, ...)             \
+  do {                                            \
+    if (TILE == 256) F<Big<RB>, __VA_ARGS__;      \
+    else if (TILE == 192) F<Mid<RB>, __VA_ARGS__; \
+    else if (TILE == 128) F<Small<RB>, __VA_ARGS__; \
+    else F<Tiny<RB>, __VA_ARGS__;                 \
   } while (0)
-    if (tall) {
-      DSX_BY_TILE(sym, launch_symmetric, false, false, true, true>(t, ws, info, cur, first, b, c, skip, s));
-      DSX_BY_TILE(sym, launch_symmetric, true, true, false, false>(t, ws, info, cur, first, b, c, skip, s));
-      DSX_BY_TILE(app, launch_apply, true, true, true, MUON>(t, ws, info, cur, first, last, a, ma, out_dt, s));
-    } else {
-      DSX_BY_TILE(sym, launch_symmetric, true, true, true, false>(t, ws, info, cur, first, b, c, skip, s));
-      DSX_BY_TILE(sym, launch_symmetric, true, true, false, false>(t, ws, info, cur, first, b, c, skip, s));
-      DSX_BY_TILE(app, launch_apply, true, false, false, MUON>(t, ws, info, cur, first, last, a, ma, out_dt, s));
-    }
+    DSX_BY_TILE(sym, launch_symmetric, true, true>(t, ws, info, cur, first, b, c, skip, s));
+    DSX_BY_TILE(sym, launch_symmetric, true, false>(t, ws, info, cur, first, b, c, skip, s));
+    DSX_BY_TILE(app, launch_apply, false, MUON>(t, ws, info, cur, first, last, a, ma, out_dt, s));
 #undef DSX_BY_TILE
   }
 }
@@ -512,7 +575,7 @@ void iterate(Table& t, bool tall, short* ws, const Info* info, int steps, const 
 template <int DT, bool MUON>
 int drive(const Source* src, int32_t count, int steps, const double* coef, double eps, MuonArgs ma, int out_dt,
           char* base, int64_t bytes, const char* what, hipStream_t s) {
-  const Plan plan = each_run(src, count, [](Table&, bool, int) {});
+  const Plan plan = each_run(src, count, [](Table&, int) {});
   const int64_t need = plan.info_bytes + plan.partial_bytes + 2 * plan.halves;
   if (bytes < need)
     return fail(DSX_EINVAL, "%s: the workspace has %lld bytes, %lld are needed", what, (long long)bytes,
@@ -522,20 +585,19 @@ int drive(const Source* src, int32_t count, int steps, const double* coef, doubl
   double* partials = (double*)(base + plan.info_bytes);
   short* ws = (short*)(base + plan.info_bytes + plan.partial_bytes);
   ma.skip = MUON ? skip : nullptr;
-  auto sums = [&](Table& t, bool, int) {
+  auto sums = [&](Table& t, int) {
     const int64_t n = tiles_of(t, [](const Mat& m) { return (int64_t)m.parts; });
     k_sumsq<DT, MUON><<<dim3((unsigned)n), 256, 0, s>>>(t, partials, ma);
   };
-  auto norms = [&](Table& t, bool, int at) { k_norms<<<t.n, 64, 0, s>>>(t, partials, info + at, eps, ma.skip); };
-  auto rest = [&](Table& t, bool tall, int at) {
-    const int64_t n = tiles_of(t, [](const Mat& m) {
-      return ceil_div(m.rows8, kNormTile) * ceil_div(m.cols8, kNormTile);
-    });
-    k_cast<DT, MUON><<<dim3((unsigned)n), 256, 0, s>>>(t, ws, info + at, ma);
-    iterate<MUON>(t, tall, ws, info + at, steps, coef, ma, out_dt, s);
+  auto rest = [&](Table& t, int at) {
+    const int64_t n =
+        tiles_of(t, [](const Mat& m) { return ceil_div(m.s, kNormTile) * ceil_div(m.l, kNormTile); });
+    k_cast<DT, MUON><<<dim3((unsigned)n), 256, 0, s>>>(t, ws, partials, info + at, eps, ma);
+    iterate<MUON>(t, ws, info + at, steps, coef, ma, out_dt, s);
   };
   each_run(src, count, sums);
-  each_run(src, count, norms);
+  if (MUON)
+    each_run(src, count, [&](Table& t, int) { k_norms<<<t.n, 64, 0, s>>>(t, partials, eps, skip); });
   each_run(src, count, rest);
   return launch_status(what);
 }
@@ -578,7 +640,7 @@ int64_t dsx_orthogonalize_workspace(const DsxMatrix* mats, int32_t count) {
     src[k].rows = (int32_t)mats[k].rows;
     src[k].cols = (int32_t)mats[k].cols;
   }
-  const Plan plan = each_run(src, count, [](Table&, bool, int) {});
+  const Plan plan = each_run(src, count, [](Table&, int) {});
   delete[] src;
   return plan.info_bytes + plan.partial_bytes + 2 * plan.halves;
 }
