@@ -91,6 +91,12 @@ def __getattr__(name: str):
     if name in ("AdamWOptimizer", "MultiTensorAdamWOptimizer"):
         from . import optimizers as _o
         return getattr(_o, name)
+    if name in ("orthogonalize", "MuonOptimizer"):
+        from . import muon as _m
+        return getattr(_m, name)
+    if name in ("gated_ffn", "gated_residual_norm", "GatedFFNBlock"):
+        from . import block as _b
+        return getattr(_b, name)
     if name in ("DistributedSpeedConfig", "load_config", "fp16_config", "bf16_config", "zero_config"):
         from . import config as _c
         return getattr(_c, name)
@@ -98,5 +104,7 @@ def __getattr__(name: str):
 
 
 __all__ = ["initialize", "is_initialized", "get_config", "get_rank", "get_world_size", "get_local_rank", "destroy",
-           "DistributedSpeedEngine", "ZeROOptimizer", "AdamWOptimizer", "MultiTensorAdamWOptimizer", "DistributedSpeedConfig", "load_config",
+           "DistributedSpeedEngine", "ZeROOptimizer", "AdamWOptimizer", "MultiTensorAdamWOptimizer",
+           "MuonOptimizer", "orthogonalize", "gated_ffn", "gated_residual_norm", "GatedFFNBlock",
+           "DistributedSpeedConfig", "load_config",
            "fp16_config", "bf16_config", "zero_config"]

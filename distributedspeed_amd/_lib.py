@@ -82,6 +82,16 @@ class DsxMatrix(_c.Structure):
                 ("cols", _c.c_int64)]
 
 
+class DsxMuonParam(_c.Structure):
+    _fields_ = [("grad", _P), ("momentum", _P), ("master", _P), ("param16", _P), ("ld_grad", _c.c_int64),
+                ("rows", _c.c_int64), ("cols", _c.c_int64), ("lr", _c.c_float), ("reserved", _c.c_int32)]
+
+
+class DsxMuonHyper(_c.Structure):
+    _fields_ = [("momentum", _c.c_double), ("decay", _c.c_double), ("eps", _c.c_double), ("nesterov", _c.c_int32),
+                ("steps", _c.c_int32)]
+
+
 class DsxFfn(_c.Structure):
     _fields_ = [("x", _P), ("w_gate", _P), ("w_up", _P), ("w_down", _P)] + \
                [(k, _c.c_int64) for k in ("ld_x", "ld_gate", "ld_up", "ld_down", "tokens", "width", "inner")] + \
@@ -98,7 +108,7 @@ class DsxNorm(_c.Structure):
 
 for _s, _n in ((DsxState, 64), (DsxScalerConfig, 32), (DsxAdamwHyper, 56), (DsxStepScalars, 64),
                (DsxTensorRef, 56), (DsxChunk, 24), (DsxGroupsDev, 1112), (DsxFlatPlan, 248),
-               (DsxMatrix, 48), (DsxFfn, 128), (DsxNorm, 104)):
+               (DsxMatrix, 48), (DsxMuonParam, 64), (DsxMuonHyper, 32), (DsxFfn, 128), (DsxNorm, 104)):
     assert _c.sizeof(_s) == _n, (_s.__name__, _c.sizeof(_s))
 
 # name -> (restype, argtypes); every symbol include/dsx.h declares.
@@ -150,6 +160,8 @@ SIGNATURES = {
                                        _P, _c.c_int32, _P, _P]),
     "dsx_orthogonalize_workspace": (_c.c_int64, [_P, _c.c_int32]),
     "dsx_orthogonalize": (_c.c_int, [_P, _c.c_int32, _c.c_int, _c.c_int32, _P, _c.c_double, _P, _c.c_int64, _P]),
+    "dsx_muon_workspace": (_c.c_int64, [_P, _c.c_int32]),
+    "dsx_muon_step": (_c.c_int, [_P, _c.c_int32, _c.c_int, _c.c_int, DsxMuonHyper, _P, _P, _P, _c.c_int64, _P]),
     "dsx_ffn_saved_bytes": (_c.c_int64, [_c.c_int64, _c.c_int64, _c.c_int32]),
     "dsx_ffn_workspace_bytes": (_c.c_int64, [_P, _c.c_int32]),
     "dsx_ffn_forward": (_c.c_int, [_P, _P, _c.c_int64, _P]),

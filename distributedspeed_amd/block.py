@@ -3,6 +3,7 @@
     gated_ffn(x, w_gate, w_up, w_down)            (act(x Wg^T) * (x Wu^T)) Wd^T
     gated_residual_norm(residual, branch, ...)    the norms before and after it,
                                                   with its gate and residual
+    GatedFFNBlock                                 both as a module
 
 Both directions run the library's own kernels on the current stream, without a
 host synchronisation; the gradients work with torch.autograd and so with the
@@ -250,3 +251,37 @@ def gated_residual_norm(residual: torch.Tensor, branch: torch.Tensor | None = No
         hidden = hidden.view(residual.shape)
         normed = None if normed is None else normed.view(residual.shape)
     return hidden, normed
+
+
+class GatedFFNBlock(torch.nn.Module):
+    """One block of a stack: (hidden, normed) -> (hidden, normed), where normed
+    is the block's input and, in turn, the next block's:
+
+        y      = gated_ffn(normed, w_gate, w_up, w_down)
+        hidden = hidden + branch_scale * gate * rms(y) * post_weight
+        normed = rms(hidden) * next_weight
+
+    The stack begins with gated_residual_norm(x, next_weight=...). The gate is
+    a value a channel; w_gate, w_up and w_down are the matrices that Muon
+    steps, the others vectors."""
+
+    def __init__(self, width: int, inner: int, *, activation: str = "silu", branch_scale: float = 1.0,
+                 gate_init: float = 1.0, eps: float = 1e-6, device=None, dtype=None):
+        super().__init__()
+        if activation not in ACTIVATIONS:
+            raise ValueError(f"activation must be one of {sorted(ACTIVATIONS)}, got {activation!r}")
+        self.activation, self.branch_scale, self.eps = activation, float(branch_scale), float(eps)
+        kw = dict(device=device, dtype=dtype)
+
+        def matrix(rows, cols):
+            return torch.nn.Parameter(torch.empty(rows, cols, **kw).normal_(std=cols ** -0.5))
+
+        self.w_gate, self.w_up, self.w_down = matrix(inner, width), matrix(inner, width), matrix(width, inner)
+        self.post_weight = torch.nn.Parameter(torch.ones(width, **kw))
+        self.gate = torch.nn.Parameter(torch.full((width,), float(gate_init), **kw))
+        self.next_weight = torch.nn.Parameter(torch.ones(width, **kw))
+
+    def forward(self, hidden: torch.Tensor, normed: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+        y = gated_ffn(normed, self.w_gate, self.w_up, self.w_down, activation=self.activation)
+        return gated_residual_norm(hidden, y, post_weight=self.post_weight, gate=self.gate,
+                                   next_weight=self.next_weight, branch_scale=self.branch_scale, eps=self.eps)

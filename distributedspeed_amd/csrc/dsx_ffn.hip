@@ -449,6 +449,7 @@ Direct direct_of(const DsxFfn& q, const void* dy, int64_t ld_dy) {
 
 int64_t workspace_of(const DsxFfn& q, bool backward) {
   const Sizes z = sizes_of(q);
+  if (!z.m) return 256;
   // both load forms, so that the size does not hang on addresses
   int64_t part = 0;
   for (int direct = 0; direct < 2; direct++) {

@@ -34,6 +34,7 @@ typedef short    s4v __attribute__((ext_vector_type(4)));
 typedef short    s8v __attribute__((ext_vector_type(8)));
 typedef short    s8u __attribute__((ext_vector_type(8), aligned(2)));  // any element address
 typedef float    f4v __attribute__((ext_vector_type(4)));
+typedef float    f4u __attribute__((ext_vector_type(4), aligned(4)));
 typedef _Float16 h8v __attribute__((ext_vector_type(8)));
 typedef __bf16   b8v __attribute__((ext_vector_type(8)));
 

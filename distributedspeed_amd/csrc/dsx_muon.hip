@@ -19,6 +19,12 @@
 // alone, so a 16-bit input is not rounded at all; the rest of 1 / |G|, the
 // factor r in (1/2, 1], is folded into the first step's sums:
 //   A = X0~ X0~^T / (kScale r)^2,  X1 = (a X0~ + B X0~) / (r kScale).
+// What rounding X adds has full rank, and a X multiplies it by 3.4 in every
+// later step, while a direction that holds something stops growing at 1: a
+// matrix of low rank would end up 14% off. So the iterates before the last two
+// steps keep a second fp16 with what the first lost, which joins in a X (22
+// bits); the products take the first alone, as their noise lies in the
+// matrix's own row space. Rank one, 64 x 64: 1.4e-1 without, 2.7e-3 with it.
 
 #include <hip/hip_runtime.h>
 #include <math.h>
@@ -41,7 +47,7 @@ using dsxi::launch_status;
 using dsxi::round_up;
 
 constexpr float kScale = 4096.0f;
-constexpr int kMats = 24;        // matrices of one launch (the table is a kernel argument)
+constexpr int kMats = 22;        // matrices of one launch (the table is a kernel argument)
 constexpr int kMaxParts = 2048;  // norm partials per matrix
 constexpr int kNormTile = 64;    // the norm and cast kernels' square tile
 
@@ -51,7 +57,7 @@ struct Mat {
   float* momentum;
   float* master;
   int64_t ld_in, ld_out;
-  int64_t x[2], a, b;   // offsets in the workspace, in 16-bit elements
+  int64_t x[2], lo[2], a, b;  // offsets in the workspace, in 16-bit elements
   int32_t rows, cols;   // of the caller's matrix
   int32_t s, l;         // of X: its sides rounded up to multiples of 8, s <= l
   int32_t tall;         // X is the matrix transposed
@@ -199,7 +205,8 @@ __global__ __launch_bounds__(64) void k_norms(Table t, const double* __restrict_
 template <int DT, bool MUON>
 __global__ __launch_bounds__(256) void k_cast(Table t, short* __restrict__ ws, const double* __restrict__ partials,
                                               Info* __restrict__ info, double eps, MuonArgs ma) {
-  __shared__ short turn[kNormTile][kNormTile + 4];
+  constexpr bool LO = MUON || DT == DSX_F32;  // a 16-bit input loses nothing
+  __shared__ short turn[LO ? 2 : 1][kNormTile][kNormTile + 4];
   if (MUON && *ma.skip) return;
   const int i = find(t, blockIdx.x);
   const Mat& m = t.m[i];
@@ -222,23 +229,34 @@ __global__ __launch_bounds__(256) void k_cast(Table t, short* __restrict__ ws, c
           if (c + e < m.cols) m.momentum[(int64_t)r * m.cols + c + e] = buf[e];
       for (int e = 0; e < 4; e++) u[e] = f.bad ? __builtin_nanf("") : c + e < m.cols ? u[e] * f.p : 0.0f;
     }
-    s4v o;
+    s4v o, lo;
 #pragma unroll
-    for (int e = 0; e < 4; e++) o[e] = F16::round(u[e]);
+    for (int e = 0; e < 4; e++) {
+      o[e] = F16::round(u[e]);
+      lo[e] = F16::round(u[e] - F16::widen(o[e]));
+    }
     if (!m.tall) {
-      if (r < m.s && c < m.l) *(s4v*)(ws + m.x[0] + (int64_t)r * m.l + c) = o;
+      if (r < m.s && c < m.l) {
+        *(s4v*)(ws + m.x[0] + (int64_t)r * m.l + c) = o;
+        if (LO) *(s4v*)(ws + m.lo[0] + (int64_t)r * m.l + c) = lo;
+      }
     } else {
 #pragma unroll
-      for (int e = 0; e < 4; e++) turn[(tid & 15) * 4 + e][(tid >> 4) + 16 * k] = o[e];
+      for (int e = 0; e < 4; e++) {
+        turn[0][(tid & 15) * 4 + e][(tid >> 4) + 16 * k] = o[e];
+        if (LO) turn[LO ? 1 : 0][(tid & 15) * 4 + e][(tid >> 4) + 16 * k] = lo[e];
+      }
     }
   }
   if (!m.tall) return;
   __syncthreads();
 #pragma unroll
   for (int k = 0; k < 4; k++) {
-    const int r = xr + (tid >> 4) + 16 * k, q = xc + (tid & 15) * 4;
-    if (r < m.s && q < m.l)
-      *(s4v*)(ws + m.x[0] + (int64_t)r * m.l + q) = *(const s4v*)&turn[(tid >> 4) + 16 * k][(tid & 15) * 4];
+    const int r = (tid >> 4) + 16 * k, q = (tid & 15) * 4;
+    if (xr + r >= m.s || xc + q >= m.l) continue;
+    const int64_t at = (int64_t)(xr + r) * m.l + xc + q;
+    *(s4v*)(ws + m.x[0] + at) = *(const s4v*)&turn[0][r][q];
+    if (LO) *(s4v*)(ws + m.lo[0] + at) = *(const s4v*)&turn[LO ? 1 : 0][r][q];
   }
 }
 
@@ -305,17 +323,46 @@ __global__ DSX_TILE_KERNEL(G) void k_symmetric(Table t, short* __restrict__ ws, 
     g.template emit<true>(lds, pre, put, mirror);
 }
 
-// Muon's update of `n` <= 16 parameters: w = w decay - lr O (v holds kScale O).
+// Muon's update of N parameters of a row: w = w decay - lr O (v holds kScale O).
 template <int N>
 __device__ inline void step_params(const Mat& m, const MuonArgs& ma, int out_dt, int64_t r, int c, const float* v) {
   float* w = m.master + r * m.cols + c;
   short* o = (short*)m.out + r * m.ld_out + c;
 #pragma unroll
-  for (int e = 0; e < N; e++) {
-    if (c + e >= m.cols) break;
-    const float n = fmaf(-m.lr * (1.0f / kScale), v[e], w[e] * ma.decay);
-    w[e] = n;
-    if (out_dt) o[e] = out_dt == DSX_F16 ? F16::round(n) : BF16::round(n);
+  for (int h = 0; h < N; h += 8) {
+    const int left = m.cols - c - h;
+    if (left <= 0) continue;
+    float p[8];
+    s8v q;
+    if (left >= 8) {
+      const f4v lo = *(const f4u*)(w + h), hi = *(const f4u*)(w + h + 4);
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        p[e] = lo[e];
+        p[e + 4] = hi[e];
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; e++) p[e] = e < left ? w[h + e] : 0.0f;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      p[e] = fmaf(-m.lr * (1.0f / kScale), v[h + e], p[e] * ma.decay);
+      asm("" : "+v"(p[e]));  // the cast is of the rounded master, not of the exact sum (a fused add and cast)
+      q[e] = out_dt == DSX_F16 ? F16::round(p[e]) : BF16::round(p[e]);
+    }
+    if (left >= 8) {
+      *(f4u*)(w + h) = f4v{p[0], p[1], p[2], p[3]};
+      *(f4u*)(w + h + 4) = f4v{p[4], p[5], p[6], p[7]};
+      if (m.out) *(s8u*)(o + h) = q;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; e++)
+        if (e < left) {
+          w[h + e] = p[e];
+          if (m.out) o[h + e] = q[e];
+        }
+    }
   }
 }
 // N values of a row of the result in bf16 (v holds kScale O).
@@ -337,10 +384,14 @@ __device__ inline void store_row(const Mat& m, int64_t r, int c, const float* v)
 
 // X <- (a X + B X) / r. LAST: the result itself, transposed back where the
 // matrix was, to the output in bf16 or as Muon's parameter update (fp32 master
-// and 16-bit copy of out_dt, 0 for none).
+// and, where there is one, its 16-bit copy of out_dt). take_lo, give_lo: whether
+// the iterate read and the one written have their second fp16.
+struct XRaw {
+  s8v hi, lo;
+};
 template <class G, bool LAST, bool MUON>
 __global__ DSX_TILE_KERNEL(G) void k_apply(Table t, short* __restrict__ ws, const Info* __restrict__ info, int cur,
-                                           int first, float a, MuonArgs ma, int out_dt) {
+                                           int first, float a, int take_lo, int give_lo, MuonArgs ma, int out_dt) {
   __shared__ __attribute__((aligned(1024))) char lds[G::kLds];
   if (MUON && *ma.skip) return;
   const int bid = xcd_order(blockIdx.x, gridDim.x);
@@ -351,7 +402,9 @@ __global__ DSX_TILE_KERNEL(G) void k_apply(Table t, short* __restrict__ ws, cons
   band_order(bid - t.tile0[i], (s + G::TM - 1) / G::TM, (l + G::TN - 1) / G::TN, 8, &ti, &tj);
   const float inv_r = first ? info[i].inv_r : 1.0f;
   const short* x = ws + m.x[cur];
+  const short* x_lo = ws + m.lo[cur];
   short* y = ws + m.x[cur ^ 1];
+  short* y_lo = ws + m.lo[cur ^ 1];
   const Operand ob{ws + m.b, s, s}, ox{x, l, l};
   const int r0 = ti * G::TM, c0 = tj * G::TN;
   G g;
@@ -360,30 +413,43 @@ __global__ DSX_TILE_KERNEL(G) void k_apply(Table t, short* __restrict__ ws, cons
   auto pre = [&](int r, int c) {
     r += r0;
     c += c0;
-    return r >= s || c >= l ? s8v{} : *(const s8v*)(x + (int64_t)r * l + c);
+    XRaw raw{};
+    if (r < s && c < l) {
+      const int64_t at = (int64_t)r * l + c;
+      raw.hi = *(const s8v*)(x + at);
+      if (take_lo) raw.lo = *(const s8v*)(x_lo + at);
+    }
+    return raw;
   };
-  auto value = [&](float* v, const s8v& old) {
+  auto value = [&](float* v, const XRaw& old) {
 #pragma unroll
-    for (int e = 0; e < 8; e++) v[e] = fmaf(a, F16::widen(old[e]), v[e] * (1.0f / kScale)) * inv_r;
+    for (int e = 0; e < 8; e++)
+      v[e] = fmaf(a, F16::widen(old.hi[e]) + F16::widen(old.lo[e]), v[e] * (1.0f / kScale)) * inv_r;
   };
   auto none = [](int, int, const float*) {};
   if (!LAST) {
     g.template emit<false>(
         lds, pre,
-        [&](int r, int c, float* v, float*, const s8v& old) {
+        [&](int r, int c, float* v, float*, const XRaw& old) {
           value(v, old);
-          s8v w;
+          s8v w, lo;
 #pragma unroll
-          for (int e = 0; e < 8; e++) w[e] = F16::round(v[e]);
+          for (int e = 0; e < 8; e++) {
+            w[e] = F16::round(v[e]);
+            lo[e] = F16::round(v[e] - F16::widen(w[e]));
+          }
           r += r0;
           c += c0;
-          if (r < s && c < l) *(s8v*)(y + (int64_t)r * l + c) = w;
+          if (r >= s || c >= l) return;
+          const int64_t at = (int64_t)r * l + c;
+          *(s8v*)(y + at) = w;
+          if (give_lo) *(s8v*)(y_lo + at) = lo;
         },
         none);
   } else if (!m.tall) {
     g.template emit<false>(
         lds, pre,
-        [&](int r, int c, float* v, float*, const s8v& old) {
+        [&](int r, int c, float* v, float*, const XRaw& old) {
           value(v, old);
           r += r0;
           c += c0;
@@ -394,7 +460,7 @@ __global__ DSX_TILE_KERNEL(G) void k_apply(Table t, short* __restrict__ ws, cons
         none);
   } else {
     g.template emit<true>(
-        lds, pre, [&](int, int, float* v, float*, const s8v& old) { value(v, old); },
+        lds, pre, [&](int, int, float* v, float*, const XRaw& old) { value(v, old); },
         [&](int r, int c, const float* v) {  // a column of X is a row of the matrix
           r += c0;
           c += r0;
@@ -471,7 +537,9 @@ Plan each_run(const Source* src, int32_t count, F&& f) {
     const int64_t x = round_up((int64_t)m.s * m.l, 128), sq = round_up((int64_t)m.s * m.s, 128);
     m.x[0] = at;
     m.x[1] = at + x;
-    m.a = at + 2 * x;
+    m.lo[0] = at + 2 * x;
+    m.lo[1] = at + 3 * x;
+    m.a = at + 4 * x;
     m.b = m.a + sq;
     at = m.b + sq;
     m.parts = parts_of(q.rows, q.cols);
@@ -508,56 +576,48 @@ void launch_symmetric(Table& t, short* ws, const Info* info, int cur, int first,
 }
 
 template <class G, bool MUON>
-void launch_apply(Table& t, short* ws, const Info* info, int cur, int first, bool last, float a, const MuonArgs& ma,
-                  int out_dt, hipStream_t s) {
+void launch_apply(Table& t, short* ws, const Info* info, int cur, int first, bool last, float a, int take_lo,
+                  int give_lo, const MuonArgs& ma, int out_dt, hipStream_t s) {
   const int64_t n = tiles_of(t, [](const Mat& m) { return ceil_div(m.s, G::TM) * ceil_div(m.l, G::TN); });
   if (last)
-    k_apply<G, true, MUON><<<dim3((unsigned)n), G::THREADS, 0, s>>>(t, ws, info, cur, first, a, ma, out_dt);
+    k_apply<G, true, MUON><<<dim3((unsigned)n), G::THREADS, 0, s>>>(t, ws, info, cur, first, a, take_lo, give_lo, ma, out_dt);
   else
-    k_apply<G, false, false><<<dim3((unsigned)n), G::THREADS, 0, s>>>(t, ws, info, cur, first, a, ma, out_dt);
+    k_apply<G, false, false><<<dim3((unsigned)n), G::THREADS, 0, s>>>(t, ws, info, cur, first, a, take_lo, give_lo, ma, out_dt);
 }
 
-// The square tile of a launch. A CU runs one block of 256 or 192 at a time, or
-// two of 128, whose products take 1.2 times as long for the same area (a lone
-// block of 128 on a CU: 1.4 times); the rounds over the CUs decide. (The Gram
-// matrix of 4096 x 14336: 136, 253 and 528 tiles, of which only the 192s fill
-// the chip once and no more: 370, 327 and 520 us.)
+// The square tile of a launch. Few tiles are bound by the latency of a K tile,
+// not by products: 64-tiles while three a CU cover the launch (one 1001 x 2731:
+// 281 us with 64-tiles, 385 with 128; one 1024^2: 195 and 251; beyond it, as
+// for twelve 768^2, 308 and 297). Else a CU runs one block of 256 or 192 at a
+// time or two of 128, whose products take 1.2 times as long for the same area
+// (a lone block of 128 on a CU: 1.4 times), and the rounds over the CUs decide.
+// (The Gram matrix of 4096 x 14336: 136, 253 and 528 tiles, of which only the
+// 192s fill the chip once and no more: 370, 247 and 520 us.)
 int tile_of(const Table& t, bool triangle) {
-#ifdef FORCE_TILE
-  return FORCE_TILE;
-#endif
-  const int64_t cus = 256, size[3] = {256, 192, 128};
-  int best = 0;
-  int64_t least = INT64_MAX;
-  for (int k = 0; k < 3; k++) {
-    int64_t n = 0;
+  const int64_t cus = 256, size[4] = {256, 192, 128, 64};
+  int64_t n[4] = {0, 0, 0, 0};
+  for (int k = 0; k < 4; k++)
     for (int i = 0; i < t.n; i++) {
       const int64_t a = ceil_div(t.m[i].s, size[k]), b = ceil_div(t.m[i].l, size[k]);
-      n += triangle ? a * (a + 1) / 2 : a * b;
+      n[k] += triangle ? a * (a + 1) / 2 : a * b;
     }
-    int64_t cost;
-    if (size[k] > 128) {
-      cost = ceil_div(n, cus) * size[k] * size[k] * (size[k] == 256 ? 10 : 12);
-    } else {
-      const int64_t rest = n % (2 * cus);
-      cost = (n / (2 * cus) * 24 + (rest > cus ? 24 : rest ? 14 : 0)) * 128 * 128;
-    }
-    if (cost < least) {
-      least = cost;
-      best = k;
-    }
-  }
-  return (int)size[best];
+  if (n[3] <= 3 * cus) return 64;
+  const int64_t rest = n[2] % (2 * cus);
+  const int64_t cost[3] = {ceil_div(n[0], cus) * 256 * 256 * 10, ceil_div(n[1], cus) * 192 * 192 * 12,
+                           (n[2] / (2 * cus) * 24 + (rest > cus ? 24 : rest ? 14 : 0)) * 128 * 128};
+  const int k = cost[0] <= cost[1] ? (cost[0] <= cost[2] ? 0 : 2) : (cost[1] <= cost[2] ? 1 : 2);
+  return (int)size[k];
 }
 
 template <bool MUON>
-void iterate(Table& t, short* ws, const Info* info, int steps, const double* coef, const MuonArgs& ma, int out_dt,
-             hipStream_t s) {
+void iterate(Table& t, short* ws, const Info* info, int steps, const double* coef, bool input_lo, const MuonArgs& ma,
+             int out_dt, hipStream_t s) {
   const int sym = tile_of(t, true), app = tile_of(t, false);
   const int32_t* skip = MUON ? ma.skip : nullptr;
   for (int k = 0; k < steps; k++) {
     const float a = (float)coef[3 * k], b = (float)coef[3 * k + 1], c = (float)coef[3 * k + 2];
     const int cur = k & 1, first = k == 0, last = k == steps - 1;
+    auto lo = [&](int i) { return i < steps - 2 && (i || input_lo); };
 #define DSX_BY_TILE(TILE, F, RB, ...)             \
   do {                                            \
     if (TILE == 256) F<Big<RB>, __VA_ARGS__;      \
@@ -567,7 +627,7 @@ void iterate(Table& t, short* ws, const Info* info, int steps, const double* coe
   } while (0)
     DSX_BY_TILE(sym, launch_symmetric, true, true>(t, ws, info, cur, first, b, c, skip, s));
     DSX_BY_TILE(sym, launch_symmetric, true, false>(t, ws, info, cur, first, b, c, skip, s));
-    DSX_BY_TILE(app, launch_apply, false, MUON>(t, ws, info, cur, first, last, a, ma, out_dt, s));
+    DSX_BY_TILE(app, launch_apply, false, MUON>(t, ws, info, cur, first, last, a, lo(k), lo(k + 1), ma, out_dt, s));
 #undef DSX_BY_TILE
   }
 }
@@ -593,7 +653,7 @@ int drive(const Source* src, int32_t count, int steps, const double* coef, doubl
     const int64_t n =
         tiles_of(t, [](const Mat& m) { return ceil_div(m.s, kNormTile) * ceil_div(m.l, kNormTile); });
     k_cast<DT, MUON><<<dim3((unsigned)n), 256, 0, s>>>(t, ws, partials, info + at, eps, ma);
-    iterate<MUON>(t, ws, info + at, steps, coef, ma, out_dt, s);
+    iterate<MUON>(t, ws, info + at, steps, coef, MUON || DT == DSX_F32, ma, out_dt, s);
   };
   each_run(src, count, sums);
   if (MUON)
@@ -679,6 +739,78 @@ int dsx_orthogonalize(const DsxMatrix* mats, int32_t count, int dtype, int32_t s
       rc = drive<DSX_F16, false>(src, count, steps, coefficients, eps, ma, DSX_BF16, base, workspace_bytes, what, s);
     else
       rc = drive<DSX_BF16, false>(src, count, steps, coefficients, eps, ma, DSX_BF16, base, workspace_bytes, what, s);
+  }
+  delete[] src;
+  return rc;
+}
+
+
+int64_t dsx_muon_workspace(const DsxMuonParam* params, int32_t count) {
+  if (count < 0 || count > kMaxList || (count && !params)) return fail(-1, "dsx_muon_workspace: bad list");
+  Source* src = new (std::nothrow) Source[count ? count : 1];
+  if (!src) return fail(-1, "dsx_muon_workspace: out of memory");
+  for (int32_t k = 0; k < count; k++) {
+    if (check_shape("dsx_muon_workspace", k, params[k].rows, params[k].cols)) {
+      delete[] src;
+      return -1;
+    }
+    src[k] = Source{};
+    src[k].rows = (int32_t)params[k].rows;
+    src[k].cols = (int32_t)params[k].cols;
+  }
+  const Plan plan = each_run(src, count, [](Table&, int) {});
+  delete[] src;
+  return plan.info_bytes + plan.partial_bytes + 2 * plan.halves;
+}
+
+int dsx_muon_step(const DsxMuonParam* params, int32_t count, int grad_dtype, int param_dtype, DsxMuonHyper hyper,
+                  const float* grad_scale, const double* coefficients, void* workspace, int64_t workspace_bytes,
+                  void* stream) {
+  const char* what = "dsx_muon_step";
+  if (count > kMaxList) return fail(DSX_EINVAL, "%s: at most %d matrices", what, kMaxList);
+  if (int rc = check_common(what, count, hyper.steps, coefficients, hyper.eps, workspace)) return rc;
+  if (count && !params) return fail(DSX_EINVAL, "%s: params is NULL", what);
+  if (grad_dtype != DSX_F32 && !dsxi::is16(grad_dtype)) return fail(DSX_EINVAL, "%s: bad grad dtype", what);
+  if (!dsxi::is16(param_dtype)) return fail(DSX_EINVAL, "%s: bad param dtype", what);
+  if (!(hyper.momentum >= 0.0 && hyper.momentum < 1.0)) return fail(DSX_EINVAL, "%s: momentum in [0, 1)", what);
+  if (!(hyper.decay >= 0.0 && hyper.decay <= 1.0)) return fail(DSX_EINVAL, "%s: decay in [0, 1]", what);
+  if ((uintptr_t)grad_scale & 3) return fail(DSX_EINVAL, "%s: misaligned grad_scale", what);
+  Source* src = new (std::nothrow) Source[count ? count : 1];
+  if (!src) return fail(DSX_EINVAL, "%s: out of memory", what);
+  int rc = DSX_OK;
+  const uintptr_t unit = grad_dtype == DSX_F32 ? 3 : 1;
+  for (int32_t k = 0; k < count && !rc; k++) {
+    const DsxMuonParam& q = params[k];
+    src[k] = Source{};
+    rc = check_shape(what, k, q.rows, q.cols);
+    if (rc || !q.rows || !q.cols) continue;
+    if (!q.grad || !q.momentum || !q.master || ((uintptr_t)q.grad & unit) || ((uintptr_t)q.momentum & 15) ||
+        ((uintptr_t)q.master & 15) || ((uintptr_t)q.param16 & 1))
+      rc = fail(DSX_EINVAL, "%s: matrix %d has a NULL or misaligned pointer", what, (int)k);
+    else if (q.ld_grad < q.cols)
+      rc = fail(DSX_EINVAL, "%s: matrix %d has a row stride below its columns", what, (int)k);
+    else if (!isfinite(q.lr))
+      rc = fail(DSX_EINVAL, "%s: matrix %d has a step size that is not finite", what, (int)k);
+    src[k] = Source{q.grad, q.param16, q.momentum, q.master, q.ld_grad, q.cols, (int32_t)q.rows, (int32_t)q.cols,
+                    q.lr};
+  }
+  if (!rc) {
+    MuonArgs ma{};
+    ma.grad_scale = grad_scale;
+    ma.momentum = (float)hyper.momentum;
+    ma.decay = (float)hyper.decay;
+    ma.nesterov = hyper.nesterov;
+    char* base = (char*)workspace;
+    hipStream_t s = as_stream(stream);
+    if (grad_dtype == DSX_F32)
+      rc = drive<DSX_F32, true>(src, count, hyper.steps, coefficients, hyper.eps, ma, param_dtype, base,
+                                workspace_bytes, what, s);
+    else if (grad_dtype == DSX_F16)
+      rc = drive<DSX_F16, true>(src, count, hyper.steps, coefficients, hyper.eps, ma, param_dtype, base,
+                                workspace_bytes, what, s);
+    else
+      rc = drive<DSX_BF16, true>(src, count, hyper.steps, coefficients, hyper.eps, ma, param_dtype, base,
+                                 workspace_bytes, what, s);
   }
   delete[] src;
   return rc;

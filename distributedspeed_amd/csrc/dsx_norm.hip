@@ -42,8 +42,6 @@ using dsxi::fail;
 using dsxi::launch_status;
 using dsxi::round_up;
 
-typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
-
 constexpr int kWidest = 8192;  // of a row kept in registers: 1024 threads of eight elements
 
 struct Args {
@@ -563,7 +561,7 @@ int check(const char* what, const DsxNorm* q) {
   if (q->dtype != DSX_F32 && !dsxi::is16(q->dtype)) return fail(DSX_EINVAL, "%s: bad dtype %d", what, q->dtype);
   if (q->rows < 0 || q->rows > DSX_NORM_MAX_ROWS || q->width < 1 || q->width > DSX_MATRIX_MAX_DIM)
     return fail(DSX_EINVAL, "%s: rows in [0, %d], width in [1, %d]", what, DSX_NORM_MAX_ROWS, DSX_MATRIX_MAX_DIM);
-  if (!q->branch && (q->post_weight || q->gate))
+  if (q->rows && !q->branch && (q->post_weight || q->gate))
     return fail(DSX_EINVAL, "%s: a weight or gate of a branch that is NULL", what);
   if (q->gate && (q->gate_rows < 1 || q->gate_rows > 65533 || (q->rows && q->rows % q->gate_rows)))
     return fail(DSX_EINVAL, "%s: gate_rows must divide rows and lie in [1, 65533]", what);

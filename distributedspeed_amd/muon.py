@@ -2,6 +2,7 @@
 optimizer built on it.
 
     orthogonalize(updates)     the orthogonalised matrices, in bf16
+    MuonOptimizer(params)      the optimizer, for the matrices of a model
 
 For a matrix G with singular value decomposition U S V^T the iteration drives
 every singular value of G / |G| towards 1 without computing the decomposition:
@@ -18,7 +19,7 @@ from typing import Sequence
 import torch
 
 from . import _lib, ops
-from ._lib import DsxMatrix
+from ._lib import DsxMatrix, DsxMuonHyper, DsxMuonParam
 
 NS_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 
@@ -131,3 +132,140 @@ def orthogonalize(updates: torch.Tensor | Sequence[torch.Tensor], *, steps: int 
         _lib.call("dsx_orthogonalize", table, len(ms), code, steps, coef, eps, ops._ptr(work), nbytes,
                   ops.stream_of(dev))
     return result
+
+
+class MuonOptimizer(torch.optim.Optimizer):
+    """Muon for matrix parameters, with torch.optim.Muon's arguments:
+
+        buf = momentum * buf + (1 - momentum) * grad
+        u   = momentum * buf + (1 - momentum) * grad   (nesterov; else buf)
+        w   = w * (1 - lr * weight_decay) - lr * factor * orthogonalize(u)
+
+    where factor is sqrt(max(1, rows / cols)) for adjust_lr "original" and
+    0.2 * sqrt(max(rows, cols)) for "match_rms_adamw", which lets AdamW's
+    learning rate and weight decay carry over. Parameters are 2-D and
+    contiguous; fp16 and bf16 ones get an fp32 master (state[p]["master"])
+    that the step updates and rounds to the parameter, in the launch that
+    forms the last Newton-Schulz product: the orthogonalised update is never
+    written to memory. Vectors, embeddings and output heads belong to another
+    optimizer (AdamWOptimizer).
+
+    step(grad_scale=...) divides the grads by a one-element fp32 device tensor
+    (AdamWOptimizer.loss_scale_tensor()). A grad that is not finite skips the
+    step of its param group (and type): nothing of it changes, and
+    last_step_skipped() says so. Nothing here synchronises the host with the
+    device."""
+
+    def __init__(self, params, lr: float = 1e-3, weight_decay: float = 0.1, momentum: float = 0.95,
+                 nesterov: bool = True, ns_coefficients=NS_COEFFICIENTS, eps: float = 1e-7, ns_steps: int = 5,
+                 adjust_lr: str = "original"):
+        if not 0.0 <= lr or not math.isfinite(lr):
+            raise ValueError(f"Invalid learning rate: {lr}")
+        if not 0.0 <= weight_decay:
+            raise ValueError(f"Invalid weight_decay value: {weight_decay}")
+        if not 0.0 <= momentum < 1.0:
+            raise ValueError(f"Invalid momentum value: {momentum}")
+        if adjust_lr not in ("original", "match_rms_adamw"):
+            raise ValueError(f"adjust_lr must be 'original' or 'match_rms_adamw', got {adjust_lr!r}")
+        ns_steps, eps = _check_ns(ns_steps, eps)
+        _coefficients(ns_coefficients, ns_steps)
+        super().__init__(params, dict(lr=lr, weight_decay=weight_decay, momentum=momentum, nesterov=bool(nesterov),
+                                      ns_coefficients=ns_coefficients, eps=eps, ns_steps=ns_steps,
+                                      adjust_lr=adjust_lr))
+        self._skips: list[torch.Tensor] = []
+
+    def add_param_group(self, param_group: dict) -> None:
+        super().add_param_group(param_group)
+        for p in self.param_groups[-1]["params"]:
+            ops._device(p)
+            ops.grad_code(p.dtype)
+            if p.dim() != 2:
+                raise ValueError(f"Muon steps matrices; got a parameter of shape {tuple(p.shape)}")
+            if not p.is_contiguous():
+                raise ValueError("Muon's parameters must be contiguous")
+
+    def _state_of(self, p: torch.Tensor) -> dict:
+        st = self.state[p]
+        if not st:
+            st["momentum_buffer"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
+            if p.dtype != torch.float32:
+                st["master"] = p.detach().float()
+        return st
+
+    def refresh_master(self) -> None:
+        """Take the fp32 masters from the current params (after they were
+        written from outside the step, as by a module's load_state_dict)."""
+        for p, st in self.state.items():
+            if "master" in st:
+                st["master"].copy_(p.detach())
+
+    @torch.no_grad()
+    def step(self, closure=None, *, grad_scale: torch.Tensor | None = None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        if grad_scale is not None and (not isinstance(grad_scale, torch.Tensor) or grad_scale.numel() != 1
+                                       or grad_scale.dtype != torch.float32 or not grad_scale.is_cuda):
+            raise ValueError("grad_scale must be a one-element float32 tensor on the GPU")
+        self._skips = []
+        for g in self.param_groups:
+            lists: dict[tuple, list[torch.Tensor]] = {}
+            for p in g["params"]:
+                if p.grad is None:
+                    continue
+                if p.grad.is_sparse:
+                    raise RuntimeError("Muon does not support sparse gradients")
+                lists.setdefault((p.device, p.grad.dtype, p.dtype), []).append(p)
+            for (dev, gdt, pdt), ps in lists.items():
+                self._step_list(g, dev, gdt, pdt, ps, grad_scale)
+        return loss
+
+    def _step_list(self, g: dict, dev, gdt, pdt, ps: list, grad_scale) -> None:
+        lr, steps = float(g["lr"]), int(g["ns_steps"])
+        decay = 1.0 - lr * g["weight_decay"]
+        if not 0.0 <= decay <= 1.0:
+            raise ValueError(f"lr * weight_decay must be in [0, 1], got {lr * g['weight_decay']}")
+        table = (DsxMuonParam * len(ps))()
+        grads = [_rows_contiguous(p.grad) for p in ps]
+        for q, p, gr in zip(table, ps, grads):
+            if not p.is_contiguous():
+                raise ValueError("Muon's parameters must be contiguous")
+            st = self._state_of(p)
+            rows, cols = p.shape
+            factor = (0.2 * math.sqrt(max(rows, cols)) if g["adjust_lr"] == "match_rms_adamw"
+                      else math.sqrt(max(1.0, rows / cols)) if cols else 1.0)
+            q.grad, q.momentum = gr.data_ptr(), st["momentum_buffer"].data_ptr()
+            if "master" in st:
+                q.master, q.param16 = st["master"].data_ptr(), p.data_ptr()
+            else:
+                q.master = p.data_ptr()
+            q.ld_grad, q.rows, q.cols, q.lr = _row_stride(gr), rows, cols, lr * factor
+        coef = (ctypes.c_double * (3 * steps))(*(v for r in _coefficients(g["ns_coefficients"], steps) for v in r))
+        hyper = DsxMuonHyper(float(g["momentum"]), decay, float(g["eps"]), int(g["nesterov"]), steps)
+        nbytes = _lib.load().dsx_muon_workspace(table, len(ps))
+        if nbytes < 0:
+            raise ValueError(_lib.last_error())
+        with torch.cuda.device(dev):
+            work = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+            skip = work[:4].view(torch.int32)
+            _lib.call("dsx_muon_step", table, len(ps), ops.grad_code(gdt),
+                      ops.dtype_code(torch.float16 if pdt == torch.float32 else pdt), hyper, ops._ptr(grad_scale), coef,
+                      ops._ptr(work), nbytes, ops.stream_of(dev))
+            self._skips.append(skip.clone())
+
+    def last_step_skipped(self) -> bool:
+        """Whether any part of the last step was skipped (synchronises)."""
+        return any(bool(s.item()) for s in self._skips)
+
+    def load_state_dict(self, state_dict: dict) -> None:
+        """torch's, but the fp32 state stays fp32 for 16-bit parameters."""
+        super().load_state_dict(state_dict)
+        saved = state_dict["state"]
+        index = 0
+        for g in self.param_groups:
+            for p in g["params"]:
+                for key, value in saved.get(index, {}).items():
+                    if isinstance(value, torch.Tensor):
+                        self.state[p][key] = value.detach().to(device=p.device, dtype=torch.float32, copy=True)
+                index += 1

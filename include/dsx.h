@@ -628,6 +628,48 @@ int dsx_orthogonalize(const DsxMatrix* mats /* host */, int32_t count,
                       const double* coefficients /* host */, double eps,
                       void* workspace, int64_t workspace_bytes, void* stream);
 
+/* One matrix parameter of a Muon step (a host array), all contiguous but the
+ * grad (row stride ld_grad): momentum and master fp32, 16-byte aligned,
+ * param16 (may be NULL) of the call's param dtype. lr is the step size of this
+ * matrix, any factor of its shape included. */
+typedef struct DsxMuonParam {
+  const void* grad;
+  float*      momentum;
+  float*      master;
+  void*       param16;
+  int64_t     ld_grad;
+  int64_t     rows;
+  int64_t     cols;
+  float       lr;
+  int32_t     reserved;
+} DsxMuonParam;
+
+typedef struct DsxMuonHyper {
+  double  momentum;  /* mu, in [0, 1)                                        */
+  double  decay;     /* 1 - lr * weight_decay, in [0, 1]                     */
+  double  eps;       /* added to the norm                                    */
+  int32_t nesterov;
+  int32_t steps;     /* Newton-Schulz steps                                  */
+} DsxMuonHyper;
+
+/* Bytes of device scratch for the list; -1 with dsx_last_error. Host only. */
+int64_t dsx_muon_workspace(const DsxMuonParam* params /* host */,
+                           int32_t count);
+
+/* One Muon step over the list, with g = grad / *grad_scale (a device float;
+ * NULL: 1):
+ *   buf = mu buf + (1 - mu) g
+ *   u   = mu buf + (1 - mu) g  with nesterov, else buf
+ *   O   = the Newton-Schulz iterate of u (as dsx_orthogonalize, unrounded)
+ *   w   = w decay - lr O;  param16 = round_to_nearest_even(w)
+ * If any matrix's u has a norm that is not finite (an overflowed grad), the
+ * whole step does nothing. The first 4 bytes of the workspace then hold 1, else
+ * 0. No counterpart in the reference. */
+int dsx_muon_step(const DsxMuonParam* params /* host */, int32_t count,
+                  int grad_dtype, int param_dtype, DsxMuonHyper hyper,
+                  const float* grad_scale, const double* coefficients /* host */,
+                  void* workspace, int64_t workspace_bytes, void* stream);
+
 /* ---- the gated feed-forward block ------------------------------------- */
 
 /* activations */
