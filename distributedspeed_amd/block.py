@@ -11,20 +11,44 @@ optimizers of this package.
 """
 from __future__ import annotations
 
-import ctypes
+import struct
 
 import torch
 
 from . import _lib, ops
-from ._lib import DsxFfn, DsxNorm
 
 ACTIVATIONS = {"silu": 0, "gelu": 1, "gelu_tanh": 2, "relu": 3}
+
+# The argument blocks as bytes (DsxFfn and DsxNorm of include/dsx.h). These
+# calls are a few microseconds of GPU time each for small inputs, so their host
+# side is kept short: a block is packed once, the library's functions are bound
+# once, and the autograd thread's part reuses what the forward worked out.
+_FFN = struct.Struct("=4Q7q4i2Qq")
+_NORM = struct.Struct("=5Q5qi3fQ")
+
+
+class _Bound:
+    """The library's functions, bound at first use."""
+
+    def __getattr__(self, name: str):
+        fn = getattr(_lib.load(), name)
+        setattr(self, name, fn)
+        return fn
+
+
+_bound = _Bound()
+
+
+def _raise(name: str, rc: int) -> None:
+    raise _lib.DsxError(name, rc, _lib.last_error())
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """t [n, d], or a copy where its columns are not adjacent or its rows overlap."""
-    n, d = t.shape
-    if (d > 1 and t.stride(1) != 1) or (n > 1 and t.stride(0) < d):
+    if t.is_contiguous():
+        return t
+    (n, d), (row, col) = t.shape, t.stride()
+    if (d > 1 and col != 1) or (n > 1 and row < d):
         return t.contiguous()
     return t
 
@@ -33,59 +57,91 @@ def _ld(t: torch.Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
-def _describe(x, w_gate, w_up, w_down, activation: int, keep: bool) -> DsxFfn:
-    f, d = w_gate.shape
-    return DsxFfn(x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(), _ld(x), _ld(w_gate), _ld(w_up),
-                  _ld(w_down), x.shape[0], d, f, ops.dtype_code(x.dtype), activation, int(keep), 0, None, None, 0)
-
-
 def _scratch(nbytes: int, device: torch.device) -> torch.Tensor:
     if nbytes < 0:
         raise ValueError(_lib.last_error())
     return torch.empty(nbytes, dtype=torch.uint8, device=device)
 
 
-def _forward(x, w_gate, w_up, w_down, activation: int, keep: bool):
+def _on(device: torch.device, run, *args):
+    """run(*args) with `device` current."""
+    if torch.cuda.current_device() == device.index:
+        return run(*args)
+    with torch.cuda.device(device):
+        return run(*args)
+
+
+def _refuse(name: str, t, first: torch.Tensor, optional: bool = False) -> None:
+    """Why t cannot go with `first`."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a tensor" + (" or None" if optional else ""))
+    if t.device != first.device:
+        raise ValueError(f"{name} is on {t.device}, expected {first.device}")
+    raise TypeError(f"{name} must be {first.dtype}, got {t.dtype}")
+
+
+# ---- the gated feed-forward block ----------------------------------------------------------------
+
+def _pack_ffn(x, w_gate, w_up, w_down, activation: int, keep: bool, saved: int, work: int, nbytes: int) -> bytes:
+    f, d = w_gate.shape
+    return _FFN.pack(x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(), _ld(x), _ld(w_gate),
+                     _ld(w_up), _ld(w_down), x.shape[0], d, f, ops.dtype_code(x.dtype), activation, keep, 0, saved,
+                     work, nbytes)
+
+
+def _ffn_forward(x, w_gate, w_up, w_down, activation: int, keep: bool):
     """y, and the buffer the forward kept; x [tokens, width] and the weights row-contiguous."""
-    lib, dev = _lib.load(), x.device
-    tokens, inner = x.shape[0], w_gate.shape[0]
-    y = torch.empty_like(x, memory_format=torch.contiguous_format)
-    q = _describe(x, w_gate, w_up, w_down, activation, keep)
-    with torch.cuda.device(dev):
-        saved = _scratch(lib.dsx_ffn_saved_bytes(tokens, inner, int(keep)), dev)
-        work = _scratch(lib.dsx_ffn_workspace_bytes(ctypes.byref(q), 0), dev)
-        q.saved, q.workspace, q.workspace_bytes = saved.data_ptr(), work.data_ptr(), work.numel()
-        _lib.call("dsx_ffn_forward", ctypes.byref(q), ops._ptr(y), y.shape[1], ops.stream_of(dev))
+    dev = x.device
+    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    saved = _scratch(_bound.dsx_ffn_saved_bytes(x.shape[0], w_gate.shape[0], keep), dev)
+    nbytes = _bound.dsx_ffn_workspace_bytes(_pack_ffn(x, w_gate, w_up, w_down, activation, keep, 0, 0, 0), 0)
+    work = _scratch(nbytes, dev)
+    q = _pack_ffn(x, w_gate, w_up, w_down, activation, keep, saved.data_ptr(), work.data_ptr(), nbytes)
+    rc = _bound.dsx_ffn_forward(q, y.data_ptr(), y.shape[1], ops.stream_of(dev))
+    if rc:
+        _raise("dsx_ffn_forward", rc)
     return y, saved
+
+
+def _ffn_backward(ctx, dy):
+    x, w_gate, w_up, w_down, saved = ctx.saved_tensors
+    dev, dy = x.device, _rows(dy)
+    make = torch.empty if x.shape[0] else torch.zeros  # with no token the weights' gradients are zero
+    grads = [make(t.shape, dtype=t.dtype, device=dev) if n else None
+             for t, n in zip((x, w_gate, w_up, w_down), ctx.needs_input_grad)]
+    nbytes = ctx.backward_bytes
+    work = _scratch(nbytes, dev)
+    q = _pack_ffn(x, w_gate, w_up, w_down, ctx.activation, True, saved.data_ptr(), work.data_ptr(), nbytes)
+    at = [None if g is None else g.data_ptr() for g in grads]
+    rc = _bound.dsx_ffn_backward(q, dy.data_ptr(), _ld(dy), at[0], x.shape[1], at[1], at[2], at[3], ops.stream_of(dev))
+    if rc:
+        _raise("dsx_ffn_backward", rc)
+    return (*grads, None)
 
 
 class _GatedFFN(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w_gate, w_up, w_down, activation):
         keep = any(ctx.needs_input_grad[:4])
-        x, w_gate, w_up, w_down = (_rows(t) for t in (x, w_gate, w_up, w_down))
-        y, saved = _forward(x, w_gate, w_up, w_down, activation, keep)
+        x, w_gate, w_up, w_down = _rows(x), _rows(w_gate), _rows(w_up), _rows(w_down)
+        y, saved = _on(x.device, _ffn_forward, x, w_gate, w_up, w_down, activation, keep)
         if keep:
             ctx.save_for_backward(x, w_gate, w_up, w_down, saved)
             ctx.activation = activation
+            ctx.backward_bytes = _bound.dsx_ffn_workspace_bytes(
+                _pack_ffn(x, w_gate, w_up, w_down, activation, True, 0, 0, 0), 1)
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, w_gate, w_up, w_down, saved = ctx.saved_tensors
-        need, dev = ctx.needs_input_grad, x.device
-        dy = _rows(dy)
-        make = torch.empty if x.shape[0] else torch.zeros  # with no token the weights' gradients are zero
-        grads = [make(t.shape, dtype=t.dtype, device=dev) if n else None
-                 for t, n in zip((x, w_gate, w_up, w_down), need)]
-        q = _describe(x, w_gate, w_up, w_down, ctx.activation, True)
-        with torch.cuda.device(dev):
-            work = _scratch(_lib.load().dsx_ffn_workspace_bytes(ctypes.byref(q), 1), dev)
-            q.saved, q.workspace, q.workspace_bytes = saved.data_ptr(), work.data_ptr(), work.numel()
-            _lib.call("dsx_ffn_backward", ctypes.byref(q), ops._ptr(dy), _ld(dy), ops._ptr(grads[0]), x.shape[1],
-                      *(ops._ptr(g) for g in grads[1:]), ops.stream_of(dev))
-        return (*grads, None)
+        if torch.is_grad_enabled():
+            return _ffn_backward_once(ctx, dy)
+        return _on(dy.device, _ffn_backward, ctx, dy)
+
+
+@torch.autograd.function.once_differentiable
+def _ffn_backward_once(ctx, dy):
+    return _on(dy.device, _ffn_backward, ctx, dy)
 
 
 def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor, *,
@@ -99,17 +155,18 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
 
     Differentiable once in all four tensors. The backward keeps 8 bytes for
     every token and inner feature; without gradients nothing is kept."""
-    try:
-        act = ACTIVATIONS[activation]
-    except KeyError:
-        raise ValueError(f"activation must be one of {sorted(ACTIVATIONS)}, got {activation!r}") from None
-    for name, t in (("x", x), ("w_gate", w_gate), ("w_up", w_up), ("w_down", w_down)):
-        if not isinstance(t, torch.Tensor):
-            raise TypeError(f"{name} must be a tensor")
+    act = ACTIVATIONS.get(activation)
+    if act is None:
+        raise ValueError(f"activation must be one of {sorted(ACTIVATIONS)}, got {activation!r}")
+    if not isinstance(x, torch.Tensor):
+        raise TypeError("x must be a tensor")
     dev = ops._device(x)
     ops.dtype_code(x.dtype)
     if x.dim() < 1:
         raise ValueError("x must have at least one dimension")
+    for name, t in (("w_gate", w_gate), ("w_up", w_up), ("w_down", w_down)):
+        if not isinstance(t, torch.Tensor) or t.dtype != x.dtype or t.device != dev:
+            _refuse(name, t, x)
     d = x.shape[-1]
     if w_gate.dim() != 2:
         raise ValueError(f"w_gate must be [inner, width], got {tuple(w_gate.shape)}")
@@ -117,18 +174,63 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     if d < 1 or f < 1:
         raise ValueError(f"width and inner must be at least 1, got {d} and {f}")
     for name, t, shape in (("w_gate", w_gate, (f, d)), ("w_up", w_up, (f, d)), ("w_down", w_down, (d, f))):
-        if tuple(t.shape) != shape:
+        if t.shape != shape:
             raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
-        if t.device != dev:
-            raise ValueError(f"{name} is on {t.device}, expected {dev}")
-        if t.dtype != x.dtype:
-            raise TypeError(f"{name} must be {x.dtype}, got {t.dtype}")
     flat = x.reshape(-1, d) if x.dim() != 2 else x
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (x, w_gate, w_up, w_down)):
+    if torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad
+                                    or w_down.requires_grad):
         y = _GatedFFN.apply(flat, w_gate, w_up, w_down, act)
     else:
-        y, _ = _forward(*(_rows(t.detach()) for t in (flat, w_gate, w_up, w_down)), act, False)
+        y, _ = _on(dev, _ffn_forward, _rows(flat), _rows(w_gate), _rows(w_up), _rows(w_down), act, False)
     return y.view(x.shape) if x.dim() != 2 else y
+
+
+# ---- the norms around a block --------------------------------------------------------------------
+
+def _at(t: torch.Tensor | None) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
+def _norm_forward(residual, branch, post_weight, gate, next_weight, scales, keep: bool):
+    """hidden, normed, the saved rstd and the packed arguments."""
+    dev = residual.device
+    rows, d = residual.shape
+    hidden = torch.empty(residual.shape, dtype=residual.dtype, device=dev)
+    normed = None if next_weight is None else torch.empty(residual.shape, dtype=residual.dtype, device=dev)
+    rstd = torch.empty((2, rows), dtype=torch.float32, device=dev) if keep else None
+    q = _NORM.pack(residual.data_ptr(), _at(branch), _at(post_weight), _at(gate), _at(next_weight), _ld(residual),
+                   0 if branch is None else _ld(branch), rows, d, 0 if gate is None else gate.numel() // d,
+                   ops.grad_code(residual.dtype), *scales, _at(rstd))
+    rc = _bound.dsx_norm_forward(q, hidden.data_ptr(), None if normed is None else normed.data_ptr(),
+                                 ops.stream_of(dev))
+    if rc:
+        _raise("dsx_norm_forward", rc)
+    return hidden, normed, rstd, q
+
+
+def _norm_backward(ctx, d_hidden, d_normed):
+    saved = ctx.saved_tensors  # kept alive, and checked for changes in place; their addresses are in ctx.packed
+    residual = saved[0]
+    dev = residual.device
+    make = torch.empty if residual.shape[0] else torch.zeros  # with no row the vectors' gradients are zero
+    grads = [make(t.shape, dtype=t.dtype, device=dev) if t is not None and n else None
+             for t, n in zip(saved, ctx.needs_input_grad[:5])]
+    dh = dn = None
+    ld_dh = ld_dn = 0
+    if d_hidden is not None:
+        d_hidden = _rows(d_hidden)
+        dh, ld_dh = d_hidden.data_ptr(), _ld(d_hidden)
+    if d_normed is not None:
+        d_normed = _rows(d_normed)
+        dn, ld_dn = d_normed.data_ptr(), _ld(d_normed)
+    nbytes = ctx.backward_bytes
+    work = _scratch(nbytes, dev)
+    rc = _bound.dsx_norm_backward(ctx.packed, dh, ld_dh, dn, ld_dn,
+                                  *[None if g is None else g.data_ptr() for g in grads], work.data_ptr(), nbytes,
+                                  ops.stream_of(dev))
+    if rc:
+        _raise("dsx_norm_backward", rc)
+    return (*grads, None)
 
 
 class _GatedResidualNorm(torch.autograd.Function):
@@ -136,53 +238,35 @@ class _GatedResidualNorm(torch.autograd.Function):
     def forward(ctx, residual, branch, post_weight, gate, next_weight, scales):
         keep = any(ctx.needs_input_grad[:5])
         residual = _rows(residual)
-        branch = None if branch is None else _rows(branch)
-        post_weight, gate, next_weight = (None if t is None else t.contiguous()
-                                          for t in (post_weight, gate, next_weight))
-        hidden, normed, rstd = _norm_forward(residual, branch, post_weight, gate, next_weight, scales, keep)
+        if branch is not None:
+            branch = _rows(branch)
+        if post_weight is not None:
+            post_weight = post_weight.contiguous()
+        if gate is not None:
+            gate = gate.contiguous()
+        if next_weight is not None:
+            next_weight = next_weight.contiguous()
+        hidden, normed, rstd, q = _on(residual.device, _norm_forward, residual, branch, post_weight, gate, next_weight,
+                                      scales, keep)
         ctx.set_materialize_grads(False)
         if keep:
             ctx.save_for_backward(residual, branch, post_weight, gate, next_weight, rstd)
-            ctx.scales = scales
+            ctx.packed = q
+            ctx.backward_bytes = _bound.dsx_norm_workspace_bytes(q)
         return hidden, normed
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, d_hidden, d_normed):
-        *inputs, rstd = ctx.saved_tensors
-        residual, dev = inputs[0], inputs[0].device
         if d_hidden is None and d_normed is None:
             return (None,) * 6
-        d_hidden, d_normed = (None if t is None else _rows(t) for t in (d_hidden, d_normed))
-        make = torch.empty if residual.shape[0] else torch.zeros  # with no row the vectors' gradients are zero
-        grads = [make(t.shape, dtype=t.dtype, device=dev) if t is not None and need else None
-                 for t, need in zip(inputs, ctx.needs_input_grad)]
-        q = _describe_norm(*inputs, ctx.scales, rstd)
-        with torch.cuda.device(dev):
-            work = _scratch(_lib.load().dsx_norm_workspace_bytes(ctypes.byref(q)), dev)
-            _lib.call("dsx_norm_backward", ctypes.byref(q), ops._ptr(d_hidden), 0 if d_hidden is None else _ld(d_hidden),
-                      ops._ptr(d_normed), 0 if d_normed is None else _ld(d_normed), *(ops._ptr(g) for g in grads),
-                      ops._ptr(work), work.numel(), ops.stream_of(dev))
-        return (*grads, None)
+        if torch.is_grad_enabled():
+            return _norm_backward_once(ctx, d_hidden, d_normed)
+        return _on((d_normed if d_hidden is None else d_hidden).device, _norm_backward, ctx, d_hidden, d_normed)
 
 
-def _describe_norm(residual, branch, post_weight, gate, next_weight, scales, rstd) -> DsxNorm:
-    at = [None if t is None else t.data_ptr() for t in (residual, branch, post_weight, gate, next_weight)]
-    rows, d = residual.shape
-    gate_rows = 0 if gate is None else gate.numel() // d
-    return DsxNorm(*at, _ld(residual), 0 if branch is None else _ld(branch), rows, d, gate_rows,
-                   ops.grad_code(residual.dtype), *scales, None if rstd is None else rstd.data_ptr())
-
-
-def _norm_forward(residual, branch, post_weight, gate, next_weight, scales, keep: bool):
-    dev = residual.device
-    hidden = torch.empty(residual.shape, dtype=residual.dtype, device=dev)
-    normed = None if next_weight is None else torch.empty_like(hidden)
-    rstd = torch.empty(2, residual.shape[0], dtype=torch.float32, device=dev) if keep else None
-    q = _describe_norm(residual, branch, post_weight, gate, next_weight, scales, rstd)
-    with torch.cuda.device(dev):
-        _lib.call("dsx_norm_forward", ctypes.byref(q), ops._ptr(hidden), ops._ptr(normed), ops.stream_of(dev))
-    return hidden, normed, rstd
+@torch.autograd.function.once_differentiable
+def _norm_backward_once(ctx, d_hidden, d_normed):
+    return _on((d_normed if d_hidden is None else d_hidden).device, _norm_backward, ctx, d_hidden, d_normed)
 
 
 def gated_residual_norm(residual: torch.Tensor, branch: torch.Tensor | None = None, *,
@@ -213,26 +297,24 @@ def gated_residual_norm(residual: torch.Tensor, branch: torch.Tensor | None = No
     if residual.dim() < 1 or residual.shape[-1] < 1:
         raise ValueError(f"residual must be [..., width] with a width of at least 1, got {tuple(residual.shape)}")
     d = residual.shape[-1]
-    rows = residual.numel() // d
     if branch is None and (post_weight is not None or gate is not None):
         raise ValueError("post_weight and gate belong to a branch, and there is none")
+    wants_grad = residual.requires_grad
     for name, t in (("branch", branch), ("post_weight", post_weight), ("gate", gate), ("next_weight", next_weight)):
         if t is None:
             continue
-        if not isinstance(t, torch.Tensor):
-            raise TypeError(f"{name} must be a tensor or None")
-        if t.device != dev:
-            raise ValueError(f"{name} is on {t.device}, expected {dev}")
-        if t.dtype != residual.dtype:
-            raise TypeError(f"{name} must be {residual.dtype}, got {t.dtype}")
+        if not isinstance(t, torch.Tensor) or t.dtype != residual.dtype or t.device != dev:
+            _refuse(name, t, residual, True)
+        wants_grad = wants_grad or t.requires_grad
     if branch is not None and branch.shape != residual.shape:
         raise ValueError(f"branch must be {list(residual.shape)}, got {list(branch.shape)}")
     for name, t in (("post_weight", post_weight), ("next_weight", next_weight)):
-        if t is not None and tuple(t.shape) != (d,):
+        if t is not None and t.shape != (d,):
             raise ValueError(f"{name} must be [{d}], got {list(t.shape)}")
     if gate is not None:
         if gate.dim() not in (1, 2) or gate.shape[-1] != d or gate.numel() == 0:
             raise ValueError(f"gate must be [{d}] or [samples, {d}], got {list(gate.shape)}")
+        rows = residual.numel() // d
         if gate.dim() == 2 and rows % gate.shape[0]:
             raise ValueError(f"gate has {gate.shape[0]} rows, which do not divide the {rows} rows")
     if not eps >= 0:
@@ -240,13 +322,12 @@ def gated_residual_norm(residual: torch.Tensor, branch: torch.Tensor | None = No
     scales = (float(branch_scale), float(residual_scale), float(eps))
     flat = residual if residual.dim() == 2 else residual.reshape(-1, d)
     flat_branch = branch if branch is None or branch.dim() == 2 else branch.reshape(-1, d)
-    inputs = (flat, flat_branch, post_weight, gate, next_weight)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in inputs):
-        hidden, normed = _GatedResidualNorm.apply(*inputs, scales)
+    if wants_grad and torch.is_grad_enabled():
+        hidden, normed = _GatedResidualNorm.apply(flat, flat_branch, post_weight, gate, next_weight, scales)
     else:
-        vectors = (None if t is None else t.detach().contiguous() for t in inputs[2:])
-        hidden, normed, _ = _norm_forward(_rows(flat.detach()), None if branch is None else _rows(flat_branch.detach()),
-                                          *vectors, scales, False)
+        vectors = [None if t is None else t.contiguous() for t in (post_weight, gate, next_weight)]
+        hidden, normed, _, _ = _on(dev, _norm_forward, _rows(flat), None if branch is None else _rows(flat_branch),
+                                   *vectors, scales, False)
     if residual.dim() != 2:
         hidden = hidden.view(residual.shape)
         normed = None if normed is None else normed.view(residual.shape)

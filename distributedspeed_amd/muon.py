@@ -14,14 +14,16 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 from typing import Sequence
 
 import torch
 
 from . import _lib, ops
-from ._lib import DsxMatrix, DsxMuonHyper, DsxMuonParam
+from ._lib import DsxMuonHyper, DsxMuonParam
 
 NS_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+_MATRIX = struct.Struct("=2Q4q")  # DsxMatrix of include/dsx.h
 
 
 def _coefficients(coefficients, steps: int) -> tuple[tuple[float, float, float], ...]:
@@ -65,7 +67,7 @@ def _matrices(updates, name: str) -> list[torch.Tensor]:
 
 def _rows_contiguous(t: torch.Tensor) -> torch.Tensor:
     """t, or a copy where its columns are not adjacent or its rows overlap."""
-    if t.numel() and ((t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1])):
+    if not t.is_contiguous() and t.numel() and ((t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1])):
         return t.contiguous()
     return t
 
@@ -118,19 +120,26 @@ def orthogonalize(updates: torch.Tensor | Sequence[torch.Tensor], *, steps: int 
                                  f"{tuple(o.shape)} on {o.device}")
             if _rows_contiguous(o) is not o:
                 raise ValueError("out must have adjacent columns and rows that do not overlap")
-    ms = [_rows_contiguous(t.detach()) for t in ms]
-    table = (DsxMatrix * len(ms))()
-    for q, t, o in zip(table, ms, outs):
-        q.in_, q.out, q.ld_in, q.ld_out = t.data_ptr(), o.data_ptr(), _row_stride(t), _row_stride(o)
-        q.rows, q.cols = t.shape
-    coef = (ctypes.c_double * (3 * steps))(*(v for r in rows for v in r))
-    nbytes = _lib.load().dsx_orthogonalize_workspace(table, len(ms))
+    ms = [_rows_contiguous(t) for t in ms]
+    table = b"".join(_MATRIX.pack(t.data_ptr(), o.data_ptr(), _row_stride(t), _row_stride(o), *t.shape)
+                     for t, o in zip(ms, outs))
+    coef = struct.pack(f"={3 * steps}d", *(v for r in rows for v in r))
+    lib = _lib.load()
+    nbytes = lib.dsx_orthogonalize_workspace(table, len(ms))
     if nbytes < 0:
         raise ValueError(_lib.last_error())
-    with torch.cuda.device(dev):
+
+    def run():
         work = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        _lib.call("dsx_orthogonalize", table, len(ms), code, steps, coef, eps, ops._ptr(work), nbytes,
-                  ops.stream_of(dev))
+        rc = lib.dsx_orthogonalize(table, len(ms), code, steps, coef, eps, work.data_ptr(), nbytes, ops.stream_of(dev))
+        if rc:
+            raise _lib.DsxError("dsx_orthogonalize", rc, _lib.last_error())
+
+    if torch.cuda.current_device() == dev.index:
+        run()
+    else:
+        with torch.cuda.device(dev):
+            run()
     return result
 
 
