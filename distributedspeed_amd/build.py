@@ -1,4 +1,5 @@
-"""Build libdsx.so in-tree with hipcc for gfx950.
+"""Build libdsx.so in-tree with hipcc for gfx950, and the autograd nodes of the
+block operators (_block_autograd.so, host C++).
 
     python -m distributedspeed_amd.build
 
@@ -24,6 +25,7 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+import sysconfig
 import tempfile
 from concurrent.futures import ThreadPoolExecutor
 
@@ -32,6 +34,7 @@ ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 INCLUDE = os.path.join(ROOT, "include")
 OUT = os.path.join(HERE, "libdsx.so")
+AUTOGRAD = os.path.join(HERE, "_block_autograd.so")
 ARCH = os.environ.get("DSX_OFFLOAD_ARCH", "gfx950")
 
 # source -> its own flags. The optimizer step rounds where torch rounds; the
@@ -60,24 +63,39 @@ def command(source: str, out: str, extra: list[str] | None = None) -> list[str]:
             f"-I{INCLUDE}", f"-I{CSRC}", os.path.join(CSRC, source), "-o", out] + list(extra or [])
 
 
+def autograd_command(out: str) -> list[str]:
+    """The compile command of the autograd nodes of the block operators: host
+    C++ against torch, calling libdsx through addresses bound at load."""
+    import torch
+    from torch.utils import cpp_extension
+    includes = [*cpp_extension.include_paths(), sysconfig.get_paths()["include"], INCLUDE]
+    return ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+            *[a for i in includes for a in ("-isystem" if "torch" in i else "-I", i)],
+            os.path.join(CSRC, "block_autograd.cpp"), "-o", out,
+            *[f"-L{d}" for d in cpp_extension.library_paths()], "-lc10", "-ltorch", "-ltorch_cpu", "-ltorch_python"]
+
+
 def _run(cmd: list[str]) -> list[str]:
     res = subprocess.run(cmd, capture_output=True, text=True)
     # hipcc's host pass warns that it does not know the packed-fp32 feature: harmless.
     noise = [ln for ln in (res.stderr or "").splitlines() if "packed-fp32-ops" not in ln and ln.strip()]
     if res.returncode != 0:
-        raise RuntimeError("hipcc failed:\n" + "\n".join(noise))
+        raise RuntimeError(f"{os.path.basename(cmd[0])} failed:\n" + "\n".join(noise))
     return noise
 
 
-def build(out: str = OUT, verbose: bool = False) -> str:
+def build(out: str = OUT, autograd: str = AUTOGRAD, verbose: bool = False) -> str:
     with tempfile.TemporaryDirectory(prefix="dsx_build_") as tmp:
         objects = {src: os.path.join(tmp, src + ".o") for src in SOURCES}
-        with ThreadPoolExecutor(max_workers=min(4, len(SOURCES))) as pool:
-            noise = [ln for got in pool.map(lambda src: _run(command(src, objects[src])), SOURCES) for ln in got]
+        jobs = [command(src, objects[src]) for src in SOURCES] + [autograd_command(autograd + ".tmp")]
+        with ThreadPoolExecutor(max_workers=min(5, len(jobs))) as pool:
+            noise = [ln for got in pool.map(_run, jobs) for ln in got]
         _run([hipcc(), f"--offload-arch={ARCH}", "-fPIC", "-shared", *objects.values(), "-o", out + ".tmp"])
     if verbose and noise:
         print("\n".join(noise), file=sys.stderr)
     os.replace(out + ".tmp", out)
+    os.replace(autograd + ".tmp", autograd)
     return out
 
 
