@@ -133,6 +133,7 @@ struct Store {  // C in the inputs' type
   short* c;
   int64_t ld;
   __device__ inline Raw load(int, int) const { return {}; }
+  __device__ inline void one(int m, int n, float v, float) const { c[m * ld + n] = T::round(v); }
   __device__ inline void operator()(int m, int n, int N, const float* v, const float*, const Raw&) const {
     short* o = c + m * ld + n;
     const s8v w = round8<T>(v);
@@ -151,6 +152,18 @@ struct Up {  // h and the factors from g and u
   Saved s;
   int act, keep;
   __device__ inline Raw load(int, int) const { return {}; }
+  __device__ inline void one(int m, int n, float g, float u) const {
+    const int64_t at = m * s.ld + n;
+    const ActValue a = activate(act, g);
+    s.h[at] = T::round(a.f * u);
+    if (keep) {
+      const uint32_t p = top24(u * a.d), q = top24(a.f);
+      s.p_hi[at] = (uint16_t)(p >> 16);
+      s.p_lo[at] = (uint8_t)(p >> 8);
+      s.q_hi[at] = (uint16_t)(q >> 16);
+      s.q_lo[at] = (uint8_t)(q >> 8);
+    }
+  }
   __device__ inline void operator()(int m, int n, int, const float* g, const float* u, const Raw&) const {
     const int64_t at = m * s.ld + n;
     float h[8], p[8], q[8];
@@ -289,6 +302,86 @@ __global__ __launch_bounds__(256) void k_join(const float* __restrict__ part, in
   e(r, c, n, v, w, e.load(r, c));
 }
 
+// ---- up to three tokens ------------------------------------------------------
+
+// With so few tokens the forward is the weights' stream: a wave takes two rows
+// of weights (one feature of the gate and the up projection, or two outputs)
+// and their products with each token's row, eight elements a lane and load,
+// sums in fp32. No shared memory, nothing split, and any alignment; the weights
+// are read past the caches, being used once. 4096 x 14336, bf16, 1 to 4 tokens:
+// 59, 62, 69 and 74 us (5.9 TB/s for one; 64 us through the caches); as matrix-
+// instruction tiles of 16 rows with split sums 68, 68, 70 and 71.
+constexpr int kFewTokens = 3;
+
+template <class T, int M, class E>
+__global__ __launch_bounds__(256) void k_few(const short* __restrict__ w0, const short* __restrict__ w1, int64_t ld0,
+                                             int64_t ld1, const short* __restrict__ x, int64_t ld_x, int n, int k,
+                                             E e) {
+  const int lane = threadIdx.x & 63;
+  const int i = blockIdx.x * 4 + (threadIdx.x >> 6);  // the pair of rows
+  if (E::kPair ? i >= n : 2 * i >= n) return;
+  const bool second = E::kPair || 2 * i + 1 < n;
+  const short* p = E::kPair ? w0 + i * ld0 : w0 + 2 * i * ld0;
+  const short* q = E::kPair ? w1 + i * ld1 : second ? p + ld0 : p;
+  float u[M], v[M];
+#pragma unroll
+  for (int m = 0; m < M; m++) u[m] = v[m] = 0.0f;
+  auto add = [&](const s8v& a, const s8v& b, const s8v* c) {
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      const float f = T::widen(a[j]), g = T::widen(b[j]);
+#pragma unroll
+      for (int m = 0; m < M; m++) {
+        const float h = T::widen(c[m][j]);
+        u[m] = fmaf(f, h, u[m]);
+        v[m] = fmaf(g, h, v[m]);
+      }
+    }
+  };
+  int c = lane * 8;
+#pragma unroll 4
+  for (; c + 8 <= k; c += 512) {
+    s8v t[M];
+    const s8v a = __builtin_nontemporal_load((const s8u*)(p + c)), b = __builtin_nontemporal_load((const s8u*)(q + c));
+#pragma unroll
+    for (int m = 0; m < M; m++) t[m] = *(const s8u*)(x + m * ld_x + c);
+    add(a, b, t);
+  }
+  if (c < k) {  // the row's last elements
+    s8v a = {0, 0, 0, 0, 0, 0, 0, 0}, b = a, t[M];
+#pragma unroll
+    for (int m = 0; m < M; m++) t[m] = a;
+    for (int j = 0; j < 8; j++)
+      if (c + j < k) {
+        a[j] = p[c + j];
+        b[j] = q[c + j];
+        for (int m = 0; m < M; m++) t[m][j] = x[m * ld_x + c + j];
+      }
+    add(a, b, t);
+  }
+#pragma unroll
+  for (int m = 0; m < M; m++)
+#pragma unroll
+    for (int d = 32; d; d >>= 1) {
+      u[m] += __shfl_xor(u[m], d);
+      v[m] += __shfl_xor(v[m], d);
+    }
+  if (lane < M) {
+    float f = u[0], g = v[0];
+#pragma unroll
+    for (int m = 1; m < M; m++) {
+      f = lane == m ? u[m] : f;
+      g = lane == m ? v[m] : g;
+    }
+    if (E::kPair) {
+      e.one(lane, i, f, g);
+    } else {
+      e.one(lane, 2 * i, f, 0.0f);
+      if (second) e.one(lane, 2 * i + 1, g, 0.0f);
+    }
+  }
+}
+
 // ---- the weight gradients: up to three products over the tokens ------------
 
 struct WeightGrad {
@@ -345,19 +438,26 @@ int square_tile(int64_t n256, int64_t n128) {
 Shape shape_of(int64_t m, int64_t n, int64_t kt, bool pair, bool direct) {
   Shape s{};
   const int64_t cols = pair ? 2 * n : n;
+  const int64_t want = 2 * kCus;  // blocks to fill the chip
+  int64_t most = kt / 2;          // splits, of two K tiles each at least
   if (!direct) {
     s.tm = m <= 32 ? 32 : 128;
     s.tn = 128;
   } else if (m <= 64) {
     s.tm = m <= 16 ? 16 : m <= 32 ? 32 : 64;
-    s.tn = 128;
+    // 4096 x 14336, 16 tokens forward: 82 us with 128 columns a tile, 94 with 64;
+    // 64 x 2048 x 8192 forward and backward: 104 and 96
+    s.tn = m <= 16 ? 128 : 64;
+    // A split writes and reads m n fp32 sums: at most half as many bytes as the
+    // weights' own 2 n k. (Without the bound, 64 x 2048 x 8192: 135 us.)
+    const int64_t bound = kt * kBK / (8 * m);
+    if (bound < most) most = bound;
   } else {
     s.tm = s.tn = square_tile(ceil_div(m, 256) * ceil_div(cols, 256), ceil_div(m, 128) * ceil_div(cols, 128));
   }
   const int64_t tiles = ceil_div(m, s.tm) * ceil_div(cols, s.tn);
-  const int64_t want = s.tm <= 64 ? 4 * kCus : 2 * kCus;  // blocks that a CU holds at once, over all CUs
   int64_t splits = tiles >= want / 2 ? 1 : ceil_div(want, tiles);
-  if (splits > kt / 2) splits = kt / 2;  // two K tiles each at least
+  if (splits > most) splits = most;
   if (splits < 1) splits = 1;
   s.per = (int)ceil_div(kt, splits);
   s.splits = (int)ceil_div(kt, s.per);
@@ -388,8 +488,8 @@ void launch_product(Product p, const Shape& s, bool direct, float* part, const E
   } while (0)
   if (direct) {
     if (s.tm == 16) DSX_RUN(16, 128, 1, 4, true);
-    else if (s.tm == 32) DSX_RUN(32, 128, 1, 4, true);
-    else if (s.tm == 64) DSX_RUN(64, 128, 1, 4, true);
+    else if (s.tm == 32) DSX_RUN(32, 64, 2, 2, true);
+    else if (s.tm == 64) DSX_RUN(64, 64, 2, 2, true);
     else if (s.tm == 128) DSX_RUN(128, 128, 2, 4, true);
     else DSX_RUN(256, 256, 2, 4, true);
   } else {
@@ -466,11 +566,27 @@ int64_t workspace_of(const DsxFfn& q, bool backward) {
   return round_up(part, 256) + (backward ? 2 * round_up(z.m * z.ldf * 2, 256) : 0) + 256;
 }
 
+template <class T, int M>
+void forward_few(const DsxFfn& q, const Saved& s, void* y, int64_t ld_y, hipStream_t st) {
+  const int d = (int)q.width, f = (int)q.inner;
+  const short *wg = (const short*)q.w_gate, *wu = (const short*)q.w_up, *wd = (const short*)q.w_down;
+  k_few<T, M, Up<T>><<<dim3((unsigned)ceil_div(f, 4)), 256, 0, st>>>(wg, wu, q.ld_gate, q.ld_up, (const short*)q.x,
+                                                                     q.ld_x, f, d, Up<T>{s, q.activation, q.keep});
+  k_few<T, M, Store<T>><<<dim3((unsigned)ceil_div(d, 8)), 256, 0, st>>>(wd, wd, q.ld_down, q.ld_down, s.h, s.ld, d, f,
+                                                                        Store<T>{(short*)y, ld_y});
+}
+
 template <class T>
 int forward(const DsxFfn& q, void* y, int64_t ld_y, hipStream_t st) {
   const Sizes z = sizes_of(q);
   const Direct dir = direct_of(q, nullptr, 0);
   const Saved s = saved_of(q);
+  if (z.m <= kFewTokens) {
+    if (z.m == 1) forward_few<T, 1>(q, s, y, ld_y, st);
+    else if (z.m == 2) forward_few<T, 2>(q, s, y, ld_y, st);
+    else forward_few<T, 3>(q, s, y, ld_y, st);
+    return launch_status("dsx_ffn_forward");
+  }
   float* part = (float*)q.workspace;
   Product p{};
   p.a[0] = {(const short*)q.x, q.ld_x, (int)z.m};

@@ -42,7 +42,7 @@ using dsxi::fail;
 using dsxi::launch_status;
 using dsxi::round_up;
 
-constexpr int kWidest = 8192;  // of a row kept in registers: 1024 threads of eight elements
+constexpr int kWidest = 8192;  // of a row kept in registers: 512 threads of two chunks of eight elements
 
 struct Args {
   const void* r;
@@ -149,62 +149,84 @@ __device__ inline void widen8(const typename Elem<DT>::Raw& v, float* f) {
   for (int e = 0; e < 8; e++) f[e] = Elem<DT>::at(v, e);
 }
 
-template <int DT, int W>
+// Eight elements a thread and chunk; chunk v of a row begins at column
+// (v W + thread) 8.
+template <int DT, int W, int NV>
 __global__ __launch_bounds__(W) void k_forward(Args a, void* __restrict__ hidden, void* __restrict__ normed) {
   using E = Elem<DT>;
   __shared__ float buf[2][16][1];
-  const int c = threadIdx.x * 8, left = a.width - c;
-  const bool in = left > 0;
-  typename E::Raw zero{};
+  int c[NV], left[NV];
+#pragma unroll
+  for (int v = 0; v < NV; v++) {
+    c[v] = (v * W + threadIdx.x) * 8;
+    left[v] = a.width - c[v];
+  }
   const float inv_width = 1.0f / a.width;
-  float w1[8], w2[8], gate[8];
-  if (a.w1) widen8<DT>(in ? E::load(a.w1, c, left) : zero, w1);
-  if (a.w2) widen8<DT>(in ? E::load(a.w2, c, left) : zero, w2);
+  float w1[NV][8], w2[NV][8], gate[NV][8];
+  auto vector = [&](const void* p, int64_t at, float (*f)[8]) {
+#pragma unroll
+    for (int v = 0; v < NV; v++) widen8<DT>(left[v] > 0 ? E::load(p, at + c[v], left[v]) : typename E::Raw{}, f[v]);
+  };
+  if (a.w1) vector(a.w1, 0, w1);
+  if (a.w2) vector(a.w2, 0, w2);
   int sample = -1, turn = 0;
   int row = blockIdx.x;
-  typename E::Raw nr = zero, ny = zero;
-  if (in && row < a.rows) {
-    nr = E::load(a.r, row * a.ld_r + c, left);
-    if (a.y) ny = E::load(a.y, row * a.ld_y + c, left);
-  }
-  for (; row < a.rows; row += gridDim.x) {
-    float r[8], y[8], h[8];
-    widen8<DT>(nr, r);
-    widen8<DT>(ny, y);
-    const int next = row + gridDim.x;
-    if (in && next < a.rows) {
-      nr = E::load(a.r, next * a.ld_r + c, left);
-      if (a.y) ny = E::load(a.y, next * a.ld_y + c, left);
+  typename E::Raw nr[NV] = {}, ny[NV] = {};
+  auto fetch = [&](int k) {
+    if (k >= a.rows) return;
+#pragma unroll
+    for (int v = 0; v < NV; v++) {
+      if (left[v] <= 0) continue;
+      nr[v] = E::load(a.r, k * a.ld_r + c[v], left[v]);
+      if (a.y) ny[v] = E::load(a.y, k * a.ld_y + c[v], left[v]);
     }
+  };
+  fetch(row);
+  for (; row < a.rows; row += gridDim.x) {
+    float r[NV][8], y[NV][8], h[NV][8];
+#pragma unroll
+    for (int v = 0; v < NV; v++) {
+      widen8<DT>(nr[v], r[v]);
+      widen8<DT>(ny[v], y[v]);
+    }
+    fetch(row + gridDim.x);
     if (a.gate && row / a.per_sample != sample) {
       sample = row / a.per_sample;
-      widen8<DT>(in ? E::load(a.gate, (int64_t)sample * a.width + c, left) : zero, gate);
+      vector(a.gate, (int64_t)sample * a.width, gate);
     }
     float rstd1 = 1.0f;
     if (a.w1) {
       float s = 0;
 #pragma unroll
-      for (int e = 0; e < 8; e++) s = fmaf(y[e], y[e], s);
+      for (int v = 0; v < NV; v++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) s = fmaf(y[v][e], y[v][e], s);
       block_sum<W, 1>(&s, buf, turn++);
       rstd1 = 1.0f / sqrtf(s * inv_width + a.eps);
     }
     float s = 0;
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
-      float z = y[e];
-      if (a.w1) z = z * rstd1 * w1[e];
-      if (a.gate) z *= gate[e];
-      h[e] = fmaf(a.beta, r[e], a.alpha * z);
-      s = fmaf(h[e], h[e], s);
+    for (int v = 0; v < NV; v++) {
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        float z = y[v][e];
+        if (a.w1) z = z * rstd1 * w1[v][e];
+        if (a.gate) z *= gate[v][e];
+        h[v][e] = fmaf(a.beta, r[v][e], a.alpha * z);
+        s = fmaf(h[v][e], h[v][e], s);
+      }
+      if (left[v] > 0) E::store(hidden, (int64_t)row * a.width + c[v], left[v], h[v]);
     }
-    if (in) E::store(hidden, (int64_t)row * a.width + c, left, h);
     float rstd2 = 1.0f;
     if (a.w2) {
       block_sum<W, 1>(&s, buf, turn++);
       rstd2 = 1.0f / sqrtf(s * inv_width + a.eps);
 #pragma unroll
-      for (int e = 0; e < 8; e++) h[e] *= rstd2 * w2[e];
-      if (in) E::store(normed, (int64_t)row * a.width + c, left, h);
+      for (int v = 0; v < NV; v++) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) h[v][e] *= rstd2 * w2[v][e];
+        if (left[v] > 0) E::store(normed, (int64_t)row * a.width + c[v], left[v], h[v]);
+      }
     }
     if (a.rstd && threadIdx.x == 0) {
       a.rstd[row] = rstd1;
@@ -235,86 +257,113 @@ __device__ inline void unit_rows(const Args& a, const Grads& g, int u, int* lo, 
   *hi = first + (int)((int64_t)a.per_sample * (slice + 1) / g.slices);
 }
 
-template <int DT, int W>
+template <int DT, int W, int NV>
 __global__ __launch_bounds__(W) void k_backward(Args a, Grads g) {
   using E = Elem<DT>;
   __shared__ float buf[2][16][3];
-  const int c = threadIdx.x * 8, left = a.width - c;
-  const bool in = left > 0;
-  typename E::Raw zero{};
-  const float inv_width = 1.0f / a.width;
-  float w1[8], w2[8], gate[8];
+  int c[NV], left[NV];
 #pragma unroll
-  for (int e = 0; e < 8; e++) w1[e] = w2[e] = gate[e] = 1.0f;
-  if (a.w1) widen8<DT>(in ? E::load(a.w1, c, left) : zero, w1);
-  if (a.w2) widen8<DT>(in ? E::load(a.w2, c, left) : zero, w2);
+  for (int v = 0; v < NV; v++) {
+    c[v] = (v * W + threadIdx.x) * 8;
+    left[v] = a.width - c[v];
+  }
+  const float inv_width = 1.0f / a.width;
+  float w1[NV][8], w2[NV][8], gate[NV][8];
+  auto vector = [&](const void* p, int64_t at, float (*f)[8]) {
+#pragma unroll
+    for (int v = 0; v < NV; v++) {
+      if (p) {
+        widen8<DT>(left[v] > 0 ? E::load(p, at + c[v], left[v]) : typename E::Raw{}, f[v]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++) f[v][e] = 1.0f;
+      }
+    }
+  };
+  vector(a.w1, 0, w1);
+  vector(a.w2, 0, w2);
+  vector(a.gate, (int64_t)(blockIdx.x / g.slices) * a.width, gate);
   int row, end, turn = 0;
   unit_rows(a, g, blockIdx.x, &row, &end);
-  if (a.gate) widen8<DT>(in ? E::load(a.gate, (int64_t)(blockIdx.x / g.slices) * a.width + c, left) : zero, gate);
-  float s1[8], sg[8], s2[8];
-#pragma unroll
-  for (int e = 0; e < 8; e++) s1[e] = sg[e] = s2[e] = 0.0f;
-  typename E::Raw nr = zero, ny = zero, nh = zero, nn = zero;
+  float s1[NV][8] = {}, sg[NV][8] = {}, s2[NV][8] = {};
+  typename E::Raw nr[NV] = {}, ny[NV] = {}, nh[NV] = {}, nn[NV] = {};
   auto fetch = [&](int k) {
-    if (!in || k >= end) return;
-    nr = E::load(a.r, k * a.ld_r + c, left);
-    if (a.y) ny = E::load(a.y, k * a.ld_y + c, left);
-    if (g.dh) nh = E::load(g.dh, k * g.ld_dh + c, left);
-    if (g.dn) nn = E::load(g.dn, k * g.ld_dn + c, left);
+    if (k >= end) return;
+#pragma unroll
+    for (int v = 0; v < NV; v++) {
+      if (left[v] <= 0) continue;
+      nr[v] = E::load(a.r, k * a.ld_r + c[v], left[v]);
+      if (a.y) ny[v] = E::load(a.y, k * a.ld_y + c[v], left[v]);
+      if (g.dh) nh[v] = E::load(g.dh, k * g.ld_dh + c[v], left[v]);
+      if (g.dn) nn[v] = E::load(g.dn, k * g.ld_dn + c[v], left[v]);
+    }
   };
   fetch(row);
   for (; row < end; row++) {
-    float r[8], y[8], dh[8], dn[8], h[8];
-    widen8<DT>(nr, r);
-    widen8<DT>(ny, y);
-    widen8<DT>(nh, dh);
-    widen8<DT>(nn, dn);
+    float y[NV][8], dh[NV][8], dn[NV][8], h[NV][8];
+#pragma unroll
+    for (int v = 0; v < NV; v++) {
+      widen8<DT>(nr[v], h[v]);
+      widen8<DT>(ny[v], y[v]);
+      widen8<DT>(nh[v], dh[v]);
+      widen8<DT>(nn[v], dn[v]);
+    }
     fetch(row + 1);
     const float rstd1 = a.rstd[row], rstd2 = a.rstd[a.rows + row];
     float sum[3] = {0, 0, 0};  // of t h, q (dh + rstd2 t), q h
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
-      const float az = a.alpha * gate[e] * w1[e] * y[e];  // q
-      h[e] = fmaf(a.beta, r[e], az * rstd1);
-      const float t = w2[e] * dn[e];
-      sum[0] = fmaf(t, h[e], sum[0]);
-      sum[1] = fmaf(az, fmaf(rstd2, t, dh[e]), sum[1]);
-      sum[2] = fmaf(az, h[e], sum[2]);
-    }
+    for (int v = 0; v < NV; v++)
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const float q = a.alpha * gate[v][e] * w1[v][e] * y[v][e];
+        h[v][e] = fmaf(a.beta, h[v][e], q * rstd1);
+        const float t = w2[v][e] * dn[v][e];
+        sum[0] = fmaf(t, h[v][e], sum[0]);
+        sum[1] = fmaf(q, fmaf(rstd2, t, dh[v][e]), sum[1]);
+        sum[2] = fmaf(q, h[v][e], sum[2]);
+      }
     block_sum<W, 3>(sum, buf, turn++);
     const float mean2 = a.w2 ? sum[0] * rstd2 * inv_width : 0.0f;  // mean(t hhat)
     const float k2 = rstd2 * rstd2 * mean2;
     const float mean1 = (sum[1] - k2 * sum[2]) * rstd1 * inv_width;  // mean(w1 dz yhat)
-    float dr[8], dy[8];
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
-      float d = dh[e];
-      if (a.w2) {
-        d = fmaf(rstd2, w2[e] * dn[e], d) - k2 * h[e];
-        s2[e] = fmaf(dn[e], h[e] * rstd2, s2[e]);
+    for (int v = 0; v < NV; v++) {
+      float dr[8], dy[8];
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        float d = dh[v][e];
+        if (a.w2) {
+          d = fmaf(rstd2, w2[v][e] * dn[v][e], d) - k2 * h[v][e];
+          s2[v][e] = fmaf(dn[v][e], h[v][e] * rstd2, s2[v][e]);
+        }
+        dr[e] = a.beta * d;
+        const float yhat = y[v][e] * rstd1;
+        sg[v][e] = fmaf(a.alpha * (yhat * w1[v][e]), d, sg[v][e]);
+        const float dz = a.alpha * gate[v][e] * d;
+        s1[v][e] = fmaf(dz, yhat, s1[v][e]);
+        dy[e] = a.w1 ? rstd1 * (w1[v][e] * dz - yhat * mean1) : dz;
       }
-      dr[e] = a.beta * d;
-      const float yhat = y[e] * rstd1;
-      sg[e] = fmaf(a.alpha * (yhat * w1[e]), d, sg[e]);
-      const float dz = a.alpha * gate[e] * d;
-      s1[e] = fmaf(dz, yhat, s1[e]);
-      dy[e] = a.w1 ? rstd1 * (w1[e] * dz - yhat * mean1) : dz;
-    }
-    if (in) {
-      if (g.dr) E::store(g.dr, (int64_t)row * a.width + c, left, dr);
-      if (g.dy) E::store(g.dy, (int64_t)row * a.width + c, left, dy);
+      if (left[v] > 0) {
+        const int64_t at = (int64_t)row * a.width + c[v];
+        if (g.dr) E::store(g.dr, at, left[v], dr);
+        if (g.dy) E::store(g.dy, at, left[v], dy);
+      }
     }
   }
-  if (!in) return;
-  const int64_t plane = (int64_t)g.units * a.width, at = (int64_t)blockIdx.x * a.width + c;
-  if (g.dw1) Elem<DSX_F32>::store(g.part, at, left, s1);
-  if (g.dgate) {
-    if (g.slices == 1)
-      E::store(g.dgate, at, left, sg);  // a unit is a whole sample
-    else
-      Elem<DSX_F32>::store(g.part, plane + at, left, sg);
+  const int64_t plane = (int64_t)g.units * a.width;
+#pragma unroll
+  for (int v = 0; v < NV; v++) {
+    if (left[v] <= 0) continue;
+    const int64_t at = (int64_t)blockIdx.x * a.width + c[v];
+    if (g.dw1) Elem<DSX_F32>::store(g.part, at, left[v], s1[v]);
+    if (g.dgate) {
+      if (g.slices == 1)
+        E::store(g.dgate, at, left[v], sg[v]);  // a unit is a whole sample
+      else
+        Elem<DSX_F32>::store(g.part, plane + at, left[v], sg[v]);
+    }
+    if (g.dw2) Elem<DSX_F32>::store(g.part, 2 * plane + at, left[v], s2[v]);
   }
-  if (g.dw2) Elem<DSX_F32>::store(g.part, 2 * plane + at, left, s2);
 }
 
 // The partial rows of up to three vectors, added in order: for each, out[sample]
@@ -462,15 +511,16 @@ __global__ __launch_bounds__(256) void k_wide_backward(Args a, Grads g, const fl
 
 int block_of(int64_t width) {
   int w = 64;
-  while (w < 1024 && w * 8 < width) w *= 2;
+  while (w < 512 && w * 8 < width) w *= 2;
   return w;
 }
 
-// Runs of rows for the backward: several for each sample until the chip is
-// full, but four rows each at least, since every run costs a row of partial
-// sums for each of up to three vectors.
+// Runs of rows for the backward: enough blocks for eight waves a CU, but four
+// rows a run at least, since every run costs a row of partial sums for each of
+// up to three vectors. (8192 rows of 4096, bf16, forward and backward: 152 us;
+// with two, four and eight times as many blocks 157, 170 and 198.)
 int slices_of(int64_t rows, int64_t samples, int64_t width) {
-  const int64_t per = rows / samples, target = 1024 * 512 / block_of(width);
+  const int64_t per = rows / samples, target = 256 * 512 / block_of(width);
   int64_t s = ceil_div(target, samples);
   if (s > per / 4) s = per / 4;
   return (int)(s < 1 ? 1 : s);
@@ -515,11 +565,12 @@ void forward(const Args& a, void* hidden, void* normed, hipStream_t s) {
   const int64_t most = (int64_t)256 * (2048 / w);
   const unsigned grid = (unsigned)(a.rows < most ? a.rows : most);
   switch (w) {
-    case 64: k_forward<DT, 64><<<grid, 64, 0, s>>>(a, hidden, normed); break;
-    case 128: k_forward<DT, 128><<<grid, 128, 0, s>>>(a, hidden, normed); break;
-    case 256: k_forward<DT, 256><<<grid, 256, 0, s>>>(a, hidden, normed); break;
-    case 512: k_forward<DT, 512><<<grid, 512, 0, s>>>(a, hidden, normed); break;
-    default: k_forward<DT, 1024><<<grid, 1024, 0, s>>>(a, hidden, normed); break;
+    case 64: k_forward<DT, 64, 1><<<grid, 64, 0, s>>>(a, hidden, normed); break;
+    case 128: k_forward<DT, 128, 1><<<grid, 128, 0, s>>>(a, hidden, normed); break;
+    case 256: k_forward<DT, 256, 1><<<grid, 256, 0, s>>>(a, hidden, normed); break;
+    default:
+      if (a.width <= 4096) k_forward<DT, 512, 1><<<grid, 512, 0, s>>>(a, hidden, normed);
+      else k_forward<DT, 512, 2><<<grid, 512, 0, s>>>(a, hidden, normed);
   }
 }
 
@@ -531,11 +582,12 @@ void backward(const Args& a, Grads g, float* means, int samples, hipStream_t s) 
   } else {
     const unsigned grid = (unsigned)g.units;
     switch (block_of(a.width)) {
-      case 64: k_backward<DT, 64><<<grid, 64, 0, s>>>(a, g); break;
-      case 128: k_backward<DT, 128><<<grid, 128, 0, s>>>(a, g); break;
-      case 256: k_backward<DT, 256><<<grid, 256, 0, s>>>(a, g); break;
-      case 512: k_backward<DT, 512><<<grid, 512, 0, s>>>(a, g); break;
-      default: k_backward<DT, 1024><<<grid, 1024, 0, s>>>(a, g); break;
+      case 64: k_backward<DT, 64, 1><<<grid, 64, 0, s>>>(a, g); break;
+      case 128: k_backward<DT, 128, 1><<<grid, 128, 0, s>>>(a, g); break;
+      case 256: k_backward<DT, 256, 1><<<grid, 256, 0, s>>>(a, g); break;
+      default:
+        if (a.width <= 4096) k_backward<DT, 512, 1><<<grid, 512, 0, s>>>(a, g);
+        else k_backward<DT, 512, 2><<<grid, 512, 0, s>>>(a, g);
     }
   }
   const int64_t plane = (int64_t)g.units * a.width;
