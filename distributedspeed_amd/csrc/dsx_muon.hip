@@ -25,6 +25,14 @@
 // steps keep a second fp16 with what the first lost, which joins in a X (22
 // bits); the products take the first alone, as their noise lies in the
 // matrix's own row space. Rank one, 64 x 64: 1.4e-1 without, 2.7e-3 with it.
+//
+// Matrices whose shorter side is at most 64 take another way to the same
+// result, in fp32 throughout: every iterate is a polynomial of A0 = X0 X0^T
+// times X0, so with P_k = a I + b A_k + c A_k^2 and A_{k+1} = P_k A_k P_k the
+// result is (P_K ... P_1) X0. Three launches: A0 in parts along the longer side,
+// everything s x s in one block's shared memory, and the product with X0.
+// (In 16 bits that recurrence would lose the small singular values, which A
+// holds squared; in fp32 it is 3e-4 off at worst over spectra of any kind.)
 
 #include <hip/hip_runtime.h>
 #include <math.h>
@@ -69,7 +77,7 @@ struct Table {
   int32_t n, reserved;
   Mat m[kMats];
 };
-static_assert(sizeof(Table) <= 3840, "the table travels in the kernel arguments");
+static_assert(sizeof(Table) <= 3072, "the table travels in the kernel arguments, at most 4 KB with the others");
 
 struct Info {
   float p;      // X0~ = G p, a power of two
@@ -114,6 +122,12 @@ __device__ inline void load4(const void* p, int64_t at, bool vec, int left, floa
   }
 }
 
+// Whether four values of a row are one aligned load.
+template <int DT>
+__device__ inline bool vectors(const Mat& m) {
+  return (m.ld_in & 3) == 0 && ((uintptr_t)m.in & (DT == DSX_F32 ? 15 : 7)) == 0;
+}
+
 // The matrix that is orthogonalised, four values of a row: the input itself,
 // or Muon's update (buf = mu buf + (1 - mu) g; u = mu buf + (1 - mu) g with
 // Nesterov's correction, else buf).
@@ -143,9 +157,8 @@ __global__ __launch_bounds__(256) void k_sumsq(Table t, double* __restrict__ par
   const Mat& m = t.m[i];
   const int part = blockIdx.x - t.tile0[i], tid = threadIdx.x;
   const int tc = (m.cols + kNormTile - 1) / kNormTile, tiles = tc * ((m.rows + kNormTile - 1) / kNormTile);
-  const bool vec = (m.ld_in & 3) == 0 && ((uintptr_t)m.in & (DT == DSX_F32 ? 15 : 7)) == 0;
+  const bool vec = vectors<DT>(m);
   const float inv = MUON ? inverse_scale(ma) : 1.0f;
-  if (MUON && ma.skip && blockIdx.x == 0 && part == 0 && tid == 0 && m.part0 == 0) *ma.skip = 0;
   double sum = 0;
   for (int tile = part; tile < tiles; tile += m.parts) {
     const int r0 = tile / tc * kNormTile + (tid >> 4), c = tile % tc * kNormTile + (tid & 15) * 4;
@@ -216,7 +229,7 @@ __global__ __launch_bounds__(256) void k_cast(Table t, short* __restrict__ ws, c
   const int tc = (m.l + kNormTile - 1) / kNormTile;  // X's tile, and where it lies in the matrix
   const int xr = tile / tc * kNormTile, xc = tile % tc * kNormTile;
   const int r0 = (m.tall ? xc : xr) + (tid >> 4), c = (m.tall ? xr : xc) + (tid & 15) * 4;
-  const bool vec = (m.ld_in & 3) == 0 && ((uintptr_t)m.in & (DT == DSX_F32 ? 15 : 7)) == 0;
+  const bool vec = vectors<DT>(m);
   const float inv = MUON ? inverse_scale(ma) : 1.0f;
 #pragma unroll
   for (int k = 0; k < 4; k++) {
@@ -471,6 +484,241 @@ __global__ DSX_TILE_KERNEL(G) void k_apply(Table t, short* __restrict__ ws, cons
   }
 }
 
+// ---- a shorter side of at most 64 --------------------------------------------
+
+constexpr int kSmall = 64;       // X's rows, padded
+constexpr int kLdS = kSmall + 4;  // floats: a fragment's 16 rows and 4 columns fall on 64 banks
+constexpr int kLdX = 80;          // the same for 4 rows and 16 columns
+constexpr int kSmallParts = 16;
+
+// 64 columns of X from `x0` on, as fp32, handed to put(row of X, column within
+// the 64, four values along the matrix's row): along X's row unless tall.
+template <int DT, bool MUON, class F>
+__device__ inline void small_tile(const Mat& m, const MuonArgs& ma, float inv, bool vec, int x0, F&& put) {
+  const int tid = threadIdx.x;
+#pragma unroll
+  for (int k = 0; k < 4; k++) {
+    const int r = (m.tall ? x0 : 0) + (tid >> 4) + 16 * k, c = (m.tall ? 0 : x0) + (tid & 15) * 4;
+    float u[4] = {0, 0, 0, 0}, buf[4] = {0, 0, 0, 0};
+    const bool in = r < m.rows && c < m.cols;
+    if (in) update4<DT, MUON>(m, ma, inv, r, c, vec, u, buf);
+    put(r, c, in, u, buf);
+  }
+}
+
+typedef float f4acc __attribute__((ext_vector_type(4)));
+
+// A0's partial sums over a run of X's columns: parts[part][64][64].
+template <int DT, bool MUON>
+__global__ __launch_bounds__(256) void k_small_gram(Table t, float* __restrict__ ws, MuonArgs ma) {
+  __shared__ float x[kSmall * kLdS];
+  const int i = find(t, blockIdx.x);
+  const Mat& m = t.m[i];
+  const int part = blockIdx.x - t.tile0[i], tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  const bool vec = vectors<DT>(m);
+  const float inv = MUON ? inverse_scale(ma) : 1.0f;
+  const int tiles = (m.l + 63) / 64, lo = (int)((int64_t)tiles * part / m.parts),
+            hi = (int)((int64_t)tiles * (part + 1) / m.parts), nb = (m.s + 15) / 16;
+  f4acc acc[4] = {};
+  for (int tile = lo; tile < hi; tile++) {
+    const int x0 = tile * 64;
+    __syncthreads();
+    small_tile<DT, MUON>(m, ma, inv, vec, x0, [&](int r, int c, bool, const float* u, const float*) {
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const bool in = c + e < m.cols;
+        if (m.tall) {
+          if (c + e < kSmall) x[(c + e) * kLdS + r - x0] = in ? u[e] : 0.0f;
+        } else {
+          x[r * kLdS + c - x0 + e] = in ? u[e] : 0.0f;
+        }
+      }
+    });
+    __syncthreads();
+    if (w < nb)
+#pragma unroll 4
+      for (int k = 0; k < 64; k += 4) {
+        const float a = x[(w * 16 + (lane & 15)) * kLdS + k + (lane >> 4)];
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+          if (j < nb)
+            acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(a, x[(j * 16 + (lane & 15)) * kLdS + k + (lane >> 4)],
+                                                          acc[j], 0, 0, 0);
+      }
+  }
+  float* out = ws + m.a + (int64_t)part * kSmall * kSmall;
+  if (w < nb)
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+      if (j < nb)
+#pragma unroll
+        for (int e = 0; e < 4; e++) out[(w * 16 + (lane >> 4) * 4 + e) * kSmall + j * 16 + (lane & 15)] = acc[j][e];
+}
+
+// Ten waves, one for each 16 x 16 tile on or above the diagonal of a product of
+// two symmetric matrices that commute (polynomials of the same A0), so that the
+// product is symmetric too and rows serve as columns.
+struct SmallProduct {
+  int ti, tj, lane, steps;
+  bool on;
+  __device__ inline f4acc operator()(const float* a, const float* b) const {
+    f4acc acc = {0, 0, 0, 0};
+    if (on)
+#pragma unroll 4
+      for (int k = 0; k < steps; k++)
+        acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a[(ti * 16 + (lane & 15)) * kLdS + 4 * k + (lane >> 4)],
+                                                   b[(tj * 16 + (lane & 15)) * kLdS + 4 * k + (lane >> 4)], acc, 0, 0,
+                                                   0);
+    return acc;
+  }
+  __device__ inline void put(float* c, const f4acc& v) const {
+    if (!on) return;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const int r = ti * 16 + (lane >> 4) * 4 + e, q = tj * 16 + (lane & 15);
+      if (r > q) continue;  // of a tile on the diagonal: its other half is written from above
+      c[r * kLdS + q] = v[e];
+      c[q * kLdS + r] = v[e];
+    }
+  }
+};
+
+struct SmallCoef {
+  float c[3 * 64];
+};
+
+// All steps on A0 in shared memory; (P_K ... P_1) / |G| to ws + m.b.
+__global__ __launch_bounds__(640) void k_small_steps(Table t, float* __restrict__ ws, SmallCoef coef, int steps,
+                                                     double eps, int32_t* skip) {
+  __shared__ float A[kSmall * kLdS], P[kSmall * kLdS], T[kSmall * kLdS], Q[kSmall * kLdS];
+  __shared__ double norm2;
+  const Mat& m = t.m[blockIdx.x];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int nb = (m.s + 15) / 16, n = nb * 16;
+  SmallProduct mul;
+  triangle(__builtin_amdgcn_readfirstlane(tid >> 6), &mul.ti, &mul.tj);
+  mul.lane = lane;
+  mul.steps = nb * 4;
+  mul.on = mul.tj < nb;
+  const float* in = ws + m.a;
+  for (int e = tid; e < n * n; e += 640) {
+    const int r = e / n, c = e - r * n;
+    float sum = 0;
+#pragma unroll 8
+    for (int p = 0; p < m.parts; p++) sum += in[(int64_t)p * kSmall * kSmall + r * kSmall + c];
+    A[r * kLdS + c] = sum;
+  }
+  __syncthreads();
+  if (tid < 64) {
+    double d = tid < n ? (double)A[tid * kLdS + tid] : 0.0;
+    for (int k = 32; k; k >>= 1) d += __shfl_xor(d, k);
+    if (tid == 0) norm2 = d;
+  }
+  __syncthreads();
+  const bool bad = !isfinite(norm2);
+  if (bad && skip && tid == 0) atomicOr(skip, 1);
+  const double inv = bad ? __builtin_nan("") : 1.0 / (sqrt(norm2) + eps);
+  for (int e = tid; e < n * n; e += 640) {
+    const int r = e / n, c = e - r * n;
+    A[r * kLdS + c] = (float)(A[r * kLdS + c] * inv * inv);
+  }
+  __syncthreads();
+  for (int k = 0; k < steps; k++) {
+    const float a = coef.c[3 * k], b = coef.c[3 * k + 1], c = coef.c[3 * k + 2];
+    f4acc p = mul(A, A);
+    if (mul.on)
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const int r = mul.ti * 16 + (lane >> 4) * 4 + e, q = mul.tj * 16 + (lane & 15);
+        p[e] = fmaf(c, p[e], b * A[r * kLdS + q]) + (r == q ? a : 0.0f);
+      }
+    mul.put(P, p);
+    if (k == 0) mul.put(Q, p);
+    __syncthreads();
+    const bool more = k + 1 < steps;
+    f4acc s = {0, 0, 0, 0}, q = s;
+    if (more) s = mul(P, A);
+    if (k) q = mul(P, Q);
+    __syncthreads();
+    if (more) mul.put(T, s);
+    if (k) mul.put(Q, q);
+    __syncthreads();
+    if (more) {
+      s = mul(P, T);
+      __syncthreads();
+      mul.put(A, s);
+      __syncthreads();
+    }
+  }
+  float* out = ws + m.b;
+  for (int e = tid; e < n * n; e += 640) {
+    const int r = e / n, c = e - r * n;
+    out[r * kSmall + c] = (float)(Q[r * kLdS + c] * inv);
+  }
+}
+
+// The result's 64 columns: (P_K ... P_1 / |G|) X, to the output or the parameters.
+template <int DT, bool MUON>
+__global__ __launch_bounds__(256) void k_small_apply(Table t, const float* __restrict__ ws, MuonArgs ma, int out_dt) {
+  __shared__ float q[kSmall * kLdS], x[kSmall * kLdX];
+  if (MUON && *ma.skip) return;
+  const int i = find(t, blockIdx.x);
+  const Mat& m = t.m[i];
+  const int x0 = (blockIdx.x - t.tile0[i]) * 64, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  const int nb = (m.s + 15) / 16, n = nb * 16;
+  const bool vec = vectors<DT>(m);
+  const float inv = MUON ? inverse_scale(ma) : 1.0f;
+  for (int e = tid; e < n * n; e += 256) {
+    const int r = e / n, c = e - r * n;
+    q[r * kLdS + c] = ws[m.b + r * kSmall + c];
+  }
+  small_tile<DT, MUON>(m, ma, inv, vec, x0, [&](int r, int c, bool in, const float* u, const float* buf) {
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const bool here = in && c + e < m.cols;
+      if (MUON && here) m.momentum[(int64_t)r * m.cols + c + e] = buf[e];
+      if (m.tall) {
+        if (c + e < kSmall) x[(c + e) * kLdX + r - x0] = here ? u[e] : 0.0f;
+      } else {
+        x[r * kLdX + c - x0 + e] = here ? u[e] : 0.0f;
+      }
+    }
+  });
+  __syncthreads();
+  f4acc acc[4] = {};  // the wave's 16 columns
+#pragma unroll 4
+  for (int k = 0; k < n; k += 4) {
+    const float b = x[(k + (lane >> 4)) * kLdX + w * 16 + (lane & 15)];
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+      if (j < nb)
+        acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(q[(j * 16 + (lane & 15)) * kLdS + k + (lane >> 4)], b, acc[j], 0,
+                                                      0, 0);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < 4; j++)
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+      x[(j * 16 + (lane >> 4) * 4 + e) * kLdX + w * 16 + (lane & 15)] = acc[j][e] * kScale;
+  __syncthreads();
+  // eight values of a row of the matrix a thread
+#pragma unroll
+  for (int k = 0; k < 2; k++) {
+    const int r = (tid >> 3) + 32 * k, c = (tid & 7) * 8;
+    const int row = m.tall ? x0 + r : r, col = m.tall ? c : x0 + c;
+    if (row < m.rows && col < m.cols) {
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 8; e++) v[e] = m.tall ? x[(c + e) * kLdX + r] : x[r * kLdX + c + e];
+      if (MUON) step_params<8>(m, ma, out_dt, row, col, v);
+      else store_row<8>(m, row, col, v);
+    }
+  }
+}
+
+__global__ void k_clear(int32_t* p) { *p = 0; }
+
 // ---- host ------------------------------------------------------------------
 
 template <bool RB>
@@ -499,56 +747,71 @@ int32_t parts_of(int32_t rows, int32_t cols) {
 }
 
 struct Plan {
-  int64_t info_bytes = 0, partial_bytes = 0, halves = 0;
+  int64_t info_bytes = 0, partial_bytes = 0, run_bytes = 0;
 };
 
-// The list in runs of at most kMats matrices, f(table, index of the first).
-// The workspace: skip flag, norm records, partials, then the fp16 matrices of
-// the largest run.
+bool is_small(const Source& q) { return (q.rows < q.cols ? q.rows : q.cols) <= kSmall; }
+
+// The list in runs of at most kMats matrices, the ones with a side of at most
+// 64 apart: f(table, index of the first, small). The workspace: skip flag, norm
+// records, partials, then what the largest run needs (a small matrix's offsets
+// count floats from there, another's 16-bit elements).
 template <class F>
 Plan each_run(const Source* src, int32_t count, F&& f) {
   Plan plan;
-  Table t{};
-  int64_t part0 = 0, at = 0;
+  int64_t part0 = 0;
   int32_t index = 0;
-  auto flush = [&]() {
-    if (t.n) f(t, index - t.n);
-    if (at > plan.halves) plan.halves = at;
-    t.n = 0;
-    at = 0;
-  };
-  for (int32_t k = 0; k < count; k++) {
-    const Source& q = src[k];
-    if (q.rows <= 0 || q.cols <= 0) continue;
-    Mat& m = t.m[t.n++];
-    m = Mat{};
-    m.in = q.in;
-    m.out = q.out;
-    m.momentum = q.momentum;
-    m.master = q.master;
-    m.ld_in = q.ld_in;
-    m.ld_out = q.ld_out;
-    m.rows = q.rows;
-    m.cols = q.cols;
-    m.tall = q.rows > q.cols;
-    m.s = (int32_t)round_up(m.tall ? q.cols : q.rows, 8);
-    m.l = (int32_t)round_up(m.tall ? q.rows : q.cols, 8);
-    m.lr = q.lr;
-    const int64_t x = round_up((int64_t)m.s * m.l, 128), sq = round_up((int64_t)m.s * m.s, 128);
-    m.x[0] = at;
-    m.x[1] = at + x;
-    m.lo[0] = at + 2 * x;
-    m.lo[1] = at + 3 * x;
-    m.a = at + 4 * x;
-    m.b = m.a + sq;
-    at = m.b + sq;
-    m.parts = parts_of(q.rows, q.cols);
-    m.part0 = (int32_t)part0;
-    part0 += m.parts;
-    index++;
-    if (t.n == kMats) flush();
+  for (int small = 0; small < 2; small++) {
+    Table t{};
+    int64_t at = 0;
+    auto flush = [&]() {
+      if (t.n) f(t, index - t.n, small != 0);
+      const int64_t bytes = at * (small ? 4 : 2);
+      if (bytes > plan.run_bytes) plan.run_bytes = bytes;
+      t.n = 0;
+      at = 0;
+    };
+    for (int32_t k = 0; k < count; k++) {
+      const Source& q = src[k];
+      if (q.rows <= 0 || q.cols <= 0 || is_small(q) != (small != 0)) continue;
+      Mat& m = t.m[t.n++];
+      m = Mat{};
+      m.in = q.in;
+      m.out = q.out;
+      m.momentum = q.momentum;
+      m.master = q.master;
+      m.ld_in = q.ld_in;
+      m.ld_out = q.ld_out;
+      m.rows = q.rows;
+      m.cols = q.cols;
+      m.tall = q.rows > q.cols;
+      m.s = (int32_t)round_up(m.tall ? q.cols : q.rows, 8);
+      m.l = (int32_t)round_up(m.tall ? q.rows : q.cols, 8);
+      m.lr = q.lr;
+      if (small) {
+        const int64_t p = ceil_div(m.l, 256);
+        m.parts = (int32_t)(p > kSmallParts ? kSmallParts : p);
+        m.a = at;
+        m.b = at + (int64_t)m.parts * kSmall * kSmall;
+        at = m.b + kSmall * kSmall;
+      } else {
+        const int64_t x = round_up((int64_t)m.s * m.l, 128), sq = round_up((int64_t)m.s * m.s, 128);
+        m.x[0] = at;
+        m.x[1] = at + x;
+        m.lo[0] = at + 2 * x;
+        m.lo[1] = at + 3 * x;
+        m.a = at + 4 * x;
+        m.b = m.a + sq;
+        at = m.b + sq;
+        m.parts = parts_of(q.rows, q.cols);
+        m.part0 = (int32_t)part0;
+        part0 += m.parts;
+        index++;
+      }
+      if (t.n == kMats) flush();
+    }
+    flush();
   }
-  flush();
   plan.info_bytes = 256 + round_up((int64_t)index * (int64_t)sizeof(Info), 256);
   plan.partial_bytes = round_up(part0 * 8, 256);
   return plan;
@@ -635,30 +898,63 @@ void iterate(Table& t, short* ws, const Info* info, int steps, const double* coe
 template <int DT, bool MUON>
 int drive(const Source* src, int32_t count, int steps, const double* coef, double eps, MuonArgs ma, int out_dt,
           char* base, int64_t bytes, const char* what, hipStream_t s) {
-  const Plan plan = each_run(src, count, [](Table&, int) {});
-  const int64_t need = plan.info_bytes + plan.partial_bytes + 2 * plan.halves;
+  const Plan plan = each_run(src, count, [](Table&, int, bool) {});
+  const int64_t need = plan.info_bytes + plan.partial_bytes + plan.run_bytes;
   if (bytes < need)
     return fail(DSX_EINVAL, "%s: the workspace has %lld bytes, %lld are needed", what, (long long)bytes,
                 (long long)need);
   int32_t* skip = (int32_t*)base;
   Info* info = (Info*)(base + 256);
   double* partials = (double*)(base + plan.info_bytes);
-  short* ws = (short*)(base + plan.info_bytes + plan.partial_bytes);
+  char* run = base + plan.info_bytes + plan.partial_bytes;
   ma.skip = MUON ? skip : nullptr;
-  auto sums = [&](Table& t, int) {
+  SmallCoef sc{};
+  for (int k = 0; k < 3 * steps; k++) sc.c[k] = (float)coef[k];
+  auto small_steps = [&](Table& t) {
+    const int64_t n = tiles_of(t, [](const Mat& m) { return (int64_t)m.parts; });
+    k_small_gram<DT, MUON><<<dim3((unsigned)n), 256, 0, s>>>(t, (float*)run, ma);
+    k_small_steps<<<t.n, 640, 0, s>>>(t, (float*)run, sc, steps, eps, ma.skip);
+  };
+  auto small_apply = [&](Table& t) {
+    const int64_t n = tiles_of(t, [](const Mat& m) { return ceil_div(m.l, 64); });
+    k_small_apply<DT, MUON><<<dim3((unsigned)n), 256, 0, s>>>(t, (const float*)run, ma, out_dt);
+  };
+  auto sums = [&](Table& t) {
     const int64_t n = tiles_of(t, [](const Mat& m) { return (int64_t)m.parts; });
     k_sumsq<DT, MUON><<<dim3((unsigned)n), 256, 0, s>>>(t, partials, ma);
   };
   auto rest = [&](Table& t, int at) {
     const int64_t n =
         tiles_of(t, [](const Mat& m) { return ceil_div(m.s, kNormTile) * ceil_div(m.l, kNormTile); });
-    k_cast<DT, MUON><<<dim3((unsigned)n), 256, 0, s>>>(t, ws, partials, info + at, eps, ma);
-    iterate<MUON>(t, ws, info + at, steps, coef, MUON || DT == DSX_F32, ma, out_dt, s);
+    k_cast<DT, MUON><<<dim3((unsigned)n), 256, 0, s>>>(t, (short*)run, partials, info + at, eps, ma);
+    iterate<MUON>(t, (short*)run, info + at, steps, coef, MUON || DT == DSX_F32, ma, out_dt, s);
   };
-  each_run(src, count, sums);
-  if (MUON)
-    each_run(src, count, [&](Table& t, int) { k_norms<<<t.n, 64, 0, s>>>(t, partials, eps, skip); });
-  each_run(src, count, rest);
+  if (MUON) {
+    // Every norm is known before anything is written: a small matrix's is the
+    // trace of A0, so its steps run (and are run again below, as the runs share
+    // their place) before the first cast.
+    k_clear<<<1, 1, 0, s>>>(skip);
+    each_run(src, count, [&](Table& t, int, bool small) {
+      if (small) {
+        small_steps(t);
+      } else {
+        sums(t);
+        k_norms<<<t.n, 64, 0, s>>>(t, partials, eps, skip);
+      }
+    });
+  } else {
+    each_run(src, count, [&](Table& t, int, bool small) {
+      if (!small) sums(t);
+    });
+  }
+  each_run(src, count, [&](Table& t, int at, bool small) {
+    if (small) {
+      small_steps(t);
+      small_apply(t);
+    } else {
+      rest(t, at);
+    }
+  });
   return launch_status(what);
 }
 
@@ -700,9 +996,9 @@ int64_t dsx_orthogonalize_workspace(const DsxMatrix* mats, int32_t count) {
     src[k].rows = (int32_t)mats[k].rows;
     src[k].cols = (int32_t)mats[k].cols;
   }
-  const Plan plan = each_run(src, count, [](Table&, int) {});
+  const Plan plan = each_run(src, count, [](Table&, int, bool) {});
   delete[] src;
-  return plan.info_bytes + plan.partial_bytes + 2 * plan.halves;
+  return plan.info_bytes + plan.partial_bytes + plan.run_bytes;
 }
 
 int dsx_orthogonalize(const DsxMatrix* mats, int32_t count, int dtype, int32_t steps, const double* coefficients,
@@ -758,9 +1054,9 @@ int64_t dsx_muon_workspace(const DsxMuonParam* params, int32_t count) {
     src[k].rows = (int32_t)params[k].rows;
     src[k].cols = (int32_t)params[k].cols;
   }
-  const Plan plan = each_run(src, count, [](Table&, int) {});
+  const Plan plan = each_run(src, count, [](Table&, int, bool) {});
   delete[] src;
-  return plan.info_bytes + plan.partial_bytes + 2 * plan.halves;
+  return plan.info_bytes + plan.partial_bytes + plan.run_bytes;
 }
 
 int dsx_muon_step(const DsxMuonParam* params, int32_t count, int grad_dtype, int param_dtype, DsxMuonHyper hyper,
