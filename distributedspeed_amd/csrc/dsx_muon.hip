@@ -55,7 +55,7 @@ using dsxi::launch_status;
 using dsxi::round_up;
 
 constexpr float kScale = 4096.0f;
-constexpr int kMats = 22;        // matrices of one launch (the table is a kernel argument)
+constexpr int kMats = 20;        // matrices of one launch (the table is a kernel argument)
 constexpr int kMaxParts = 2048;  // norm partials per matrix
 constexpr int kNormTile = 64;    // the norm and cast kernels' square tile
 
@@ -69,6 +69,8 @@ struct Mat {
   int32_t rows, cols;   // of the caller's matrix
   int32_t s, l;         // of X: its sides rounded up to multiples of 8, s <= l
   int32_t tall;         // X is the matrix transposed
+  int32_t splits;       // of the Gram matrix's sums along l, into ws + part (fp32, a 64-tile after another)
+  int64_t part;
   int32_t part0, parts;
   float   lr;           // Muon: the step size of this matrix
 };
@@ -283,7 +285,7 @@ __device__ inline void triangle(int t, int* i, int* j) {
 
 // A symmetric product's tile, written at (m, n) and, off the diagonal, at (n, m).
 // GRAM: A = X X^T of the current X; else B = b A + c A A.
-template <class G, bool GRAM>
+template <class G, bool GRAM, bool SPLIT>
 __global__ DSX_TILE_KERNEL(G) void k_symmetric(Table t, short* __restrict__ ws, const Info* __restrict__ info, int cur,
                                                int first, float b, float c, const int32_t* skip) {
   __shared__ __attribute__((aligned(1024))) char lds[G::kLds];
@@ -293,14 +295,32 @@ __global__ DSX_TILE_KERNEL(G) void k_symmetric(Table t, short* __restrict__ ws, 
   const Mat& m = t.m[i];
   const int s = m.s;
   int ti, tj;
-  triangle(bid - t.tile0[i], &ti, &tj);
+  const int side = (s + G::TM - 1) / G::TM, tiles = side * (side + 1) / 2;
+  const bool split = SPLIT && m.splits > 1;
+  const int at = bid - t.tile0[i], run = split ? at / tiles : 0, tile = at - run * tiles;
+  triangle(tile, &ti, &tj);
   G g;
   g.init();
   const float inv_r = first ? info[i].inv_r : 1.0f;
   const short* src = ws + (GRAM ? m.x[cur] : m.a);
-  const Operand o{src, GRAM ? m.l : s, s};
+  Operand o{src, GRAM ? m.l : s, s};
+  int k_all = GRAM ? m.l : s;
+  if (split) {  // K tiles [lo, hi) of l
+    const int kt = (m.l + kBK - 1) / kBK, lo = (int)((int64_t)kt * run / m.splits),
+              hi = (int)((int64_t)kt * (run + 1) / m.splits);
+    o.p += lo * kBK;
+    k_all = min(hi * kBK, m.l) - lo * kBK;
+  }
   const int r0 = ti * G::TM, c0 = tj * G::TN;
-  g.run(lds, o, o, o, r0, c0, GRAM ? m.l : s);
+  g.run(lds, o, o, o, r0, c0, k_all);
+  if (split) {
+    float* out = (float*)(ws + m.part) + ((int64_t)run * tiles + tile) * G::TM * G::TN;
+    g.template emit<false>(
+        lds, [](int, int) { return Nothing{}; },
+        [&](int r, int q, float* v, float*, const Nothing&) { G::put8(out + r * G::TN + q, v); },
+        [](int, int, const float*) {});
+    return;
+  }
   const float k = GRAM ? inv_r * inv_r * (1.0f / kScale) : c * (1.0f / kScale);
   short* dst = ws + (GRAM ? m.a : m.b);
   auto pre = [&](int r, int q) {  // s is a multiple of 8: eight values are inside or outside together
@@ -334,6 +354,43 @@ __global__ DSX_TILE_KERNEL(G) void k_symmetric(Table t, short* __restrict__ ws, 
     g.template emit<false>(lds, pre, put, mirror);
   else
     g.template emit<true>(lds, pre, put, mirror);
+}
+
+// A from the partial sums of a split Gram matrix's 64-tiles, added in order.
+__global__ __launch_bounds__(256) void k_gram_join(Table t, short* __restrict__ ws, const Info* __restrict__ info,
+                                                   int first, const int32_t* skip) {
+  __shared__ float x[64][68];
+  if (skip && *skip) return;
+  const int i = find(t, blockIdx.x);
+  const Mat& m = t.m[i];
+  const int tile = blockIdx.x - t.tile0[i], s = m.s, side = (s + 63) / 64, tiles = side * (side + 1) / 2;
+  if (m.splits <= 1) return;
+  int ti, tj;
+  triangle(tile, &ti, &tj);
+  const float inv_r = first ? info[i].inv_r : 1.0f, k = inv_r * inv_r * (1.0f / kScale);
+  const float* p = (const float*)(ws + m.part) + (int64_t)tile * 4096;
+  short* dst = ws + m.a;
+  const int r = threadIdx.x >> 2, c = (threadIdx.x & 3) * 16;
+  f4v v[4] = {};
+#pragma unroll 4
+  for (int n = 0; n < m.splits; n++, p += (int64_t)tiles * 4096)
+#pragma unroll
+    for (int e = 0; e < 4; e++) v[e] += *(const f4v*)(p + r * 64 + c + 4 * e);
+#pragma unroll
+  for (int e = 0; e < 16; e++) x[r][c + e] = k * v[e >> 2][e & 3];
+  __syncthreads();
+#pragma unroll
+  for (int h = 0; h < 16; h += 8) {
+    s8v w, z;
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      w[e] = F16::round(x[r][c + h + e]);
+      z[e] = F16::round(x[c + h + e][r]);
+    }
+    const int a = ti * 64, b = tj * 64;
+    if (a + r < s && b + c + h < s) *(s8v*)(dst + (int64_t)(a + r) * s + b + c + h) = w;
+    if (ti != tj && b + r < s && a + c + h < s) *(s8v*)(dst + (int64_t)(b + r) * s + a + c + h) = z;
+  }
 }
 
 // Muon's update of N parameters of a row: w = w decay - lr O (v holds kScale O).
@@ -489,22 +546,43 @@ __global__ DSX_TILE_KERNEL(G) void k_apply(Table t, short* __restrict__ ws, cons
 constexpr int kSmall = 64;       // X's rows, padded
 constexpr int kLdS = kSmall + 4;  // floats: a fragment's 16 rows and 4 columns fall on 64 banks
 constexpr int kLdX = 80;          // the same for 4 rows and 16 columns
-constexpr int kSmallParts = 16;
+constexpr int kSmallParts = 32;
 
-// 64 columns of X from `x0` on, as fp32, handed to put(row of X, column within
-// the 64, four values along the matrix's row): along X's row unless tall.
-template <int DT, bool MUON, class F>
-__device__ inline void small_tile(const Mat& m, const MuonArgs& ma, float inv, bool vec, int x0, F&& put) {
-  const int tid = threadIdx.x;
-#pragma unroll
-  for (int k = 0; k < 4; k++) {
-    const int r = (m.tall ? x0 : 0) + (tid >> 4) + 16 * k, c = (m.tall ? 0 : x0) + (tid & 15) * 4;
-    float u[4] = {0, 0, 0, 0}, buf[4] = {0, 0, 0, 0};
-    const bool in = r < m.rows && c < m.cols;
-    if (in) update4<DT, MUON>(m, ma, inv, r, c, vec, u, buf);
-    put(r, c, in, u, buf);
+// 64 columns of X from `x0` on, as fp32: four values along the matrix's row in
+// each of four rows a thread, and their places in the tile.
+template <int DT, bool MUON>
+struct SmallTile {
+  float u[4][4], buf[4][4];
+  static __device__ inline void place(const Mat& m, int x0, int k, int* r, int* c) {
+    *r = (m.tall ? x0 : 0) + (threadIdx.x >> 4) + 16 * k;
+    *c = (m.tall ? 0 : x0) + (threadIdx.x & 15) * 4;
   }
-}
+  __device__ inline void load(const Mat& m, const MuonArgs& ma, float inv, bool vec, int x0) {
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      int r, c;
+      place(m, x0, k, &r, &c);
+#pragma unroll
+      for (int e = 0; e < 4; e++) u[k][e] = 0.0f;
+      if (r < m.rows && c < m.cols) update4<DT, MUON>(m, ma, inv, r, c, vec, u[k], buf[k]);
+    }
+  }
+  // Into x [row of X][column], rows LD apart.
+  template <int LD>
+  __device__ inline void store(const Mat& m, int x0, float* x) const {
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      int r, c;
+      place(m, x0, k, &r, &c);
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const float v = c + e < m.cols ? u[k][e] : 0.0f;
+        if (m.tall) x[(c + e) * LD + r - x0] = v;
+        else x[r * LD + c - x0 + e] = v;
+      }
+    }
+  }
+};
 
 typedef float f4acc __attribute__((ext_vector_type(4)));
 
@@ -520,20 +598,12 @@ __global__ __launch_bounds__(256) void k_small_gram(Table t, float* __restrict__
   const int tiles = (m.l + 63) / 64, lo = (int)((int64_t)tiles * part / m.parts),
             hi = (int)((int64_t)tiles * (part + 1) / m.parts), nb = (m.s + 15) / 16;
   f4acc acc[4] = {};
+  SmallTile<DT, MUON> next;
+  next.load(m, ma, inv, vec, lo * 64);
   for (int tile = lo; tile < hi; tile++) {
-    const int x0 = tile * 64;
     __syncthreads();
-    small_tile<DT, MUON>(m, ma, inv, vec, x0, [&](int r, int c, bool, const float* u, const float*) {
-#pragma unroll
-      for (int e = 0; e < 4; e++) {
-        const bool in = c + e < m.cols;
-        if (m.tall) {
-          if (c + e < kSmall) x[(c + e) * kLdS + r - x0] = in ? u[e] : 0.0f;
-        } else {
-          x[r * kLdS + c - x0 + e] = in ? u[e] : 0.0f;
-        }
-      }
-    });
+    next.template store<kLdS>(m, tile * 64, x);
+    if (tile + 1 < hi) next.load(m, ma, inv, vec, (tile + 1) * 64);
     __syncthreads();
     if (w < nb)
 #pragma unroll 4
@@ -558,14 +628,15 @@ __global__ __launch_bounds__(256) void k_small_gram(Table t, float* __restrict__
 // Ten waves, one for each 16 x 16 tile on or above the diagonal of a product of
 // two symmetric matrices that commute (polynomials of the same A0), so that the
 // product is symmetric too and rows serve as columns.
+template <int NB>
 struct SmallProduct {
-  int ti, tj, lane, steps;
+  int ti, tj, lane;
   bool on;
   __device__ inline f4acc operator()(const float* a, const float* b) const {
     f4acc acc = {0, 0, 0, 0};
     if (on)
-#pragma unroll 4
-      for (int k = 0; k < steps; k++)
+#pragma unroll
+      for (int k = 0; k < 4 * NB; k++)
         acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a[(ti * 16 + (lane & 15)) * kLdS + 4 * k + (lane >> 4)],
                                                    b[(tj * 16 + (lane & 15)) * kLdS + 4 * k + (lane >> 4)], acc, 0, 0,
                                                    0);
@@ -587,19 +658,16 @@ struct SmallCoef {
   float c[3 * 64];
 };
 
-// All steps on A0 in shared memory; (P_K ... P_1) / |G| to ws + m.b.
-__global__ __launch_bounds__(640) void k_small_steps(Table t, float* __restrict__ ws, SmallCoef coef, int steps,
-                                                     double eps, int32_t* skip) {
-  __shared__ float A[kSmall * kLdS], P[kSmall * kLdS], T[kSmall * kLdS], Q[kSmall * kLdS];
-  __shared__ double norm2;
-  const Mat& m = t.m[blockIdx.x];
+// All steps on A0 in shared memory; (P_K ... P_1) / |G| to ws + m.b. NB: 16-tiles a side.
+template <int NB>
+__device__ inline void small_steps(const Mat& m, float* __restrict__ ws, const SmallCoef& coef, int steps, double eps,
+                                   int32_t* skip, float* A, float* P, float* T, float* Q, double& norm2) {
   const int tid = threadIdx.x, lane = tid & 63;
-  const int nb = (m.s + 15) / 16, n = nb * 16;
-  SmallProduct mul;
+  constexpr int n = NB * 16;
+  SmallProduct<NB> mul;
   triangle(__builtin_amdgcn_readfirstlane(tid >> 6), &mul.ti, &mul.tj);
   mul.lane = lane;
-  mul.steps = nb * 4;
-  mul.on = mul.tj < nb;
+  mul.on = mul.tj < NB;
   const float* in = ws + m.a;
   for (int e = tid; e < n * n; e += 640) {
     const int r = e / n, c = e - r * n;
@@ -657,6 +725,17 @@ __global__ __launch_bounds__(640) void k_small_steps(Table t, float* __restrict_
   }
 }
 
+__global__ __launch_bounds__(640) void k_small_steps(Table t, float* __restrict__ ws, SmallCoef coef, int steps,
+                                                     double eps, int32_t* skip) {
+  __shared__ float A[kSmall * kLdS], P[kSmall * kLdS], T[kSmall * kLdS], Q[kSmall * kLdS];
+  __shared__ double norm2;
+  const Mat& m = t.m[blockIdx.x];
+  if (m.s <= 16) small_steps<1>(m, ws, coef, steps, eps, skip, A, P, T, Q, norm2);
+  else if (m.s <= 32) small_steps<2>(m, ws, coef, steps, eps, skip, A, P, T, Q, norm2);
+  else if (m.s <= 48) small_steps<3>(m, ws, coef, steps, eps, skip, A, P, T, Q, norm2);
+  else small_steps<4>(m, ws, coef, steps, eps, skip, A, P, T, Q, norm2);
+}
+
 // The result's 64 columns: (P_K ... P_1 / |G|) X, to the output or the parameters.
 template <int DT, bool MUON>
 __global__ __launch_bounds__(256) void k_small_apply(Table t, const float* __restrict__ ws, MuonArgs ma, int out_dt) {
@@ -672,18 +751,18 @@ __global__ __launch_bounds__(256) void k_small_apply(Table t, const float* __res
     const int r = e / n, c = e - r * n;
     q[r * kLdS + c] = ws[m.b + r * kSmall + c];
   }
-  small_tile<DT, MUON>(m, ma, inv, vec, x0, [&](int r, int c, bool in, const float* u, const float* buf) {
+  SmallTile<DT, MUON> tile;
+  tile.load(m, ma, inv, vec, x0);
+  tile.template store<kLdX>(m, x0, x);
+  if (MUON)
 #pragma unroll
-    for (int e = 0; e < 4; e++) {
-      const bool here = in && c + e < m.cols;
-      if (MUON && here) m.momentum[(int64_t)r * m.cols + c + e] = buf[e];
-      if (m.tall) {
-        if (c + e < kSmall) x[(c + e) * kLdX + r - x0] = here ? u[e] : 0.0f;
-      } else {
-        x[r * kLdX + c - x0 + e] = here ? u[e] : 0.0f;
-      }
+    for (int k = 0; k < 4; k++) {
+      int r, c;
+      tile.place(m, x0, k, &r, &c);
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+        if (r < m.rows && c + e < m.cols) m.momentum[(int64_t)r * m.cols + c + e] = tile.buf[k][e];
     }
-  });
   __syncthreads();
   f4acc acc[4] = {};  // the wave's 16 columns
 #pragma unroll 4
@@ -765,6 +844,24 @@ Plan each_run(const Source* src, int32_t count, F&& f) {
     Table t{};
     int64_t at = 0;
     auto flush = [&]() {
+      if (t.n && !small) {
+        // A Gram matrix of few 64-tiles leaves CUs idle while each walks all of
+        // l: its sums are split so that there are about two blocks a CU, eight
+        // K tiles each at least, and only below 160 tiles (65 x 8192: 326 us without,
+        // 117 with; 1001 x 2731, 136 tiles: 277 and 247; 1024 x 784 with 1024 x 1024,
+        // 227 tiles: 12.0 us a launch without, 15.2 with).
+        int64_t n = 0;
+        auto tiles = [](const Mat& m) { return ceil_div(m.s, 64) * (ceil_div(m.s, 64) + 1) / 2; };
+        for (int i = 0; i < t.n; i++) n += tiles(t.m[i]);
+        for (int i = 0; i < t.n; i++) {
+          Mat& m = t.m[i];
+          int64_t splits = n >= 160 ? 1 : ceil_div(512, n);
+          if (splits > m.l / (8 * kBK)) splits = m.l / (8 * kBK);
+          m.splits = (int32_t)(splits < 1 ? 1 : splits);
+          m.part = at;
+          if (m.splits > 1) at += m.splits * tiles(m) * 64 * 64 * 2;
+        }
+      }
       if (t.n) f(t, index - t.n, small != 0);
       const int64_t bytes = at * (small ? 4 : 2);
       if (bytes > plan.run_bytes) plan.run_bytes = bytes;
@@ -789,7 +886,7 @@ Plan each_run(const Source* src, int32_t count, F&& f) {
       m.l = (int32_t)round_up(m.tall ? q.rows : q.cols, 8);
       m.lr = q.lr;
       if (small) {
-        const int64_t p = ceil_div(m.l, 256);
+        const int64_t p = ceil_div(m.l, 128);
         m.parts = (int32_t)(p > kSmallParts ? kSmallParts : p);
         m.a = at;
         m.b = at + (int64_t)m.parts * kSmall * kSmall;
@@ -831,11 +928,18 @@ int64_t tiles_of(Table& t, F&& per) {
 template <class G, bool GRAM>
 void launch_symmetric(Table& t, short* ws, const Info* info, int cur, int first, float b, float c, const int32_t* skip,
                       hipStream_t s) {
-  const int64_t n = tiles_of(t, [](const Mat& m) {
+  constexpr bool SPLIT = GRAM && G::TM == 64;
+  auto tiles = [](const Mat& m) {
     const int64_t k = ceil_div(m.s, G::TM);
     return k * (k + 1) / 2;
+  };
+  bool any = false;
+  const int64_t n = tiles_of(t, [&](const Mat& m) {
+    any = any || (SPLIT && m.splits > 1);
+    return tiles(m) * (SPLIT ? m.splits : 1);
   });
-  k_symmetric<G, GRAM><<<dim3((unsigned)n), G::THREADS, 0, s>>>(t, ws, info, cur, first, b, c, skip);
+  k_symmetric<G, GRAM, SPLIT><<<dim3((unsigned)n), G::THREADS, 0, s>>>(t, ws, info, cur, first, b, c, skip);
+  if (any) k_gram_join<<<dim3((unsigned)tiles_of(t, tiles)), 256, 0, s>>>(t, ws, info, first, skip);
 }
 
 template <class G, bool MUON>
