@@ -146,7 +146,7 @@ struct Stage {
 // instruction: without any, the compiler waits for every direct load in flight
 // before each such read (tile t + 1's loads before tile t is multiplied),
 // although the loads fill the other tile and are waited for at the barrier.
-// Measured with a col operand, 8192^3: XXXX TFLOP/s.
+// 256-tiles of col operands, 8192^3: 1122 TFLOP/s so, 1277 with it.
 typedef __attribute__((address_space(3))) s4v LdsBlock;
 static __device__ inline s4v read_transposed(LdsBlock* __restrict__ p) {
   return __builtin_amdgcn_ds_read_tr16_b64_v4i16(p);

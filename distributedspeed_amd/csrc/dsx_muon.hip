@@ -13,7 +13,8 @@
 // Numbers. The iterates are fp16 with fp32 sums: entries of X, A and B are
 // bounded by their spectral norms (about 1.2, 1.5 and 2.9 with Muon's
 // coefficients), so range is no concern and fp16's 11 bits leave 8 times less
-// rounding error than bf16 (against 64 bits, 1024 x 1024: 1.1e-3 and 8.8e-3).
+// rounding error than bf16 (all of A, B and X rounded, against 64 bits,
+// 1024 x 1024: 1.1e-3 and 8.8e-3).
 // All three are stored times kScale, which keeps the small entries of large
 // matrices (1e-6 for A) in fp16's normal range. X0 is scaled by a power of two
 // alone, so a 16-bit input is not rounded at all; the rest of 1 / |G|, the
@@ -26,6 +27,12 @@
 // bits); the products take the first alone, as their noise lies in the
 // matrix's own row space. Rank one, 64 x 64: 1.4e-1 without, 2.7e-3 with it.
 //
+// The diagonals of A and B stay in fp32, apart from the matrices: they are the
+// large entries, and in a wide or random matrix nearly equal ones, so that
+// rounding them moves all of X by the same 2^-12 and more. With them out, A A is
+// A' A' + (d_i + d_j) A' + d_i^2 on the diagonal for the rest A', and B X has
+// d_i X added where a X is. Against 64 bits, 192 x 4416: 3.3e-4, with rounded
+// diagonals 1.2e-3; 512 x 512: 6.9e-4 and 1.3e-3.
 // Matrices whose shorter side is at most 64 take another way to the same
 // result, in fp32 throughout: every iterate is a polynomial of A0 = X0 X0^T
 // times X0, so with P_k = a I + b A_k + c A_k^2 and A_{k+1} = P_k A_k P_k the
@@ -55,7 +62,7 @@ using dsxi::launch_status;
 using dsxi::round_up;
 
 constexpr float kScale = 4096.0f;
-constexpr int kMats = 20;        // matrices of one launch (the table is a kernel argument)
+constexpr int kMats = 19;        // matrices of one launch (the table is a kernel argument)
 constexpr int kMaxParts = 2048;  // norm partials per matrix
 constexpr int kNormTile = 64;    // the norm and cast kernels' square tile
 
@@ -71,6 +78,7 @@ struct Mat {
   int32_t tall;         // X is the matrix transposed
   int32_t splits;       // of the Gram matrix's sums along l, into ws + part (fp32, a 64-tile after another)
   int64_t part;
+  int64_t diag;         // the diagonals of A and of B, s fp32 each
   int32_t part0, parts;
   float   lr;           // Muon: the step size of this matrix
 };
@@ -321,22 +329,42 @@ __global__ DSX_TILE_KERNEL(G) void k_symmetric(Table t, short* __restrict__ ws, 
         [](int, int, const float*) {});
     return;
   }
-  const float k = GRAM ? inv_r * inv_r * (1.0f / kScale) : c * (1.0f / kScale);
+  const float k = inv_r * inv_r * (1.0f / kScale);
   short* dst = ws + (GRAM ? m.a : m.b);
+  float* da = (float*)(ws + m.diag);
+  float* db = da + s;
+  struct Raw {
+    s8v a;
+    float row;
+    f4v lo, hi;  // the diagonal of A at the row and at the eight columns
+  };
   auto pre = [&](int r, int q) {  // s is a multiple of 8: eight values are inside or outside together
     r += r0;
     q += c0;
-    return GRAM || r >= s || q >= s ? s8v{} : *(const s8v*)(src + (int64_t)r * s + q);
+    Raw raw{};
+    if (!GRAM && r < s && q < s)
+      raw = {*(const s8v*)(src + (int64_t)r * s + q), da[r], *(const f4v*)(da + q), *(const f4v*)(da + q + 4)};
+    return raw;
   };
-  auto put = [&](int r, int q, float* v, float*, const s8v& a) {
+  auto put = [&](int r, int q, float* v, float*, const Raw& raw) {
+    r += r0;
+    q += c0;
     s8v w;
 #pragma unroll
     for (int e = 0; e < 8; e++) {
-      v[e] = GRAM ? k * v[e] : fmaf(k, v[e], b * F16::widen(a[e]));
+      const bool on = r == q + e;
+      if (GRAM) {
+        v[e] *= k;
+        if (on && r < s) da[r] = v[e] * (1.0f / kScale);
+      } else {
+        const float a = F16::widen(raw.a[e]), d = raw.row + (e < 4 ? raw.lo[e & 3] : raw.hi[e & 3]);
+        if (on && r < s)
+          db[r] = fmaf(c, fmaf(v[e], 1.0f / (kScale * kScale), raw.row * raw.row), b * raw.row);
+        v[e] = fmaf(c, fmaf(d, a, v[e] * (1.0f / kScale)), b * a);
+      }
+      if (on) v[e] = 0.0f;
       w[e] = F16::round(v[e]);
     }
-    r += r0;
-    q += c0;
     if (r < s && q < s) *(s8v*)(dst + (int64_t)r * s + q) = w;
   };
   auto mirror = [&](int q, int r, const float* v) {
@@ -377,7 +405,11 @@ __global__ __launch_bounds__(256) void k_gram_join(Table t, short* __restrict__ 
 #pragma unroll
     for (int e = 0; e < 4; e++) v[e] += *(const f4v*)(p + r * 64 + c + 4 * e);
 #pragma unroll
-  for (int e = 0; e < 16; e++) x[r][c + e] = k * v[e >> 2][e & 3];
+  for (int e = 0; e < 16; e++) {
+    const bool on = ti == tj && r == c + e;
+    x[r][c + e] = on ? 0.0f : k * v[e >> 2][e & 3];
+    if (on && ti * 64 + r < s) ((float*)(ws + m.diag))[ti * 64 + r] = k * v[e >> 2][e & 3] * (1.0f / kScale);
+  }
   __syncthreads();
 #pragma unroll
   for (int h = 0; h < 16; h += 8) {
@@ -458,6 +490,7 @@ __device__ inline void store_row(const Mat& m, int64_t r, int c, const float* v)
 // the iterate read and the one written have their second fp16.
 struct XRaw {
   s8v hi, lo;
+  float d;  // B's diagonal at the row
 };
 template <class G, bool LAST, bool MUON>
 __global__ DSX_TILE_KERNEL(G) void k_apply(Table t, short* __restrict__ ws, const Info* __restrict__ info, int cur,
@@ -473,6 +506,7 @@ __global__ DSX_TILE_KERNEL(G) void k_apply(Table t, short* __restrict__ ws, cons
   const float inv_r = first ? info[i].inv_r : 1.0f;
   const short* x = ws + m.x[cur];
   const short* x_lo = ws + m.lo[cur];
+  const float* db = (const float*)(ws + m.diag) + s;
   short* y = ws + m.x[cur ^ 1];
   short* y_lo = ws + m.lo[cur ^ 1];
   const Operand ob{ws + m.b, s, s}, ox{x, l, l};
@@ -487,6 +521,7 @@ __global__ DSX_TILE_KERNEL(G) void k_apply(Table t, short* __restrict__ ws, cons
     if (r < s && c < l) {
       const int64_t at = (int64_t)r * l + c;
       raw.hi = *(const s8v*)(x + at);
+      raw.d = db[r];
       if (take_lo) raw.lo = *(const s8v*)(x_lo + at);
     }
     return raw;
@@ -494,7 +529,7 @@ __global__ DSX_TILE_KERNEL(G) void k_apply(Table t, short* __restrict__ ws, cons
   auto value = [&](float* v, const XRaw& old) {
 #pragma unroll
     for (int e = 0; e < 8; e++)
-      v[e] = fmaf(a, F16::widen(old.hi[e]) + F16::widen(old.lo[e]), v[e] * (1.0f / kScale)) * inv_r;
+      v[e] = fmaf(a + old.d, F16::widen(old.hi[e]) + F16::widen(old.lo[e]), v[e] * (1.0f / kScale)) * inv_r;
   };
   auto none = [](int, int, const float*) {};
   if (!LAST) {
@@ -899,7 +934,8 @@ Plan each_run(const Source* src, int32_t count, F&& f) {
         m.lo[1] = at + 3 * x;
         m.a = at + 4 * x;
         m.b = m.a + sq;
-        at = m.b + sq;
+        m.diag = m.b + sq;
+        at = m.diag + round_up(4 * (int64_t)m.s, 128);
         m.parts = parts_of(q.rows, q.cols);
         m.part0 = (int32_t)part0;
         part0 += m.parts;
