@@ -452,6 +452,16 @@ Shape shape_of(int64_t m, int64_t n, int64_t kt, bool pair, bool direct) {
     // weights' own 2 n k. (Without the bound, 64 x 2048 x 8192: 135 us.)
     const int64_t bound = kt * kBK / (8 * m);
     if (bound < most) most = bound;
+  } else if (const int64_t n64 = ceil_div(m, 64) * ceil_div(cols, 64);
+             n64 <= 4 * kCus && kt <= 96 && n64 * kt <= 128 * kCus) {
+    // A product of at most about 128 K tiles of 64 x 64 a CU, four blocks to a
+    // CU: larger tiles would have to be split over K and joined, or leave CUs
+    // idle. Forward, against 128-tiles: 256 x 1024 x 4096 24 us and 56,
+    // 2048 x 512 x 1024 23 and 36, 200 x 2048 x 5632 38 and 58. Beyond the bounds
+    // the twice as many loads cost more: forward and backward, with n64 <= 1024
+    // alone, 1024 x 2048 x 5632 takes 375 us (319 with 128-tiles) and
+    // 100 x 4096 x 14336 takes 398 (361).
+    s.tm = s.tn = 64;
   } else {
     s.tm = s.tn = square_tile(ceil_div(m, 256) * ceil_div(cols, 256), ceil_div(m, 128) * ceil_div(cols, 128));
   }

@@ -102,6 +102,16 @@ def test_large_tiles(gpu):
     _check(_run(*args, "silu"), _exact(*args, "silu"), 3 * U["bfloat16"])
 
 
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("tokens,d,f", [(70, 6208, 72), (70, 72, 6216), (1100, 136, 2056), (2060, 520, 1160)])
+def test_middle_tiles(gpu, tokens, d, f, dtype):
+    """The 128-tiles: sums too long for the 64-tiles, which are split, along
+    either size; more tiles than the 64-tiles are used for, which are not."""
+    args = _make(tokens, d, f, dtype, seed=tokens + d + f)
+    _say(f"gated_ffn {tokens}x{d}x{f} {dtype}")
+    _check(_run(*args, "silu"), _exact(*args, "silu"), 3 * U[dtype])
+
+
 def test_gradients_against_differences(gpu):
     """(L(p + e v) - L(p - e v)) / 2e against <dL/dp, v> for L = <y, dy>, v
     with the parameter's own scale: at e = 1/32 the cubic term is of the order
