@@ -19,6 +19,9 @@
 // bits, which the matrix instruction's types do demand. h, dg and du are
 // rounded to the inputs' type once.
 //
+// Operands whose rows are not whole 16-byte chunks are copied first to rows
+// that are, where that pays (kRealignTokens).
+//
 // With few tokens there are fewer tiles than CUs while the weights' bytes
 // bound the time: the sum over k is split over blocks, each writing fp32
 // partial sums, and a second launch adds them in order and applies the
@@ -73,7 +76,8 @@ __device__ inline ActValue activate(int act, float g) {
 // ---- what the forward keeps ------------------------------------------------
 
 // Planes of [tokens][ldf]: h (16 bit), then the upper 16 and the next 8 bits
-// of the two factors.
+// of the two factors. Columns from F to ldf hold zeros, so that a sum over F
+// may be taken in whole chunks of eight.
 struct Saved {
   short* h;
   uint16_t* p_hi;
@@ -117,6 +121,12 @@ __device__ inline float widen24(const Raw24& r, int e) {
 }
 
 // ---- epilogues: eight columns of a row (n is a multiple of 8, below N) ------
+
+// Zeros in the place of columns past the end.
+__device__ inline void trim(float* v, int n, int N) {
+#pragma unroll
+  for (int e = 0; e < 8; e++) v[e] = n + e < N ? v[e] : 0.0f;
+}
 
 template <class T>
 __device__ inline s8v round8(const float* v) {
@@ -164,7 +174,7 @@ struct Up {  // h and the factors from g and u
       s.q_lo[at] = (uint8_t)(q >> 8);
     }
   }
-  __device__ inline void operator()(int m, int n, int, const float* g, const float* u, const Raw&) const {
+  __device__ inline void operator()(int m, int n, int N, const float* g, const float* u, const Raw&) const {
     const int64_t at = m * s.ld + n;
     float h[8], p[8], q[8];
 #pragma unroll
@@ -173,6 +183,11 @@ struct Up {  // h and the factors from g and u
       h[e] = a.f * u[e];
       p[e] = u[e] * a.d;
       q[e] = a.f;
+    }
+    if (n + 8 > N) {
+      trim(h, n, N);
+      trim(p, n, N);
+      trim(q, n, N);
     }
     *(s8v*)(s.h + at) = round8<T>(h);
     if (keep) {
@@ -197,13 +212,17 @@ struct Factors {  // dg and du from dh
     const int64_t at = m * s.ld + n;
     return {get24(s.p_hi, s.p_lo, at), get24(s.q_hi, s.q_lo, at)};
   }
-  __device__ inline void operator()(int m, int n, int, const float* v, const float*, const Raw& r) const {
+  __device__ inline void operator()(int m, int n, int N, const float* v, const float*, const Raw& r) const {
     const int64_t at = m * s.ld + n;
     float p[8], q[8];
 #pragma unroll
     for (int e = 0; e < 8; e++) {
       p[e] = widen24(r.p, e) * v[e];
       q[e] = widen24(r.q, e) * v[e];
+    }
+    if (n + 8 > N) {
+      trim(p, n, N);
+      trim(q, n, N);
     }
     *(s8v*)(dg + at) = round8<T>(p);
     *(s8v*)(du + at) = round8<T>(q);
@@ -416,6 +435,47 @@ __global__ DSX_TILE_KERNEL(G) void k_weight_grads(WeightGrads t) {
       [](int, int, const float*) {});
 }
 
+// ---- operands off the direct loads' alignment --------------------------------
+
+// Rows of any length and stride to rows of whole 16-byte chunks, zeros past the
+// end; up to five matrices in one launch, a chunk a thread and pass.
+struct Realign {
+  const short* from;
+  short* to;
+  int64_t ld;
+  int rows, cols, block0;
+};
+struct Realigns {
+  Realign r[5];
+  int count;
+};
+constexpr int kRealignChunks = 1024;  // of a block
+
+__global__ __launch_bounds__(256) void k_realign(Realigns t) {
+  int i = 0;
+  while (i + 1 < t.count && (int)blockIdx.x >= t.r[i + 1].block0) i++;
+  const Realign& q = t.r[i];
+  const uint32_t per = (uint32_t)(q.cols + 7) / 8, n = per * (uint32_t)q.rows;
+  const uint32_t at = (blockIdx.x - q.block0) * kRealignChunks + threadIdx.x;
+  s8v v[4];
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    const uint32_t k = at + j * 256;
+    v[j] = s8v{0, 0, 0, 0, 0, 0, 0, 0};
+    if (k >= n) continue;
+    const int r = (int)(k / per), c = (int)(k % per) * 8;
+    const short* p = q.from + r * q.ld + c;
+    if (c + 8 <= q.cols)
+      v[j] = *(const s8u*)p;
+    else
+      for (int e = 0; e < 8; e++)
+        if (c + e < q.cols) v[j][e] = p[e];
+  }
+#pragma unroll
+  for (int j = 0; j < 4; j++)
+    if (at + j * 256 < n) *(s8v*)(q.to + (int64_t)(at + j * 256) * 8) = v[j];
+}
+
 // ---- host ------------------------------------------------------------------
 
 // Tile rows and splits of a product of m x n over kt K tiles.
@@ -544,22 +604,68 @@ Saved saved_of(const DsxFfn& q) {
 struct Direct {
   bool up, down, dh, dx, dw;
 };
-Direct direct_of(const DsxFfn& q, const void* dy, int64_t ld_dy) {
-  const bool x = direct_ok(q.x, q.ld_x, q.width), wg = direct_ok(q.w_gate, q.ld_gate, q.width),
-             wu = direct_ok(q.w_up, q.ld_up, q.width), wd = direct_ok(q.w_down, q.ld_down, q.inner),
-             y = dy && direct_ok(dy, ld_dy, q.width), f = q.inner % 8 == 0;
+// Elements of each operand's rows that may be read (and, past the row's own,
+// are zeros).
+struct Lengths {
+  int64_t x, gate, up, down, dy;
+};
+Direct direct_of(const DsxFfn& q, const void* dy, int64_t ld_dy, const Lengths& n) {
+  const bool x = direct_ok(q.x, q.ld_x, n.x), wg = direct_ok(q.w_gate, q.ld_gate, n.gate),
+             wu = direct_ok(q.w_up, q.ld_up, n.up), wd = direct_ok(q.w_down, q.ld_down, n.down),
+             y = dy && direct_ok(dy, ld_dy, n.dy);
   Direct d{};
   d.up = x && wg && wu;
-  d.down = wd && f;
+  d.down = wd;
   d.dh = y && wd;
-  d.dx = wg && wu && f;
-  d.dw = x && y && f;
+  d.dx = wg && wu;
+  d.dw = x && y;
   return d;
 }
 
-int64_t workspace_of(const DsxFfn& q, bool backward) {
+// Operands whose rows' length or stride rule the direct loads out are first
+// copied to rows that do not: always in the backward, which reads each twice or
+// more, and in a forward of more than kRealignTokens. Forward and backward in
+// us, with the loads through registers and with the copies: 3000 x 2049 x 8001
+// 494 / 1734 and 410 / 1299, 200 x 2047 x 5631 78 / 280 and 68 / 181,
+// 3000 x 255 x 1023 43 / 444 and 36 / 104; forward only, 128 x 2047 x 5631 65
+// and 63, 130 x 1025 x 1025 26 and 31, 16 x 2047 x 5631 36 and 53 (there the
+// weights' bytes bound the time, which the copies triple). An operand that is
+// off by its address alone is not copied.
+constexpr int64_t kRealignTokens = 192;
+bool realigns(int64_t tokens, bool backward) { return backward || tokens > kRealignTokens; }
+
+bool realigned(int64_t rows, int64_t ld, int64_t cols) {
+  return !direct_ok(nullptr, ld, cols) &&
+         rows * ceil_div(cols, 8) < (int64_t)1 << 31;  // the copy's 32-bit chunk numbers
+}
+int64_t realigned_bytes(int64_t rows, int64_t ld, int64_t cols) {
+  return realigned(rows, ld, cols) ? round_up(rows * ld_inner(cols) * 2, 256) : 0;
+}
+
+// Collects the copies and puts the operands in their place.
+struct Realigner {
+  bool wanted;
+  char* at;
+  Realigns t;
+  int64_t blocks;
+
+  void add(const void** p, int64_t* ld, int64_t rows, int64_t* cols) {
+    if (!wanted || !realigned(rows, *ld, *cols)) return;
+    t.r[t.count++] = {(const short*)*p, (short*)at, *ld, (int)rows, (int)*cols, (int)blocks};
+    blocks += ceil_div(rows * ceil_div(*cols, 8), kRealignChunks);
+    *p = at;
+    at += realigned_bytes(rows, *ld, *cols);
+    *ld = *cols = ld_inner(*cols);
+  }
+  void launch(hipStream_t st) {
+    if (t.count) k_realign<<<dim3((unsigned)blocks), 256, 0, st>>>(t);
+  }
+};
+
+// Bytes of the split sums, which follow dg and du in the workspace; the copies
+// follow them.
+int64_t part_of(const DsxFfn& q, bool backward) {
   const Sizes z = sizes_of(q);
-  if (!z.m) return 256;
   // both load forms, so that the size does not hang on addresses
   int64_t part = 0;
   for (int direct = 0; direct < 2; direct++) {
@@ -573,7 +679,18 @@ int64_t workspace_of(const DsxFfn& q, bool backward) {
     for (int64_t v : b)
       if (v > part) part = v;
   }
-  return round_up(part, 256) + (backward ? 2 * round_up(z.m * z.ldf * 2, 256) : 0) + 256;
+  return round_up(part, 256);
+}
+
+int64_t workspace_of(const DsxFfn& q, bool backward) {
+  const Sizes z = sizes_of(q);
+  if (!z.m) return 256;
+  int64_t bytes = part_of(q, backward) + 256;
+  if (backward) bytes += 2 * round_up(z.m * z.ldf * 2, 256) + realigned_bytes(z.m, z.d, z.d);
+  if (realigns(z.m, backward))
+    bytes += realigned_bytes(z.m, q.ld_x, z.d) + realigned_bytes(z.f, q.ld_gate, z.d) +
+             realigned_bytes(z.f, q.ld_up, z.d) + realigned_bytes(z.d, q.ld_down, z.f);
+  return bytes;
 }
 
 template <class T, int M>
@@ -587,9 +704,8 @@ void forward_few(const DsxFfn& q, const Saved& s, void* y, int64_t ld_y, hipStre
 }
 
 template <class T>
-int forward(const DsxFfn& q, void* y, int64_t ld_y, hipStream_t st) {
+int forward(DsxFfn q, void* y, int64_t ld_y, hipStream_t st) {
   const Sizes z = sizes_of(q);
-  const Direct dir = direct_of(q, nullptr, 0);
   const Saved s = saved_of(q);
   if (z.m <= kFewTokens) {
     if (z.m == 1) forward_few<T, 1>(q, s, y, ld_y, st);
@@ -598,6 +714,14 @@ int forward(const DsxFfn& q, void* y, int64_t ld_y, hipStream_t st) {
     return launch_status("dsx_ffn_forward");
   }
   float* part = (float*)q.workspace;
+  Lengths len{z.d, z.d, z.d, z.f, z.d};
+  Realigner copies{realigns(z.m, false), (char*)q.workspace + part_of(q, false), {}, 0};
+  copies.add(&q.x, &q.ld_x, z.m, &len.x);
+  copies.add(&q.w_gate, &q.ld_gate, z.f, &len.gate);
+  copies.add(&q.w_up, &q.ld_up, z.f, &len.up);
+  copies.add(&q.w_down, &q.ld_down, z.d, &len.down);
+  copies.launch(st);
+  const Direct dir = direct_of(q, nullptr, 0, len);
   Product p{};
   p.a[0] = {(const short*)q.x, q.ld_x, (int)z.m};
   p.b[0] = {(const short*)q.w_gate, q.ld_gate, (int)z.f};
@@ -647,16 +771,26 @@ void launch_weight_grads(WeightGrads& w, hipStream_t st) {
 }
 
 template <class T>
-int backward(const DsxFfn& q, const void* dy, int64_t ld_dy, void* dx, int64_t ld_dx, void* dw_gate, void* dw_up,
+int backward(DsxFfn q, const void* dy, int64_t ld_dy, void* dx, int64_t ld_dx, void* dw_gate, void* dw_up,
              void* dw_down, hipStream_t st) {
   const Sizes z = sizes_of(q);
-  const Direct dir = direct_of(q, dy, ld_dy);
   const Saved s = saved_of(q);
   const int64_t plane = round_up(z.m * z.ldf * 2, 256);
   short* dg = (short*)q.workspace;
   short* du = (short*)((char*)q.workspace + plane);
   float* part = (float*)((char*)q.workspace + 2 * plane);
   const int m = (int)z.m;
+  Lengths len{z.d, z.d, z.d, z.f, z.d};
+  Realigner copies{realigns(z.m, true), (char*)part + part_of(q, true), {}, 0};
+  if (dw_gate || dw_up) copies.add(&q.x, &q.ld_x, z.m, &len.x);
+  if (dx) {
+    copies.add(&q.w_gate, &q.ld_gate, z.f, &len.gate);
+    copies.add(&q.w_up, &q.ld_up, z.f, &len.up);
+  }
+  if (dx || dw_gate || dw_up) copies.add(&q.w_down, &q.ld_down, z.d, &len.down);
+  if (z.d % 8) copies.add(&dy, &ld_dy, z.m, &len.dy);  // the workspace's size knows the width, not this stride
+  copies.launch(st);
+  const Direct dir = direct_of(q, dy, ld_dy, len);
   if (dx || dw_gate || dw_up) {
     Product p{};
     p.a[0] = {(const short*)dy, ld_dy, m};

@@ -19,9 +19,10 @@
 // Edges. A row or column of C past the end reads some valid element instead
 // (clamped address) and its sums are not stored. A k past the end must add
 // nothing: the places of the last tile that hold no k are written with zeros
-// after the loads have landed. The direct loads need 16-byte aligned operands
-// whose leading dimension and contiguous length are multiples of 8; anything
-// else goes through registers (kRegs), element by element at the edges.
+// after the loads have landed, by whole chunks. The direct loads need 16-byte
+// aligned operands whose leading dimension is a multiple of 8 and whose rows
+// are either as long or hold zeros up to there; anything else goes through
+// registers (DIRECT = false), element by element at the edges.
 #ifndef DSX_GEMM_H_
 #define DSX_GEMM_H_
 
@@ -152,7 +153,7 @@ static __device__ inline s4v read_transposed(LdsBlock* __restrict__ p) {
   return __builtin_amdgcn_ds_read_tr16_b64_v4i16(p);
 }
 
-// The product tile. NT = threads, WM x WN waves of (TM/WM) x (TN/WN).
+// The product tile: WM x WN waves of (TM/WM) x (TN/WN).
 // SPLIT: B's tile is two half tiles from two operands (the gate and the up
 // projection), and a wave's columns are half of one and half of the other.
 template <class T, int TM_, int TN_, int WM, int WN, bool RA, bool RB, bool DIRECT, bool SPLIT = false>

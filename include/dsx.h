@@ -705,8 +705,10 @@ typedef struct DsxFfn {
   int64_t     workspace_bytes;
 } DsxFfn;
 
-/* Bytes of `saved` and of `workspace` (host only; the addresses in `block`
- * are not read); -1 with dsx_last_error for sizes out of range. */
+/* Bytes of `saved` and of `workspace` (host only; the sizes and row strides in
+ * `block` count, the addresses are not read): operands whose rows are not whole
+ * 16-byte chunks may be copied there. -1 with dsx_last_error for sizes out of
+ * range. */
 int64_t dsx_ffn_saved_bytes(int64_t tokens, int64_t inner, int32_t keep);
 int64_t dsx_ffn_workspace_bytes(const DsxFfn* block /* host */,
                                 int32_t backward);

@@ -112,6 +112,24 @@ def test_middle_tiles(gpu, tokens, d, f, dtype):
     _check(_run(*args, "silu"), _exact(*args, "silu"), 3 * U[dtype])
 
 
+@pytest.mark.parametrize("tokens,d,f,pad", [(200, 129, 260, 0), (200, 136, 261, 0), (333, 515, 1021, 3),
+                                           (193, 512, 1024, 5), (260, 264, 1023, 6)])
+def test_rows_off_the_chunks(gpu, tokens, d, f, pad):
+    """Odd lengths and strides at enough tokens for the aligned copies, forward
+    and backward, with NaN between the rows and an output gradient whose
+    stride is odd too."""
+    import torch
+    args = _make(tokens, d, f, "bfloat16", seed=tokens + d + f + pad)
+    want = _exact(*args, "silu")
+    views = []
+    for t in args:
+        big = torch.full((t.shape[0], t.shape[1] + pad), float("nan"), device="cuda", dtype=t.dtype)
+        big[:, :t.shape[1]] = t
+        views.append(big[:, :t.shape[1]])
+    _say(f"gated_ffn {tokens}x{d}x{f} rows {pad} longer")
+    _check(_run(*views, "silu"), want, 3 * U["bfloat16"])
+
+
 def test_gradients_against_differences(gpu):
     """(L(p + e v) - L(p - e v)) / 2e against <dL/dp, v> for L = <y, dy>, v
     with the parameter's own scale: at e = 1/32 the cubic term is of the order
