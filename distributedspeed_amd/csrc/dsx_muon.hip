@@ -110,12 +110,14 @@ __device__ inline int find(const Table& t, int tile) {
   return __popcll(__ballot(begun)) - 1;
 }
 
+// Four values of a row at any element's address (zeros past its end).
+typedef s4v s4u __attribute__((aligned(2)));
 template <int DT>
-__device__ inline void load4(const void* p, int64_t at, bool vec, int left, float* v) {
+__device__ inline void load4(const void* p, int64_t at, int left, float* v) {
   if (DT == DSX_F32) {
     const float* q = (const float*)p + at;
-    if (vec && left >= 4) {
-      const f4v w = *(const f4v*)q;
+    if (left >= 4) {
+      const f4v w = *(const f4u*)q;
       for (int e = 0; e < 4; e++) v[e] = w[e];
     } else {
       for (int e = 0; e < 4; e++) v[e] = e < left ? q[e] : 0.0f;
@@ -123,8 +125,8 @@ __device__ inline void load4(const void* p, int64_t at, bool vec, int left, floa
   } else {
     using T = typename std::conditional<DT == DSX_F16, F16, BF16>::type;
     const short* q = (const short*)p + at;
-    if (vec && left >= 4) {
-      const s4v w = *(const s4v*)q;
+    if (left >= 4) {
+      const s4v w = *(const s4u*)q;
       for (int e = 0; e < 4; e++) v[e] = T::widen(w[e]);
     } else {
       for (int e = 0; e < 4; e++) v[e] = e < left ? T::widen(q[e]) : 0.0f;
@@ -132,22 +134,23 @@ __device__ inline void load4(const void* p, int64_t at, bool vec, int left, floa
   }
 }
 
-// Whether four values of a row are one aligned load.
-template <int DT>
-__device__ inline bool vectors(const Mat& m) {
-  return (m.ld_in & 3) == 0 && ((uintptr_t)m.in & (DT == DSX_F32 ? 15 : 7)) == 0;
+__device__ inline void store4(float* p, int left, const float* v) {
+  if (left >= 4)
+    *(f4u*)p = f4v{v[0], v[1], v[2], v[3]};
+  else
+    for (int e = 0; e < left; e++) p[e] = v[e];
 }
 
 // The matrix that is orthogonalised, four values of a row: the input itself,
 // or Muon's update (buf = mu buf + (1 - mu) g; u = mu buf + (1 - mu) g with
 // Nesterov's correction, else buf).
 template <int DT, bool MUON>
-__device__ inline void update4(const Mat& m, const MuonArgs& ma, float inv, int r, int c, bool vec, float* u,
+__device__ inline void update4(const Mat& m, const MuonArgs& ma, float inv, int r, int c, float* u,
                                float* buf) {
   const int left = m.cols - c;
-  load4<DT>(m.in, r * m.ld_in + c, vec, left, u);
+  load4<DT>(m.in, r * m.ld_in + c, left, u);
   if (MUON) {
-    load4<DSX_F32>(m.momentum, (int64_t)r * m.cols + c, (m.cols & 3) == 0, left, buf);
+    load4<DSX_F32>(m.momentum, (int64_t)r * m.cols + c, left, buf);
 #pragma unroll
     for (int e = 0; e < 4; e++) {
       const float g = u[e] * inv;
@@ -160,14 +163,15 @@ __device__ inline void update4(const Mat& m, const MuonArgs& ma, float inv, int 
 __device__ inline float inverse_scale(const MuonArgs& ma) { return ma.grad_scale ? 1.0f / *ma.grad_scale : 1.0f; }
 
 // Sums of squares: `parts` blocks per matrix, each over every parts-th tile;
-// squares and sums in fp64 (an fp32 input's squares may leave fp32's range).
+// squares and sums in fp64 (an fp32 input's squares may leave fp32's range). A
+// tile a block up to kMaxParts: four a block, the loads waiting for each other's
+// sums, took 10.6 us for twelve of 768 x 768 in bf16, one takes 6.4.
 template <int DT, bool MUON>
 __global__ __launch_bounds__(256) void k_sumsq(Table t, double* __restrict__ partials, MuonArgs ma) {
   const int i = find(t, blockIdx.x);
   const Mat& m = t.m[i];
   const int part = blockIdx.x - t.tile0[i], tid = threadIdx.x;
   const int tc = (m.cols + kNormTile - 1) / kNormTile, tiles = tc * ((m.rows + kNormTile - 1) / kNormTile);
-  const bool vec = vectors<DT>(m);
   const float inv = MUON ? inverse_scale(ma) : 1.0f;
   double sum = 0;
   for (int tile = part; tile < tiles; tile += m.parts) {
@@ -178,7 +182,7 @@ __global__ __launch_bounds__(256) void k_sumsq(Table t, double* __restrict__ par
       const int r = r0 + 16 * k;
       if (r >= m.rows) break;
       float u[4], buf[4];
-      update4<DT, MUON>(m, ma, inv, r, c, vec, u, buf);
+      update4<DT, MUON>(m, ma, inv, r, c, u, buf);
 #pragma unroll
       for (int e = 0; e < 4; e++) sum += (double)u[e] * u[e];
     }
@@ -205,20 +209,28 @@ __device__ inline Info info_of(double sum, double eps) {
   return f;
 }
 
-// A wave's sum of a matrix's partials, in an order set by their count.
-__device__ inline double total(const double* __restrict__ p, int parts) {
+// A matrix's Info by a block: its partials' sum, in an order set by their
+// count, shared by its waves (each wave for itself: 14336 x 4096, whose 2048
+// partials every block reads, 85 us for k_cast, 59 so).
+__device__ inline Info info_by_block(const double* __restrict__ p, int parts, double eps) {
+  __shared__ double of_wave[4];
+  __shared__ Info info;
   double sum = 0;
 #pragma unroll 4
-  for (int k = threadIdx.x & 63; k < parts; k += 64) sum += p[k];
+  for (int k = threadIdx.x; k < parts; k += 256) sum += p[k];
   for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
-  return sum;
+  if ((threadIdx.x & 63) == 0) of_wave[threadIdx.x >> 6] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0) info = info_of(of_wave[0] + of_wave[1] + of_wave[2] + of_wave[3], eps);
+  __syncthreads();
+  return info;
 }
 
 // Muon: whether any matrix's norm is not finite, before anything is written.
-__global__ __launch_bounds__(64) void k_norms(Table t, const double* __restrict__ partials, double eps,
+__global__ __launch_bounds__(256) void k_norms(Table t, const double* __restrict__ partials, double eps,
                                               int32_t* skip) {
   const Mat& m = t.m[blockIdx.x];
-  const Info f = info_of(total(partials + m.part0, m.parts), eps);
+  const Info f = info_by_block(partials + m.part0, m.parts, eps);
   if (threadIdx.x == 0 && f.bad) atomicOr(skip, 1);
 }
 
@@ -234,29 +246,28 @@ __global__ __launch_bounds__(256) void k_cast(Table t, short* __restrict__ ws, c
   const int i = find(t, blockIdx.x);
   const Mat& m = t.m[i];
   const int tile = blockIdx.x - t.tile0[i], tid = threadIdx.x;
-  const Info f = info_of(total(partials + m.part0, m.parts), eps);
-  if (tile == 0 && tid == 0) info[i] = f;
   const int tc = (m.l + kNormTile - 1) / kNormTile;  // X's tile, and where it lies in the matrix
   const int xr = tile / tc * kNormTile, xc = tile % tc * kNormTile;
   const int r0 = (m.tall ? xc : xr) + (tid >> 4), c = (m.tall ? xr : xc) + (tid & 15) * 4;
-  const bool vec = vectors<DT>(m);
   const float inv = MUON ? inverse_scale(ma) : 1.0f;
+  float u[4][4] = {}, buf[4][4];
+#pragma unroll
+  for (int k = 0; k < 4; k++)
+    if (r0 + 16 * k < m.rows && c < m.cols) update4<DT, MUON>(m, ma, inv, r0 + 16 * k, c, u[k], buf[k]);
+  const Info f = info_by_block(partials + m.part0, m.parts, eps);  // while the tile is on its way
+  if (tile == 0 && tid == 0) info[i] = f;
 #pragma unroll
   for (int k = 0; k < 4; k++) {
     const int r = r0 + 16 * k;
-    float u[4] = {0, 0, 0, 0}, buf[4];
     if (r < m.rows && c < m.cols) {
-      update4<DT, MUON>(m, ma, inv, r, c, vec, u, buf);
-      if (MUON)
-        for (int e = 0; e < 4; e++)
-          if (c + e < m.cols) m.momentum[(int64_t)r * m.cols + c + e] = buf[e];
-      for (int e = 0; e < 4; e++) u[e] = f.bad ? __builtin_nanf("") : c + e < m.cols ? u[e] * f.p : 0.0f;
+      if (MUON) store4(m.momentum + (int64_t)r * m.cols + c, m.cols - c, buf[k]);
+      for (int e = 0; e < 4; e++) u[k][e] = f.bad ? __builtin_nanf("") : c + e < m.cols ? u[k][e] * f.p : 0.0f;
     }
     s4v o, lo;
 #pragma unroll
     for (int e = 0; e < 4; e++) {
-      o[e] = F16::round(u[e]);
-      lo[e] = F16::round(u[e] - F16::widen(o[e]));
+      o[e] = F16::round(u[k][e]);
+      lo[e] = F16::round(u[k][e] - F16::widen(o[e]));
     }
     if (!m.tall) {
       if (r < m.s && c < m.l) {
@@ -592,14 +603,14 @@ struct SmallTile {
     *r = (m.tall ? x0 : 0) + (threadIdx.x >> 4) + 16 * k;
     *c = (m.tall ? 0 : x0) + (threadIdx.x & 15) * 4;
   }
-  __device__ inline void load(const Mat& m, const MuonArgs& ma, float inv, bool vec, int x0) {
+  __device__ inline void load(const Mat& m, const MuonArgs& ma, float inv, int x0) {
 #pragma unroll
     for (int k = 0; k < 4; k++) {
       int r, c;
       place(m, x0, k, &r, &c);
 #pragma unroll
       for (int e = 0; e < 4; e++) u[k][e] = 0.0f;
-      if (r < m.rows && c < m.cols) update4<DT, MUON>(m, ma, inv, r, c, vec, u[k], buf[k]);
+      if (r < m.rows && c < m.cols) update4<DT, MUON>(m, ma, inv, r, c, u[k], buf[k]);
     }
   }
   // Into x [row of X][column], rows LD apart.
@@ -628,17 +639,16 @@ __global__ __launch_bounds__(256) void k_small_gram(Table t, float* __restrict__
   const int i = find(t, blockIdx.x);
   const Mat& m = t.m[i];
   const int part = blockIdx.x - t.tile0[i], tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-  const bool vec = vectors<DT>(m);
   const float inv = MUON ? inverse_scale(ma) : 1.0f;
   const int tiles = (m.l + 63) / 64, lo = (int)((int64_t)tiles * part / m.parts),
             hi = (int)((int64_t)tiles * (part + 1) / m.parts), nb = (m.s + 15) / 16;
   f4acc acc[4] = {};
   SmallTile<DT, MUON> next;
-  next.load(m, ma, inv, vec, lo * 64);
+  next.load(m, ma, inv, lo * 64);
   for (int tile = lo; tile < hi; tile++) {
     __syncthreads();
     next.template store<kLdS>(m, tile * 64, x);
-    if (tile + 1 < hi) next.load(m, ma, inv, vec, (tile + 1) * 64);
+    if (tile + 1 < hi) next.load(m, ma, inv, (tile + 1) * 64);
     __syncthreads();
     if (w < nb)
 #pragma unroll 4
@@ -780,23 +790,20 @@ __global__ __launch_bounds__(256) void k_small_apply(Table t, const float* __res
   const Mat& m = t.m[i];
   const int x0 = (blockIdx.x - t.tile0[i]) * 64, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const int nb = (m.s + 15) / 16, n = nb * 16;
-  const bool vec = vectors<DT>(m);
   const float inv = MUON ? inverse_scale(ma) : 1.0f;
   for (int e = tid; e < n * n; e += 256) {
     const int r = e / n, c = e - r * n;
     q[r * kLdS + c] = ws[m.b + r * kSmall + c];
   }
   SmallTile<DT, MUON> tile;
-  tile.load(m, ma, inv, vec, x0);
+  tile.load(m, ma, inv, x0);
   tile.template store<kLdX>(m, x0, x);
   if (MUON)
 #pragma unroll
     for (int k = 0; k < 4; k++) {
       int r, c;
       tile.place(m, x0, k, &r, &c);
-#pragma unroll
-      for (int e = 0; e < 4; e++)
-        if (r < m.rows && c + e < m.cols) m.momentum[(int64_t)r * m.cols + c + e] = tile.buf[k][e];
+      if (r < m.rows) store4(m.momentum + (int64_t)r * m.cols + c, m.cols - c, tile.buf[k]);
     }
   __syncthreads();
   f4acc acc[4] = {};  // the wave's 16 columns
@@ -855,8 +862,7 @@ struct Source {  // one matrix of the caller's list
 };
 
 int32_t parts_of(int32_t rows, int32_t cols) {
-  const int64_t tiles = ceil_div(rows, kNormTile) * ceil_div(cols, kNormTile);
-  const int64_t p = ceil_div(tiles, 4);
+  const int64_t p = ceil_div(rows, kNormTile) * ceil_div(cols, kNormTile);
   return (int32_t)(p < 1 ? 1 : p > kMaxParts ? kMaxParts : p);
 }
 
@@ -1079,7 +1085,7 @@ int drive(const Source* src, int32_t count, int steps, const double* coef, doubl
         small_steps(t);
       } else {
         sums(t);
-        k_norms<<<t.n, 64, 0, s>>>(t, partials, eps, skip);
+        k_norms<<<t.n, 256, 0, s>>>(t, partials, eps, skip);
       }
     });
   } else {
