@@ -506,7 +506,7 @@ Shape shape_of(int64_t m, int64_t n, int64_t kt, bool pair, bool direct) {
   } else if (m <= 64) {
     s.tm = m <= 16 ? 16 : m <= 32 ? 32 : 64;
     // 4096 x 14336, 16 tokens forward: 82 us with 128 columns a tile, 94 with 64;
-    // 64 x 2048 x 8192 forward and backward: 104 and 96
+    // 64 x 2048 x 8192 forward and backward: 104 and 96 (two K tiles in shared memory)
     s.tn = m <= 16 ? 128 : 64;
     // A split writes and reads m n fp32 sums: at most half as many bytes as the
     // weights' own 2 n k. (Without the bound, 64 x 2048 x 8192: 135 us.)
@@ -516,11 +516,11 @@ Shape shape_of(int64_t m, int64_t n, int64_t kt, bool pair, bool direct) {
              n64 <= 4 * kCus && kt <= 96 && n64 * kt <= 128 * kCus) {
     // A product of at most about 128 K tiles of 64 x 64 a CU, four blocks to a
     // CU: larger tiles would have to be split over K and joined, or leave CUs
-    // idle. Forward, against 128-tiles: 256 x 1024 x 4096 24 us and 56,
-    // 2048 x 512 x 1024 23 and 36, 200 x 2048 x 5632 38 and 58. Beyond the bounds
+    // idle. Forward, against 128-tiles: 256 x 1024 x 4096 22 us and 56,
+    // 2048 x 512 x 1024 23 and 36, 200 x 2048 x 5632 37 and 58. Beyond the bounds
     // the twice as many loads cost more: forward and backward, with n64 <= 1024
-    // alone, 1024 x 2048 x 5632 takes 375 us (319 with 128-tiles) and
-    // 100 x 4096 x 14336 takes 398 (361).
+    // alone, 1024 x 2048 x 5632 takes 334 us (308 with 128-tiles) and
+    // 256 x 4096 x 14336 takes 561 (480).
     s.tm = s.tn = 64;
   } else {
     s.tm = s.tn = square_tile(ceil_div(m, 256) * ceil_div(cols, 256), ceil_div(m, 128) * ceil_div(cols, 128));
@@ -551,20 +551,27 @@ void launch_product(Product p, const Shape& s, bool direct, float* part, const E
   p.part = part;
   p.ldp = round_up(p.n, 8) * (PAIR ? 2 : 1);
   const dim3 grid((unsigned)(p.mt * p.nt * p.splits));
-#define DSX_RUN(TM, TN, WM, WN, DIRECT)                              \
+  // At most two blocks a CU of the 32- and 64-tiles: four K tiles in shared
+  // memory (forward, 64 x 2048 x 8192 33 us, 44 with two, 32 x 2048 x 8192 28 and
+  // 40; at three blocks a CU 200 x 2048 x 5632 takes 43, with two 37; the 16-tiles
+  // gain nothing: 5 x 4096 x 14336 71.5 and 70.9).
+  const bool deep = (int)grid.x <= 2 * kCus;
+#define DSX_RUN(TM, TN, WM, WN, DIRECT, STAGES)                      \
   do {                                                               \
-    using G = Gemm<T, TM, TN, WM, WN, RA, RB, DIRECT, PAIR>;         \
+    using G = Gemm<T, TM, TN, WM, WN, RA, RB, DIRECT, PAIR, STAGES>; \
     k_product<G, RA, RB, E><<<grid, G::THREADS, 0, st>>>(p, e);      \
   } while (0)
   if (direct) {
-    if (s.tm == 16) DSX_RUN(16, 128, 1, 4, true);
-    else if (s.tm == 32) DSX_RUN(32, 64, 2, 2, true);
-    else if (s.tm == 64) DSX_RUN(64, 64, 2, 2, true);
-    else if (s.tm == 128) DSX_RUN(128, 128, 2, 4, true);
-    else DSX_RUN(256, 256, 2, 4, true);
+    if (s.tm == 16) DSX_RUN(16, 128, 1, 4, true, 2);
+    else if (s.tm == 32 && deep) DSX_RUN(32, 64, 2, 2, true, 4);
+    else if (s.tm == 32) DSX_RUN(32, 64, 2, 2, true, 2);
+    else if (s.tm == 64 && deep) DSX_RUN(64, 64, 2, 2, true, 4);
+    else if (s.tm == 64) DSX_RUN(64, 64, 2, 2, true, 2);
+    else if (s.tm == 128) DSX_RUN(128, 128, 2, 4, true, 2);
+    else DSX_RUN(256, 256, 2, 4, true, 2);
   } else {
-    if (s.tm == 32) DSX_RUN(32, 128, 1, 4, false);
-    else DSX_RUN(128, 128, 2, 4, false);
+    if (s.tm == 32) DSX_RUN(32, 128, 1, 4, false, 2);
+    else DSX_RUN(128, 128, 2, 4, false, 2);
   }
 #undef DSX_RUN
   if (p.splits > 1)

@@ -9,9 +9,10 @@
 // registers by the transposing LDS read (16 lanes read a 4 x 16 block, each
 // lane gets one column of it).
 //
-// A block walks K in tiles of 64, two of them in shared memory: while the waves
-// multiply one, the other is filled by 16-byte loads that go straight to
-// shared memory (no registers, no LDS store instructions). A tile is kept in
+// A block walks K in tiles of 64, two of them in shared memory (four for few
+// small tiles, see Gemm): while the waves multiply one, the others are filled by
+// 16-byte loads that go straight to shared memory (no registers, no LDS store
+// instructions). A tile is kept in
 // 16-byte chunks at permuted places, so that the 16 lanes of a fragment read
 // fall on different banks; a direct load writes lane after lane, so it is the
 // global address that is permuted.
@@ -156,16 +157,26 @@ static __device__ inline s4v read_transposed(LdsBlock* __restrict__ p) {
 // The product tile: WM x WN waves of (TM/WM) x (TN/WN).
 // SPLIT: B's tile is two half tiles from two operands (the gate and the up
 // projection), and a wave's columns are half of one and half of the other.
-template <class T, int TM_, int TN_, int WM, int WN, bool RA, bool RB, bool DIRECT, bool SPLIT = false>
+// STAGES: K tiles in shared memory. Two suffice where the tile's products, or
+// other blocks on the CU, cover the next one's loads; where a launch has at most
+// two blocks of 64-tiles a CU each K tile waits for its loads, and four of them
+// hide that: A A of 1024 x 1024 with 784 (227 tiles) 12.3 us with two, 9.7 with
+// four; beyond two blocks a CU their shared memory costs more than it gives
+// (1001 x 2731, 688 tiles: 17.0 and 20.9).
+template <class T, int TM_, int TN_, int WM, int WN, bool RA, bool RB, bool DIRECT, bool SPLIT = false,
+          int STAGES = 2>
 struct Gemm {
   static constexpr int TM = TM_, TN = TN_, THREADS = WM * WN * 64;
   static constexpr int WTM = TM / WM, WTN = TN / WN, MF = WTM / 16, NF = WTN / 16;
   static constexpr int BROWS = SPLIT ? TN / 2 : TN;
+  template <int S>
+  using Staged = Gemm<T, TM_, TN_, WM, WN, RA, RB, DIRECT, SPLIT, S>;
   using SA = Stage<TM, RA, THREADS>;
   using SB = Stage<BROWS, RB, THREADS>;
   static constexpr int NB = SPLIT ? 2 : 1;
   static constexpr int kTile = SA::kBytes + NB * SB::kBytes;
-  static constexpr int kLds = 2 * kTile;
+  static constexpr int kLds = STAGES * kTile;
+  static_assert((STAGES & (STAGES - 1)) == 0 && (DIRECT || STAGES == 2), "slots by a mask; registers hold one tile");
   static constexpr int kWavesFit = 163840 / kLds * (WM * WN) / 4;
   static constexpr int kWavesPerSimd = kWavesFit < 4 ? kWavesFit : 4;
 
@@ -280,9 +291,19 @@ struct Gemm {
     return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
   }
 
-  // A barrier once this wave's direct loads have landed and its LDS reads are done.
-  static __device__ inline void sync_loads() {
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  // Waits until all but the last LEFT of this wave's direct loads have landed
+  // (they land in order) and its LDS reads are done.
+  template <int LEFT>
+  static __device__ inline void wait_loads() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LEFT) : "memory");
+  }
+  // A barrier after such a wait for the next tile, `after` more tiles being on
+  // their way behind it. The STAGES - 2 last of them may stay so.
+  __device__ inline void sync_loads(int after) const {
+    constexpr int ahead = STAGES - 2;
+    static_assert(STAGES == 2 || !(SA::kPart || SB::kPart), "as many loads in every wave");
+    if (ahead && after >= ahead) wait_loads<ahead * (SA::kInstr + NB * SB::kInstr)>();
+    else wait_loads<0>();
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
   }
@@ -402,17 +423,22 @@ struct Gemm {
         pb1 += sb1;
       };
       Frags f0, f1;
+      auto fill = [&](int t) {
+        const int left = K - t * kBK;
+        if (left < kBK) set(left);
+        load(lds + (t & (STAGES - 1)) * kTile);
+      };
       set(K);
-      load(lds);
-      sync_loads();
-      if (nt > 1) {
-        if (K - kBK < kBK) set(K - kBK);
-        load(lds + kTile);
-      }
+      fill(0);
+      if (STAGES == 2) sync_loads(0);
+#pragma unroll
+      for (int t = 1; t < STAGES; t++)
+        if (t < nt) fill(t);
+      if (STAGES > 2) sync_loads(nt >= STAGES ? nt : 0);
       auto tail = [&](int t) {
         const int left = K - t * kBK;
         if (left >= kBK) return;
-        char* cur = lds + (t & 1) * kTile;
+        char* cur = lds + (t & (STAGES - 1)) * kTile;
         zero_tail<SA>(cur, RA, left);
         zero_tail<SB>(cur + SA::kBytes, RB, left);
         if (SPLIT) zero_tail<SB>(cur + SA::kBytes + SB::kBytes, RB, left);
@@ -421,24 +447,19 @@ struct Gemm {
       if (nt == 1) tail(0);
       read(f0, lds, 0);
       for (int t = 0; t + 1 < nt; t++) {
-        char* cur = lds + (t & 1) * kTile;
-        char* nxt = lds + ((t + 1) & 1) * kTile;
+        char* cur = lds + (t & (STAGES - 1)) * kTile;
+        char* nxt = lds + ((t + 1) & (STAGES - 1)) * kTile;
         read(f1, cur, 1);
         multiply(f0);
         interleave();
-        sync_loads();  // all of this tile is in registers, all of the next in shared memory
-        if (t + 2 < nt) {
-          const int left = K - (t + 2) * kBK;
-          if (left < kBK) set(left);
-          load(cur);
-        } else {
-          tail(t + 1);
-        }
+        sync_loads(nt - t - 2);  // all of this tile is in registers, all of the next in shared memory
+        if (t + STAGES < nt) fill(t + STAGES);
+        if (t + 2 >= nt) tail(t + 1);
         read(f0, nxt, 0);
         multiply(f1);
         interleave();
       }
-      read(f1, lds + ((nt - 1) & 1) * kTile, 1);
+      read(f1, lds + ((nt - 1) & (STAGES - 1)) * kTile, 1);
       multiply(f0);
       multiply(f1);
     } else {

@@ -887,16 +887,16 @@ Plan each_run(const Source* src, int32_t count, F&& f) {
     auto flush = [&]() {
       if (t.n && !small) {
         // A Gram matrix of few 64-tiles leaves CUs idle while each walks all of
-        // l: its sums are split so that there are about two blocks a CU, eight
+        // l: its sums are split so that there are up to two blocks a CU, eight
         // K tiles each at least, and only below 160 tiles (65 x 8192: 326 us without,
         // 117 with; 1001 x 2731, 136 tiles: 277 and 247; 1024 x 784 with 1024 x 1024,
-        // 227 tiles: 12.0 us a launch without, 15.2 with).
+        // 227 tiles, two K tiles in shared memory: 12.0 us a launch without, 15.2 with).
         int64_t n = 0;
         auto tiles = [](const Mat& m) { return ceil_div(m.s, 64) * (ceil_div(m.s, 64) + 1) / 2; };
         for (int i = 0; i < t.n; i++) n += tiles(t.m[i]);
         for (int i = 0; i < t.n; i++) {
           Mat& m = t.m[i];
-          int64_t splits = n >= 160 ? 1 : ceil_div(512, n);
+          int64_t splits = n >= 160 ? 1 : 512 / n;
           if (splits > m.l / (8 * kBK)) splits = m.l / (8 * kBK);
           m.splits = (int32_t)(splits < 1 ? 1 : splits);
           m.part = at;
@@ -967,6 +967,14 @@ int64_t tiles_of(Table& t, F&& per) {
   return n;
 }
 
+// The 64-tiles of a launch of at most two blocks a CU keep four K tiles (Gemm).
+template <class G>
+using Deep = typename G::template Staged<G::TM == 64 ? 4 : 2>;
+template <class G>
+bool is_deep(int64_t blocks) {
+  return G::TM == 64 && blocks <= 512;
+}
+
 template <class G, bool GRAM>
 void launch_symmetric(Table& t, short* ws, const Info* info, int cur, int first, float b, float c, const int32_t* skip,
                       hipStream_t s) {
@@ -980,7 +988,12 @@ void launch_symmetric(Table& t, short* ws, const Info* info, int cur, int first,
     any = any || (SPLIT && m.splits > 1);
     return tiles(m) * (SPLIT ? m.splits : 1);
   });
-  k_symmetric<G, GRAM, SPLIT><<<dim3((unsigned)n), G::THREADS, 0, s>>>(t, ws, info, cur, first, b, c, skip);
+  auto go = [&](auto tile) {
+    using H = decltype(tile);
+    k_symmetric<H, GRAM, SPLIT><<<dim3((unsigned)n), H::THREADS, 0, s>>>(t, ws, info, cur, first, b, c, skip);
+  };
+  if (is_deep<G>(n)) go(Deep<G>{});
+  else go(G{});
   if (any) k_gram_join<<<dim3((unsigned)tiles_of(t, tiles)), 256, 0, s>>>(t, ws, info, first, skip);
 }
 
@@ -988,10 +1001,16 @@ template <class G, bool MUON>
 void launch_apply(Table& t, short* ws, const Info* info, int cur, int first, bool last, float a, int take_lo,
                   int give_lo, const MuonArgs& ma, int out_dt, hipStream_t s) {
   const int64_t n = tiles_of(t, [](const Mat& m) { return ceil_div(m.s, G::TM) * ceil_div(m.l, G::TN); });
-  if (last)
-    k_apply<G, true, MUON><<<dim3((unsigned)n), G::THREADS, 0, s>>>(t, ws, info, cur, first, a, take_lo, give_lo, ma, out_dt);
-  else
-    k_apply<G, false, false><<<dim3((unsigned)n), G::THREADS, 0, s>>>(t, ws, info, cur, first, a, take_lo, give_lo, ma, out_dt);
+  auto go = [&](auto tile) {
+    using H = decltype(tile);
+    const dim3 grid((unsigned)n);
+    if (last)
+      k_apply<H, true, MUON><<<grid, H::THREADS, 0, s>>>(t, ws, info, cur, first, a, take_lo, give_lo, ma, out_dt);
+    else
+      k_apply<H, false, false><<<grid, H::THREADS, 0, s>>>(t, ws, info, cur, first, a, take_lo, give_lo, ma, out_dt);
+  };
+  if (is_deep<G>(n)) go(Deep<G>{});
+  else go(G{});
 }
 
 // The square tile of a launch. Few tiles are bound by the latency of a K tile,
