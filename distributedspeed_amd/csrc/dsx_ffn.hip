@@ -17,7 +17,7 @@
 // fp32 value (16 bits and 8 bits in separate planes): kept in bf16 they would
 // add a rounding to both gradients as large as the one of dg and du to 16
 // bits, which the matrix instruction's types do demand. h, dg and du are
-// rounded to the inputs' type once.
+// rounded to the inputs' type once (but for up to three tokens' forward, k_few).
 //
 // Operands whose rows are not whole 16-byte chunks are copied first to rows
 // that are, where that pays (kRealignTokens).
@@ -161,12 +161,14 @@ struct Up {  // h and the factors from g and u
   typedef Nothing Raw;
   Saved s;
   int act, keep;
+  float* h32;  // for `one`: h unrounded, which the few tokens' second product takes
   __device__ inline Raw load(int, int) const { return {}; }
   __device__ inline void one(int m, int n, float g, float u) const {
     const int64_t at = m * s.ld + n;
     const ActValue a = activate(act, g);
-    s.h[at] = T::round(a.f * u);
+    h32[at] = a.f * u;
     if (keep) {
+      s.h[at] = T::round(a.f * u);
       const uint32_t p = top24(u * a.d), q = top24(a.f);
       s.p_hi[at] = (uint16_t)(p >> 16);
       s.p_lo[at] = (uint8_t)(p >> 8);
@@ -327,15 +329,42 @@ __global__ __launch_bounds__(256) void k_join(const float* __restrict__ part, in
 // of weights (one feature of the gate and the up projection, or two outputs)
 // and their products with each token's row, eight elements a lane and load,
 // sums in fp32. No shared memory, nothing split, and any alignment; the weights
-// are read past the caches, being used once. 4096 x 14336, bf16, 1 to 4 tokens:
-// 59, 62, 69 and 74 us (5.9 TB/s for one; 64 us through the caches); as matrix-
-// instruction tiles of 16 rows with split sums 68, 68, 70 and 71.
+// are read past the caches, being used once. No matrix instruction asks for 16
+// bits here, so the second product takes h in fp32 and y is rounded once; what
+// the backward keeps of h is 16 bits as ever. 4096 x 14336, bf16, 1 to 3 tokens:
+// 59, 62 and 71 us (5.9 TB/s for one; 64 us through the caches; with h in 16
+// bits 59, 62 and 68); as matrix-instruction tiles of 16 rows with split sums
+// 68, 68 and 70.
 constexpr int kFewTokens = 3;
 
-template <class T, int M, class E>
+struct Eight {
+  float v[8];
+};
+template <class T>
+__device__ inline Eight eight(const short* p) {
+  const s8v w = *(const s8u*)p;
+  Eight r;
+#pragma unroll
+  for (int j = 0; j < 8; j++) r.v[j] = T::widen(w[j]);
+  return r;
+}
+template <class T>
+__device__ inline Eight eight(const float* p) {
+  const f4v a = *(const f4u*)p, b = *(const f4u*)(p + 4);
+  return {{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]}};
+}
+template <class T>
+__device__ inline float element(const short* p) {
+  return T::widen(*p);
+}
+template <class T>
+__device__ inline float element(const float* p) {
+  return *p;
+}
+
+template <class T, int M, class X, class E>
 __global__ __launch_bounds__(256) void k_few(const short* __restrict__ w0, const short* __restrict__ w1, int64_t ld0,
-                                             int64_t ld1, const short* __restrict__ x, int64_t ld_x, int n, int k,
-                                             E e) {
+                                             int64_t ld1, const X* __restrict__ x, int64_t ld_x, int n, int k, E e) {
   const int lane = threadIdx.x & 63;
   const int i = blockIdx.x * 4 + (threadIdx.x >> 6);  // the pair of rows
   if (E::kPair ? i >= n : 2 * i >= n) return;
@@ -345,13 +374,13 @@ __global__ __launch_bounds__(256) void k_few(const short* __restrict__ w0, const
   float u[M], v[M];
 #pragma unroll
   for (int m = 0; m < M; m++) u[m] = v[m] = 0.0f;
-  auto add = [&](const s8v& a, const s8v& b, const s8v* c) {
+  auto add = [&](const s8v& a, const s8v& b, const Eight* c) {
 #pragma unroll
     for (int j = 0; j < 8; j++) {
       const float f = T::widen(a[j]), g = T::widen(b[j]);
 #pragma unroll
       for (int m = 0; m < M; m++) {
-        const float h = T::widen(c[m][j]);
+        const float h = c[m].v[j];
         u[m] = fmaf(f, h, u[m]);
         v[m] = fmaf(g, h, v[m]);
       }
@@ -360,21 +389,20 @@ __global__ __launch_bounds__(256) void k_few(const short* __restrict__ w0, const
   int c = lane * 8;
 #pragma unroll 4
   for (; c + 8 <= k; c += 512) {
-    s8v t[M];
+    Eight t[M];
     const s8v a = __builtin_nontemporal_load((const s8u*)(p + c)), b = __builtin_nontemporal_load((const s8u*)(q + c));
 #pragma unroll
-    for (int m = 0; m < M; m++) t[m] = *(const s8u*)(x + m * ld_x + c);
+    for (int m = 0; m < M; m++) t[m] = eight<T>(x + m * ld_x + c);
     add(a, b, t);
   }
   if (c < k) {  // the row's last elements
-    s8v a = {0, 0, 0, 0, 0, 0, 0, 0}, b = a, t[M];
-#pragma unroll
-    for (int m = 0; m < M; m++) t[m] = a;
+    s8v a = {0, 0, 0, 0, 0, 0, 0, 0}, b = a;
+    Eight t[M] = {};
     for (int j = 0; j < 8; j++)
       if (c + j < k) {
         a[j] = p[c + j];
         b[j] = q[c + j];
-        for (int m = 0; m < M; m++) t[m][j] = x[m * ld_x + c + j];
+        for (int m = 0; m < M; m++) t[m].v[j] = element<T>(x + m * ld_x + c + j);
       }
     add(a, b, t);
   }
@@ -693,6 +721,7 @@ int64_t workspace_of(const DsxFfn& q, bool backward) {
   const Sizes z = sizes_of(q);
   if (!z.m) return 256;
   int64_t bytes = part_of(q, backward) + 256;
+  if (!backward && z.m <= kFewTokens) bytes += z.m * z.ldf * 4;  // h
   if (backward) bytes += 2 * round_up(z.m * z.ldf * 2, 256) + realigned_bytes(z.m, z.d, z.d);
   if (realigns(z.m, backward))
     bytes += realigned_bytes(z.m, q.ld_x, z.d) + realigned_bytes(z.f, q.ld_gate, z.d) +
@@ -704,10 +733,11 @@ template <class T, int M>
 void forward_few(const DsxFfn& q, const Saved& s, void* y, int64_t ld_y, hipStream_t st) {
   const int d = (int)q.width, f = (int)q.inner;
   const short *wg = (const short*)q.w_gate, *wu = (const short*)q.w_up, *wd = (const short*)q.w_down;
-  k_few<T, M, Up<T>><<<dim3((unsigned)ceil_div(f, 4)), 256, 0, st>>>(wg, wu, q.ld_gate, q.ld_up, (const short*)q.x,
-                                                                     q.ld_x, f, d, Up<T>{s, q.activation, q.keep});
-  k_few<T, M, Store<T>><<<dim3((unsigned)ceil_div(d, 8)), 256, 0, st>>>(wd, wd, q.ld_down, q.ld_down, s.h, s.ld, d, f,
-                                                                        Store<T>{(short*)y, ld_y});
+  float* h = (float*)q.workspace;
+  k_few<T, M, short><<<dim3((unsigned)ceil_div(f, 4)), 256, 0, st>>>(
+      wg, wu, q.ld_gate, q.ld_up, (const short*)q.x, q.ld_x, f, d, Up<T>{s, q.activation, q.keep, h});
+  k_few<T, M, float><<<dim3((unsigned)ceil_div(d, 8)), 256, 0, st>>>(wd, wd, q.ld_down, q.ld_down, h, s.ld, d, f,
+                                                                     Store<T>{(short*)y, ld_y});
 }
 
 template <class T>
@@ -738,7 +768,7 @@ int forward(DsxFfn q, void* y, int64_t ld_y, hipStream_t st) {
   p.m = (int)z.m;
   p.n = (int)z.f;
   launch_product<T, true, true>(p, shape_of(z.m, z.f, z.kd, true, dir.up), dir.up, part,
-                                Up<T>{s, q.activation, q.keep}, st);
+                                Up<T>{s, q.activation, q.keep, nullptr}, st);
   Product r{};
   r.a[0] = {s.h, s.ld, (int)z.m};
   r.b[0] = {(const short*)q.w_down, q.ld_down, (int)z.d};

@@ -714,8 +714,8 @@ int64_t dsx_ffn_workspace_bytes(const DsxFfn* block /* host */,
                                 int32_t backward);
 
 /* y = (act(x w_gate^T) * (x w_up^T)) w_down^T, y [tokens][width] with row
- * stride ld_y. fp32 sums; h is rounded to `dtype`. No counterpart in the
- * reference. */
+ * stride ld_y. fp32 sums; h is rounded to `dtype`, but stays in fp32 for up to
+ * three tokens. No counterpart in the reference. */
 int dsx_ffn_forward(const DsxFfn* block /* host */, void* y, int64_t ld_y,
                     void* stream);
 

@@ -130,6 +130,20 @@ def test_rows_off_the_chunks(gpu, tokens, d, f, pad):
     _check(_run(*views, "silu"), want, 3 * U["bfloat16"])
 
 
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("tokens,d,f", [(1, 896, 320), (2, 520, 1027), (3, 129, 2048)])
+def test_few_tokens_are_rounded_once(gpu, tokens, d, f, dtype):
+    """Up to three tokens' forward is as far off as the exact result rounded to
+    the type: fp32 sums of a few thousand terms (relative 2^-24 each, 2^-17 at
+    most) move one element in about 2^8 over a rounding boundary; bound 5%."""
+    args = _make(tokens, d, f, dtype, seed=tokens + d + f)
+    _say(f"gated_ffn {tokens}x{d}x{f} {dtype}")
+    want = _exact(*args, "silu")[0]
+    got = _run(*args, "silu")[0].double()
+    once = (want.to(args[0].dtype).double() - want).norm()
+    assert (got - want).norm() <= 1.05 * once
+
+
 def test_gradients_against_differences(gpu):
     """(L(p + e v) - L(p - e v)) / 2e against <dL/dp, v> for L = <y, dy>, v
     with the parameter's own scale: at e = 1/32 the cubic term is of the order
