@@ -17,7 +17,7 @@
 // fp32 value (16 bits and 8 bits in separate planes): kept in bf16 they would
 // add a rounding to both gradients as large as the one of dg and du to 16
 // bits, which the matrix instruction's types do demand. h, dg and du are
-// rounded to the inputs' type once (but for up to three tokens' forward, k_few).
+// rounded to the inputs' type once (up to three tokens: k_few and WeightGrad).
 //
 // Operands whose rows are not whole 16-byte chunks are copied first to rows
 // that are, where that pays (kRealignTokens).
@@ -84,6 +84,7 @@ struct Saved {
   uint16_t* q_hi;
   uint8_t* p_lo;
   uint8_t* q_lo;
+  short* h_lo;  // up to kFewTokens: what h lost in rounding, as rows below h's
   int64_t ld;
 };
 
@@ -136,6 +137,14 @@ __device__ inline s8v round8(const float* v) {
   return w;
 }
 
+// What a rounded value lost, in the same type: together they hold 16 (bf16) or
+// 22 bits. Nothing beside an infinity or NaN.
+template <class T>
+__device__ inline short rest(float v) {
+  const float w = T::widen(T::round(v));
+  return T::round(__builtin_isfinite(w) ? v - w : 0.0f);
+}
+
 template <class T>
 struct Store {  // C in the inputs' type
   static constexpr bool kPair = false;
@@ -169,6 +178,7 @@ struct Up {  // h and the factors from g and u
     h32[at] = a.f * u;
     if (keep) {
       s.h[at] = T::round(a.f * u);
+      s.h_lo[at] = rest<T>(a.f * u);
       const uint32_t p = top24(u * a.d), q = top24(a.f);
       s.p_hi[at] = (uint16_t)(p >> 16);
       s.p_lo[at] = (uint8_t)(p >> 8);
@@ -208,6 +218,8 @@ struct Factors {  // dg and du from dh
   Saved s;
   short* dg;
   short* du;
+  short* dg_lo;  // up to kFewTokens (else null): what dg and du lost in rounding
+  short* du_lo;
   int rows, cols;
   __device__ inline Raw load(int m, int n) const {
     if (m >= rows || n >= cols) return {};
@@ -228,6 +240,16 @@ struct Factors {  // dg and du from dh
     }
     *(s8v*)(dg + at) = round8<T>(p);
     *(s8v*)(du + at) = round8<T>(q);
+    if (dg_lo) {
+      s8v a, b;
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        a[e] = rest<T>(p[e]);
+        b[e] = rest<T>(q[e]);
+      }
+      *(s8v*)(dg_lo + at) = a;
+      *(s8v*)(du_lo + at) = b;
+    }
   }
 };
 
@@ -431,6 +453,10 @@ __global__ __launch_bounds__(256) void k_few(const short* __restrict__ w0, const
 
 // ---- the weight gradients: up to three products over the tokens ------------
 
+// Of many tokens the rounding errors of dg, du and h average out in the sums;
+// of up to kFewTokens they would be as large as the gradients' own rounding, so
+// what those three lost is as many more rows of theirs, which meet x and dy a
+// second time within the one K tile.
 struct WeightGrad {
   Operand a, b;
   short* out;
@@ -466,7 +492,7 @@ __global__ DSX_TILE_KERNEL(G) void k_weight_grads(WeightGrads t) {
 // ---- operands off the direct loads' alignment --------------------------------
 
 // Rows of any length and stride to rows of whole 16-byte chunks, zeros past the
-// end; up to five matrices in one launch, a chunk a thread and pass.
+// end; up to seven matrices in one launch, a chunk a thread and pass.
 struct Realign {
   const short* from;
   short* to;
@@ -474,7 +500,7 @@ struct Realign {
   int rows, cols, block0;
 };
 struct Realigns {
-  Realign r[5];
+  Realign r[7];
   int count;
 };
 constexpr int kRealignChunks = 1024;  // of a block
@@ -629,6 +655,8 @@ Saved saved_of(const DsxFfn& q) {
   char* p = (char*)q.saved;
   s.ld = ld;
   s.h = (short*)p;
+  if (q.tokens <= kFewTokens) p += 2 * n;
+  s.h_lo = (short*)p;
   s.p_hi = (uint16_t*)(p + 2 * n);
   s.q_hi = (uint16_t*)(p + 4 * n);
   s.p_lo = (uint8_t*)(p + 6 * n);
@@ -677,6 +705,8 @@ int64_t realigned_bytes(int64_t rows, int64_t ld, int64_t cols) {
   return realigned(rows, ld, cols) ? round_up(rows * ld_inner(cols) * 2, 256) : 0;
 }
 
+int64_t twice_bytes(int64_t rows, int64_t cols) { return round_up(2 * rows * ld_inner(cols) * 2, 256); }
+
 // Collects the copies and puts the operands in their place.
 struct Realigner {
   bool wanted;
@@ -691,6 +721,17 @@ struct Realigner {
     *p = at;
     at += realigned_bytes(rows, *ld, *cols);
     *ld = *cols = ld_inner(*cols);
+  }
+  // Of few rows: two copies, one below the other.
+  void twice(const void** p, int64_t* ld, int64_t rows, int64_t* cols) {
+    const int64_t to = ld_inner(*cols);
+    for (int k = 0; k < 2; k++) {
+      t.r[t.count++] = {(const short*)*p, (short*)at + k * rows * to, *ld, (int)rows, (int)*cols, (int)blocks};
+      blocks += ceil_div(rows * to / 8, kRealignChunks);
+    }
+    *p = at;
+    at += twice_bytes(rows, *cols);
+    *ld = *cols = to;
   }
   void launch(hipStream_t st) {
     if (t.count) k_realign<<<dim3((unsigned)blocks), 256, 0, st>>>(t);
@@ -721,7 +762,8 @@ int64_t workspace_of(const DsxFfn& q, bool backward) {
   const Sizes z = sizes_of(q);
   if (!z.m) return 256;
   int64_t bytes = part_of(q, backward) + 256;
-  if (!backward && z.m <= kFewTokens) bytes += z.m * z.ldf * 4;  // h
+  if (z.m <= kFewTokens)  // h in fp32; what dg and du lost, and x and dy twice
+    bytes += backward ? 2 * round_up(z.m * z.ldf * 2, 256) + 2 * twice_bytes(z.m, z.d) : z.m * z.ldf * 4;
   if (backward) bytes += 2 * round_up(z.m * z.ldf * 2, 256) + realigned_bytes(z.m, z.d, z.d);
   if (realigns(z.m, backward))
     bytes += realigned_bytes(z.m, q.ld_x, z.d) + realigned_bytes(z.f, q.ld_gate, z.d) +
@@ -812,20 +854,28 @@ int backward(DsxFfn q, const void* dy, int64_t ld_dy, void* dx, int64_t ld_dx, v
              void* dw_down, hipStream_t st) {
   const Sizes z = sizes_of(q);
   const Saved s = saved_of(q);
-  const int64_t plane = round_up(z.m * z.ldf * 2, 256);
+  const bool few = z.m <= kFewTokens;
+  const int64_t plane = round_up(z.m * z.ldf * 2 * (few ? 2 : 1), 256);
   short* dg = (short*)q.workspace;
   short* du = (short*)((char*)q.workspace + plane);
+  short* dg_lo = few ? dg + z.m * z.ldf : nullptr;  // rows below
+  short* du_lo = few ? du + z.m * z.ldf : nullptr;
   float* part = (float*)((char*)q.workspace + 2 * plane);
   const int m = (int)z.m;
   Lengths len{z.d, z.d, z.d, z.f, z.d};
   Realigner copies{realigns(z.m, true), (char*)part + part_of(q, true), {}, 0};
-  if (dw_gate || dw_up) copies.add(&q.x, &q.ld_x, z.m, &len.x);
+  if (few) {
+    copies.twice(&q.x, &q.ld_x, z.m, &len.x);
+    copies.twice(&dy, &ld_dy, z.m, &len.dy);
+  } else {
+    if (dw_gate || dw_up) copies.add(&q.x, &q.ld_x, z.m, &len.x);
+    if (z.d % 8) copies.add(&dy, &ld_dy, z.m, &len.dy);  // the workspace's size knows the width, not this stride
+  }
   if (dx) {
     copies.add(&q.w_gate, &q.ld_gate, z.f, &len.gate);
     copies.add(&q.w_up, &q.ld_up, z.f, &len.up);
   }
   if (dx || dw_gate || dw_up) copies.add(&q.w_down, &q.ld_down, z.d, &len.down);
-  if (z.d % 8) copies.add(&dy, &ld_dy, z.m, &len.dy);  // the workspace's size knows the width, not this stride
   copies.launch(st);
   const Direct dir = direct_of(q, dy, ld_dy, len);
   if (dx || dw_gate || dw_up) {
@@ -836,8 +886,8 @@ int backward(DsxFfn q, const void* dy, int64_t ld_dy, void* dx, int64_t ld_dx, v
     p.segments = 1;
     p.m = m;
     p.n = (int)z.f;
-    launch_product<T, true, false>(p, shape_of(z.m, z.f, z.kd, false, dir.dh), dir.dh, part, Factors<T>{s, dg, du, m, (int)z.f},
-                                   st);
+    launch_product<T, true, false>(p, shape_of(z.m, z.f, z.kd, false, dir.dh), dir.dh, part,
+                                   Factors<T>{s, dg, du, dg_lo, du_lo, m, (int)z.f}, st);
   }
   if (dx) {
     Product r{};
@@ -853,7 +903,7 @@ int backward(DsxFfn q, const void* dy, int64_t ld_dy, void* dx, int64_t ld_dx, v
                                    Store<T>{(short*)dx, ld_dx}, st);
   }
   WeightGrads w{};
-  w.tokens = m;
+  w.tokens = few ? 2 * m : m;
   const Operand x{(const short*)q.x, q.ld_x, (int)z.d}, oy{(const short*)dy, ld_dy, (int)z.d};
   const Operand og{dg, z.ldf, (int)z.f}, ou{du, z.ldf, (int)z.f}, oh{s.h, s.ld, (int)z.f};
   if (dw_gate) w.w[w.count++] = {og, x, (short*)dw_gate, (int)z.f, (int)z.d, 0, 0};
@@ -901,7 +951,7 @@ extern "C" {
 int64_t dsx_ffn_saved_bytes(int64_t tokens, int64_t inner, int32_t keep) {
   if (tokens < 0 || inner < 1 || tokens > DSX_MATRIX_MAX_DIM || inner > DSX_MATRIX_MAX_DIM)
     return fail(-1, "dsx_ffn_saved_bytes: sizes out of range");
-  return tokens * ld_inner(inner) * (keep ? 8 : 2);
+  return tokens * ld_inner(inner) * (!keep ? 2 : tokens <= kFewTokens ? 10 : 8);
 }
 
 int64_t dsx_ffn_workspace_bytes(const DsxFfn* block, int32_t backward) {

@@ -144,6 +144,18 @@ def test_few_tokens_are_rounded_once(gpu, tokens, d, f, dtype):
     assert (got - want).norm() <= 1.05 * once
 
 
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("tokens,d,f", [(1, 896, 320), (2, 520, 1027), (3, 129, 2048), (1, 64, 8)])
+def test_few_tokens_weight_gradients_are_rounded_once(gpu, tokens, d, f, dtype):
+    """As above: dg, du and h enter with 16 bits (bf16) or 22, an error of 2^-8
+    of the result's own rounding or less."""
+    args = _make(tokens, d, f, dtype, seed=tokens + d + f)
+    _say(f"gated_ffn {tokens}x{d}x{f} {dtype}")
+    for name, got, want in zip(("gate", "up", "down"), _run(*args, "silu")[2:], _exact(*args, "silu")[2:]):
+        once = (want.to(args[0].dtype).double() - want).norm()
+        assert (got.double() - want).norm() <= 1.05 * once, name
+
+
 def test_gradients_against_differences(gpu):
     """(L(p + e v) - L(p - e v)) / 2e against <dL/dp, v> for L = <y, dy>, v
     with the parameter's own scale: at e = 1/32 the cubic term is of the order
