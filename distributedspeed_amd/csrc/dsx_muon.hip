@@ -888,9 +888,10 @@ Plan each_run(const Source* src, int32_t count, F&& f) {
       if (t.n && !small) {
         // A Gram matrix of few 64-tiles leaves CUs idle while each walks all of
         // l: its sums are split so that there are up to two blocks a CU, eight
-        // K tiles each at least, and only below 160 tiles (65 x 8192: 326 us without,
-        // 117 with; 1001 x 2731, 136 tiles: 277 and 247; 1024 x 784 with 1024 x 1024,
-        // 227 tiles, two K tiles in shared memory: 12.0 us a launch without, 15.2 with).
+        // K tiles each at least, and only below 160 tiles (65 x 8192: 326 us
+        // without, 117 with; 1001 x 2731, 136 tiles: 277 and 247; 1024 x 784 with
+        // 1024 x 1024, 227 tiles: 12.0 us a launch without, 15.2 with; all with
+        // two K tiles in shared memory).
         int64_t n = 0;
         auto tiles = [](const Mat& m) { return ceil_div(m.s, 64) * (ceil_div(m.s, 64) + 1) / 2; };
         for (int i = 0; i < t.n; i++) n += tiles(t.m[i]);
@@ -1015,8 +1016,8 @@ void launch_apply(Table& t, short* ws, const Info* info, int cur, int first, boo
 
 // The square tile of a launch. Few tiles are bound by the latency of a K tile,
 // not by products: 64-tiles while three a CU cover the launch (one 1001 x 2731:
-// 281 us with 64-tiles, 385 with 128; one 1024^2: 195 and 251; beyond it, as
-// for twelve 768^2, 308 and 297). Else a CU runs one block of 256 or 192 at a
+// 233 us with 64-tiles, 382 with 128; one 1024^2: 176 and 250; beyond it, as
+// for twelve 768^2, 297 and 279). Else a CU runs one block of 256 or 192 at a
 // time or two of 128, whose products take 1.2 times as long for the same area
 // (a lone block of 128 on a CU: 1.4 times), and the rounds over the CUs decide.
 // (The Gram matrix of 4096 x 14336: 136, 253 and 528 tiles, of which only the
