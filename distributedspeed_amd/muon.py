@@ -24,6 +24,7 @@ from ._lib import DsxMuonHyper, DsxMuonParam
 
 NS_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 _MATRIX = struct.Struct("=2Q4q")  # DsxMatrix of include/dsx.h
+_BUFFERS = ("momentum_buffer", "master")  # of a parameter's state: fp32, of its shape
 
 
 def _coefficients(coefficients, steps: int) -> tuple[tuple[float, float, float], ...]:
@@ -194,19 +195,36 @@ class MuonOptimizer(torch.optim.Optimizer):
                 raise ValueError("Muon's parameters must be contiguous")
 
     def _state_of(self, p: torch.Tensor) -> dict:
+        """p's buffers as the step needs them for p's type of now: a momentum,
+        and a master where p is 16-bit. The state may have been loaded from a
+        run of another type, or p cast since the last step: a 16-bit p without
+        a master begins one from its own values, an fp32 p takes the values of
+        a master left over and goes on without it. The kernels walk every
+        buffer by p's shape, so anything else is refused."""
         st = self.state[p]
-        if not st:
+        if "momentum_buffer" not in st:
             st["momentum_buffer"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
-            if p.dtype != torch.float32:
-                st["master"] = p.detach().float()
+        if p.dtype != torch.float32 and "master" not in st:
+            st["master"] = p.detach().float()
+        for key in _BUFFERS:
+            t = st.get(key)
+            if t is not None and (t.shape != p.shape or t.dtype != torch.float32 or t.device != p.device
+                                  or not t.is_contiguous()):
+                raise ValueError(f"{key} must be a contiguous fp32 tensor of shape {tuple(p.shape)} on {p.device}, got "
+                                 f"{t.dtype} {tuple(t.shape)} on {t.device}")
+        if p.dtype == torch.float32 and "master" in st:
+            p.copy_(st.pop("master"))
         return st
 
+    @torch.no_grad()
     def refresh_master(self) -> None:
         """Take the fp32 masters from the current params (after they were
         written from outside the step, as by a module's load_state_dict)."""
         for p, st in self.state.items():
-            if "master" in st:
-                st["master"].copy_(p.detach())
+            if p.dtype == torch.float32:
+                st.pop("master", None)
+            elif "master" in st:
+                st["master"].copy_(p)
 
     @torch.no_grad()
     def step(self, closure=None, *, grad_scale: torch.Tensor | None = None):
@@ -225,6 +243,9 @@ class MuonOptimizer(torch.optim.Optimizer):
                     continue
                 if p.grad.is_sparse:
                     raise RuntimeError("Muon does not support sparse gradients")
+                if p.grad.shape != p.shape or p.grad.device != p.device:
+                    raise ValueError(f"a grad of shape {tuple(p.grad.shape)} on {p.grad.device} for a parameter of "
+                                     f"shape {tuple(p.shape)} on {p.device}")
                 lists.setdefault((p.device, p.grad.dtype, p.dtype), []).append(p)
             for (dev, gdt, pdt), ps in lists.items():
                 self._step_list(g, dev, gdt, pdt, ps, grad_scale)
@@ -245,10 +266,10 @@ class MuonOptimizer(torch.optim.Optimizer):
             factor = (0.2 * math.sqrt(max(rows, cols)) if g["adjust_lr"] == "match_rms_adamw"
                       else math.sqrt(max(1.0, rows / cols)) if cols else 1.0)
             q.grad, q.momentum = gr.data_ptr(), st["momentum_buffer"].data_ptr()
-            if "master" in st:
-                q.master, q.param16 = st["master"].data_ptr(), p.data_ptr()
-            else:
+            if pdt == torch.float32:
                 q.master = p.data_ptr()
+            else:
+                q.master, q.param16 = st["master"].data_ptr(), p.data_ptr()
             q.ld_grad, q.rows, q.cols, q.lr = _row_stride(gr), rows, cols, lr * factor
         coef = (ctypes.c_double * (3 * steps))(*(v for r in _coefficients(g["ns_coefficients"], steps) for v in r))
         hyper = DsxMuonHyper(float(g["momentum"]), decay, float(g["eps"]), int(g["nesterov"]), steps)
@@ -268,13 +289,21 @@ class MuonOptimizer(torch.optim.Optimizer):
         return any(bool(s.item()) for s in self._skips)
 
     def load_state_dict(self, state_dict: dict) -> None:
-        """torch's, but the fp32 state stays fp32 for 16-bit parameters."""
+        """torch's, but the fp32 state stays fp32 for 16-bit parameters. A
+        buffer of another shape than its parameter's is refused (ValueError)
+        before anything changes. State of a run of another parameter type is
+        taken over by the next step (see _state_of)."""
+        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
+        pairs = [(p, state_dict["state"].get(i, {})) for i, p in
+                 zip(ids, (p for g in self.param_groups for p in g["params"]))]
+        for p, saved in pairs:
+            for key in _BUFFERS:
+                t = saved.get(key)
+                if t is not None and tuple(t.shape) != tuple(p.shape):
+                    raise ValueError(f"{key} has shape {tuple(t.shape)}, its parameter {tuple(p.shape)}")
         super().load_state_dict(state_dict)
-        saved = state_dict["state"]
-        index = 0
-        for g in self.param_groups:
-            for p in g["params"]:
-                for key, value in saved.get(index, {}).items():
-                    if isinstance(value, torch.Tensor):
-                        self.state[p][key] = value.detach().to(device=p.device, dtype=torch.float32, copy=True)
-                index += 1
+        for p, saved in pairs:
+            for key in _BUFFERS:
+                if saved.get(key) is not None:
+                    self.state[p][key] = saved[key].detach().to(device=p.device, dtype=torch.float32, copy=True,
+                                                                memory_format=torch.contiguous_format)

@@ -1,0 +1,98 @@
+"""MuonOptimizer steps after its state or its parameters changed their type,
+on the GPU against the step in 64 bits. Tolerance of a step: 15 roundings of
+2^-12 in the iteration, in units of the update's norm, and fp32's rounding of
+the weights (as for steps of one type)."""
+from __future__ import annotations
+
+import copy
+import math
+import sys
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+COEF = (3.4445, -4.7750, 2.0315)
+SHAPES = ((70, 50), (33, 129), (40, 40))
+
+
+def _say(msg):
+    print(f"[gpu-test] {msg}", file=sys.stderr, flush=True)
+
+
+def _exact(g):
+    x = g.double()
+    tall = x.shape[0] > x.shape[1]
+    x = x.t().contiguous() if tall else x
+    x = x / (x.norm() + 1e-7)
+    for _ in range(5):
+        p = x.mm(x.t().contiguous())
+        x = COEF[0] * x + (COEF[1] * p + COEF[2] * p.mm(p)).mm(x)
+    return x.t() if tall else x
+
+
+def _normal(gen, shape, std):
+    import torch
+    return torch.randn(shape, generator=gen, device="cuda") * std
+
+
+def _build(dtype, seed):
+    import torch
+    from distributedspeed_amd import MuonOptimizer
+    gen = torch.Generator("cuda").manual_seed(seed)
+    ps = [torch.nn.Parameter(_normal(gen, s, 0.05).to(getattr(torch, dtype))) for s in SHAPES]
+    return ps, MuonOptimizer(ps, lr=0.02, weight_decay=0.1), gen
+
+
+def _grads(ps, gen):
+    for p in ps:
+        p.grad = _normal(gen, p.shape, 1e-2).to(p.dtype)
+
+
+def _weights(opt, p):
+    return opt.state[p].get("master", p.detach()).double()
+
+
+def _step_and_check(opt, ps, weights, buffers):
+    """One step from the given fp64 weights and momenta."""
+    opt.step()
+    assert not opt.last_step_skipped()
+    for p, w, buf in zip(ps, weights, buffers):
+        g = p.grad.double()
+        buf = 0.95 * buf + 0.05 * g
+        factor = 0.02 * math.sqrt(max(1.0, p.shape[0] / p.shape[1]))
+        want = w * (1 - 0.02 * 0.1) - factor * _exact(0.95 * buf + 0.05 * g)
+        unit = factor * math.sqrt(min(p.shape))
+        assert (_weights(opt, p) - want).norm().item() <= 15 * 2.0 ** -12 * unit + 1e-6 * w.norm().item()
+        got = opt.state[p]["momentum_buffer"].double()
+        assert (got - buf).norm().item() <= 3 * 2.0 ** -23 * buf.norm().item()
+
+
+@pytest.mark.parametrize("saved", ["float32", "bfloat16", "float16"])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+def test_state_of_one_type_into_parameters_of_another(gpu, saved, dtype):
+    ps, opt, gen = _build(saved, 1)
+    _grads(ps, gen)
+    opt.step()
+    qs, other, gen2 = _build(dtype, 2)
+    other.load_state_dict(copy.deepcopy(opt.state_dict()))
+    _grads(qs, gen2)
+    _say(f"state of {saved} into {dtype}")
+    weights = [q.detach().double() if saved == "float32" else _weights(opt, p) for p, q in zip(ps, qs)]
+    _step_and_check(other, qs, weights, [opt.state[p]["momentum_buffer"].double() for p in ps])
+
+
+@pytest.mark.parametrize("before,after", [("float32", "bfloat16"), ("bfloat16", "float32"), ("float16", "bfloat16")])
+def test_parameters_cast_between_steps(gpu, before, after):
+    import torch
+    ps, opt, gen = _build(before, 3)
+    _grads(ps, gen)
+    opt.step()
+    kept = [_weights(opt, p) for p in ps]
+    for p in ps:
+        p.grad = None
+        p.data = p.data.to(getattr(torch, after))
+    weights = [p.detach().double() for p in ps] if before == "float32" else kept
+    _grads(ps, gen)
+    _say(f"{before} cast to {after}")
+    _step_and_check(opt, ps, weights, [opt.state[p]["momentum_buffer"].double() for p in ps])
