@@ -145,7 +145,8 @@ def orthogonalize(updates: torch.Tensor | Sequence[torch.Tensor], *, steps: int 
 
 
 class MuonOptimizer(torch.optim.Optimizer):
-    """Muon for matrix parameters, with torch.optim.Muon's arguments:
+    """Muon for matrix parameters, with torch.optim.Muon's arguments (but
+    adjust_lr, which is adjust_lr_fn there) and its state dicts:
 
         buf = momentum * buf + (1 - momentum) * grad
         u   = momentum * buf + (1 - momentum) * grad   (nesterov; else buf)
@@ -193,6 +194,15 @@ class MuonOptimizer(torch.optim.Optimizer):
                 raise ValueError(f"Muon steps matrices; got a parameter of shape {tuple(p.shape)}")
             if not p.is_contiguous():
                 raise ValueError("Muon's parameters must be contiguous")
+
+    def __setstate__(self, state: dict) -> None:
+        """Groups as this class has them, also from torch.optim.Muon's state
+        dict, whose adjust_lr_fn is adjust_lr here (None: "original")."""
+        super().__setstate__(state)
+        self._skips = []
+        for g in self.param_groups:
+            if "adjust_lr" not in g:
+                g["adjust_lr"] = g.pop("adjust_lr_fn", None) or "original"
 
     def _state_of(self, p: torch.Tensor) -> dict:
         """p's buffers as the step needs them for p's type of now: a momentum,

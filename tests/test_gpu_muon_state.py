@@ -96,3 +96,31 @@ def test_parameters_cast_between_steps(gpu, before, after):
     _grads(ps, gen)
     _say(f"{before} cast to {after}")
     _step_and_check(opt, ps, weights, [opt.state[p]["momentum_buffer"].double() for p in ps])
+
+
+@pytest.mark.parametrize("adjust", [None, "match_rms_adamw"])
+def test_goes_on_from_torchs_muon(gpu, adjust):
+    """torch.optim.Muon's state dict, then one step of each from there. Torch
+    rounds its input and three products a step to bf16 (2^-9 each): 16
+    roundings of 2^-9 beside this class's own."""
+    import torch
+    from distributedspeed_amd import MuonOptimizer
+    gen = torch.Generator("cuda").manual_seed(4)
+    ps = [torch.nn.Parameter(_normal(gen, s, 0.05)) for s in SHAPES]
+    theirs = torch.optim.Muon(ps, lr=0.02, weight_decay=0.1, adjust_lr_fn=adjust)
+    _grads(ps, gen)
+    theirs.step()
+    qs = [torch.nn.Parameter(p.detach().clone()) for p in ps]
+    opt = MuonOptimizer(qs)
+    opt.load_state_dict(copy.deepcopy(theirs.state_dict()))
+    _grads(ps, gen)
+    for p, q in zip(ps, qs):
+        q.grad = p.grad.clone()
+    _say(f"one step of each, adjust_lr_fn={adjust}")
+    theirs.step()
+    opt.step()
+    for p, q in zip(ps, qs):
+        factor = 0.2 * math.sqrt(max(p.shape)) if adjust else math.sqrt(max(1.0, p.shape[0] / p.shape[1]))
+        unit = 0.02 * factor * math.sqrt(min(p.shape))
+        far = (p.detach().double() - q.detach().double()).norm().item()
+        assert far <= (16 * 2.0 ** -9 + 15 * 2.0 ** -12) * unit + 1e-6 * p.detach().norm().item(), far / unit

@@ -93,6 +93,24 @@ def test_state_of_one_type_into_parameters_of_another(muon, saved, dtype):
         assert bool((weights == torch.tensor(0.7512 if saved != F32 else 0.5)).all())
 
 
+def test_state_of_torchs_muon(muon):
+    import torch
+    make, tables = muon
+    source = _params(BF16)
+    theirs = torch.optim.Muon(source, lr=0.125, weight_decay=0.25, adjust_lr_fn="match_rms_adamw")
+    for p in source:
+        theirs.state[p]["momentum_buffer"] = torch.full_like(p, 0.25)
+    params = _params(BF16)
+    opt = make(params, lr=0.01)
+    opt.load_state_dict(theirs.state_dict())
+    _grads(params)
+    opt.step()
+    _check_table(opt, params, tables[-1])
+    group = opt.param_groups[0]
+    assert group["lr"] == 0.125 and group["weight_decay"] == 0.25 and group["adjust_lr"] == "match_rms_adamw"
+    assert all(bool((opt.state[p]["momentum_buffer"] == 0.25).all()) for p in params)
+
+
 @pytest.mark.parametrize("before,after", [(F32, BF16), (BF16, F32), (BF16, F16)])
 def test_parameters_cast_between_steps(muon, before, after):
     import torch
