@@ -59,7 +59,8 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     type once. Rows may be strided; a tensor whose columns are not adjacent is
     copied first. Any number of tokens, none included.
 
-    Differentiable once in all four tensors. The backward keeps 8 bytes for
+    Differentiable once in all four tensors, backwards (a forward-mode tangent
+    is refused). The backward keeps 8 bytes for
     every token and inner feature; without gradients nothing is kept."""
     act = ACTIVATIONS.get(activation)
     if act is None:
@@ -106,7 +107,8 @@ def gated_residual_norm(residual: torch.Tensor, branch: torch.Tensor | None = No
     arithmetic is fp32 and rounded once; normed is taken from hidden before its
     rounding. Rows may be strided.
 
-    Differentiable once in all five tensors; the backward computes hidden again
+    Differentiable once in all five tensors, backwards (a forward-mode tangent
+    is refused); the backward computes hidden again
     from the inputs and keeps 8 bytes a row beside them."""
     if not isinstance(residual, torch.Tensor):
         raise TypeError("residual must be a tensor")

@@ -41,6 +41,13 @@ void check(const char* name, int rc) {
   if (rc) throw std::runtime_error(std::string(name) + " failed (status " + std::to_string(rc) + "): " + entry.last_error());
 }
 
+// The library's kernels see values alone: a forward-mode tangent of an input
+// would be lost on the way to the output, which reads as a tangent of zero.
+void refuse_tangent(const char* name, const Tensor& t) {
+  if (t.defined() && t._fw_grad(0).defined())
+    throw std::runtime_error(std::string(name) + " has no forward-mode derivative: an input carries a tangent");
+}
+
 int32_t code_of(at::ScalarType t) { return t == at::kFloat ? DSX_F32 : t == at::kHalf ? DSX_F16 : DSX_BF16; }
 
 // t [n, d], or a copy where its columns are not adjacent or its rows overlap.
@@ -153,6 +160,7 @@ struct GatedFfn : torch::autograd::Function<GatedFfn> {
 };
 
 Tensor gated_ffn(const Tensor& x, const Tensor& wg, const Tensor& wu, const Tensor& wd, int64_t act, int64_t stream) {
+  for (const Tensor* t : {&x, &wg, &wu, &wd}) refuse_tangent("gated_ffn", *t);
   if (at::GradMode::is_enabled() &&
       (x.requires_grad() || wg.requires_grad() || wu.requires_grad() || wd.requires_grad()))
     return GatedFfn::apply(x, wg, wu, wd, act, stream);
@@ -236,6 +244,7 @@ std::pair<Tensor, MaybeTensor> gated_residual_norm(const Tensor& residual, const
                                                    const MaybeTensor& next, double alpha, double beta, double eps,
                                                    int64_t stream) {
   Tensor in[5] = {residual, or_undefined(branch), or_undefined(post), or_undefined(gate), or_undefined(next)};
+  for (const auto& t : in) refuse_tangent("gated_residual_norm", t);
   bool wanted = false;
   for (const auto& t : in) wanted = wanted || (t.defined() && t.requires_grad());
   variable_list out = wanted && at::GradMode::is_enabled()
