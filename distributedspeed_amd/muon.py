@@ -18,6 +18,7 @@ import struct
 from typing import Sequence
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib, ops
 from ._lib import DsxMuonHyper, DsxMuonParam
@@ -66,6 +67,15 @@ def _matrices(updates, name: str) -> list[torch.Tensor]:
     return ms
 
 
+def _refuse_tracked(ts: list[torch.Tensor]) -> None:
+    """The kernels see values alone: a tensor that autograd follows, in either
+    direction, would lose its derivative without a word."""
+    tracked = torch.is_grad_enabled()
+    for t in ts:
+        if (tracked and t.requires_grad) or forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError("orthogonalize is not differentiable: pass t.detach(), or call it under torch.no_grad()")
+
+
 def _rows_contiguous(t: torch.Tensor) -> torch.Tensor:
     """t, or a copy where its columns are not adjacent or its rows overlap."""
     if not t.is_contiguous() and t.numel() and ((t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1])):
@@ -88,8 +98,9 @@ def orthogonalize(updates: torch.Tensor | Sequence[torch.Tensor], *, steps: int 
     keep the iterates' singular values below 4 (the iterates are fp16: their
     11 bits are why the result is bf16). A matrix whose norm is not finite
     becomes NaN; a zero matrix stays zero. A matrix whose columns are not
-    adjacent is copied first. Runs on the current stream without a host
-    synchronisation."""
+    adjacent is copied first. Not differentiable: a tensor that requires grad
+    (while grad mode is on) or carries a forward-mode tangent is refused. Runs
+    on the current stream without a host synchronisation."""
     steps, eps = _check_ns(steps, eps)
     rows = _coefficients(coefficients, steps)
     ms = _matrices(updates, "updates")
@@ -98,6 +109,7 @@ def orthogonalize(updates: torch.Tensor | Sequence[torch.Tensor], *, steps: int 
         if single:
             return updates.new_empty(updates.shape, dtype=torch.bfloat16) if out is None else out
         return []
+    _refuse_tracked(ms)
     dev = ops._device(ms[0])
     code = ops.grad_code(ms[0].dtype)
     for t in ms:
@@ -113,6 +125,7 @@ def orthogonalize(updates: torch.Tensor | Sequence[torch.Tensor], *, steps: int 
             result = outs = [torch.empty(t.shape, dtype=torch.bfloat16, device=dev) for t in ms]
     else:
         result, outs = out, _matrices(out, "out")
+        _refuse_tracked(outs)
         if len(outs) != len(ms):
             raise ValueError(f"out has {len(outs)} matrices, updates {len(ms)}")
         for t, o in zip(ms, outs):
