@@ -54,10 +54,10 @@ def _matrices(updates, name: str) -> list[torch.Tensor]:
     if isinstance(updates, torch.Tensor):
         if updates.dim() < 2:
             raise ValueError(f"{name} must have at least two dimensions, got {tuple(updates.shape)}")
-        if updates.dim() == 2:
-            return [updates]
-        flat = updates.flatten(0, -3) if updates.numel() else updates.reshape(-1, *updates.shape[-2:])
-        return list(flat.unbind(0))
+        ms = [updates]
+        for _ in range(updates.dim() - 2):  # views, whatever the batch dimensions' order in memory
+            ms = [u for t in ms for u in t.unbind(0)]
+        return ms
     ms = list(updates)
     for t in ms:
         if not isinstance(t, torch.Tensor):
@@ -126,6 +126,8 @@ def orthogonalize(updates: torch.Tensor | Sequence[torch.Tensor], *, steps: int 
     else:
         result, outs = out, _matrices(out, "out")
         _refuse_tracked(outs)
+        if isinstance(out, torch.Tensor) and any(n > 1 and k == 0 for n, k in zip(out.shape, out.stride())):
+            raise ValueError("out's matrices must not overlap")
         if len(outs) != len(ms):
             raise ValueError(f"out has {len(outs)} matrices, updates {len(ms)}")
         for t, o in zip(ms, outs):

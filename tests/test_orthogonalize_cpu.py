@@ -54,3 +54,30 @@ def test_inputs_whose_derivative_would_be_lost_are_refused(calls):
         assert not orthogonalize(p).requires_grad
         orthogonalize(g, out=torch.nn.Parameter(torch.ones(4, 6, dtype=torch.bfloat16)))
     assert len(calls) == 4
+
+
+@pytest.mark.parametrize("shape,order", [((4, 2, 5, 7), (1, 0, 2, 3)), ((2, 3, 4, 5, 6), (2, 0, 1, 3, 4)),
+                                         ((3, 5, 7), (0, 1, 2)), ((2, 2, 5, 7), (0, 1, 2, 3))])
+def test_out_is_written_where_it_lies(calls, shape, order):
+    """Batch dimensions in any order of memory: every matrix of `out` is a view of it."""
+    import torch
+    from distributedspeed_amd import orthogonalize
+    out = torch.zeros(shape, dtype=torch.bfloat16).permute(order)
+    updates = torch.ones(out.shape)
+    assert orthogonalize(updates, out=out) is out
+    rows, cols = out.shape[-2:]
+    batch = [[]]
+    for n in out.shape[:-2]:
+        batch = [b + [k] for b in batch for k in range(n)]
+    want = [(updates[tuple(b)].data_ptr(), out[tuple(b)].data_ptr(), cols, out.stride(-2), rows, cols) for b in batch]
+    assert calls[-1] == want
+
+
+def test_an_out_whose_matrices_share_memory_is_refused(calls):
+    import torch
+    from distributedspeed_amd import orthogonalize
+    with pytest.raises(ValueError, match="overlap"):
+        orthogonalize(torch.ones(3, 4, 5), out=torch.zeros(4, 5, dtype=torch.bfloat16).expand(3, 4, 5))
+    with pytest.raises(ValueError, match="overlap"):
+        orthogonalize(torch.ones(2, 3, 4, 5), out=torch.zeros(2, 1, 4, 5, dtype=torch.bfloat16).expand(2, 3, 4, 5))
+    assert not calls
