@@ -53,3 +53,14 @@ def test_out_with_batch_dimensions_in_any_order(gpu, n, m):
     for i in range(2):
         for j in range(4):
             assert _far(out[i, j], _exact(g[i, j])) <= _tol(5)
+
+
+def test_batches_of_empty_matrices(gpu):
+    import torch
+    from distributedspeed_amd import orthogonalize
+    for shape in ((2, 0, 4), (2, 4, 0), (2, 3, 0, 0), (0, 2, 3, 4)):
+        _say(f"empty {shape}")
+        assert orthogonalize(torch.ones(shape, device="cuda")).shape == shape
+    good = _normal((30, 20), 2)
+    got = orthogonalize([torch.ones(0, 4, device="cuda"), good, torch.ones(4, 0, device="cuda")])
+    assert _far(got[1], _exact(good)) <= _tol(5)

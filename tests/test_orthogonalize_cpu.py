@@ -81,3 +81,14 @@ def test_an_out_whose_matrices_share_memory_is_refused(calls):
     with pytest.raises(ValueError, match="overlap"):
         orthogonalize(torch.ones(2, 3, 4, 5), out=torch.zeros(2, 1, 4, 5, dtype=torch.bfloat16).expand(2, 3, 4, 5))
     assert not calls
+
+
+@pytest.mark.parametrize("shape", [(0, 4, 5), (2, 0, 4), (2, 4, 0), (2, 3, 0, 0), (0, 2, 3, 4), (2, 0, 3, 4), (0, 0, 4),
+                                   (0, 0)])
+def test_batches_of_empty_matrices_and_empty_batches(calls, shape):
+    import torch
+    from distributedspeed_amd import orthogonalize
+    got = orthogonalize(torch.ones(shape))
+    assert got.shape == shape and got.dtype == torch.bfloat16
+    out = torch.zeros(shape, dtype=torch.bfloat16)
+    assert orthogonalize(torch.ones(shape), out=out) is out
