@@ -38,8 +38,16 @@
 // times X0, so with P_k = a I + b A_k + c A_k^2 and A_{k+1} = P_k A_k P_k the
 // result is (P_K ... P_1) X0. Three launches: A0 in parts along the longer side,
 // everything s x s in one block's shared memory, and the product with X0.
-// (In 16 bits that recurrence would lose the small singular values, which A
-// holds squared; in fp32 it is 3e-4 off at worst over spectra of any kind.)
+// The recurrence is not stable: A0's rounding moves an eigenvalue near zero by
+// about 2^-24, each step multiplies that by a^2, and a negative one runs away.
+// So a run of steps ends where the product of their a^2 would pass 2^18
+// (small_run; five steps of Muon's coefficients just stay below): X is formed
+// in fp32 and the next run begins with its Gram matrix. Modelled in fp32
+// against 64 bits, 64 x 64, five steps: 3e-4 off for singular values spread over
+// 1e4, 1.4e-4 for rank four, 1e-5 for a random matrix; eight steps 4e-4, 7e-4
+// and 2e-5 (in one run 1.1e-1, 9e-3 and 8e-5; twelve in one run: NaN for rank
+// four). Where every X is formed, 5e-5, 7e-4 and 2e-6: the rest is the matrix's
+// own condition.
 
 #include <hip/hip_runtime.h>
 #include <math.h>
@@ -595,13 +603,25 @@ constexpr int kLdX = 80;          // the same for 4 rows and 16 columns
 constexpr int kSmallParts = 32;
 
 // 64 columns of X from `x0` on, as fp32: four values along the matrix's row in
-// each of four rows a thread, and their places in the tile.
-template <int DT, bool MUON>
+// each of four rows a thread, and their places in the tile. KEPT: of the X that
+// an earlier run of steps left in the workspace, s x l and never transposed.
+template <int DT, bool MUON, bool KEPT>
 struct SmallTile {
   float u[4][4], buf[4][4];
   static __device__ inline void place(const Mat& m, int x0, int k, int* r, int* c) {
-    *r = (m.tall ? x0 : 0) + (threadIdx.x >> 4) + 16 * k;
-    *c = (m.tall ? 0 : x0) + (threadIdx.x & 15) * 4;
+    const bool tall = !KEPT && m.tall;
+    *r = (tall ? x0 : 0) + (threadIdx.x >> 4) + 16 * k;
+    *c = (tall ? 0 : x0) + (threadIdx.x & 15) * 4;
+  }
+  __device__ inline void load_kept(const Mat& m, const float* ws, int x0) {
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      int r, c;
+      place(m, x0, k, &r, &c);
+      const f4v v = r < m.s && c < m.l ? *(const f4v*)(ws + m.x[0] + (int64_t)r * m.l + c) : f4v{0, 0, 0, 0};
+#pragma unroll
+      for (int e = 0; e < 4; e++) u[k][e] = v[e];
+    }
   }
   __device__ inline void load(const Mat& m, const MuonArgs& ma, float inv, int x0) {
 #pragma unroll
@@ -622,8 +642,8 @@ struct SmallTile {
       place(m, x0, k, &r, &c);
 #pragma unroll
       for (int e = 0; e < 4; e++) {
-        const float v = c + e < m.cols ? u[k][e] : 0.0f;
-        if (m.tall) x[(c + e) * LD + r - x0] = v;
+        const float v = KEPT || c + e < m.cols ? u[k][e] : 0.0f;
+        if (!KEPT && m.tall) x[(c + e) * LD + r - x0] = v;
         else x[r * LD + c - x0 + e] = v;
       }
     }
@@ -633,7 +653,7 @@ struct SmallTile {
 typedef float f4acc __attribute__((ext_vector_type(4)));
 
 // A0's partial sums over a run of X's columns: parts[part][64][64].
-template <int DT, bool MUON>
+template <int DT, bool MUON, bool KEPT>
 __global__ __launch_bounds__(256) void k_small_gram(Table t, float* __restrict__ ws, MuonArgs ma) {
   __shared__ float x[kSmall * kLdS];
   const int i = find(t, blockIdx.x);
@@ -643,12 +663,16 @@ __global__ __launch_bounds__(256) void k_small_gram(Table t, float* __restrict__
   const int tiles = (m.l + 63) / 64, lo = (int)((int64_t)tiles * part / m.parts),
             hi = (int)((int64_t)tiles * (part + 1) / m.parts), nb = (m.s + 15) / 16;
   f4acc acc[4] = {};
-  SmallTile<DT, MUON> next;
-  next.load(m, ma, inv, lo * 64);
+  SmallTile<DT, MUON, KEPT> next;
+  auto load = [&](int tile) {
+    if (KEPT) next.load_kept(m, ws, tile * 64);
+    else next.load(m, ma, inv, tile * 64);
+  };
+  load(lo);
   for (int tile = lo; tile < hi; tile++) {
     __syncthreads();
     next.template store<kLdS>(m, tile * 64, x);
-    if (tile + 1 < hi) next.load(m, ma, inv, (tile + 1) * 64);
+    if (tile + 1 < hi) load(tile + 1);
     __syncthreads();
     if (w < nb)
 #pragma unroll 4
@@ -703,10 +727,11 @@ struct SmallCoef {
   float c[3 * 64];
 };
 
-// All steps on A0 in shared memory; (P_K ... P_1) / |G| to ws + m.b. NB: 16-tiles a side.
+// A run of steps (from step k0 on) on its Gram matrix in shared memory;
+// P_K ... P_1, over |G| in the first run, to ws + m.b. NB: 16-tiles a side.
 template <int NB>
-__device__ inline void small_steps(const Mat& m, float* __restrict__ ws, const SmallCoef& coef, int steps, double eps,
-                                   int32_t* skip, float* A, float* P, float* T, float* Q, double& norm2) {
+__device__ inline void small_steps(const Mat& m, float* __restrict__ ws, const SmallCoef& coef, int k0, int steps,
+                                   double eps, int32_t* skip, float* A, float* P, float* T, float* Q, double& norm2) {
   const int tid = threadIdx.x, lane = tid & 63;
   constexpr int n = NB * 16;
   SmallProduct<NB> mul;
@@ -730,14 +755,14 @@ __device__ inline void small_steps(const Mat& m, float* __restrict__ ws, const S
   __syncthreads();
   const bool bad = !isfinite(norm2);
   if (bad && skip && tid == 0) atomicOr(skip, 1);
-  const double inv = bad ? __builtin_nan("") : 1.0 / (sqrt(norm2) + eps);
+  const double inv = bad ? __builtin_nan("") : k0 ? 1.0 : 1.0 / (sqrt(norm2) + eps);
   for (int e = tid; e < n * n; e += 640) {
     const int r = e / n, c = e - r * n;
     A[r * kLdS + c] = (float)(A[r * kLdS + c] * inv * inv);
   }
   __syncthreads();
   for (int k = 0; k < steps; k++) {
-    const float a = coef.c[3 * k], b = coef.c[3 * k + 1], c = coef.c[3 * k + 2];
+    const float a = coef.c[3 * (k0 + k)], b = coef.c[3 * (k0 + k) + 1], c = coef.c[3 * (k0 + k) + 2];
     f4acc p = mul(A, A);
     if (mul.on)
 #pragma unroll
@@ -770,21 +795,23 @@ __device__ inline void small_steps(const Mat& m, float* __restrict__ ws, const S
   }
 }
 
-__global__ __launch_bounds__(640) void k_small_steps(Table t, float* __restrict__ ws, SmallCoef coef, int steps,
-                                                     double eps, int32_t* skip) {
+__global__ __launch_bounds__(640) void k_small_steps(Table t, float* __restrict__ ws, SmallCoef coef, int k0,
+                                                     int steps, double eps, int32_t* skip) {
   __shared__ float A[kSmall * kLdS], P[kSmall * kLdS], T[kSmall * kLdS], Q[kSmall * kLdS];
   __shared__ double norm2;
   const Mat& m = t.m[blockIdx.x];
-  if (m.s <= 16) small_steps<1>(m, ws, coef, steps, eps, skip, A, P, T, Q, norm2);
-  else if (m.s <= 32) small_steps<2>(m, ws, coef, steps, eps, skip, A, P, T, Q, norm2);
-  else if (m.s <= 48) small_steps<3>(m, ws, coef, steps, eps, skip, A, P, T, Q, norm2);
-  else small_steps<4>(m, ws, coef, steps, eps, skip, A, P, T, Q, norm2);
+  if (m.s <= 16) small_steps<1>(m, ws, coef, k0, steps, eps, skip, A, P, T, Q, norm2);
+  else if (m.s <= 32) small_steps<2>(m, ws, coef, k0, steps, eps, skip, A, P, T, Q, norm2);
+  else if (m.s <= 48) small_steps<3>(m, ws, coef, k0, steps, eps, skip, A, P, T, Q, norm2);
+  else small_steps<4>(m, ws, coef, k0, steps, eps, skip, A, P, T, Q, norm2);
 }
 
-// The result's 64 columns: (P_K ... P_1 / |G|) X, to the output or the parameters.
-template <int DT, bool MUON>
-__global__ __launch_bounds__(256) void k_small_apply(Table t, const float* __restrict__ ws, MuonArgs ma, int out_dt) {
-  __shared__ float q[kSmall * kLdS], x[kSmall * kLdX];
+// 64 columns of the product of a run's P_K ... P_1 and X: the result, to the
+// output or the parameters, after the LAST run, else the next run's X (a block
+// reads and writes its own columns alone).
+template <int DT, bool MUON, bool KEPT, bool LAST>
+__global__ __launch_bounds__(256) void k_small_apply(Table t, float* __restrict__ ws, MuonArgs ma, int out_dt) {
+  __shared__ __attribute__((aligned(16))) float q[kSmall * kLdS], x[kSmall * kLdX];
   if (MUON && *ma.skip) return;
   const int i = find(t, blockIdx.x);
   const Mat& m = t.m[i];
@@ -795,10 +822,11 @@ __global__ __launch_bounds__(256) void k_small_apply(Table t, const float* __res
     const int r = e / n, c = e - r * n;
     q[r * kLdS + c] = ws[m.b + r * kSmall + c];
   }
-  SmallTile<DT, MUON> tile;
-  tile.load(m, ma, inv, x0);
+  SmallTile<DT, MUON, KEPT> tile;
+  if (KEPT) tile.load_kept(m, ws, x0);
+  else tile.load(m, ma, inv, x0);
   tile.template store<kLdX>(m, x0, x);
-  if (MUON)
+  if (MUON && !KEPT)
 #pragma unroll
     for (int k = 0; k < 4; k++) {
       int r, c;
@@ -821,8 +849,17 @@ __global__ __launch_bounds__(256) void k_small_apply(Table t, const float* __res
   for (int j = 0; j < 4; j++)
 #pragma unroll
     for (int e = 0; e < 4; e++)
-      x[(j * 16 + (lane >> 4) * 4 + e) * kLdX + w * 16 + (lane & 15)] = acc[j][e] * kScale;
+      x[(j * 16 + (lane >> 4) * 4 + e) * kLdX + w * 16 + (lane & 15)] = acc[j][e] * (LAST ? kScale : 1.0f);
   __syncthreads();
+  if (!LAST) {
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      const int r = (tid >> 4) + 16 * k, c = (tid & 15) * 4;
+      if (r < m.s && x0 + c < m.l)
+        *(f4v*)(ws + m.x[0] + (int64_t)r * m.l + x0 + c) = *(const f4v*)&x[r * kLdX + c];
+    }
+    return;
+  }
   // eight values of a row of the matrix a thread
 #pragma unroll
   for (int k = 0; k < 2; k++) {
@@ -932,7 +969,8 @@ Plan each_run(const Source* src, int32_t count, F&& f) {
         m.parts = (int32_t)(p > kSmallParts ? kSmallParts : p);
         m.a = at;
         m.b = at + (int64_t)m.parts * kSmall * kSmall;
-        at = m.b + kSmall * kSmall;
+        m.x[0] = m.b + kSmall * kSmall;
+        at = m.x[0] + round_up((int64_t)m.s * m.l, 64);
       } else {
         const int64_t x = round_up((int64_t)m.s * m.l, 128), sq = round_up((int64_t)m.s * m.s, 128);
         m.x[0] = at;
@@ -1061,6 +1099,18 @@ void iterate(Table& t, short* ws, const Info* info, int steps, const double* coe
   }
 }
 
+// Steps from k0 on that one Gram matrix carries: see the top of this file.
+int small_run(const double* coef, int k0, int steps) {
+  double growth = 1.0;
+  int n = 0;
+  for (; k0 + n < steps; n++) {
+    const double a = coef[3 * (k0 + n)];
+    if (a * a > 1.0) growth *= a * a;
+    if (n && growth > 262144.0) break;
+  }
+  return n;
+}
+
 template <int DT, bool MUON>
 int drive(const Source* src, int32_t count, int steps, const double* coef, double eps, MuonArgs ma, int out_dt,
           char* base, int64_t bytes, const char* what, hipStream_t s) {
@@ -1076,14 +1126,22 @@ int drive(const Source* src, int32_t count, int steps, const double* coef, doubl
   ma.skip = MUON ? skip : nullptr;
   SmallCoef sc{};
   for (int k = 0; k < 3 * steps; k++) sc.c[k] = (float)coef[k];
-  auto small_steps = [&](Table& t) {
-    const int64_t n = tiles_of(t, [](const Mat& m) { return (int64_t)m.parts; });
-    k_small_gram<DT, MUON><<<dim3((unsigned)n), 256, 0, s>>>(t, (float*)run, ma);
-    k_small_steps<<<t.n, 640, 0, s>>>(t, (float*)run, sc, steps, eps, ma.skip);
+  // The run of steps from k0 on, without its product; the flag is the input's alone.
+  auto small_steps = [&](Table& t, int k0) {
+    const dim3 grid((unsigned)tiles_of(t, [](const Mat& m) { return (int64_t)m.parts; }));
+    const int n = small_run(coef, k0, steps);
+    if (k0) k_small_gram<DSX_F32, false, true><<<grid, 256, 0, s>>>(t, (float*)run, ma);
+    else k_small_gram<DT, MUON, false><<<grid, 256, 0, s>>>(t, (float*)run, ma);
+    k_small_steps<<<t.n, 640, 0, s>>>(t, (float*)run, sc, k0, n, eps, k0 ? nullptr : ma.skip);
+    return k0 + n;
   };
-  auto small_apply = [&](Table& t) {
-    const int64_t n = tiles_of(t, [](const Mat& m) { return ceil_div(m.l, 64); });
-    k_small_apply<DT, MUON><<<dim3((unsigned)n), 256, 0, s>>>(t, (const float*)run, ma, out_dt);
+  auto small_apply = [&](Table& t, int k0, bool last) {
+    const dim3 grid((unsigned)tiles_of(t, [](const Mat& m) { return ceil_div(m.l, 64); }));
+    float* ws = (float*)run;
+    if (k0 && last) k_small_apply<DSX_F32, MUON, true, true><<<grid, 256, 0, s>>>(t, ws, ma, out_dt);
+    else if (k0) k_small_apply<DSX_F32, MUON, true, false><<<grid, 256, 0, s>>>(t, ws, ma, out_dt);
+    else if (last) k_small_apply<DT, MUON, false, true><<<grid, 256, 0, s>>>(t, ws, ma, out_dt);
+    else k_small_apply<DT, MUON, false, false><<<grid, 256, 0, s>>>(t, ws, ma, out_dt);
   };
   auto sums = [&](Table& t) {
     const int64_t n = tiles_of(t, [](const Mat& m) { return (int64_t)m.parts; });
@@ -1102,7 +1160,7 @@ int drive(const Source* src, int32_t count, int steps, const double* coef, doubl
     k_clear<<<1, 1, 0, s>>>(skip);
     each_run(src, count, [&](Table& t, int, bool small) {
       if (small) {
-        small_steps(t);
+        small_steps(t, 0);
       } else {
         sums(t);
         k_norms<<<t.n, 256, 0, s>>>(t, partials, eps, skip);
@@ -1115,8 +1173,11 @@ int drive(const Source* src, int32_t count, int steps, const double* coef, doubl
   }
   each_run(src, count, [&](Table& t, int at, bool small) {
     if (small) {
-      small_steps(t);
-      small_apply(t);
+      for (int k = 0; k < steps;) {
+        const int next = small_steps(t, k);
+        small_apply(t, k, next == steps);
+        k = next;
+      }
     } else {
       rest(t, at);
     }
