@@ -48,6 +48,10 @@
 // and 2e-5 (in one run 1.1e-1, 9e-3 and 8e-5; twelve in one run: NaN for rank
 // four). Where every X is formed, 5e-5, 7e-4 and 2e-6: the rest is the matrix's
 // own condition.
+// The squares of an fp32 or bf16 matrix may leave fp32's range at either end: the
+// input is taken times a power of two, which changes no bit of the result, such
+// that no value is above 1 (each part of A0 with its own, joined where the parts
+// are added).
 
 #include <hip/hip_runtime.h>
 #include <math.h>
@@ -86,7 +90,7 @@ struct Mat {
   int32_t tall;         // X is the matrix transposed
   int32_t splits;       // of the Gram matrix's sums along l, into ws + part (fp32, a 64-tile after another)
   int64_t part;
-  int64_t diag;         // the diagonals of A and of B, s fp32 each
+  int64_t diag;         // the diagonals of A and of B, s fp32 each (a short side: exponents)
   int32_t part0, parts;
   float   lr;           // Muon: the step size of this matrix
 };
@@ -601,6 +605,7 @@ constexpr int kSmall = 64;       // X's rows, padded
 constexpr int kLdS = kSmall + 4;  // floats: a fragment's 16 rows and 4 columns fall on 64 banks
 constexpr int kLdX = 80;          // the same for 4 rows and 16 columns
 constexpr int kSmallParts = 32;
+constexpr int kNoExponent = -200;  // of zeros: below every fp32's
 
 // 64 columns of X from `x0` on, as fp32: four values along the matrix's row in
 // each of four rows a thread, and their places in the tile. KEPT: of the X that
@@ -633,16 +638,25 @@ struct SmallTile {
       if (r < m.rows && c < m.cols) update4<DT, MUON>(m, ma, inv, r, c, u[k], buf[k]);
     }
   }
-  // Into x [row of X][column], rows LD apart.
+  // The largest magnitude (a NaN aside, which stays one at any scale).
+  __device__ inline float most() const {
+    float v = 0;
+#pragma unroll
+    for (int k = 0; k < 4; k++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) v = fmaxf(v, fabsf(u[k][e]));
+    return v;
+  }
+  // Times 2^-scale into x [row of X][column], rows LD apart; KEPT as it is.
   template <int LD>
-  __device__ inline void store(const Mat& m, int x0, float* x) const {
+  __device__ inline void store(const Mat& m, int x0, float* x, int scale) const {
 #pragma unroll
     for (int k = 0; k < 4; k++) {
       int r, c;
       place(m, x0, k, &r, &c);
 #pragma unroll
       for (int e = 0; e < 4; e++) {
-        const float v = KEPT || c + e < m.cols ? u[k][e] : 0.0f;
+        const float v = KEPT ? u[k][e] : c + e < m.cols ? ldexpf(u[k][e], -scale) : 0.0f;
         if (!KEPT && m.tall) x[(c + e) * LD + r - x0] = v;
         else x[r * LD + c - x0 + e] = v;
       }
@@ -652,10 +666,11 @@ struct SmallTile {
 
 typedef float f4acc __attribute__((ext_vector_type(4)));
 
-// A0's partial sums over a run of X's columns: parts[part][64][64].
+// The partial sums of X X^T over a run of X's columns: parts[part][64][64], and
+// the exponent of two that a part's values were divided by.
 template <int DT, bool MUON, bool KEPT>
 __global__ __launch_bounds__(256) void k_small_gram(Table t, float* __restrict__ ws, MuonArgs ma) {
-  __shared__ float x[kSmall * kLdS];
+  __shared__ float x[kSmall * kLdS], of_wave[4];
   const int i = find(t, blockIdx.x);
   const Mat& m = t.m[i];
   const int part = blockIdx.x - t.tile0[i], tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
@@ -669,9 +684,27 @@ __global__ __launch_bounds__(256) void k_small_gram(Table t, float* __restrict__
     else next.load(m, ma, inv, tile * 64);
   };
   load(lo);
+  int scale = kNoExponent;
   for (int tile = lo; tile < hi; tile++) {
+    if (!KEPT) {
+      float most = next.most();
+      for (int d = 32; d; d >>= 1) most = fmaxf(most, __shfl_xor(most, d));
+      if (lane == 0) of_wave[w] = most;
+    }
     __syncthreads();
-    next.template store<kLdS>(m, tile * 64, x);
+    if (!KEPT) {
+      const float most = fmaxf(fmaxf(of_wave[0], of_wave[1]), fmaxf(of_wave[2], of_wave[3]));
+      int e = kNoExponent;
+      if (most > 0.0f) frexpf(most, &e);
+      if (e > scale) {  // what is summed already goes on at the tile's scale
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+#pragma unroll
+          for (int v = 0; v < 4; v++) acc[j][v] = ldexpf(acc[j][v], 2 * (scale - e));
+        scale = e;
+      }
+    }
+    next.template store<kLdS>(m, tile * 64, x, scale);
     if (tile + 1 < hi) load(tile + 1);
     __syncthreads();
     if (w < nb)
@@ -685,6 +718,7 @@ __global__ __launch_bounds__(256) void k_small_gram(Table t, float* __restrict__
                                                           acc[j], 0, 0, 0);
       }
   }
+  if (!KEPT && tid == 0) ((int*)(ws + m.diag))[part] = scale;
   float* out = ws + m.a + (int64_t)part * kSmall * kSmall;
   if (w < nb)
 #pragma unroll
@@ -728,7 +762,8 @@ struct SmallCoef {
 };
 
 // A run of steps (from step k0 on) on its Gram matrix in shared memory;
-// P_K ... P_1, over |G| in the first run, to ws + m.b. NB: 16-tiles a side.
+// P_K ... P_1, over |G| (at the input's scale) in the first run, to ws + m.b. NB:
+// 16-tiles a side.
 template <int NB>
 __device__ inline void small_steps(const Mat& m, float* __restrict__ ws, const SmallCoef& coef, int k0, int steps,
                                    double eps, int32_t* skip, float* A, float* P, float* T, float* Q, double& norm2) {
@@ -739,11 +774,21 @@ __device__ inline void small_steps(const Mat& m, float* __restrict__ ws, const S
   mul.lane = lane;
   mul.on = mul.tj < NB;
   const float* in = ws + m.a;
+  int* exps = (int*)(ws + m.diag);
+  int scale = 0, shift = 0;  // the matrix's exponent; twice a part's below it, in lane `part`
+  if (!k0) {
+    const int e = lane < m.parts ? exps[lane] : kNoExponent;
+    scale = e;
+    for (int d = 32; d; d >>= 1) scale = max(scale, __shfl_xor(scale, d));
+    shift = 2 * (e - scale);
+    if (tid == 0) exps[kSmallParts] = scale;
+  }
   for (int e = tid; e < n * n; e += 640) {
     const int r = e / n, c = e - r * n;
     float sum = 0;
 #pragma unroll 8
-    for (int p = 0; p < m.parts; p++) sum += in[(int64_t)p * kSmall * kSmall + r * kSmall + c];
+    for (int p = 0; p < m.parts; p++)
+      sum += ldexpf(in[(int64_t)p * kSmall * kSmall + r * kSmall + c], __builtin_amdgcn_readlane(shift, p));
     A[r * kLdS + c] = sum;
   }
   __syncthreads();
@@ -755,7 +800,7 @@ __device__ inline void small_steps(const Mat& m, float* __restrict__ ws, const S
   __syncthreads();
   const bool bad = !isfinite(norm2);
   if (bad && skip && tid == 0) atomicOr(skip, 1);
-  const double inv = bad ? __builtin_nan("") : k0 ? 1.0 : 1.0 / (sqrt(norm2) + eps);
+  const double inv = bad ? __builtin_nan("") : k0 ? 1.0 : 1.0 / (sqrt(norm2) + ldexp(eps, -scale));  // 2^scale / (|G| + eps)
   for (int e = tid; e < n * n; e += 640) {
     const int r = e / n, c = e - r * n;
     A[r * kLdS + c] = (float)(A[r * kLdS + c] * inv * inv);
@@ -825,7 +870,7 @@ __global__ __launch_bounds__(256) void k_small_apply(Table t, float* __restrict_
   SmallTile<DT, MUON, KEPT> tile;
   if (KEPT) tile.load_kept(m, ws, x0);
   else tile.load(m, ma, inv, x0);
-  tile.template store<kLdX>(m, x0, x);
+  tile.template store<kLdX>(m, x0, x, KEPT ? 0 : ((const int*)(ws + m.diag))[kSmallParts]);
   if (MUON && !KEPT)
 #pragma unroll
     for (int k = 0; k < 4; k++) {
@@ -969,7 +1014,8 @@ Plan each_run(const Source* src, int32_t count, F&& f) {
         m.parts = (int32_t)(p > kSmallParts ? kSmallParts : p);
         m.a = at;
         m.b = at + (int64_t)m.parts * kSmall * kSmall;
-        m.x[0] = m.b + kSmall * kSmall;
+        m.diag = m.b + kSmall * kSmall;  // the parts' exponents and the matrix's
+        m.x[0] = m.diag + 64;
         at = m.x[0] + round_up((int64_t)m.s * m.l, 64);
       } else {
         const int64_t x = round_up((int64_t)m.s * m.l, 128), sq = round_up((int64_t)m.s * m.s, 128);

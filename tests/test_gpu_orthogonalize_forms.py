@@ -151,3 +151,72 @@ def test_muon_steps_of_many_iterations(gpu):
         want = _exact(p.grad * 0.0975, (COEF,) * 12)  # (1 - mu^2) g of a first Nesterov step
         inside = [u.t().contiguous().mm(t).mm(v.t().contiguous()) for t in (o, want)]
         assert _far(*inside) <= 2.0 ** -8
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("n,m", [(64, 1024), (1024, 40), (16, 16), (5, 3000), (96, 200), (300, 130)])
+def test_scale_does_not_matter_at_either_end(gpu, n, m, dtype):
+    """Entries from 1e-30 to 1e37 (their squares leave fp32's range from 1e-19
+    down and 1e19 up), in a list and alone, eps far below or, at 1e-19 and
+    below, beside and above the norm. A short side takes a power of two out, so
+    that its bits are the scaled matrix's own. With a longer one the iterates
+    are fp16 times 4096: where the norm is far below eps, they lose bits to
+    their range, so that those scales are left to the short sides."""
+    import torch
+    from distributedspeed_amd import orthogonalize
+    base = _normal((n, m), 31, dtype).clamp_(-8, 8)
+    small = min(n, m) <= 64
+    for power in (-100, -80, -67, -63, -40, 40, 63, 80, 120):
+        if not small and power < -50:
+            continue
+        g = (base.double() * 2.0 ** power).to(base.dtype)
+        _say(f"{n}x{m} {dtype} times 2^{power}")
+        got = orthogonalize(g, eps=1e-20)
+        assert bool(got.isfinite().all())
+        want = _exact(g, eps=1e-20)
+        if want.norm() > 1e-30:  # of bf16's range
+            assert _far(got, want) <= _tol(5)
+    if small:
+        a, b = orthogonalize(base, eps=2.0 ** -60), orthogonalize((base.double() * 2.0 ** 30).to(base.dtype), eps=2.0 ** -30)
+        assert torch.equal(a, b)
+    both = orthogonalize([base, (base.double() * 2.0 ** 110).to(base.dtype), torch.zeros_like(base)])
+    assert _far(both[0], _exact(base)) <= _tol(5) and _far(both[1], _exact(base)) <= _tol(5) and not bool(both[2].any())
+
+
+def test_one_large_value_among_small_ones(gpu):
+    """The parts of a long side at scales of their own: a column of 1e30 and
+    one of 1e-30 in different ones, and an infinity or a NaN at any place."""
+    import torch
+    from distributedspeed_amd import orthogonalize
+    for n, m in ((20, 5000), (5000, 20)):
+        for at in (0, 2500, 4999):
+            g = _normal((n, m), 41, std=1e-30)
+            (g if n < m else g.t())[:, at] *= 1e30
+            _say(f"{n}x{m}, 1e30 times at {at}")
+            # rank one but for 1e-30: the rest is below the result's last bit
+            assert _far(orthogonalize(g), _exact(g)) <= _tol(5)
+            for bad in (float("inf"), float("nan"), -float("inf")):
+                h = g.clone()
+                (h if n < m else h.t())[7, at] = bad
+                assert bool(orthogonalize(h).isnan().all())
+
+
+def test_muon_steps_with_grads_at_the_ends_of_fp32(gpu):
+    """A finite grad is no overflow, whatever the shorter side."""
+    import torch
+    from distributedspeed_amd import MuonOptimizer
+    for power, skipped in ((100, False), (-60, False)):
+        ps = [torch.nn.Parameter(_normal(s, 50, std=0.05)) for s in ((64, 256), (130, 100))]
+        before = [p.detach().double() for p in ps]
+        opt = MuonOptimizer(ps, lr=0.01, weight_decay=0.0, eps=1e-20)
+        for p in ps:
+            p.grad = _normal(p.shape, 51) * 2.0 ** power
+        _say(f"grads times 2^{power}")
+        opt.step()
+        assert opt.last_step_skipped() == skipped
+        for p, w in zip(ps, before):
+            factor = 0.01 * max(1.0, p.shape[0] / p.shape[1]) ** 0.5
+            o = (w - p.detach().double()) / factor
+            want = _exact(p.grad * 0.0975, eps=1e-20)
+            # fp32's rounding of weights of 0.05 in units of the update
+            assert (o - want).norm() <= 15 * 2.0 ** -12 * want.norm() + 1e-6 * w.norm() / factor
