@@ -258,8 +258,8 @@ class MuonOptimizer(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
         if grad_scale is not None and (not isinstance(grad_scale, torch.Tensor) or grad_scale.numel() != 1
-                                       or grad_scale.dtype != torch.float32 or not grad_scale.is_cuda):
-            raise ValueError("grad_scale must be a one-element float32 tensor on the GPU")
+                                       or grad_scale.dtype != torch.float32):
+            raise ValueError("grad_scale must be a one-element float32 tensor")
         self._skips = []
         for g in self.param_groups:
             lists: dict[tuple, list[torch.Tensor]] = {}
@@ -277,6 +277,8 @@ class MuonOptimizer(torch.optim.Optimizer):
         return loss
 
     def _step_list(self, g: dict, dev, gdt, pdt, ps: list, grad_scale) -> None:
+        if grad_scale is not None and grad_scale.device != dev:
+            raise ValueError(f"grad_scale is on {grad_scale.device}, the parameters on {dev}")
         lr, steps = float(g["lr"]), int(g["ns_steps"])
         decay = 1.0 - lr * g["weight_decay"]
         if not 0.0 <= decay <= 1.0:

@@ -213,3 +213,22 @@ def test_a_grad_of_another_shape_is_refused(muon):
     with pytest.raises(ValueError, match="grad"):
         opt.step()
     assert len(tables) == count
+
+
+def test_a_grad_scale_elsewhere_is_refused(muon):
+    """The kernels read it on the parameters' device."""
+    import torch
+
+    class Elsewhere(torch.Tensor):
+        is_cuda = True
+        device = torch.device("cuda", 1)
+
+    make, tables = muon
+    params, opt = _stepped(make, F32)
+    count = len(tables)
+    for scale in (torch.ones(1).as_subclass(Elsewhere), torch.ones(1, device="meta")):
+        with pytest.raises(ValueError, match="grad_scale"):
+            opt.step(grad_scale=scale)
+    assert len(tables) == count
+    opt.step(grad_scale=torch.ones(1))
+    assert len(tables) == count + 1
