@@ -79,6 +79,12 @@ constexpr float kScale = 4096.0f;
 constexpr int kMats = 19;        // matrices of one launch (the table is a kernel argument)
 constexpr int kMaxParts = 2048;  // norm partials per matrix
 constexpr int kNormTile = 64;    // the norm and cast kernels' square tile
+// Scratch of a run of matrices, where it has more than one: a list's scratch does
+// not grow with its length, and what fills the card is faster alone (four of
+// 14336 x 4096: 15.5 ms one at a time, 16.0 together with 2.1 GiB; 19 of
+// 2048 x 2048, 0.9 GiB: 3.9 ms in one run, 4.0, 4.3 and 5.1 in runs of 512, 256
+// and 128 MiB; eight of 4096 x 4096: 10.6 with this bound, 10.9 without).
+constexpr int64_t kRunBytes = (int64_t)1 << 30;
 
 struct Mat {
   const void* in;
@@ -982,7 +988,7 @@ struct Plan {
 
 bool is_small(const Source& q) { return (q.rows < q.cols ? q.rows : q.cols) <= kSmall; }
 
-// The list in runs of at most kMats matrices, the ones with a side of at most
+// The list in runs of at most kMats matrices and kRunBytes, the ones with a side of at most
 // 64 apart: f(table, index of the first, small). The workspace: skip flag, norm
 // records, partials, then what the largest run needs (a small matrix's offsets
 // count floats from there, another's 16-bit elements).
@@ -1023,8 +1029,7 @@ Plan each_run(const Source* src, int32_t count, F&& f) {
     for (int32_t k = 0; k < count; k++) {
       const Source& q = src[k];
       if (q.rows <= 0 || q.cols <= 0 || is_small(q) != (small != 0)) continue;
-      Mat& m = t.m[t.n++];
-      m = Mat{};
+      Mat m{};
       m.in = q.in;
       m.out = q.out;
       m.momentum = q.momentum;
@@ -1037,16 +1042,18 @@ Plan each_run(const Source* src, int32_t count, F&& f) {
       m.s = (int32_t)round_up(m.tall ? q.cols : q.rows, 8);
       m.l = (int32_t)round_up(m.tall ? q.rows : q.cols, 8);
       m.lr = q.lr;
+      m.parts = small ? (int32_t)(ceil_div(m.l, 128) > kSmallParts ? kSmallParts : ceil_div(m.l, 128))
+                      : parts_of(q.rows, q.cols);
+      const int64_t x = round_up((int64_t)m.s * m.l, 128), sq = round_up((int64_t)m.s * m.s, 128);
+      const int64_t need = small ? (int64_t)(m.parts + 1) * kSmall * kSmall + 64 + x
+                                 : 4 * x + 2 * sq + round_up(4 * (int64_t)m.s, 128);
+      if (t.n && (at + need) * (small ? 4 : 2) > kRunBytes) flush();
       if (small) {
-        const int64_t p = ceil_div(m.l, 128);
-        m.parts = (int32_t)(p > kSmallParts ? kSmallParts : p);
         m.a = at;
         m.b = at + (int64_t)m.parts * kSmall * kSmall;
         m.diag = m.b + kSmall * kSmall;  // the parts' exponents and the matrix's
         m.x[0] = m.diag + 64;
-        at = m.x[0] + round_up((int64_t)m.s * m.l, 64);
       } else {
-        const int64_t x = round_up((int64_t)m.s * m.l, 128), sq = round_up((int64_t)m.s * m.s, 128);
         m.x[0] = at;
         m.x[1] = at + x;
         m.lo[0] = at + 2 * x;
@@ -1054,12 +1061,12 @@ Plan each_run(const Source* src, int32_t count, F&& f) {
         m.a = at + 4 * x;
         m.b = m.a + sq;
         m.diag = m.b + sq;
-        at = m.diag + round_up(4 * (int64_t)m.s, 128);
-        m.parts = parts_of(q.rows, q.cols);
         m.part0 = (int32_t)part0;
         part0 += m.parts;
         index++;
       }
+      at += need;
+      t.m[t.n++] = m;
       if (t.n == kMats) flush();
     }
     flush();

@@ -608,7 +608,10 @@ typedef struct DsxMatrix {
 } DsxMatrix;
 
 /* Bytes of device scratch dsx_orthogonalize needs for the list (the shapes
- * alone are read); -1 with dsx_last_error for a bad list. Host only. */
+ * alone are read); -1 with dsx_last_error for a bad list. Host only. A list is
+ * worked on in runs of about 1 GiB of scratch; a matrix alone takes 8 bytes an
+ * element and 4 for each of its shorter side squared (a shorter side of at most
+ * 64: 4 bytes an element). */
 int64_t dsx_orthogonalize_workspace(const DsxMatrix* mats /* host */,
                                     int32_t count);
 

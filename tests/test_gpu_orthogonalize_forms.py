@@ -220,3 +220,15 @@ def test_muon_steps_with_grads_at_the_ends_of_fp32(gpu):
             want = _exact(p.grad * 0.0975, eps=1e-20)
             # fp32's rounding of weights of 0.05 in units of the update
             assert (o - want).norm() <= 15 * 2.0 ** -12 * want.norm() + 1e-6 * w.norm() / factor
+
+
+def test_a_list_in_several_runs_of_scratch(gpu):
+    """Five matrices whose scratch is more than a run's, small ones among them."""
+    import torch
+    from distributedspeed_amd import orthogonalize
+    big = [_normal(s, 60 + k, "bfloat16") for k, s in enumerate(((4096, 6000), (6000, 4096)) * 2 + ((4096, 6000),))]
+    small = [_normal((30, 50), 70 + k, "bfloat16") for k in range(3)] + [_normal((90, 70), 80, "bfloat16")]
+    ms = [big[0], small[0], big[1], small[3], big[2], small[1], big[3], small[2], big[4]]
+    _say("five of 4096 x 6000")
+    for g, o in zip(ms, orthogonalize(ms)):
+        assert o.shape == g.shape and _far(o, _exact(g)) <= _tol(5)

@@ -92,3 +92,20 @@ def test_batches_of_empty_matrices_and_empty_batches(calls, shape):
     assert got.shape == shape and got.dtype == torch.bfloat16
     out = torch.zeros(shape, dtype=torch.bfloat16)
     assert orthogonalize(torch.ones(shape), out=out) is out
+
+
+@pytest.mark.parametrize("n,m,count", [(14336, 4096, 1), (14336, 4096, 19), (14336, 4096, 200), (8192, 28672, 7),
+                                       (64, 1 << 20, 40), (2048, 2048, 100), (3, 5, 4000)])
+def test_scratch_is_bounded_for_any_length_of_list(n, m, count):
+    """1 GiB, or what one matrix needs; beside it the records and the partial
+    norms of every matrix (16 KiB at most) and the split sums (8 MiB)."""
+    from distributedspeed_amd import _lib
+    lib = _lib.load()
+    for struct_, name in ((_lib.DsxMatrix, "dsx_orthogonalize_workspace"), (_lib.DsxMuonParam, "dsx_muon_workspace")):
+        table = (struct_ * count)()
+        for q in table:
+            q.rows, q.cols = n, m
+        s = (min(n, m) + 7) // 8 * 8
+        one = 8 * (s * max(n, m) + 64) + 4 * (s * s + 256) + 8 * s + 1024
+        got = getattr(lib, name)(table, count)
+        assert 0 < got <= max(1 << 30, one) + count * (16384 + 32) + (8 << 20) + 1024
