@@ -176,11 +176,21 @@ class MuonOptimizer(torch.optim.Optimizer):
     written to memory. Vectors, embeddings and output heads belong to another
     optimizer (AdamWOptimizer).
 
-    step(grad_scale=...) divides the grads by a one-element fp32 device tensor
-    (AdamWOptimizer.loss_scale_tensor()). A grad that is not finite skips the
-    step of its param group (and type): nothing of it changes, and
-    last_step_skipped() says so. Nothing here synchronises the host with the
-    device."""
+    step(grad_scale=...) divides the grads by a one-element fp32 tensor on
+    their device (AdamWOptimizer.loss_scale_tensor(), before that optimizer's
+    own step, which may move it). A grad that is not finite skips the step of
+    its param group (and type): nothing of it changes, and last_step_skipped()
+    says so. It moves no loss scale: an AdamWOptimizer beside it sees its own
+    grads alone, so under a dynamic scale the caller has to halve it where only
+    a matrix's grad overflowed:
+
+        muon.step(grad_scale=adamw.loss_scale_tensor())
+        if muon.last_step_skipped():  # synchronises
+            adamw.set_scaler_state(adamw.read_state().scale / 2)
+        else:
+            adamw.step()
+
+    step() does not synchronise the host with the device."""
 
     def __init__(self, params, lr: float = 1e-3, weight_decay: float = 0.1, momentum: float = 0.95,
                  nesterov: bool = True, ns_coefficients=NS_COEFFICIENTS, eps: float = 1e-7, ns_steps: int = 5,

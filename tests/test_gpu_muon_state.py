@@ -124,3 +124,40 @@ def test_goes_on_from_torchs_muon(gpu, adjust):
         unit = 0.02 * factor * math.sqrt(min(p.shape))
         far = (p.detach().double() - q.detach().double()).norm().item()
         assert far <= (16 * 2.0 ** -9 + 15 * 2.0 ** -12) * unit + 1e-6 * p.detach().norm().item(), far / unit
+
+
+def test_a_dynamic_scale_shared_with_adamw(gpu):
+    """The loop that MuonOptimizer's documentation gives, in fp16: the matrix's
+    scaled grad overflows above 2^14, the vector's never. The scale comes down
+    until Muon steps, both optimizers step together, and the scale's growth
+    (after two clean steps) costs a skipped step, not the run."""
+    import torch
+    from distributedspeed_amd import AdamWOptimizer, MuonOptimizer
+    from distributedspeed_amd.flat_step import ScalerConfig
+    w = torch.nn.Parameter(_normal(torch.Generator("cuda").manual_seed(5), (40, 24), 0.05).half())
+    v = torch.nn.Parameter(torch.full((64,), 0.5, device="cuda", dtype=torch.float16))
+    muon = MuonOptimizer([w], lr=0.01)
+    adamw = AdamWOptimizer([v], lr=1e-3, param_dtype=torch.float16,
+                           loss_scaler=ScalerConfig(mode="dynamic", init_scale=2.0 ** 18, window=2, hysteresis=1))
+    true = torch.full((40, 24), 0.5, device="cuda")
+    true[3, 4] = 3.0  # times 2^14 below 65504, times 2^15 above
+    seen = []
+    for step in range(12):
+        scale = adamw.loss_scale_tensor()
+        w.grad = (true * scale).half()
+        v.grad = None
+        (v.float().sum() * 0.01 * scale).backward()
+        before = [p.detach().clone() for p in (w, v)]
+        muon.step(grad_scale=scale)
+        used, skipped = float(scale), muon.last_step_skipped()
+        if skipped:
+            adamw.set_scaler_state(adamw.read_state().scale / 2)
+        else:
+            adamw.step()
+        _say(f"step {step}: scale 2^{math.log2(used):g}, skipped {skipped}")
+        assert skipped == (used > 2.0 ** 14)
+        for p, old in zip((w, v), before):
+            assert torch.equal(p.detach(), old) == skipped
+        seen.append(skipped)
+    # 2^18 to 2^15 skipped; then two steps, growth, one skipped
+    assert seen == [True] * 4 + [False, False, True, False, False, True, False, False]
