@@ -212,13 +212,17 @@ class MuonOptimizer(torch.optim.Optimizer):
 
     def add_param_group(self, param_group: dict) -> None:
         super().add_param_group(param_group)
-        for p in self.param_groups[-1]["params"]:
-            ops._device(p)
-            ops.grad_code(p.dtype)
-            if p.dim() != 2:
-                raise ValueError(f"Muon steps matrices; got a parameter of shape {tuple(p.shape)}")
-            if not p.is_contiguous():
-                raise ValueError("Muon's parameters must be contiguous")
+        try:
+            for p in self.param_groups[-1]["params"]:
+                ops._device(p)
+                ops.grad_code(p.dtype)
+                if p.dim() != 2:
+                    raise ValueError(f"Muon steps matrices; got a parameter of shape {tuple(p.shape)}")
+                if not p.is_contiguous():
+                    raise ValueError("Muon's parameters must be contiguous")
+        except (TypeError, ValueError):
+            self.param_groups.pop()
+            raise
 
     def __setstate__(self, state: dict) -> None:
         """Groups as this class has them, also from torch.optim.Muon's state

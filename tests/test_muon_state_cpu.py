@@ -232,3 +232,20 @@ def test_a_grad_scale_elsewhere_is_refused(muon):
     assert len(tables) == count
     opt.step(grad_scale=torch.ones(1))
     assert len(tables) == count + 1
+
+
+def test_a_refused_group_is_not_added(muon):
+    import torch
+    make, tables = muon
+    params, opt = _stepped(make, F32)
+    good = torch.nn.Parameter(torch.ones(4, 4))
+    for bad in (torch.nn.Parameter(torch.ones(5)), torch.nn.Parameter(torch.ones(4, 6).t()),
+                torch.nn.Parameter(torch.ones(4, 4, dtype=torch.float64))):
+        for group in ([bad], [good, bad], (p for p in (good, bad)), bad):
+            with pytest.raises((ValueError, TypeError)):
+                opt.add_param_group({"params": group})
+            assert len(opt.param_groups) == 1
+    opt.add_param_group({"params": [good], "lr": 0.5})
+    good.grad = torch.ones(4, 4)
+    opt.step()
+    assert len(opt.param_groups) == 2 and [len(t) for t in tables[-2:]] == [2, 1]
