@@ -57,11 +57,11 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     fp16 or all bf16 on one GPU; `activation` is "silu", "gelu", "gelu_tanh" or
     "relu". Sums are fp32; the inner product act(g) u is rounded to the inputs'
     type once. Rows may be strided; a tensor whose columns are not adjacent is
-    copied first. Any number of tokens, none included.
+    copied first. Up to 2^20 tokens, none included.
 
     Differentiable once in all four tensors, backwards (a forward-mode tangent
-    is refused). The backward keeps 8 bytes for
-    every token and inner feature; without gradients nothing is kept."""
+    is refused). The backward keeps 8 bytes for every token and inner feature
+    (10 for up to three tokens); without gradients nothing is kept."""
     act = ACTIVATIONS.get(activation)
     if act is None:
         raise ValueError(f"activation must be one of {sorted(ACTIVATIONS)}, got {activation!r}")
@@ -103,7 +103,7 @@ def gated_residual_norm(residual: torch.Tensor, branch: torch.Tensor | None = No
     branch it is the norm before a first block. residual and branch are
     [..., width], the weights [width]; gate is [width] (a value a channel) or
     [samples, width], whose i-th row serves the i-th of `samples` equal runs of
-    rows. All tensors are of one type (fp32, fp16 or bf16) on one GPU. The
+    rows (at most 65533 samples). All tensors are of one type (fp32, fp16 or bf16) on one GPU. The
     arithmetic is fp32 and rounded once; normed is taken from hidden before its
     rounding. Rows may be strided.
 
@@ -158,7 +158,8 @@ class GatedFFNBlock(torch.nn.Module):
 
     The stack begins with gated_residual_norm(x, next_weight=...). The gate is
     a value a channel; w_gate, w_up and w_down are the matrices that Muon
-    steps, the others vectors."""
+    steps, the others vectors. The forward takes fp16 or bf16 parameters and
+    inputs: give a dtype, or leave the cast to the engine's fp16 or bf16 mode."""
 
     def __init__(self, width: int, inner: int, *, activation: str = "silu", branch_scale: float = 1.0,
                  gate_init: float = 1.0, eps: float = 1e-6, device=None, dtype=None):

@@ -1004,10 +1004,12 @@ Plan each_run(const Source* src, int32_t count, F&& f) {
       if (t.n && !small) {
         // A Gram matrix of few 64-tiles leaves CUs idle while each walks all of
         // l: its sums are split so that there are up to two blocks a CU, eight
-        // K tiles each at least, and only below 160 tiles (65 x 8192: 326 us
-        // without, 117 with; 1001 x 2731, 136 tiles: 277 and 247; 1024 x 784 with
-        // 1024 x 1024, 227 tiles: 12.0 us a launch without, 15.2 with; all with
-        // two K tiles in shared memory).
+        // K tiles each at least, and only below 160 tiles. Calls without the
+        // split and with it: 65 x 8192 241 and 135 us, 200 x 3000 163 and 136,
+        // 700 x 4000 (66 tiles) 210 and 193, 1024 x 4096 (136) 245 and 237,
+        // 512 x 512 112 and 112; 1100 x 2731 (171) 252 and 265, 1200 x 3000 (190)
+        // 270 and 290. Below the bound it loses where l is short: 768 x 1024
+        // (78) 144 and 160, 1024 x 1024 (136) 156 and 178, 1001 x 2731 226 and 233.
         int64_t n = 0;
         auto tiles = [](const Mat& m) { return ceil_div(m.s, 64) * (ceil_div(m.s, 64) + 1) / 2; };
         for (int i = 0; i < t.n; i++) n += tiles(t.m[i]);

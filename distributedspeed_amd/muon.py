@@ -96,8 +96,15 @@ def orthogonalize(updates: torch.Tensor | Sequence[torch.Tensor], *, steps: int 
 
     `coefficients` is one (a, b, c) for all steps or one for each; they must
     keep the iterates' singular values below 4 (the iterates are fp16: their
-    11 bits are why the result is bf16). A matrix whose norm is not finite
-    becomes NaN; a zero matrix stays zero. A matrix whose columns are not
+    11 bits are why the result is bf16). A matrix with an element that is not
+    finite becomes NaN; a zero matrix stays zero. At most 4096 matrices a call,
+    with sides of at most 2^20. Each step also multiplies, by its `a`, what the
+    iterates' roundings put where the matrix has nothing: an fp32 matrix of rank
+    four is 4e-3 off after five steps of Muon's coefficients, 1e-2 after six and
+    1e-1 after eight (128 x 128; singular values over 10^4: 2e-3, 3e-3, 5e-3).
+    Matrices with a side of at most 64 stay in fp32 (7e-4 beside the result's
+    own rounding after eight). A norm far below eps (1e-5 of it) leaves the fp16
+    iterates little of their bits. A matrix whose columns are not
     adjacent is copied first. Not differentiable: a tensor that requires grad
     (while grad mode is on) or carries a forward-mode tangent is refused. Runs
     on the current stream without a host synchronisation."""

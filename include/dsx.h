@@ -620,11 +620,13 @@ int64_t dsx_orthogonalize_workspace(const DsxMatrix* mats /* host */,
  *   `coefficients` (host):  A = X X^T,  X = a X + (b A + c A A) X
  * (the transposed products where rows > cols: the result is the same).
  * in is of `dtype` (DSX_F32, DSX_F16 or DSX_BF16), out is bf16. A zero matrix
- * gives zeros; a matrix with a non-finite element gives NaN throughout. The
- * iterates are held in fp16 with fp32 sums: the coefficients must keep every
- * singular value below 4 and every one of b A + c A A below 16 in magnitude
- * (Muon's 3.4445, -4.7750, 2.0315 stay below 1.3 and 2.9). Matrices with no
- * element are skipped. steps in [1, 64], eps in [1e-20, 1]; `workspace` is
+ * gives zeros; a matrix with a non-finite element gives NaN throughout. With
+ * both sides above 64 the iterates are held in fp16 with fp32 sums: the
+ * coefficients must keep every singular value below 4 and every one of
+ * b A + c A A below 16 in magnitude (Muon's 3.4445, -4.7750, 2.0315 stay below
+ * 1.3 and 2.9), and |G|_F should not be far below eps (at 1e-5 of it the first
+ * iterate leaves fp16's range). Matrices with no element are skipped. count is
+ * at most 4096, steps in [1, 64], eps in [1e-20, 1]; `workspace` is
  * 256-byte aligned device memory. No counterpart in the reference. */
 int dsx_orthogonalize(const DsxMatrix* mats /* host */, int32_t count,
                       int dtype, int32_t steps,
