@@ -56,7 +56,8 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     [inner, width] and w_down [width, inner] (torch.nn.Linear's layout), all
     fp16 or all bf16 on one GPU; `activation` is "silu", "gelu", "gelu_tanh" or
     "relu". Sums are fp32; the inner product act(g) u is rounded to the inputs'
-    type once. Rows may be strided; a tensor whose columns are not adjacent is
+    type once, or not at all for up to three tokens, so that a token's last
+    bits depend on how many run with it. Rows may be strided; a tensor whose columns are not adjacent is
     copied first. Up to 2^20 tokens, none included.
 
     Differentiable once in all four tensors, backwards (a forward-mode tangent
