@@ -248,6 +248,9 @@ class MuonOptimizer(torch.optim.Optimizer):
         a master left over and goes on without it. The kernels walk every
         buffer by p's shape, so anything else is refused."""
         st = self.state[p]
+        for key in _BUFFERS:
+            if key in st and st[key] is None:
+                del st[key]
         if "momentum_buffer" not in st:
             st["momentum_buffer"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
         if p.dtype != torch.float32 and "master" not in st:

@@ -249,3 +249,20 @@ def test_a_refused_group_is_not_added(muon):
     good.grad = torch.ones(4, 4)
     opt.step()
     assert len(opt.param_groups) == 2 and [len(t) for t in tables[-2:]] == [2, 1]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_a_buffer_saved_as_none_begins_anew(muon, dtype):
+    import copy
+    make, tables = muon
+    params, opt = _stepped(make, dtype)
+    state = copy.deepcopy(opt.state_dict())
+    for s in state["state"].values():
+        s.update(momentum_buffer=None, master=None)
+    others = _params(dtype)
+    opt2 = make(others)
+    opt2.load_state_dict(state)
+    _grads(others)
+    opt2.step()
+    _check_table(opt2, others, tables[-1])
+    assert all(not bool(opt2.state[p]["momentum_buffer"].any()) for p in others)
