@@ -97,6 +97,12 @@ def __getattr__(name: str):
     if name in ("gated_ffn", "gated_residual_norm", "GatedFFNBlock"):
         from . import block as _b
         return getattr(_b, name)
+    if name in ("PackedSequences", "packed_attention", "rotary", "AttentionBlock"):
+        from . import sequence as _s
+        return getattr(_s, name)
+    if name == "linear_cross_entropy":
+        from .loss import linear_cross_entropy
+        return linear_cross_entropy
     if name in ("DistributedSpeedConfig", "load_config", "fp16_config", "bf16_config", "zero_config"):
         from . import config as _c
         return getattr(_c, name)
@@ -106,5 +112,6 @@ def __getattr__(name: str):
 __all__ = ["initialize", "is_initialized", "get_config", "get_rank", "get_world_size", "get_local_rank", "destroy",
            "DistributedSpeedEngine", "ZeROOptimizer", "AdamWOptimizer", "MultiTensorAdamWOptimizer",
            "MuonOptimizer", "orthogonalize", "gated_ffn", "gated_residual_norm", "GatedFFNBlock",
+           "PackedSequences", "packed_attention", "rotary", "AttentionBlock", "linear_cross_entropy",
            "DistributedSpeedConfig", "load_config",
            "fp16_config", "bf16_config", "zero_config"]

@@ -106,9 +106,32 @@ class DsxNorm(_c.Structure):
                 ("eps", _c.c_float), ("rstd", _P)]
 
 
+class DsxAttention(_c.Structure):
+    _fields_ = [("q", _P), ("k", _P), ("v", _P)] + \
+               [(k, _c.c_int64) for k in ("ld_q", "ld_k", "ld_v", "head_q", "head_k", "head_v", "tokens")] + \
+               [("tiles", _P), ("tile_count", _c.c_int64)] + \
+               [(k, _c.c_int32) for k in ("heads", "kv_heads", "head_dim", "dtype", "causal")] + \
+               [("scale", _c.c_float)]
+
+
+class DsxRotary(_c.Structure):
+    _fields_ = [("q", _P), ("k", _P), ("positions", _P)] + \
+               [(k, _c.c_int64) for k in ("ld_q", "ld_k", "head_q", "head_k", "tokens")] + \
+               [(k, _c.c_int32) for k in ("heads", "kv_heads", "head_dim", "dims", "dtype", "interleaved",
+                                          "position_bytes", "reserved")] + [("base", _c.c_double)]
+
+
+class DsxLoss(_c.Structure):
+    _fields_ = [("x", _P), ("weight", _P), ("targets", _P)] + \
+               [(k, _c.c_int64) for k in ("ld_x", "ld_weight", "tokens", "width", "vocab", "ignore_index")] + \
+               [(k, _c.c_int32) for k in ("dtype", "target_bytes", "reduction", "reserved")] + \
+               [("saved", _P), ("workspace", _P), ("workspace_bytes", _c.c_int64)]
+
+
 for _s, _n in ((DsxState, 64), (DsxScalerConfig, 32), (DsxAdamwHyper, 56), (DsxStepScalars, 64),
                (DsxTensorRef, 56), (DsxChunk, 24), (DsxGroupsDev, 1112), (DsxFlatPlan, 248),
-               (DsxMatrix, 48), (DsxMuonParam, 64), (DsxMuonHyper, 32), (DsxFfn, 128), (DsxNorm, 104)):
+               (DsxMatrix, 48), (DsxMuonParam, 64), (DsxMuonHyper, 32), (DsxFfn, 128), (DsxNorm, 104),
+               (DsxAttention, 120), (DsxRotary, 104), (DsxLoss, 112)):
     assert _c.sizeof(_s) == _n, (_s.__name__, _c.sizeof(_s))
 
 # name -> (restype, argtypes); every symbol include/dsx.h declares.
@@ -169,6 +192,15 @@ SIGNATURES = {
     "dsx_norm_workspace_bytes": (_c.c_int64, [_P]),
     "dsx_norm_forward": (_c.c_int, [_P, _P, _P, _P]),
     "dsx_norm_backward": (_c.c_int, [_P, _P, _c.c_int64, _P, _c.c_int64, _P, _P, _P, _P, _P, _P, _c.c_int64, _P]),
+    "dsx_attention_tiles": (_c.c_int64, [_P, _c.c_int64, _P, _c.c_int64]),
+    "dsx_attention_forward": (_c.c_int, [_P, _P, _P, _P, _P]),
+    "dsx_attention_workspace_bytes": (_c.c_int64, [_P]),
+    "dsx_attention_backward": (_c.c_int, [_P, _P, _P, _P, _P, _c.c_int64, _c.c_int64, _P, _P, _P, _P, _c.c_int64, _P]),
+    "dsx_rotary": (_c.c_int, [_P, _P, _P, _c.c_int32, _P]),
+    "dsx_loss_saved_bytes": (_c.c_int64, [_P]),
+    "dsx_loss_workspace_bytes": (_c.c_int64, [_P, _c.c_int32]),
+    "dsx_loss_forward": (_c.c_int, [_P, _P, _P]),
+    "dsx_loss_backward": (_c.c_int, [_P, _P, _P, _P, _P]),
 }
 
 _lib: ctypes.CDLL | None = None

@@ -1,5 +1,6 @@
 """Build libdsx.so in-tree with hipcc for gfx950, and the autograd nodes of the
-block operators (_block_autograd.so, host C++).
+block and sequence operators (_block_autograd.so and _sequence_autograd.so,
+host C++).
 
     python -m distributedspeed_amd.build
 
@@ -34,16 +35,19 @@ ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 INCLUDE = os.path.join(ROOT, "include")
 OUT = os.path.join(HERE, "libdsx.so")
-AUTOGRAD = os.path.join(HERE, "_block_autograd.so")
+AUTOGRAD = {f"{name}.cpp": os.path.join(HERE, f"_{name}.so") for name in ("block_autograd", "sequence_autograd")}
 ARCH = os.environ.get("DSX_OFFLOAD_ARCH", "gfx950")
 
 # source -> its own flags. The optimizer step rounds where torch rounds; the
-# block and Muon kernels have no such partner and may contract.
+# block, sequence and Muon kernels have no such partner and may contract.
 SOURCES = {
     "dsx_step.hip": ["-ffp-contract=off"],
     "dsx_muon.hip": [],
     "dsx_ffn.hip": [],
     "dsx_norm.hip": [],
+    "dsx_attention.hip": [],
+    "dsx_rotary.hip": [],
+    "dsx_loss.hip": [],
 }
 
 
@@ -63,16 +67,16 @@ def command(source: str, out: str, extra: list[str] | None = None) -> list[str]:
             f"-I{INCLUDE}", f"-I{CSRC}", os.path.join(CSRC, source), "-o", out] + list(extra or [])
 
 
-def autograd_command(out: str) -> list[str]:
-    """The compile command of the autograd nodes of the block operators: host
-    C++ against torch, calling libdsx through addresses bound at load."""
+def autograd_command(source: str, out: str) -> list[str]:
+    """The compile command of a file of autograd nodes: host C++ against torch,
+    calling libdsx through addresses bound at load."""
     import torch
     from torch.utils import cpp_extension
     includes = [*cpp_extension.include_paths(), sysconfig.get_paths()["include"], INCLUDE]
     return ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall",
             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
             *[a for i in includes for a in ("-isystem" if "torch" in i else "-I", i)],
-            os.path.join(CSRC, "block_autograd.cpp"), "-o", out,
+            os.path.join(CSRC, source), "-o", out,
             *[f"-L{d}" for d in cpp_extension.library_paths()], "-lc10", "-ltorch", "-ltorch_cpu", "-ltorch_python"]
 
 
@@ -85,17 +89,19 @@ def _run(cmd: list[str]) -> list[str]:
     return noise
 
 
-def build(out: str = OUT, autograd: str = AUTOGRAD, verbose: bool = False) -> str:
+def build(out: str = OUT, verbose: bool = False) -> str:
     with tempfile.TemporaryDirectory(prefix="dsx_build_") as tmp:
         objects = {src: os.path.join(tmp, src + ".o") for src in SOURCES}
-        jobs = [command(src, objects[src]) for src in SOURCES] + [autograd_command(autograd + ".tmp")]
-        with ThreadPoolExecutor(max_workers=min(5, len(jobs))) as pool:
+        jobs = [autograd_command(src, so + ".tmp") for src, so in AUTOGRAD.items()]
+        jobs += [command(src, objects[src]) for src in SOURCES]
+        with ThreadPoolExecutor(max_workers=min(8, len(jobs))) as pool:
             noise = [ln for got in pool.map(_run, jobs) for ln in got]
         _run([hipcc(), f"--offload-arch={ARCH}", "-fPIC", "-shared", *objects.values(), "-o", out + ".tmp"])
     if verbose and noise:
         print("\n".join(noise), file=sys.stderr)
     os.replace(out + ".tmp", out)
-    os.replace(autograd + ".tmp", autograd)
+    for so in AUTOGRAD.values():
+        os.replace(so + ".tmp", so)
     return out
 
 

@@ -1,0 +1,837 @@
+// dsx_attention.hip -- attention over packed sequences and its gradients (see
+// include/dsx.h).
+//
+//   s_ij = q_i k_j,  P_ij = exp(scale s_ij - lse_i),  o_i = sum_j P_ij v_j
+//   dP_ij = do_i v_j,  dS_ij = P_ij (dP_ij - delta_i),  delta_i = do_i o_i
+//   dq_i = scale sum_j dS_ij k_j,  dk_j = scale sum_i dS_ij q_i,  dv_j = sum_i P_ij do_i
+//
+// over the pairs (i, j) of one sequence (causal: j <= i); heads of a group
+// share k and v, whose gradients are summed over them.
+//
+// All three kernels are one pass: a wave keeps 32 rows of its own (queries in
+// k_attend and k_query_grads, keys in k_key_grads) and the other side comes by
+// in tiles of 64 rows through shared memory, two of them there at a time. The
+// products run on the 32x32x16 matrix instruction with the wave's own rows as
+// its columns: a lane then holds one row's values of 16 rows of the other
+// side, so that a row's maximum and sum are one exchange between two lanes,
+// and the registers of P and dS, rounded, are the second operand of the next
+// product as they lie: its sum runs over the rows in the order in which the
+// first one left them, and the transposing LDS read brings the first operand
+// in the same order.
+//
+// The gradients come from two kernels that compute P twice rather than from
+// one that adds up dq across blocks: nothing is added by atomics, so that
+// results do not depend on timing.
+
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include <new>
+
+#include "dsx.h"
+#include "dsx_gemm.h"
+#include "dsx_internal.h"
+
+namespace {
+
+using dsxg::b8v;
+using dsxg::h8v;
+using dsxg::kCus;
+using dsxg::LdsBlock;
+using dsxg::read_transposed;
+using dsxg::s4v;
+using dsxg::s8v;
+using dsxi::as_stream;
+using dsxi::ceil_div;
+using dsxi::fail;
+using dsxi::launch_status;
+using dsxi::round_up;
+
+typedef float f16v __attribute__((ext_vector_type(16)));
+typedef short s2v __attribute__((ext_vector_type(2)));
+typedef float f4v __attribute__((ext_vector_type(4)));
+
+// kBias: P is held as exp2(s - m + kBias). fp16's 2^-14 would lose the small
+// values of long rows; with the running maximum up to kLazy behind (below),
+// 2^(kBias + kLazy) = 2^15 is still in its range.
+struct F16 : dsxg::F16 {
+  static constexpr float kBias = 7.0f;
+  static constexpr bool kScaled = true;
+  static __device__ inline f16v mfma(s8v a, s8v b, f16v c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8v, a), __builtin_bit_cast(h8v, b), c, 0, 0, 0);
+  }
+};
+struct BF16 : dsxg::BF16 {
+  static constexpr float kBias = 0.0f;
+  static constexpr bool kScaled = false;
+  static __device__ inline f16v mfma(s8v a, s8v b, f16v c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8v, a), __builtin_bit_cast(b8v, b), c, 0, 0, 0);
+  }
+};
+constexpr float kLazy = 8.0f;
+
+constexpr int kRows = 128;   // of a block: four waves of 32
+constexpr int kTile = 64;    // rows of the other side in shared memory
+constexpr int kThreads = 256;
+
+struct Rows {  // [tokens][heads][d], d contiguous
+  const short* p;
+  int64_t ld, head;  // strides in elements
+};
+struct Args {
+  Rows q, k, v;
+  const int4* tiles;  // first row, first and end row of its sequence
+  int heads, kv_heads, group, d;
+  int tokens, causal;
+  float scale, scale2;  // scale2: scale log2(e)
+};
+
+// ---- tiles in shared memory --------------------------------------------------
+
+template <int HD>
+struct Tile {
+  static constexpr int kChunks = HD / 8;               // of 16 bytes, in a row
+  static constexpr int kBytes = kTile * HD * 2;
+  static constexpr int kLoads = kTile * kChunks / kThreads;
+  static constexpr int kSteps = HD / 16;               // matrix instructions along a row
+  static constexpr int kBlocks = HD / 32;              // of 32 features
+
+  // Chunk c of row r lies at c ^ swizzle(r): the 16 rows of a fragment read, and
+  // the 4 x 32 bytes that 16 lanes of a transposing read touch, then fall on
+  // different banks (64 of 4 bytes).
+  static __device__ inline int swizzle(int r) {
+    return HD == 64 ? ((r >> 1) & 3) << 1 | ((r >> 3) & 1) : (r & 7) << 1 | ((r >> 3) & 1);
+  }
+
+  // Loads rows [0, left) of 64 straight to shared memory; a row past the end is
+  // the last one again and a chunk past d the row's first (the products' other
+  // operand holds zeros there).
+  static __device__ inline void load(char* dst, const short* p, int64_t ld, int left, int d) {
+    const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+#pragma unroll
+    for (int j = 0; j < kLoads; j++) {
+      const int at = j * kThreads + tid, r = at / kChunks;
+      int c = (at % kChunks) ^ swizzle(r);
+      c = c * 8 < d ? c : 0;
+      const uint32_t off = (uint32_t)min(r, left - 1) * (uint32_t)(ld * 2) + c * 16;
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)((const char*)p + off),
+                                       (__attribute__((address_space(3))) void*)(dst + j * kThreads * 16 + w * 1024), 16,
+                                       0, 0);
+    }
+  }
+  // Rows r0..r0+31 (r0 a multiple of 32), features 16 step..: one row a lane.
+  static __device__ inline s8v rows(const char* tile, int r0, int step, int lane) {
+    const int r = r0 + (lane & 31);
+    return *(const s8v*)(tile + r * HD * 2 + (((step * 2 + (lane >> 5)) ^ swizzle(lane & 31)) << 4));
+  }
+  // Features f0..f0+31 (one a lane) of the 16 rows from r0: rows 4h..4h+3 and
+  // 8+4h..8+4h+3 for the lane's half h.
+  static __device__ inline s8v columns(const char* tile, int r0, int f0, int lane) {
+    const int r = 4 * (lane >> 5) + ((lane & 15) >> 2);
+    const int c = f0 / 8 + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+    const char* row = tile + (r0 + r) * HD * 2 + (lane & 1) * 8;
+    const s4v lo = read_transposed((LdsBlock*)(row + ((c ^ swizzle(r0 + r)) << 4)));
+    const s4v hi = read_transposed((LdsBlock*)(row + 8 * HD * 2 + ((c ^ swizzle(r0 + r + 8)) << 4)));
+    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+  // The wave's own 32 rows as an operand in registers; zeros past d.
+  static __device__ inline void own(s8v* f, const short* p, int64_t ld, int row, int d, int lane) {
+    const short* at = p + row * ld;
+#pragma unroll
+    for (int s = 0; s < kSteps; s++) {
+      const int c = (s * 2 + (lane >> 5)) * 8;
+      f[s] = c < d ? *(const s8v*)(at + c) : s8v{0, 0, 0, 0, 0, 0, 0, 0};
+    }
+  }
+};
+
+// Waits for this wave's direct loads and LDS reads, then for the other waves.
+__device__ inline void sync_loads() {
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// Values of 16 rows by 32 columns as the second operand of the next product.
+template <class T>
+__device__ inline s8v pack(const f16v& v, int half) {
+  s8v r;
+#pragma unroll
+  for (int e = 0; e < 8; e++) r[e] = T::round(v[half * 8 + e]);
+  return r;
+}
+__device__ inline float other_half(float v) { return __shfl_xor(v, 32); }
+
+// The row (of 32) that register r of a lane's half holds.
+__device__ constexpr int row_of(int r, int half) { return 8 * (r >> 2) + 4 * half + (r & 3); }
+
+// Writes a wave's 32 rows of o (one a lane, features as row_of has them) by way
+// of its part of shared memory. `rest`: what rounding to 16 bits loses instead.
+template <class T, int HD>
+__device__ inline void store_rows(char* strip, const f16v* o, float factor, bool rest, short* out, int64_t ld,
+                                  int rows, int d, int lane) {
+  using L = Tile<HD>;
+  const int r = lane & 31, half = lane >> 5;
+#pragma unroll
+  for (int i = 0; i < L::kBlocks; i++)
+#pragma unroll
+    for (int c = 0; c < 4; c++) {
+      s4v w;
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const float v = o[i][c * 4 + e] * factor;
+        w[e] = T::round(v);
+        if (rest) {
+          const float back = T::widen(w[e]);
+          w[e] = T::round(__builtin_isfinite(back) ? v - back : 0.0f);
+        }
+      }
+      *(s4v*)(strip + r * HD * 2 + (((i * 4 + c) ^ L::swizzle(r)) << 4) + half * 8) = w;
+    }
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+  for (int at = 0; at < 32 * L::kChunks; at += 64) {
+    const int row = (at + lane) / L::kChunks, c = (at + lane) % L::kChunks;
+    if (row < rows && c * 8 < d) *(s8v*)(out + row * ld + c * 8) = *(const s8v*)(strip + row * HD * 2 + ((c ^ L::swizzle(row)) << 4));
+  }
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// A block's tile and heads: tile by tile (the longest first), the heads of a
+// key head eight blocks apart so that one XCD's L2 serves them.
+struct Place {
+  int row0, start, end, head, kv;
+  bool good;
+};
+__device__ inline Place place_of(const Args& a, int heads) {
+  const int t = blockIdx.x / heads, h = blockIdx.x % heads;
+  const int4 e = a.tiles[t];
+  Place p{e.x, e.y, e.z, 0, 0, false};
+  const int per = heads / a.kv_heads;
+  p.kv = h % a.kv_heads;
+  p.head = p.kv * per + h / a.kv_heads;
+  p.good = p.start >= 0 && p.start <= p.row0 && p.row0 < p.end && p.end <= a.tokens;
+  return p;
+}
+
+#define DSX_ATTENTION_KERNEL(HD) \
+  __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(HD <= 128 ? 2 : 1, HD <= 128 ? 2 : 1)))
+
+// ---- forward -------------------------------------------------------------------
+
+struct Forward {
+  short* out;     // [tokens][heads][d]
+  short* out_lo;  // what out lost in rounding; NULL: not kept
+  float* lse;     // [heads][tokens], base 2; NULL: not kept
+};
+
+template <class T, int HD>
+__global__ DSX_ATTENTION_KERNEL(HD) void k_attend(Args a, Forward f) {
+  using L = Tile<HD>;
+  __shared__ __attribute__((aligned(1024))) char lds[2][2][L::kBytes];
+  const Place p = place_of(a, a.heads);
+  if (!p.good) return;
+  const int lane = threadIdx.x & 63, half = lane >> 5, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int w0 = p.row0 + 32 * w, row = w0 + (lane & 31);
+  s8v qf[L::kSteps];
+  L::own(qf, a.q.p + p.head * a.q.head, a.q.ld, min(row, p.end - 1), a.d, lane);
+  const short* kp = a.k.p + p.kv * a.k.head + p.start * a.k.ld;
+  const short* vp = a.v.p + p.kv * a.v.head + p.start * a.v.ld;
+  const int hi = a.causal ? min(p.row0 + kRows, p.end) : p.end;
+  const int wave_hi = w0 >= p.end ? p.start : a.causal ? min(w0 + 32, p.end) : p.end;
+  const int last = a.causal ? min(row, p.end - 1) : p.end - 1;  // the row's last key
+  const int nt = (hi - p.start + kTile - 1) / kTile;
+  auto load = [&](int t) {
+    const int left = p.end - p.start - t * kTile;
+    L::load(lds[t & 1][0], kp + (int64_t)t * kTile * a.k.ld, a.k.ld, left, a.d);
+    L::load(lds[t & 1][1], vp + (int64_t)t * kTile * a.v.ld, a.v.ld, left, a.d);
+  };
+  f16v o[L::kBlocks];
+#pragma unroll
+  for (int i = 0; i < L::kBlocks; i++) o[i] = f16v{};
+  float m = -INFINITY, l = 0;
+  load(0);
+  for (int t = 0; t < nt; t++) {
+    sync_loads();
+    if (t + 1 < nt) load(t + 1);
+    const int j0 = p.start + t * kTile;
+    if (j0 >= wave_hi) continue;
+    const char *kt = lds[t & 1][0], *vt = lds[t & 1][1];
+    f16v s[2];
+#pragma unroll
+    for (int b = 0; b < 2; b++) {
+      s[b] = f16v{};
+#pragma unroll
+      for (int i = 0; i < L::kSteps; i++) s[b] = T::mfma(L::rows(kt, b * 32, i, lane), qf[i], s[b]);
+    }
+    if (j0 + kTile - 1 > (a.causal ? min(w0, p.end - 1) : p.end - 1)) {
+#pragma unroll
+      for (int b = 0; b < 2; b++)
+#pragma unroll
+        for (int r = 0; r < 16; r++)
+          s[b][r] = j0 + b * 32 + row_of(r, half) <= last ? s[b][r] : -INFINITY;
+    }
+    float top = s[0][0];
+#pragma unroll
+    for (int r = 1; r < 32; r++) top = fmaxf(top, s[r >> 4][r & 15]);
+    top = fmaxf(top, other_half(top)) * a.scale2;
+    // The maximum that P is taken against may lag behind by kLazy: the sums are
+    // the same, and most tiles need no scaling of o.
+    if (__any(top > m + kLazy || m == -INFINITY)) {
+      const float next = fmaxf(m, top), alpha = exp2f(m - next);
+      l *= alpha;
+#pragma unroll
+      for (int i = 0; i < L::kBlocks; i++) o[i] *= alpha;
+      m = next;
+    }
+    const float shift = T::kBias - m;
+#pragma unroll
+    for (int b = 0; b < 2; b++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) {
+        s[b][r] = __builtin_amdgcn_exp2f(fmaf(s[b][r], a.scale2, shift));
+        l += s[b][r];
+      }
+#pragma unroll
+    for (int g = 0; g < 4; g++) {
+      const s8v pf = pack<T>(s[g >> 1], g & 1);
+#pragma unroll
+      for (int i = 0; i < L::kBlocks; i++) o[i] = T::mfma(L::columns(vt, g * 16, i * 32, lane), pf, o[i]);
+    }
+  }
+  l += other_half(l);
+  const int rows = min(32, p.end - w0);
+  __syncthreads();  // the tiles' place is free
+  if (rows <= 0) return;
+  char* strip = (char*)lds + w * 32 * HD * 2;
+  const int64_t ld = (int64_t)a.heads * a.d, at = w0 * ld + (int64_t)p.head * a.d;
+  store_rows<T, HD>(strip, o, 1.0f / l, false, f.out + at, ld, rows, a.d, lane);
+  if (f.out_lo) store_rows<T, HD>(strip, o, 1.0f / l, true, f.out_lo + at, ld, rows, a.d, lane);
+  if (f.lse && half == 0 && row < p.end) f.lse[(int64_t)p.head * a.tokens + row] = m - T::kBias + log2f(l);
+}
+
+// ---- backward ------------------------------------------------------------------
+
+struct Backward {
+  Rows dout;
+  const short* out;     // [tokens][heads][d]
+  const short* out_lo;
+  const float* lse;     // [heads][tokens]
+  float* delta;         // [heads][tokens]
+  float* most;          // [kMost][2]: the largest |do|^2 and |v|^2 of a block's rows (fp16)
+  short* dq;            // [tokens][heads][d]
+  short* dk;            // [tokens][kv_heads][d]
+  short* dv;
+  float* part;          // where the group is split: fp32 [2][splits][tokens][kv_heads][d]
+  int splits;           // of a group's heads
+};
+constexpr int kMost = 512;
+
+// delta, and for fp16 the largest rows: a wave a row at a time.
+template <class T>
+__global__ __launch_bounds__(256) void k_delta(Args a, Backward b) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int64_t rows = (int64_t)a.tokens * a.heads, values = T::kScaled ? (int64_t)a.tokens * a.kv_heads : 0;
+  float mo = 0, mv = 0;
+  const int per = 64 / 16;  // rows of a wave, 16 lanes each
+  const int sub = lane & 15;
+  for (int64_t i = ((int64_t)blockIdx.x * 4 + w) * per + (lane >> 4); i < rows + values; i += (int64_t)gridDim.x * 4 * per) {
+    float s = 0, n = 0;
+    if (i < rows) {
+      const int64_t t = i / a.heads;
+      const int h = (int)(i - t * a.heads);
+      const short* go = b.dout.p + t * b.dout.ld + h * b.dout.head;
+      for (int c = sub * 8; c < a.d; c += 128) {
+        const s8v x = *(const s8v*)(go + c), y = *(const s8v*)(b.out + i * a.d + c),
+                  z = *(const s8v*)(b.out_lo + i * a.d + c);
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          const float v = T::widen(x[e]);
+          s = fmaf(v, T::widen(y[e]) + T::widen(z[e]), s);
+          n = fmaf(v, v, n);
+        }
+      }
+    } else {
+      const int64_t t = (i - rows) / a.kv_heads;
+      const short* v = a.v.p + t * a.v.ld + (i - rows - t * a.kv_heads) * a.v.head;
+      for (int c = sub * 8; c < a.d; c += 128) {
+        const s8v x = *(const s8v*)(v + c);
+#pragma unroll
+        for (int e = 0; e < 8; e++) n = fmaf(T::widen(x[e]), T::widen(x[e]), n);
+      }
+    }
+#pragma unroll
+    for (int k = 8; k; k >>= 1) {
+      s += __shfl_xor(s, k);
+      n += __shfl_xor(n, k);
+    }
+    if (i < rows) {
+      if (sub == 0) {
+        const int64_t t = i / a.heads;
+        b.delta[(i - t * a.heads) * a.tokens + t] = s;
+      }
+      mo = fmaxf(mo, n);
+    } else {
+      mv = fmaxf(mv, n);
+    }
+  }
+  if (!T::kScaled) return;
+  __shared__ float buf[4][2];
+#pragma unroll
+  for (int k = 32; k >= 16; k >>= 1) {
+    mo = fmaxf(mo, __shfl_xor(mo, k));
+    mv = fmaxf(mv, __shfl_xor(mv, k));
+  }
+  if (lane == 0) {
+    buf[w][0] = mo;
+    buf[w][1] = mv;
+  }
+  __syncthreads();
+  if (threadIdx.x < 2)
+    b.most[blockIdx.x * 2 + threadIdx.x] = fmaxf(fmaxf(buf[0][threadIdx.x], buf[1][threadIdx.x]),
+                                                 fmaxf(buf[2][threadIdx.x], buf[3][threadIdx.x]));
+}
+
+// A power of two that takes dS to at most 2^15 in fp16: |dP - delta| is at most
+// 2 |do| |v|, whatever the rows. `buf`: 8 floats of shared memory.
+__device__ inline float gradient_scale(const float* most, float* buf) {
+  float mo = 0, mv = 0;
+  for (int i = threadIdx.x; i < kMost; i += kThreads) {
+    mo = fmaxf(mo, most[2 * i]);
+    mv = fmaxf(mv, most[2 * i + 1]);
+  }
+#pragma unroll
+  for (int k = 32; k; k >>= 1) {
+    mo = fmaxf(mo, __shfl_xor(mo, k));
+    mv = fmaxf(mv, __shfl_xor(mv, k));
+  }
+  const int w = threadIdx.x >> 6;
+  if ((threadIdx.x & 63) == 0) {
+    buf[2 * w] = mo;
+    buf[2 * w + 1] = mv;
+  }
+  __syncthreads();
+  mo = fmaxf(fmaxf(buf[0], buf[2]), fmaxf(buf[4], buf[6]));
+  mv = fmaxf(fmaxf(buf[1], buf[3]), fmaxf(buf[5], buf[7]));
+  __syncthreads();
+  const float bound = 2.0f * sqrtf(mo) * sqrtf(mv);
+  if (!(bound > 0.0f) || !(bound < INFINITY)) return 1.0f;
+  int e;
+  frexpf(bound, &e);  // bound < 2^e
+  return ldexpf(1.0f, max(-100, min(100, 15 - e)));
+}
+
+template <class T, int HD>
+__global__ DSX_ATTENTION_KERNEL(HD) void k_query_grads(Args a, Backward b) {
+  using L = Tile<HD>;
+  __shared__ __attribute__((aligned(1024))) char lds[2][2][L::kBytes];
+  const Place p = place_of(a, a.heads);
+  if (!p.good) return;
+  const float ds_scale = T::kScaled ? gradient_scale(b.most, (float*)lds) : 1.0f;
+  const int lane = threadIdx.x & 63, half = lane >> 5, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int w0 = p.row0 + 32 * w, row = w0 + (lane & 31), there = min(row, p.end - 1);
+  s8v qf[L::kSteps], gf[L::kSteps];
+  L::own(qf, a.q.p + p.head * a.q.head, a.q.ld, there, a.d, lane);
+  L::own(gf, b.dout.p + p.head * b.dout.head, b.dout.ld, there, a.d, lane);
+  // A row with one key has P = 1 whatever its score: dS is zero, not the
+  // rounding errors of dP - delta.
+  const bool one = a.causal ? row == p.start : p.end - p.start == 1;
+  const float lse = one ? INFINITY : b.lse[(int64_t)p.head * a.tokens + there];
+  const float delta = b.delta[(int64_t)p.head * a.tokens + there];
+  const short* kp = a.k.p + p.kv * a.k.head + p.start * a.k.ld;
+  const short* vp = a.v.p + p.kv * a.v.head + p.start * a.v.ld;
+  const int hi = a.causal ? min(p.row0 + kRows, p.end) : p.end;
+  const int wave_hi = w0 >= p.end ? p.start : a.causal ? min(w0 + 32, p.end) : p.end;
+  const int last = a.causal ? there : p.end - 1;
+  const int nt = (hi - p.start + kTile - 1) / kTile;
+  auto load = [&](int t) {
+    const int left = p.end - p.start - t * kTile;
+    L::load(lds[t & 1][0], kp + (int64_t)t * kTile * a.k.ld, a.k.ld, left, a.d);
+    L::load(lds[t & 1][1], vp + (int64_t)t * kTile * a.v.ld, a.v.ld, left, a.d);
+  };
+  f16v dq[L::kBlocks];
+#pragma unroll
+  for (int i = 0; i < L::kBlocks; i++) dq[i] = f16v{};
+  load(0);
+  for (int t = 0; t < nt; t++) {
+    sync_loads();
+    if (t + 1 < nt) load(t + 1);
+    const int j0 = p.start + t * kTile;
+    if (j0 >= wave_hi) continue;
+    const char *kt = lds[t & 1][0], *vt = lds[t & 1][1];
+    const bool edge = j0 + kTile - 1 > (a.causal ? min(w0, p.end - 1) : p.end - 1);
+#pragma unroll
+    for (int c = 0; c < 2; c++) {
+      f16v s = {}, dp = {};
+#pragma unroll
+      for (int i = 0; i < L::kSteps; i++) {
+        s = T::mfma(L::rows(kt, c * 32, i, lane), qf[i], s);
+        dp = T::mfma(L::rows(vt, c * 32, i, lane), gf[i], dp);
+      }
+#pragma unroll
+      for (int r = 0; r < 16; r++) {
+        const float e = __builtin_amdgcn_exp2f(fmaf(s[r], a.scale2, -lse));
+        s[r] = e * (dp[r] - delta) * ds_scale;
+      }
+      if (edge) {
+#pragma unroll
+        for (int r = 0; r < 16; r++) s[r] = j0 + c * 32 + row_of(r, half) <= last ? s[r] : 0.0f;
+      }
+#pragma unroll
+      for (int g = 0; g < 2; g++) {
+        const s8v sf = pack<T>(s, g);
+#pragma unroll
+        for (int i = 0; i < L::kBlocks; i++) dq[i] = T::mfma(L::columns(kt, c * 32 + g * 16, i * 32, lane), sf, dq[i]);
+      }
+    }
+  }
+  const int rows = min(32, p.end - w0);
+  __syncthreads();
+  if (rows <= 0) return;
+  const int64_t ld = (int64_t)a.heads * a.d;
+  store_rows<T, HD>((char*)lds + w * 32 * HD * 2, dq, a.scale / ds_scale, false,
+                    b.dq + w0 * ld + (int64_t)p.head * a.d, ld, rows, a.d, lane);
+}
+
+// Rows of fp32 partial sums, one a lane.
+template <int HD>
+__device__ inline void store_part(float* out, const f16v* o, float factor, bool there, int d, int half) {
+  if (!there) return;
+#pragma unroll
+  for (int i = 0; i < HD / 32; i++)
+#pragma unroll
+    for (int c = 0; c < 4; c++) {
+      const int f = i * 32 + c * 8 + half * 4;
+      if (f < d) *(f4v*)(out + f) = f4v{o[i][c * 4], o[i][c * 4 + 1], o[i][c * 4 + 2], o[i][c * 4 + 3]} * factor;
+    }
+}
+
+template <class T, int HD>
+__global__ DSX_ATTENTION_KERNEL(HD) void k_key_grads(Args a, Backward b) {
+  using L = Tile<HD>;
+  __shared__ __attribute__((aligned(1024))) char lds[2][2][L::kBytes];
+  __shared__ __attribute__((aligned(256))) float stats[2][2][kTile];  // lse, delta of a tile's rows
+  const Place p = place_of(a, a.kv_heads * b.splits);
+  if (!p.good) return;
+  const float ds_scale = T::kScaled ? gradient_scale(b.most, (float*)lds) : 1.0f;
+  const int split = p.head % b.splits;  // place_of numbers the splits of a key head as its heads
+  const int g0 = a.group * split / b.splits, g1 = a.group * (split + 1) / b.splits;
+  const int lane = threadIdx.x & 63, half = lane >> 5, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int w0 = p.row0 + 32 * w, key = w0 + (lane & 31), there = min(key, p.end - 1);
+  s8v kf[L::kSteps], vf[L::kSteps];
+  L::own(kf, a.k.p + p.kv * a.k.head, a.k.ld, there, a.d, lane);
+  L::own(vf, a.v.p + p.kv * a.v.head, a.v.ld, there, a.d, lane);
+  const int first = a.causal ? p.row0 : p.start;
+  const int per = (p.end - first + kTile - 1) / kTile, nt = per * (g1 - g0);
+  auto load = [&](int t, int head, int i0) {
+    const int left = p.end - i0;
+    L::load(lds[t & 1][0], a.q.p + head * a.q.head + i0 * a.q.ld, a.q.ld, left, a.d);
+    L::load(lds[t & 1][1], b.dout.p + head * b.dout.head + i0 * b.dout.ld, b.dout.ld, left, a.d);
+    if (w < 2) {
+      const float* from = (w ? b.delta : b.lse) + (int64_t)head * a.tokens + i0 + min(lane, left - 1);
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
+                                       (__attribute__((address_space(3))) void*)stats[t & 1][w], 4, 0, 0);
+    }
+  };
+  f16v dk[L::kBlocks], dv[L::kBlocks];
+#pragma unroll
+  for (int i = 0; i < L::kBlocks; i++) dk[i] = dv[i] = f16v{};
+  int head = p.kv * a.group + g0, i0 = first;
+  load(0, head, i0);
+  for (int t = 0; t < nt; t++) {
+    sync_loads();
+    const int now = i0;
+    i0 += kTile;
+    if (i0 >= p.end) {
+      i0 = first;
+      head++;
+    }
+    if (t + 1 < nt) load(t + 1, head, i0);
+    if (w0 >= p.end || (a.causal && now + kTile - 1 < w0)) continue;
+    const char *qt = lds[t & 1][0], *gt = lds[t & 1][1];
+    const bool edge = now + kTile > p.end || (a.causal && now < w0 + 31) || p.end - p.start == 1;
+#pragma unroll
+    for (int c = 0; c < 2; c++) {
+      f16v s = {}, dp = {};
+#pragma unroll
+      for (int i = 0; i < L::kSteps; i++) {
+        s = T::mfma(L::rows(qt, c * 32, i, lane), kf[i], s);
+        dp = T::mfma(L::rows(gt, c * 32, i, lane), vf[i], dp);
+      }
+#pragma unroll
+      for (int q = 0; q < 4; q++) {
+        const f4v lse = *(const f4v*)&stats[t & 1][0][c * 32 + q * 8 + half * 4];
+        const f4v delta = *(const f4v*)&stats[t & 1][1][c * 32 + q * 8 + half * 4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const int r = q * 4 + e;
+          s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.scale2, 2.0f * T::kBias - lse[e]));
+          dp[r] = s[r] * (dp[r] - delta[e]) * (ds_scale * (T::kScaled ? 0x1p-14f : 1.0f));
+        }
+      }
+      if (edge) {
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+          const int i = now + c * 32 + row_of(r, half);
+          const bool seen = i < p.end && (!a.causal || key <= i);
+          const bool one = a.causal ? i == p.start : p.end - p.start == 1;  // as in k_query_grads
+          s[r] = seen ? s[r] : 0.0f;
+          dp[r] = seen && !one ? dp[r] : 0.0f;
+        }
+      }
+#pragma unroll
+      for (int g = 0; g < 2; g++) {
+        const s8v pf = pack<T>(s, g), sf = pack<T>(dp, g);
+#pragma unroll
+        for (int i = 0; i < L::kBlocks; i++) {
+          dv[i] = T::mfma(L::columns(gt, c * 32 + g * 16, i * 32, lane), pf, dv[i]);
+          dk[i] = T::mfma(L::columns(qt, c * 32 + g * 16, i * 32, lane), sf, dk[i]);
+        }
+      }
+    }
+  }
+  const int rows = min(32, p.end - w0);
+  __syncthreads();
+  if (rows <= 0) return;
+  const float fk = a.scale / ds_scale, fv = T::kScaled ? 0x1p-14f : 1.0f;
+  const int64_t ld = (int64_t)a.kv_heads * a.d, at = w0 * ld + (int64_t)p.kv * a.d;
+  if (b.splits > 1) {
+    const int64_t plane = (int64_t)a.tokens * ld;
+    float* out = b.part + split * plane + at + (lane & 31) * ld;
+    store_part<HD>(out, dk, fk, key < p.end, a.d, half);
+    store_part<HD>(out + b.splits * plane, dv, fv, key < p.end, a.d, half);
+    return;
+  }
+  char* strip = (char*)lds + w * 32 * HD * 2;
+  store_rows<T, HD>(strip, dk, fk, false, b.dk + at, ld, rows, a.d, lane);
+  store_rows<T, HD>(strip, dv, fv, false, b.dv + at, ld, rows, a.d, lane);
+}
+
+// The splits' sums, added in order: eight values a thread.
+template <class T>
+__global__ __launch_bounds__(256) void k_join(const float* __restrict__ part, short* __restrict__ dk,
+                                              short* __restrict__ dv, int64_t n, int splits) {
+  const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
+  if (at >= n) return;
+  const float* p = part + (blockIdx.y ? splits * n : 0) + at;
+  f4v x = {}, y = {};
+  for (int s = 0; s < splits; s++) {
+    x += *(const f4v*)(p + s * n);
+    y += *(const f4v*)(p + s * n + 4);
+  }
+  s8v r;
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    r[e] = T::round(x[e]);
+    r[e + 4] = T::round(y[e]);
+  }
+  *(s8v*)((blockIdx.y ? dv : dk) + at) = r;
+}
+
+// ---- host ------------------------------------------------------------------
+
+
+// Parts of a group's heads in k_key_grads: enough blocks for four rounds of two
+// blocks a CU, since a causal mask makes the blocks of a sequence as unequal as
+// can be.
+int splits_of(const DsxAttention& q) {
+  const int64_t blocks = q.tile_count * q.kv_heads, group = q.heads / q.kv_heads;
+  const int64_t want = ceil_div(4 * 2 * kCus, blocks > 0 ? blocks : 1);
+  return (int)(want < group ? want : group);
+}
+
+struct Layout {
+  int64_t delta, most, part, total;
+};
+Layout layout_of(const DsxAttention& q) {
+  Layout l{};
+  l.most = round_up(q.tokens * q.heads * 4, 256);
+  l.part = l.most + kMost * 2 * 4;
+  const int splits = splits_of(q);
+  l.total = l.part + (splits > 1 ? round_up(2 * splits * q.tokens * q.kv_heads * q.head_dim * 4, 256) : 0);
+  return l;
+}
+
+Args args_of(const DsxAttention& q) {
+  Args a{};
+  a.q = {(const short*)q.q, q.ld_q, q.head_q};
+  a.k = {(const short*)q.k, q.ld_k, q.head_k};
+  a.v = {(const short*)q.v, q.ld_v, q.head_v};
+  a.tiles = (const int4*)q.tiles;
+  a.heads = q.heads;
+  a.kv_heads = q.kv_heads;
+  a.group = q.heads / q.kv_heads;
+  a.d = q.head_dim;
+  a.tokens = (int)q.tokens;
+  a.causal = q.causal;
+  a.scale = q.scale;
+  a.scale2 = q.scale * 1.44269504088896340736f;
+  return a;
+}
+
+template <class T, int HD>
+void forward(const Args& a, const Forward& f, int64_t tiles, hipStream_t s) {
+  k_attend<T, HD><<<dim3((unsigned)(tiles * a.heads)), kThreads, 0, s>>>(a, f);
+}
+
+template <class T, int HD>
+void backward(Args a, const Backward& b, int64_t tiles, hipStream_t s) {
+  k_delta<T><<<kMost, 256, 0, s>>>(a, b);
+  if (b.dq) k_query_grads<T, HD><<<dim3((unsigned)(tiles * a.heads)), kThreads, 0, s>>>(a, b);
+  if (b.dk) {
+    a.tiles += tiles;  // by keys
+    k_key_grads<T, HD><<<dim3((unsigned)(tiles * a.kv_heads * b.splits)), kThreads, 0, s>>>(a, b);
+    const int64_t n = (int64_t)a.tokens * a.kv_heads * a.d;
+    if (b.splits > 1) k_join<T><<<dim3((unsigned)ceil_div(n, 2048), 2), 256, 0, s>>>(b.part, b.dk, b.dv, n, b.splits);
+  }
+}
+
+bool off16(const void* p) { return ((uintptr_t)p & 15) != 0; }
+
+int check(const char* what, const DsxAttention* q) {
+  if (!q) return fail(DSX_EINVAL, "%s: the argument block is NULL", what);
+  if (!dsxi::is16(q->dtype)) return fail(DSX_EINVAL, "%s: dtype must be DSX_F16 or DSX_BF16", what);
+  if (q->tokens < 0 || q->tokens > DSX_ATTENTION_MAX_TOKENS)
+    return fail(DSX_EINVAL, "%s: tokens in [0, %d]", what, DSX_ATTENTION_MAX_TOKENS);
+  if (q->kv_heads < 1 || q->heads < q->kv_heads || q->heads % q->kv_heads || q->heads > DSX_ATTENTION_MAX_HEADS)
+    return fail(DSX_EINVAL, "%s: heads must be a multiple of kv_heads, at most %d", what, DSX_ATTENTION_MAX_HEADS);
+  if (q->head_dim < 8 || q->head_dim % 8 || q->head_dim > DSX_ATTENTION_MAX_HEAD_DIM)
+    return fail(DSX_EINVAL, "%s: head_dim must be a multiple of 8 up to %d", what, DSX_ATTENTION_MAX_HEAD_DIM);
+  if (q->tile_count < 0 || q->tile_count > q->tokens || (q->tokens && !q->tile_count))
+    return fail(DSX_EINVAL, "%s: tile_count must lie in [1, tokens]", what);
+  if (q->tile_count * q->heads > INT32_MAX) return fail(DSX_EINVAL, "%s: more than 2^31 - 1 tiles and heads", what);
+  if (!(q->scale > 0.0f) || !(q->scale < INFINITY)) return fail(DSX_EINVAL, "%s: scale must be positive and finite", what);
+  return DSX_OK;
+}
+
+bool bad_rows(const void* p, int64_t ld, int64_t head, int64_t heads, int64_t d) {
+  return !p || off16(p) || ld % 8 || head % 8 || ld < d || (heads > 1 && head < d) || ld > DSX_ATTENTION_MAX_STRIDE ||
+         head > INT64_MAX / 4096;
+}
+
+int check_device(const char* what, const DsxAttention* q) {
+  if (bad_rows(q->q, q->ld_q, q->head_q, q->heads, q->head_dim) ||
+      bad_rows(q->k, q->ld_k, q->head_k, q->kv_heads, q->head_dim) ||
+      bad_rows(q->v, q->ld_v, q->head_v, q->kv_heads, q->head_dim))
+    return fail(DSX_EINVAL, "%s: q, k and v need 16-byte aligned rows, strides that are multiples of 8 and at least "
+                "head_dim, row strides of at most %d", what, DSX_ATTENTION_MAX_STRIDE);
+  if (!q->tiles || off16(q->tiles)) return fail(DSX_EINVAL, "%s: tiles is NULL or misaligned", what);
+  return DSX_OK;
+}
+
+#define DSX_BY_HEAD(CALL, T, ...)                                \
+  do {                                                           \
+    if (args->head_dim <= 64) CALL<T, 64>(__VA_ARGS__);          \
+    else if (args->head_dim <= 128) CALL<T, 128>(__VA_ARGS__);   \
+    else CALL<T, 256>(__VA_ARGS__);                              \
+  } while (0)
+
+}  // namespace
+
+extern "C" {
+
+int64_t dsx_attention_tiles(const int64_t* lengths, int64_t count, int32_t* tiles, int64_t capacity) {
+  if (count < 0 || (count && !lengths)) return fail(-1, "dsx_attention_tiles: bad list of lengths");
+  int64_t tokens = 0, n = 0;
+  for (int64_t i = 0; i < count; i++) {
+    if (lengths[i] < 0 || lengths[i] > DSX_ATTENTION_MAX_TOKENS - tokens)
+      return fail(-1, "dsx_attention_tiles: lengths must be >= 0 and add up to at most %d", DSX_ATTENTION_MAX_TOKENS);
+    tokens += lengths[i];
+    n += ceil_div(lengths[i], kRows);
+  }
+  if (!tiles) return n;
+  if (capacity < n) return fail(-1, "dsx_attention_tiles: %lld tiles do not fit", (long long)n);
+  // Most work first, by counting the tiles of each distance (in tiles) from the
+  // sequence's first row, or from its end.
+  int64_t longest = 0;
+  for (int64_t i = 0; i < count; i++)
+    if (ceil_div(lengths[i], kRows) > longest) longest = ceil_div(lengths[i], kRows);
+  int64_t* at = new (std::nothrow) int64_t[2 * (longest + 1)]();
+  if (!at) return fail(-1, "dsx_attention_tiles: out of memory");
+  for (int64_t i = 0; i < count; i++) at[ceil_div(lengths[i], kRows)]++;
+  // at[k]: sequences of k tiles -> tiles at distance k - 1, which sequences of k
+  // tiles and more have -> the first place of that distance, the farthest first.
+  for (int64_t k = longest - 1; k >= 1; k--) at[k] += at[k + 1];
+  int64_t place = 0;
+  for (int64_t k = longest; k >= 1; k--) {
+    const int64_t c = at[k];
+    at[k] = at[longest + 1 + k - 1] = place;
+    place += c;
+  }
+  int64_t row = 0;
+  for (int64_t i = 0; i < count; i++) {
+    const int64_t k = ceil_div(lengths[i], kRows);
+    for (int64_t t = 0; t < k; t++) {
+      const int32_t e[4] = {(int32_t)(row + t * kRows), (int32_t)row, (int32_t)(row + lengths[i]), 0};
+      int32_t* by_query = tiles + 4 * at[t + 1]++;
+      int32_t* by_key = tiles + 4 * (n + at[longest + 1 + (k - 1 - t)]++);
+      for (int c = 0; c < 4; c++) by_query[c] = by_key[c] = e[c];
+    }
+    row += lengths[i];
+  }
+  delete[] at;
+  return n;
+}
+
+int dsx_attention_forward(const DsxAttention* args, void* out, void* out_lo, float* lse, void* stream) {
+  const char* what = "dsx_attention_forward";
+  if (int rc = check(what, args)) return rc;
+  if (!args->tokens) return DSX_OK;
+  if (int rc = check_device(what, args)) return rc;
+  if (!out || off16(out) || off16(out_lo) || ((uintptr_t)lse & 3) || !out_lo != !lse)
+    return fail(DSX_EINVAL, "%s: NULL or misaligned output, or one of out_lo and lse alone", what);
+  const Args a = args_of(*args);
+  const Forward f{(short*)out, (short*)out_lo, lse};
+  hipStream_t s = as_stream(stream);
+  if (args->dtype == DSX_F16) DSX_BY_HEAD(forward, F16, a, f, args->tile_count, s);
+  else DSX_BY_HEAD(forward, BF16, a, f, args->tile_count, s);
+  return launch_status(what);
+}
+
+int64_t dsx_attention_workspace_bytes(const DsxAttention* args) {
+  if (check("dsx_attention_workspace_bytes", args)) return -1;
+  return layout_of(*args).total;
+}
+
+int dsx_attention_backward(const DsxAttention* args, const void* out, const void* out_lo, const float* lse,
+                           const void* d_out, int64_t ld_dout, int64_t head_dout, void* dq, void* dk, void* dv,
+                           void* workspace, int64_t workspace_bytes, void* stream) {
+  const char* what = "dsx_attention_backward";
+  if (int rc = check(what, args)) return rc;
+  if (!args->tokens) return DSX_OK;
+  if (int rc = check_device(what, args)) return rc;
+  if (!out || !out_lo || !lse || off16(out) || off16(out_lo) || ((uintptr_t)lse & 3))
+    return fail(DSX_EINVAL, "%s: NULL or misaligned result of the forward", what);
+  if (bad_rows(d_out, ld_dout, head_dout, args->heads, args->head_dim))
+    return fail(DSX_EINVAL, "%s: bad gradient of the output", what);
+  if (off16(dq) || off16(dk) || off16(dv) || !dk != !dv)
+    return fail(DSX_EINVAL, "%s: misaligned gradient, or one of dk and dv alone", what);
+  const Layout l = layout_of(*args);
+  if (!workspace || ((uintptr_t)workspace & 255) || workspace_bytes < l.total)
+    return fail(DSX_EINVAL, "%s: the workspace must be 256-byte aligned and of %lld bytes", what, (long long)l.total);
+  char* ws = (char*)workspace;
+  Backward b{};
+  b.dout = {(const short*)d_out, ld_dout, head_dout};
+  b.out = (const short*)out;
+  b.out_lo = (const short*)out_lo;
+  b.lse = lse;
+  b.delta = (float*)(ws + l.delta);
+  b.most = (float*)(ws + l.most);
+  b.part = (float*)(ws + l.part);
+  b.dq = (short*)dq;
+  b.dk = (short*)dk;
+  b.dv = (short*)dv;
+  b.splits = splits_of(*args);
+  const Args a = args_of(*args);
+  hipStream_t s = as_stream(stream);
+  if (args->dtype == DSX_F16) DSX_BY_HEAD(backward, F16, a, b, args->tile_count, s);
+  else DSX_BY_HEAD(backward, BF16, a, b, args->tile_count, s);
+  return launch_status(what);
+}
+
+}  // extern "C"

@@ -537,18 +537,6 @@ struct Shape {
   int tm, tn, splits, per;
 };
 
-// 256- or 128-tiles, for n256 and n128 of them: a CU runs one block of the
-// first at a time or two of the second, whose products take 1.2 times as long
-// for the same area (a lone block of 128 on a CU: 1.4 times); the rounds over
-// the CUs decide. (By sizes alone, as the split count: the same on any card.)
-constexpr int kCus = 256;
-int square_tile(int64_t n256, int64_t n128) {
-  const int64_t rest = n128 % (2 * kCus);
-  const int64_t big = ceil_div(n256, kCus) * 4 * 10;
-  const int64_t small = n128 / (2 * kCus) * 24 + (rest > kCus ? 24 : rest ? 14 : 0);
-  return big <= small ? 256 : 128;
-}
-
 Shape shape_of(int64_t m, int64_t n, int64_t kt, bool pair, bool direct) {
   Shape s{};
   const int64_t cols = pair ? 2 * n : n;

@@ -30,6 +30,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "dsx_internal.h"
+
 namespace dsxg {
 
 typedef short    s4v __attribute__((ext_vector_type(4)));
@@ -494,6 +496,20 @@ struct Gemm {
     __syncthreads();  // the tiles may be filled again
   }
 };
+
+// ---- host ------------------------------------------------------------------
+
+// 256- or 128-tiles, for n256 and n128 of them: a CU runs one block of the
+// first at a time or two of the second, whose products take 1.2 times as long
+// for the same area (a lone block of 128 on a CU: 1.4 times); the rounds over
+// the CUs decide. (By sizes alone, as the split count: the same on any card.)
+constexpr int kCus = 256;
+inline int square_tile(int64_t n256, int64_t n128) {
+  const int64_t rest = n128 % (2 * kCus);
+  const int64_t big = dsxi::ceil_div(n256, kCus) * 4 * 10;
+  const int64_t small = n128 / (2 * kCus) * 24 + (rest > kCus ? 24 : rest ? 14 : 0);
+  return big <= small ? 256 : 128;
+}
 
 }  // namespace dsxg
 

@@ -784,6 +784,161 @@ int dsx_norm_backward(const DsxNorm* args /* host */, const void* d_hidden,
                       void* d_gate, void* d_next_weight, void* workspace,
                       int64_t workspace_bytes, void* stream);
 
+/* ---- attention over packed sequences ---------------------------------- */
+
+#define DSX_ATTENTION_MAX_TOKENS   (1 << 27)
+#define DSX_ATTENTION_MAX_HEADS    1024
+#define DSX_ATTENTION_MAX_HEAD_DIM 256
+#define DSX_ATTENTION_MAX_STRIDE   (1 << 24)
+
+/* The inputs (a host struct): q is [tokens][heads][head_dim], k and v
+ * [tokens][kv_heads][head_dim], of `dtype` (DSX_F16 or DSX_BF16), with the row
+ * strides ld_* and head strides head_* in elements. Bases are 16-byte aligned,
+ * strides and head_dim multiples of 8. heads is a multiple of kv_heads; query
+ * head h reads key head h / (heads / kv_heads). `tiles` is a device copy of
+ * what dsx_attention_tiles made, whose sequences cover rows [0, tokens). */
+typedef struct DsxAttention {
+  const void*    q;
+  const void*    k;
+  const void*    v;
+  int64_t        ld_q;
+  int64_t        ld_k;
+  int64_t        ld_v;
+  int64_t        head_q;
+  int64_t        head_k;
+  int64_t        head_v;
+  int64_t        tokens;
+  const int32_t* tiles;
+  int64_t        tile_count;
+  int32_t        heads;
+  int32_t        kv_heads;
+  int32_t        head_dim;
+  int32_t        dtype;
+  int32_t        causal;
+  float          scale;
+} DsxAttention;
+
+/* The tile table of sequences of the given lengths (zero allowed), one behind
+ * the other from row 0: 2 x count entries of four int32, written to `tiles`
+ * (host, room for `capacity` entries of each half; NULL: only counted).
+ * Returns the count, -1 with dsx_last_error for bad lengths. Host only. */
+int64_t dsx_attention_tiles(const int64_t* lengths /* host */, int64_t count,
+                            int32_t* tiles /* host */, int64_t capacity);
+
+/* out = softmax(scale q k^T) v within each sequence (causal nonzero: over the
+ * keys up to the query's own), [tokens][heads][head_dim] contiguous, of
+ * `dtype`. For a backward, out_lo (like out) and lse (fp32 [heads][tokens])
+ * take what it needs; both NULL: not kept. fp32 statistics and sums; the
+ * probabilities are rounded to `dtype` for the product with v. No counterpart
+ * in the reference. */
+int dsx_attention_forward(const DsxAttention* args /* host */, void* out,
+                          void* out_lo, float* lse, void* stream);
+
+/* Bytes of device scratch the backward needs; -1 with dsx_last_error. Host
+ * only. */
+int64_t dsx_attention_workspace_bytes(const DsxAttention* args /* host */);
+
+/* The gradients for d_out [tokens][heads][head_dim] (strides as q's, aligned
+ * alike): dq like out, dk and dv [tokens][kv_heads][head_dim], contiguous, of
+ * `dtype`, written, not added to. dq may be NULL, and dk and dv together; they
+ * are then not computed. out, out_lo and lse as the forward left them. Sums are
+ * added in an order set by the sizes alone. */
+int dsx_attention_backward(const DsxAttention* args /* host */,
+                           const void* out, const void* out_lo,
+                           const float* lse, const void* d_out,
+                           int64_t ld_dout, int64_t head_dout, void* dq,
+                           void* dk, void* dv, void* workspace,
+                           int64_t workspace_bytes, void* stream);
+
+/* ---- the rotary embedding ---------------------------------------------- */
+
+/* q [tokens][heads][head_dim] and k [tokens][kv_heads][head_dim] (kv_heads 0:
+ * no k), of `dtype` (DSX_F32, DSX_F16 or DSX_BF16), with row strides ld_* and
+ * head strides head_* in elements, any alignment of the type. positions is
+ * [tokens] of int32 or int64 (position_bytes 4 or 8), negative ones included.
+ * The first `dims` features of a head are turned, the others copied: pair i is
+ * features i and i + dims/2, or with `interleaved` 2i and 2i + 1, and turns by
+ * position base^(-2i/dims). head_dim is at most 1024. */
+typedef struct DsxRotary {
+  const void* q;
+  const void* k;
+  const void* positions;
+  int64_t     ld_q;
+  int64_t     ld_k;
+  int64_t     head_q;
+  int64_t     head_k;
+  int64_t     tokens;
+  int32_t     heads;
+  int32_t     kv_heads;
+  int32_t     head_dim;
+  int32_t     dims;
+  int32_t     dtype;
+  int32_t     interleaved;
+  int32_t     position_bytes;
+  int32_t     reserved;
+  double      base;
+} DsxRotary;
+
+/* q_out and k_out (contiguous): q and k turned, by the opposite angles where
+ * `inverse` (which takes the outputs' gradients to the inputs'). Angles are
+ * formed in fp64, the arithmetic is fp32 and rounded once. No counterpart in
+ * the reference. */
+int dsx_rotary(const DsxRotary* args /* host */, void* q_out, void* k_out,
+               int32_t inverse, void* stream);
+
+/* ---- cross entropy of a linear layer's logits --------------------------- */
+
+#define DSX_REDUCE_NONE 0
+#define DSX_REDUCE_MEAN 1 /* over the rows that count                         */
+#define DSX_REDUCE_SUM  2
+
+/* x [tokens][width] and weight [vocab][width] of `dtype` (DSX_F16 or DSX_BF16),
+ * row strides in elements; targets [tokens] of int32 or int64 (target_bytes 4
+ * or 8). A row whose target is ignore_index does not count; one whose target
+ * lies outside [0, vocab) has a loss of NaN, as have its gradients. `saved`
+ * (dsx_loss_saved_bytes) is written by the forward and read by the backward;
+ * it and `workspace` are 256-byte aligned device memory. Sizes are at most
+ * 2^20 each. */
+typedef struct DsxLoss {
+  const void* x;
+  const void* weight;
+  const void* targets;
+  int64_t     ld_x;
+  int64_t     ld_weight;
+  int64_t     tokens;
+  int64_t     width;
+  int64_t     vocab;
+  int64_t     ignore_index;
+  int32_t     dtype;
+  int32_t     target_bytes;
+  int32_t     reduction;
+  int32_t     reserved;
+  void*       saved;
+  void*       workspace;
+  int64_t     workspace_bytes;
+} DsxLoss;
+
+/* Bytes of `saved` and of `workspace` (host only; no address but weight's, for
+ * its alignment, is looked at); -1 with dsx_last_error for bad sizes. */
+int64_t dsx_loss_saved_bytes(const DsxLoss* args /* host */);
+int64_t dsx_loss_workspace_bytes(const DsxLoss* args /* host */,
+                                 int32_t backward);
+
+/* loss_t = logsumexp(weight x_t) - (weight x_t)[target_t]: loss [tokens] (0 in
+ * rows that do not count) with DSX_REDUCE_NONE, else one value (the mean of no
+ * row is NaN). The logits are fp32 sums that stay in registers: a tile of them
+ * leaves its maximum and sum a row. No counterpart in the reference. */
+int dsx_loss_forward(const DsxLoss* args /* host */, float* loss,
+                     void* stream);
+
+/* The gradients for d_loss (fp32, like loss): dx [tokens][width] (zeros in rows
+ * that do not count) and dweight [vocab][width], contiguous, of `dtype`,
+ * written, not added to; either may be NULL. The logits are computed again, a
+ * piece of the vocabulary at a time, and rounded to `dtype` as gradients.
+ * `args` as the forward had it (x is not read). */
+int dsx_loss_backward(const DsxLoss* args /* host */, const float* d_loss,
+                      void* dx, void* dweight, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
