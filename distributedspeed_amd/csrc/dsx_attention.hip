@@ -144,6 +144,47 @@ struct Tile {
       f[s] = c < d ? *(const s8v*)(at + c) : s8v{0, 0, 0, 0, 0, 0, 0, 0};
     }
   }
+  // Their arrival is waited for here: left to their first use, inside a loop, the
+  // wait would be for the tiles on their way as well, in every round.
+  static __device__ inline void arrived(s8v* f) {
+#pragma unroll
+    for (int s = 0; s < kSteps; s++) asm volatile("" : "+v"(f[s]));
+  }
+};
+
+// The same reads with three registers of addresses, for a kernel that has none
+// to spare: the places of a row's chunks differ by an exclusive or. Two tiles,
+// kBytes apart.
+typedef __attribute__((address_space(3))) s8v LdsChunk;
+__device__ inline s8v read_chunk(LdsChunk* __restrict__ p) { return *p; }
+template <int HD>
+struct Reader {
+  using L = Tile<HD>;
+  uint32_t row, lo, hi;
+  __device__ inline void init(const char* lds, int lane) {
+    const uint32_t base = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)lds;
+    const int r = lane & 31, half = lane >> 5;
+    row = base + r * HD * 2 + ((half ^ L::swizzle(r)) << 4);
+    const int k = 4 * half + ((lane & 15) >> 2), c = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+    lo = base + k * HD * 2 + ((c ^ L::swizzle(k)) << 4) + (lane & 1) * 8;
+    hi = base + (k + 8) * HD * 2 + ((c ^ L::swizzle(k + 8)) << 4) + (lane & 1) * 8;
+  }
+  // For the rows from `at` bytes on.
+  __device__ inline Reader from(int at) const {
+    Reader r{row + at, lo + at, hi + at};
+    asm volatile("" : "+v"(r.row), "+v"(r.lo), "+v"(r.hi));
+    return r;
+  }
+  template <int TILE>
+  __device__ inline s8v rows(int step) const {
+    return read_chunk((LdsChunk*)(uintptr_t)((row ^ (step << 5)) + TILE * L::kBytes));
+  }
+  template <int TILE>
+  __device__ inline s8v columns(int r0, int i) const {
+    const uint32_t at = TILE * L::kBytes + r0 * HD * 2;
+    const s4v x = read_transposed((LdsBlock*)(uintptr_t)((lo ^ (i << 6)) + at)), y = read_transposed((LdsBlock*)(uintptr_t)((hi ^ (i << 6)) + at));
+    return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+  }
 };
 
 // Waits for this wave's direct loads and LDS reads, then for the other waves.
@@ -219,8 +260,31 @@ __device__ inline Place place_of(const Args& a, int heads) {
   return p;
 }
 
-#define DSX_ATTENTION_KERNEL(HD) \
-  __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(HD <= 128 ? 2 : 1, HD <= 128 ? 2 : 1)))
+// WAVES: a SIMD's, for 64 features; two for 128 and one for 256, which is what
+// their registers allow.
+#define DSX_ATTENTION_KERNEL(HD, WAVES)                                                       \
+  __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(HD == 64 ? WAVES : HD == 128 ? 2 : 1, \
+                                                                 HD == 64 ? WAVES : HD == 128 ? 2 : 1)))
+
+// v, as the compiler may not know it before this place: keeps what the masks of
+// the few tiles at a sequence's edges need out of every tile's way.
+__device__ inline int only_here(int v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
+
+// N matrix instructions with READS LDS reads each: AHEAD instructions' reads are
+// on their way before the first.
+template <int N, int READS, int AHEAD>
+__device__ inline void feed() {
+  __builtin_amdgcn_sched_group_barrier(0x100, AHEAD * READS, 0);
+#pragma unroll
+  for (int i = 0; i < N - AHEAD; i++) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+  }
+  __builtin_amdgcn_sched_group_barrier(0x008, AHEAD, 0);
+}
 
 // ---- forward -------------------------------------------------------------------
 
@@ -231,7 +295,7 @@ struct Forward {
 };
 
 template <class T, int HD>
-__global__ DSX_ATTENTION_KERNEL(HD) void k_attend(Args a, Forward f) {
+__global__ DSX_ATTENTION_KERNEL(HD, 4) void k_attend(Args a, Forward f) {
   using L = Tile<HD>;
   __shared__ __attribute__((aligned(1024))) char lds[2][2][L::kBytes];
   const Place p = place_of(a, a.heads);
@@ -246,6 +310,7 @@ __global__ DSX_ATTENTION_KERNEL(HD) void k_attend(Args a, Forward f) {
   const int wave_hi = w0 >= p.end ? p.start : a.causal ? min(w0 + 32, p.end) : p.end;
   const int last = a.causal ? min(row, p.end - 1) : p.end - 1;  // the row's last key
   const int nt = (hi - p.start + kTile - 1) / kTile;
+  L::arrived(qf);
   auto load = [&](int t) {
     const int left = p.end - p.start - t * kTile;
     L::load(lds[t & 1][0], kp + (int64_t)t * kTile * a.k.ld, a.k.ld, left, a.d);
@@ -262,19 +327,19 @@ __global__ DSX_ATTENTION_KERNEL(HD) void k_attend(Args a, Forward f) {
     const int j0 = p.start + t * kTile;
     if (j0 >= wave_hi) continue;
     const char *kt = lds[t & 1][0], *vt = lds[t & 1][1];
-    f16v s[2];
+    f16v s[2] = {};
 #pragma unroll
-    for (int b = 0; b < 2; b++) {
-      s[b] = f16v{};
+    for (int i = 0; i < L::kSteps; i++)
 #pragma unroll
-      for (int i = 0; i < L::kSteps; i++) s[b] = T::mfma(L::rows(kt, b * 32, i, lane), qf[i], s[b]);
-    }
+      for (int b = 0; b < 2; b++) s[b] = T::mfma(L::rows(kt, b * 32, i, lane), qf[i], s[b]);
+    feed<2 * L::kSteps, 1, 6>();
+    __builtin_amdgcn_sched_barrier(0);
     if (j0 + kTile - 1 > (a.causal ? min(w0, p.end - 1) : p.end - 1)) {
+      const int left = only_here(last) - j0 - 4 * half;
 #pragma unroll
       for (int b = 0; b < 2; b++)
 #pragma unroll
-        for (int r = 0; r < 16; r++)
-          s[b][r] = j0 + b * 32 + row_of(r, half) <= last ? s[b][r] : -INFINITY;
+        for (int r = 0; r < 16; r++) s[b][r] = b * 32 + row_of(r, 0) <= left ? s[b][r] : -INFINITY;
     }
     float top = s[0][0];
 #pragma unroll
@@ -303,6 +368,18 @@ __global__ DSX_ATTENTION_KERNEL(HD) void k_attend(Args a, Forward f) {
 #pragma unroll
       for (int i = 0; i < L::kBlocks; i++) o[i] = T::mfma(L::columns(vt, g * 16, i * 32, lane), pf, o[i]);
     }
+    // The first fragments are on their way while the vector unit works, and what
+    // is left of its work goes between the matrix instructions.
+    constexpr int kAhead = 4, kFrags = 4 * L::kBlocks;
+    __builtin_amdgcn_sched_group_barrier(0x100, 2 * kAhead, 0);
+    __builtin_amdgcn_sched_group_barrier(0x002, 40, 0);
+#pragma unroll
+    for (int i = 0; i < kFrags - kAhead; i++) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+      __builtin_amdgcn_sched_group_barrier(0x002, 80 / (kFrags - kAhead), 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, kAhead, 0);
   }
   l += other_half(l);
   const int rows = min(32, p.end - w0);
@@ -327,8 +404,8 @@ struct Backward {
   short* dq;            // [tokens][heads][d]
   short* dk;            // [tokens][kv_heads][d]
   short* dv;
-  float* part;          // where the group is split: fp32 [2][splits][tokens][kv_heads][d]
-  int splits;           // of a group's heads
+  float* part;          // where there are several parts: fp32 [2][parts][tokens][kv_heads][d]
+  int parts;            // of a tile's work in k_key_grads
 };
 constexpr int kMost = 512;
 
@@ -427,7 +504,7 @@ __device__ inline float gradient_scale(const float* most, float* buf) {
 }
 
 template <class T, int HD>
-__global__ DSX_ATTENTION_KERNEL(HD) void k_query_grads(Args a, Backward b) {
+__global__ DSX_ATTENTION_KERNEL(HD, 3) void k_query_grads(Args a, Backward b) {
   using L = Tile<HD>;
   __shared__ __attribute__((aligned(1024))) char lds[2][2][L::kBytes];
   const Place p = place_of(a, a.heads);
@@ -449,6 +526,8 @@ __global__ DSX_ATTENTION_KERNEL(HD) void k_query_grads(Args a, Backward b) {
   const int wave_hi = w0 >= p.end ? p.start : a.causal ? min(w0 + 32, p.end) : p.end;
   const int last = a.causal ? there : p.end - 1;
   const int nt = (hi - p.start + kTile - 1) / kTile;
+  L::arrived(qf);
+  L::arrived(gf);
   auto load = [&](int t) {
     const int left = p.end - p.start - t * kTile;
     L::load(lds[t & 1][0], kp + (int64_t)t * kTile * a.k.ld, a.k.ld, left, a.d);
@@ -479,8 +558,9 @@ __global__ DSX_ATTENTION_KERNEL(HD) void k_query_grads(Args a, Backward b) {
         s[r] = e * (dp[r] - delta) * ds_scale;
       }
       if (edge) {
+        const int left = only_here(last) - j0 - c * 32 - 4 * half;
 #pragma unroll
-        for (int r = 0; r < 16; r++) s[r] = j0 + c * 32 + row_of(r, half) <= last ? s[r] : 0.0f;
+        for (int r = 0; r < 16; r++) s[r] = row_of(r, 0) <= left ? s[r] : 0.0f;
       }
 #pragma unroll
       for (int g = 0; g < 2; g++) {
@@ -512,38 +592,44 @@ __device__ inline void store_part(float* out, const f16v* o, float factor, bool 
 }
 
 template <class T, int HD>
-__global__ DSX_ATTENTION_KERNEL(HD) void k_key_grads(Args a, Backward b) {
+__global__ DSX_ATTENTION_KERNEL(HD, 3) void k_key_grads(Args a, Backward b) {
   using L = Tile<HD>;
-  __shared__ __attribute__((aligned(1024))) char lds[2][2][L::kBytes];
-  __shared__ __attribute__((aligned(256))) float stats[2][2][kTile];  // lse, delta of a tile's rows
-  const Place p = place_of(a, a.kv_heads * b.splits);
+  // One array: with two, the compiler waits for all direct loads in flight before
+  // each read. Two pairs of tiles, then lse and delta of their rows.
+  __shared__ __attribute__((aligned(1024))) char lds[4 * L::kBytes + 4 * kTile * 4];
+  float* stats = (float*)(lds + 4 * L::kBytes);
+  const Place p = place_of(a, a.kv_heads * b.parts);
   if (!p.good) return;
   const float ds_scale = T::kScaled ? gradient_scale(b.most, (float*)lds) : 1.0f;
-  const int split = p.head % b.splits;  // place_of numbers the splits of a key head as its heads
-  const int g0 = a.group * split / b.splits, g1 = a.group * (split + 1) / b.splits;
   const int lane = threadIdx.x & 63, half = lane >> 5, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int w0 = p.row0 + 32 * w, key = w0 + (lane & 31), there = min(key, p.end - 1);
   s8v kf[L::kSteps], vf[L::kSteps];
   L::own(kf, a.k.p + p.kv * a.k.head, a.k.ld, there, a.d, lane);
   L::own(vf, a.v.p + p.kv * a.v.head, a.v.ld, there, a.d, lane);
-  const int first = a.causal ? p.row0 : p.start;
-  const int per = (p.end - first + kTile - 1) / kTile, nt = per * (g1 - g0);
+  // The tiles of queries, head by head; the part's share of them. (place_of
+  // numbers the parts of a key head as its heads.)
+  const int first = a.causal ? p.row0 : p.start, part = p.head % b.parts;
+  const int per = (p.end - first + kTile - 1) / kTile;
+  const int step0 = (int)((int64_t)per * a.group * part / b.parts);
+  const int nt = (int)((int64_t)per * a.group * (part + 1) / b.parts) - step0;
+  L::arrived(kf);
+  L::arrived(vf);
+  float stat = 0;
   auto load = [&](int t, int head, int i0) {
     const int left = p.end - i0;
-    L::load(lds[t & 1][0], a.q.p + head * a.q.head + i0 * a.q.ld, a.q.ld, left, a.d);
-    L::load(lds[t & 1][1], b.dout.p + head * b.dout.head + i0 * b.dout.ld, b.dout.ld, left, a.d);
-    if (w < 2) {
-      const float* from = (w ? b.delta : b.lse) + (int64_t)head * a.tokens + i0 + min(lane, left - 1);
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
-                                       (__attribute__((address_space(3))) void*)stats[t & 1][w], 4, 0, 0);
-    }
+    L::load(lds + (t & 1) * 2 * L::kBytes, a.q.p + head * a.q.head + i0 * a.q.ld, a.q.ld, left, a.d);
+    L::load(lds + ((t & 1) * 2 + 1) * L::kBytes, b.dout.p + head * b.dout.head + i0 * b.dout.ld, b.dout.ld, left, a.d);
+    if (w < 2) stat = (w ? b.delta : b.lse)[(int64_t)head * a.tokens + i0 + min(lane, left - 1)];
   };
+  Reader<HD> reader;
+  reader.init((const char*)lds, lane);
   f16v dk[L::kBlocks], dv[L::kBlocks];
 #pragma unroll
   for (int i = 0; i < L::kBlocks; i++) dk[i] = dv[i] = f16v{};
-  int head = p.kv * a.group + g0, i0 = first;
-  load(0, head, i0);
+  int head = p.kv * a.group + step0 / per, i0 = first + step0 % per * kTile;
+  if (nt > 0) load(0, head, i0);
   for (int t = 0; t < nt; t++) {
+    if (w < 2) stats[((t & 1) * 2 + w) * kTile + lane] = stat;
     sync_loads();
     const int now = i0;
     i0 += kTile;
@@ -553,20 +639,23 @@ __global__ DSX_ATTENTION_KERNEL(HD) void k_key_grads(Args a, Backward b) {
     }
     if (t + 1 < nt) load(t + 1, head, i0);
     if (w0 >= p.end || (a.causal && now + kTile - 1 < w0)) continue;
-    const char *qt = lds[t & 1][0], *gt = lds[t & 1][1];
     const bool edge = now + kTile > p.end || (a.causal && now < w0 + 31) || p.end - p.start == 1;
-#pragma unroll
+    constexpr int kUnroll = HD == 64 ? 2 : 1;
+#pragma unroll kUnroll
     for (int c = 0; c < 2; c++) {
+      const Reader<HD> rd = reader.from((t & 1) * 2 * L::kBytes + c * 32 * HD * 2);
       f16v s = {}, dp = {};
 #pragma unroll
       for (int i = 0; i < L::kSteps; i++) {
-        s = T::mfma(L::rows(qt, c * 32, i, lane), kf[i], s);
-        dp = T::mfma(L::rows(gt, c * 32, i, lane), vf[i], dp);
+        s = T::mfma(rd.template rows<0>(i), kf[i], s);
+        dp = T::mfma(rd.template rows<1>(i), vf[i], dp);
       }
+      feed<2 * L::kSteps, 1, 4>();
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int q = 0; q < 4; q++) {
-        const f4v lse = *(const f4v*)&stats[t & 1][0][c * 32 + q * 8 + half * 4];
-        const f4v delta = *(const f4v*)&stats[t & 1][1][c * 32 + q * 8 + half * 4];
+        const f4v lse = *(const f4v*)&stats[(t & 1) * 2 * kTile + c * 32 + q * 8 + half * 4];
+        const f4v delta = *(const f4v*)&stats[((t & 1) * 2 + 1) * kTile + c * 32 + q * 8 + half * 4];
 #pragma unroll
         for (int e = 0; e < 4; e++) {
           const int r = q * 4 + e;
@@ -574,25 +663,36 @@ __global__ DSX_ATTENTION_KERNEL(HD) void k_key_grads(Args a, Backward b) {
           dp[r] = s[r] * (dp[r] - delta[e]) * (ds_scale * (T::kScaled ? 0x1p-14f : 1.0f));
         }
       }
+      __builtin_amdgcn_sched_barrier(0);
       if (edge) {
+        // rows [lo, hi) see the key; dS is zero for rows with one key, as in k_query_grads
+        const int i0 = now + c * 32 + 4 * half;
+        const int lo = only_here(a.causal ? key : p.start) - i0, hi = p.end - i0;
+        const int more = (a.causal ? max(key, p.start + 1) : p.end - p.start == 1 ? p.end : p.start) - i0;
 #pragma unroll
         for (int r = 0; r < 16; r++) {
-          const int i = now + c * 32 + row_of(r, half);
-          const bool seen = i < p.end && (!a.causal || key <= i);
-          const bool one = a.causal ? i == p.start : p.end - p.start == 1;  // as in k_query_grads
-          s[r] = seen ? s[r] : 0.0f;
-          dp[r] = seen && !one ? dp[r] : 0.0f;
+          const int i = row_of(r, 0);
+          s[r] = i >= lo && i < hi ? s[r] : 0.0f;
+          dp[r] = i >= more && i < hi ? dp[r] : 0.0f;
         }
       }
+      s8v pf[2], sf[2];
 #pragma unroll
       for (int g = 0; g < 2; g++) {
-        const s8v pf = pack<T>(s, g), sf = pack<T>(dp, g);
+        pf[g] = pack<T>(s, g);
+        sf[g] = pack<T>(dp, g);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int g = 0; g < 2; g++) {
 #pragma unroll
         for (int i = 0; i < L::kBlocks; i++) {
-          dv[i] = T::mfma(L::columns(gt, c * 32 + g * 16, i * 32, lane), pf, dv[i]);
-          dk[i] = T::mfma(L::columns(qt, c * 32 + g * 16, i * 32, lane), sf, dk[i]);
+          dv[i] = T::mfma(rd.template columns<1>(g * 16, i), pf[g], dv[i]);
+          dk[i] = T::mfma(rd.template columns<0>(g * 16, i), sf[g], dk[i]);
         }
       }
+      feed<4 * L::kBlocks, 2, 3>();
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
   const int rows = min(32, p.end - w0);
@@ -600,11 +700,11 @@ __global__ DSX_ATTENTION_KERNEL(HD) void k_key_grads(Args a, Backward b) {
   if (rows <= 0) return;
   const float fk = a.scale / ds_scale, fv = T::kScaled ? 0x1p-14f : 1.0f;
   const int64_t ld = (int64_t)a.kv_heads * a.d, at = w0 * ld + (int64_t)p.kv * a.d;
-  if (b.splits > 1) {
+  if (b.parts > 1) {
     const int64_t plane = (int64_t)a.tokens * ld;
-    float* out = b.part + split * plane + at + (lane & 31) * ld;
+    float* out = b.part + part * plane + at + (lane & 31) * ld;
     store_part<HD>(out, dk, fk, key < p.end, a.d, half);
-    store_part<HD>(out + b.splits * plane, dv, fv, key < p.end, a.d, half);
+    store_part<HD>(out + b.parts * plane, dv, fv, key < p.end, a.d, half);
     return;
   }
   char* strip = (char*)lds + w * 32 * HD * 2;
@@ -612,15 +712,15 @@ __global__ DSX_ATTENTION_KERNEL(HD) void k_key_grads(Args a, Backward b) {
   store_rows<T, HD>(strip, dv, fv, false, b.dv + at, ld, rows, a.d, lane);
 }
 
-// The splits' sums, added in order: eight values a thread.
+// The parts' sums, added in order: eight values a thread.
 template <class T>
 __global__ __launch_bounds__(256) void k_join(const float* __restrict__ part, short* __restrict__ dk,
-                                              short* __restrict__ dv, int64_t n, int splits) {
+                                              short* __restrict__ dv, int64_t n, int parts) {
   const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
   if (at >= n) return;
-  const float* p = part + (blockIdx.y ? splits * n : 0) + at;
+  const float* p = part + (blockIdx.y ? parts * n : 0) + at;
   f4v x = {}, y = {};
-  for (int s = 0; s < splits; s++) {
+  for (int s = 0; s < parts; s++) {
     x += *(const f4v*)(p + s * n);
     y += *(const f4v*)(p + s * n + 4);
   }
@@ -636,13 +736,24 @@ __global__ __launch_bounds__(256) void k_join(const float* __restrict__ part, sh
 // ---- host ------------------------------------------------------------------
 
 
-// Parts of a group's heads in k_key_grads: enough blocks for four rounds of two
+// Parts of k_key_grads' work on a tile: enough blocks for four rounds of two
 // blocks a CU, since a causal mask makes the blocks of a sequence as unequal as
-// can be.
-int splits_of(const DsxAttention& q) {
-  const int64_t blocks = q.tile_count * q.kv_heads, group = q.heads / q.kv_heads;
-  const int64_t want = ceil_div(4 * 2 * kCus, blocks > 0 ? blocks : 1);
-  return (int)(want < group ? want : group);
+// can be, but a part walks kLeastSteps tiles at least where the sequence is long
+// enough, since its sums go through memory, of which they take at most
+// kPartBytes. Up to a group's heads a part is whole heads, which one XCD's L2
+// then serves.
+constexpr int64_t kPartBytes = (int64_t)512 << 20;
+constexpr int kLeastSteps = 8;
+int parts_of(const DsxAttention& q) {
+  const int64_t group = q.heads / q.kv_heads, blocks = q.tile_count * q.kv_heads;
+  if (!blocks) return 1;
+  int64_t parts = ceil_div((q.head_dim <= 64 ? 8 : 4) * kCus, blocks);
+  const int64_t most = ceil_div(q.longest, kTile) * group / kLeastSteps;
+  if (parts > most) parts = most;
+  if (parts > group) parts = parts / group * group;
+  const int64_t fit = kPartBytes / (2 * q.tokens * q.kv_heads * q.head_dim * 4);
+  if (parts > fit) parts = fit;
+  return parts < 1 ? 1 : (int)parts;
 }
 
 struct Layout {
@@ -652,8 +763,8 @@ Layout layout_of(const DsxAttention& q) {
   Layout l{};
   l.most = round_up(q.tokens * q.heads * 4, 256);
   l.part = l.most + kMost * 2 * 4;
-  const int splits = splits_of(q);
-  l.total = l.part + (splits > 1 ? round_up(2 * splits * q.tokens * q.kv_heads * q.head_dim * 4, 256) : 0);
+  const int parts = parts_of(q);
+  l.total = l.part + (parts > 1 ? round_up(2 * parts * q.tokens * q.kv_heads * q.head_dim * 4, 256) : 0);
   return l;
 }
 
@@ -685,9 +796,9 @@ void backward(Args a, const Backward& b, int64_t tiles, hipStream_t s) {
   if (b.dq) k_query_grads<T, HD><<<dim3((unsigned)(tiles * a.heads)), kThreads, 0, s>>>(a, b);
   if (b.dk) {
     a.tiles += tiles;  // by keys
-    k_key_grads<T, HD><<<dim3((unsigned)(tiles * a.kv_heads * b.splits)), kThreads, 0, s>>>(a, b);
+    k_key_grads<T, HD><<<dim3((unsigned)(tiles * a.kv_heads * b.parts)), kThreads, 0, s>>>(a, b);
     const int64_t n = (int64_t)a.tokens * a.kv_heads * a.d;
-    if (b.splits > 1) k_join<T><<<dim3((unsigned)ceil_div(n, 2048), 2), 256, 0, s>>>(b.part, b.dk, b.dv, n, b.splits);
+    if (b.parts > 1) k_join<T><<<dim3((unsigned)ceil_div(n, 2048), 2), 256, 0, s>>>(b.part, b.dk, b.dv, n, b.parts);
   }
 }
 
@@ -704,7 +815,8 @@ int check(const char* what, const DsxAttention* q) {
     return fail(DSX_EINVAL, "%s: head_dim must be a multiple of 8 up to %d", what, DSX_ATTENTION_MAX_HEAD_DIM);
   if (q->tile_count < 0 || q->tile_count > q->tokens || (q->tokens && !q->tile_count))
     return fail(DSX_EINVAL, "%s: tile_count must lie in [1, tokens]", what);
-  if (q->tile_count * q->heads > INT32_MAX) return fail(DSX_EINVAL, "%s: more than 2^31 - 1 tiles and heads", what);
+  if (q->tile_count * q->heads > INT32_MAX / 64) return fail(DSX_EINVAL, "%s: more than 2^25 tiles and heads", what);
+  if (q->longest < 0 || q->longest > q->tokens) return fail(DSX_EINVAL, "%s: longest must lie in [0, tokens]", what);
   if (!(q->scale > 0.0f) || !(q->scale < INFINITY)) return fail(DSX_EINVAL, "%s: scale must be positive and finite", what);
   return DSX_OK;
 }
@@ -826,7 +938,7 @@ int dsx_attention_backward(const DsxAttention* args, const void* out, const void
   b.dq = (short*)dq;
   b.dk = (short*)dk;
   b.dv = (short*)dv;
-  b.splits = splits_of(*args);
+  b.parts = parts_of(*args);
   const Args a = args_of(*args);
   hipStream_t s = as_stream(stream);
   if (args->dtype == DSX_F16) DSX_BY_HEAD(backward, F16, a, b, args->tile_count, s);

@@ -17,8 +17,8 @@
 // of the largest size and blocks without rows end at once). The copy also
 // gives the product's direct loads the aligned rows that they need.
 //
-// In fp16, dz is held times a power of two that takes the largest w_t to about
-// 2^14, so that probabilities down to 2^-28 keep their digits.
+// In fp16, dz is held times a power of two that takes the largest factor to
+// about 2^14, so that probabilities down to 2^-28 keep their digits.
 
 #include <hip/hip_runtime.h>
 #include <math.h>
@@ -42,7 +42,7 @@ constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f
 // What the forward keeps, for the rows that count: row i of them is the
 // caller's row index[i].
 struct Saved {
-  int* count;     // [0] rows that count, [1] one of them has a bad target
+  int* count;     // of them
   int* index;     // [tokens]
   int* target;    // [tokens], -1: outside the vocabulary
   float2* stat;   // [tokens]: the largest logit and log2 of the sum of exp2((z - it) log2 e)
@@ -252,36 +252,37 @@ __global__ __launch_bounds__(256) void k_fill(float* __restrict__ p, int n) {
 
 // ---- backward -----------------------------------------------------------------
 
-// A row's weight in the total; in fp16 times the power of two in scale[0],
-// whose reciprocal is scale[1].
-__global__ __launch_bounds__(1024) void k_weights(const float* __restrict__ d_loss, int reduction, int scaled, Saved s,
+// The factor of a row in dz, and in scale[0] what takes the products with dz to
+// the gradients. Where all rows weigh alike, as in a mean, that weight stays out
+// of dz: near a target dz is then close to -1, which 16 bits hold, where w times
+// it would be off by the same 2^-9 of bf16 in every row. fp16's power of two
+// goes by the largest factor.
+__global__ __launch_bounds__(1024) void k_weights(const float* __restrict__ d_loss, int reduction, int half, Saved s,
                                                   float* __restrict__ weight, float* __restrict__ scale) {
   __shared__ float tops[16];
   const int rows = *s.count;
-  auto of = [&](int r) {
-    const float w = reduction == DSX_REDUCE_NONE ? d_loss[s.index[r]]
-                    : reduction == DSX_REDUCE_MEAN ? *d_loss / (float)rows : *d_loss;
-    return s.target[r] < 0 ? NAN : w;
-  };
-  float f = 1.0f, top = 0;
-  if (scaled) {
-    for (int r = threadIdx.x; r < rows; r += 1024) top = fmaxf(top, fabsf(of(r)));
+  const bool none = reduction == DSX_REDUCE_NONE;
+  float f = 1.0f;
+  if (half) {
+    float top = none ? 0.0f : 1.0f;
+    if (none) {
+      for (int r = threadIdx.x; r < rows; r += 1024) top = fmaxf(top, fabsf(d_loss[s.index[r]]));
 #pragma unroll
-    for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
-    if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
-    __syncthreads();
-    for (int i = 0; i < 16; i++) top = fmaxf(top, tops[i]);
+      for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+      if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
+      __syncthreads();
+      for (int i = 0; i < 16; i++) top = fmaxf(top, tops[i]);
+    }
     if (top > 0.0f && top < INFINITY) {
       int e;
       frexpf(top, &e);  // top < 2^e
-      f = ldexpf(1.0f, max(-100, min(100, 14 - e)));
+      f = ldexpf(1.0f, max(-100, min(100, 15 - e)));
     }
   }
-  for (int r = threadIdx.x; r < rows; r += 1024) weight[r] = of(r) * f;
-  if (threadIdx.x == 0) {
-    scale[0] = f;
-    scale[1] = 1.0f / f;
-  }
+  for (int r = threadIdx.x; r < rows; r += 1024)
+    weight[r] = s.target[r] < 0 ? NAN : none ? d_loss[s.index[r]] * f : f;
+  if (threadIdx.x == 0)
+    scale[0] = (none ? 1.0f : reduction == DSX_REDUCE_MEAN ? *d_loss / (float)rows : *d_loss) / f;
 }
 
 // dz of a piece, [rows][ld] with zeros from the piece's end to ld.
@@ -380,7 +381,7 @@ __global__ __launch_bounds__(256) void k_input_join(const float* __restrict__ pl
                                                     int n, Saved s, const float* __restrict__ scale,
                                                     short* __restrict__ dx) {
   const int rows = min(*s.count, m);
-  const float f = scale[1];
+  const float f = scale[0];
   for (int r = blockIdx.y; r < rows; r += gridDim.y) {
     const int c = (blockIdx.x * 256 + threadIdx.x) * 8;
     if (c >= n) continue;
@@ -429,7 +430,7 @@ __global__ DSX_TILE_KERNEL(G) void k_weight_grad(WeightGrad p) {
   G g;
   g.init();
   g.run(lds, p.dz, p.x, p.x, ti * G::TM, tj * G::TN, *p.count);
-  const float f = p.scale[1];
+  const float f = p.scale[0];
   g.template emit<false>(
       lds, [](int, int) { return Nothing{}; },
       [&](int r, int c, float* v, float*, const Nothing&) {
@@ -510,7 +511,7 @@ Saved saved_of(const DsxLoss& q, int64_t* bytes) {
     return r;
   };
   s.ld = round_up(q.width, 8);
-  s.count = (int*)take(8);
+  s.count = (int*)take(4);
   s.index = (int*)take(q.tokens * 4);
   s.target = (int*)take(q.tokens * 4);
   s.stat = (float2*)take(q.tokens * 8);
@@ -546,7 +547,7 @@ Work work_of(const DsxLoss& q, const Sizes& z, bool backward) {
     w.each = (float*)take(z.t * 4);
   } else {
     w.row_weight = (float*)take(z.t * 4);
-    w.scale = (float*)take(8);
+    w.scale = (float*)take(4);
     w.dz = (short*)take(z.t * z.ld_piece * 2);
     w.planes = (float*)take(z.splits * z.t * z.ld * 4);
   }

@@ -796,7 +796,8 @@ int dsx_norm_backward(const DsxNorm* args /* host */, const void* d_hidden,
  * strides ld_* and head strides head_* in elements. Bases are 16-byte aligned,
  * strides and head_dim multiples of 8. heads is a multiple of kv_heads; query
  * head h reads key head h / (heads / kv_heads). `tiles` is a device copy of
- * what dsx_attention_tiles made, whose sequences cover rows [0, tokens). */
+ * what dsx_attention_tiles made, whose sequences cover rows [0, tokens); longest
+ * is the longest sequence's length, by which the work is shared out. */
 typedef struct DsxAttention {
   const void*    q;
   const void*    k;
@@ -816,6 +817,7 @@ typedef struct DsxAttention {
   int32_t        dtype;
   int32_t        causal;
   float          scale;
+  int64_t        longest;
 } DsxAttention;
 
 /* The tile table of sequences of the given lengths (zero allowed), one behind
