@@ -45,6 +45,7 @@ struct Saved {
   int* count;     // of them
   int* index;     // [tokens]
   int* target;    // [tokens], -1: outside the vocabulary
+  int* place;     // [tokens]: the caller's row among those that count, -1: it does not
   float2* stat;   // [tokens]: the largest logit and log2 of the sum of exp2((z - it) log2 e)
   short* x;       // [tokens][ld]
   int64_t ld;
@@ -52,10 +53,11 @@ struct Saved {
 
 // ---- the rows that count ------------------------------------------------------
 
-// One block: runs of 4096 targets, four a thread, numbered by a scan.
+// One block: runs of 4096 targets, four a thread, numbered by a scan. `each`
+// (may be NULL) gets the loss of the rows that do not count.
 template <class I>
 __global__ __launch_bounds__(1024) void k_select(const I* __restrict__ targets, int tokens, int64_t ignore, int vocab,
-                                                 Saved s) {
+                                                 Saved s, float* __restrict__ each) {
   __shared__ int sums[16];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   int base = 0;
@@ -86,9 +88,13 @@ __global__ __launch_bounds__(1024) void k_select(const I* __restrict__ targets, 
 #pragma unroll
     for (int e = 0; e < 4; e++)
       if (v[e] != ignore) {
+        s.place[at + e] = to;
         s.index[to] = at + e;
         s.target[to] = v[e] >= 0 && v[e] < vocab ? (int)v[e] : -1;
         to++;
+      } else if (at + e < tokens) {
+        s.place[at + e] = -1;
+        if (each) each[at + e] = 0.0f;
       }
     base += all;
     __syncthreads();
@@ -245,11 +251,6 @@ __global__ __launch_bounds__(1024) void k_total(const float* __restrict__ each, 
   *out = mean ? (float)(v / rows) : (float)v;
 }
 
-__global__ __launch_bounds__(256) void k_fill(float* __restrict__ p, int n) {
-  const int i = blockIdx.x * 256 + threadIdx.x;
-  if (i < n) p[i] = 0.0f;
-}
-
 // ---- backward -----------------------------------------------------------------
 
 // The factor of a row in dz, and in scale[0] what takes the products with dz to
@@ -375,18 +376,18 @@ __global__ DSX_TILE_KERNEL(G) void k_input_grad(InputGrad p) {
       [](int, int, const float*) {});
 }
 
-// The planes added in order, rounded and put in the caller's rows.
+// The planes added in order and rounded; zeros in rows that do not count.
 template <class T>
 __global__ __launch_bounds__(256) void k_input_join(const float* __restrict__ planes, int splits, int m, int64_t ld,
                                                     int n, Saved s, const float* __restrict__ scale,
                                                     short* __restrict__ dx) {
-  const int rows = min(*s.count, m);
   const float f = scale[0];
-  for (int r = blockIdx.y; r < rows; r += gridDim.y) {
-    const int c = (blockIdx.x * 256 + threadIdx.x) * 8;
-    if (c >= n) continue;
+  const int c = (blockIdx.x * 256 + threadIdx.x) * 8;
+  if (c >= n) return;
+  for (int t = blockIdx.y; t < m; t += gridDim.y) {
+    const int r = s.place[t];
     f4v a = {}, b = {};
-    for (int k = 0; k < splits; k++) {
+    for (int k = 0; k < (r < 0 ? 0 : splits); k++) {
       const float* q = planes + ((int64_t)k * m + r) * ld + c;
       a += *(const f4v*)q;
       b += *(const f4v*)(q + 4);
@@ -394,24 +395,15 @@ __global__ __launch_bounds__(256) void k_input_join(const float* __restrict__ pl
     s8v o;
 #pragma unroll
     for (int e = 0; e < 4; e++) {
-      o[e] = T::round(a[e] * f);
-      o[e + 4] = T::round(b[e] * f);
+      o[e] = r < 0 ? (short)0 : T::round(a[e] * f);
+      o[e + 4] = r < 0 ? (short)0 : T::round(b[e] * f);
     }
-    short* to = dx + (int64_t)s.index[r] * n + c;
+    short* to = dx + (int64_t)t * n + c;
     if (c + 8 <= n)
       *(s8u*)to = o;
     else
       for (int e = 0; e < 8; e++)
         if (c + e < n) to[e] = o[e];
-  }
-}
-
-// Zeros in dx's rows that do not count: those between the ones that do.
-__global__ __launch_bounds__(256) void k_zero_rows(Saved s, int tokens, int64_t n, short* __restrict__ dx) {
-  const int rows = *s.count;
-  for (int r = blockIdx.x; r <= rows; r += gridDim.x) {
-    const int64_t lo = r ? (s.index[r - 1] + 1) * n : 0, hi = (r < rows ? s.index[r] : tokens) * n;
-    for (int64_t i = lo + threadIdx.x; i < hi; i += 256) dx[i] = 0;
   }
 }
 
@@ -475,8 +467,38 @@ struct Sizes {
   int dx_tile, splits;
 };
 
-// dz of a piece: at most this many bytes.
+// dz of a piece: at most this many bytes. (8192 x 4096 against 128256 rows, bf16,
+// dz and both products: 19.0 ms with 128 MiB, 18.8 with 256, 19.4 with 512, 19.3
+// with 1 GiB; 4096 x 768 against 50257: 1.17 ms with 256, 1.06 in one piece.)
 constexpr int64_t kPieceBytes = (int64_t)512 << 20;
+
+// Tile and splits of dx's sum over k vocabulary rows, which is long where its
+// tiles are few. In us: a K tile of 64 takes a block of 256 1.6 us and two of 128
+// on a CU 1.2 times as long for the same area (square_tile); a round of small
+// tiles that fills half the CUs' places takes 0.58 of one; a split's sums are
+// written and read at 4 TB/s.
+void share_out(int64_t m, int64_t n, int64_t k, int* tile, int* splits) {
+  const int64_t kt = ceil_div(k, kBK);
+  *tile = tile_of(m, n);
+  *splits = 1;
+  double least = INFINITY;
+  for (int t = *tile < 128 ? *tile : 128; t <= (*tile < 128 ? *tile : 256); t *= 2) {
+    const int64_t tiles = ceil_div(m, rows_of_tile(t)) * ceil_div(n, cols_of_tile(t));
+    for (int64_t s = 1; s <= 64 && (s == 1 || kt / s >= 4); s++) {
+      const int64_t blocks = tiles * s, slots = t == 256 ? kCus : t == 128 ? 2 * kCus : 4 * kCus;
+      const int64_t rest = blocks % slots;
+      double rounds = (double)(blocks / slots) + (rest == 0 ? 0.0 : t == 256 || rest > slots / 2 ? 1.0 : 0.58);
+      const double area = (double)rows_of_tile(t) * cols_of_tile(t) * (double)(slots / kCus) / 65536.0;
+      const double us = rounds * (double)ceil_div(kt, s) * 1.6 * (t == 256 ? 1.0 : area < 0.3 ? 0.36 : 1.2 * area) +
+                        (double)s * (double)(m * n) * 8.0 / 4e6;
+      if (us < least) {
+        least = us;
+        *tile = t;
+        *splits = (int)s;
+      }
+    }
+  }
+}
 
 Sizes sizes_of(const DsxLoss& q) {
   Sizes z{};
@@ -492,12 +514,7 @@ Sizes sizes_of(const DsxLoss& q) {
   const int64_t pieces = ceil_div(z.v, most);
   z.piece = pieces > 1 ? round_up(ceil_div(z.v, pieces), 256) : z.v;
   z.ld_piece = round_up(z.piece, 8);
-  z.dx_tile = tile_of(z.t, z.d);
-  const int64_t tiles = ceil_div(z.t, rows_of_tile(z.dx_tile)) * ceil_div(z.d, cols_of_tile(z.dx_tile));
-  const int64_t kt = ceil_div(z.piece, kBK);
-  int64_t splits = tiles >= kCus ? 1 : ceil_div(2 * kCus, tiles > 0 ? tiles : 1);
-  if (splits > kt / 4) splits = kt / 4;
-  z.splits = (int)(splits < 1 ? 1 : splits);
+  share_out(z.t, z.d, z.piece, &z.dx_tile, &z.splits);
   return z;
 }
 
@@ -514,6 +531,7 @@ Saved saved_of(const DsxLoss& q, int64_t* bytes) {
   s.count = (int*)take(4);
   s.index = (int*)take(q.tokens * 4);
   s.target = (int*)take(q.tokens * 4);
+  s.place = (int*)take(q.tokens * 4);
   s.stat = (float2*)take(q.tokens * 8);
   s.x = (short*)take(q.tokens * s.ld * 2);
   if (bytes) *bytes = at;
@@ -596,11 +614,12 @@ int forward(const DsxLoss& q, float* loss, hipStream_t st) {
   const Sizes z = sizes_of(q);
   const Saved s = saved_of(q, nullptr);
   const Work w = work_of(q, z, false);
-  if (q.target_bytes == 8)
-    k_select<int64_t><<<1, 1024, 0, st>>>((const int64_t*)q.targets, (int)z.t, q.ignore_index, (int)z.v, s);
-  else
-    k_select<int32_t><<<1, 1024, 0, st>>>((const int32_t*)q.targets, (int)z.t, q.ignore_index, (int)z.v, s);
   const bool none = q.reduction == DSX_REDUCE_NONE;
+  float* each = none ? loss : w.each;
+  if (q.target_bytes == 8)
+    k_select<<<1, 1024, 0, st>>>((const int64_t*)q.targets, (int)z.t, q.ignore_index, (int)z.v, s, none ? loss : nullptr);
+  else
+    k_select<<<1, 1024, 0, st>>>((const int32_t*)q.targets, (int)z.t, q.ignore_index, (int)z.v, s, none ? loss : nullptr);
   if (!z.t) {
     if (!none) k_total<<<1, 1024, 0, st>>>(nullptr, s, q.reduction == DSX_REDUCE_MEAN, loss);
     return launch_status("dsx_loss_forward");
@@ -617,8 +636,6 @@ int forward(const DsxLoss& q, float* loss, hipStream_t st) {
   } while (0)
   DSX_BY_TILE(z.tile, (int64_t)p.mt * p.nt, RUN);
 #undef RUN
-  float* each = none ? loss : w.each;
-  if (none) k_fill<<<dim3((unsigned)ceil_div(z.t, 256)), 256, 0, st>>>(loss, (int)z.t);
   k_rows<<<dim3((unsigned)ceil_div(z.t, 32)), 1024, 0, st>>>(w.part, w.hit, (int)z.t, (int)z.nt, s, each);
   if (!none) k_total<<<1, 1024, 0, st>>>(each, s, q.reduction == DSX_REDUCE_MEAN, loss);
   return launch_status("dsx_loss_forward");
@@ -690,11 +707,9 @@ int backward(const DsxLoss& q, const float* d_loss, short* dx, short* dw, hipStr
       }
     }
   }
-  if (dx && z.t) {
+  if (dx && z.t)
     k_input_join<T><<<dim3((unsigned)ceil_div(z.d, 2048), (unsigned)(z.t < 65535 ? z.t : 65535)), 256, 0, st>>>(
         w.planes, z.splits, (int)z.t, z.ld, (int)z.d, s, w.scale, dx);
-    k_zero_rows<<<dim3((unsigned)(z.t + 1 < 4096 ? z.t + 1 : 4096)), 256, 0, st>>>(s, (int)z.t, z.d, dx);
-  }
   return launch_status("dsx_loss_backward");
 }
 
