@@ -298,7 +298,7 @@ __device__ inline void feed() {
 
 struct Forward {
   short* out;     // [tokens][heads][d]
-  short* out_lo;  // what out lost in rounding; NULL: not kept
+  short* out_lo;  // what out lost in rounding, for delta (k_delta); NULL: not kept
   float* lse;     // [heads][tokens], base 2; NULL: not kept
 };
 
@@ -417,7 +417,11 @@ struct Backward {
 };
 constexpr int kMost = 512;
 
-// delta, and for fp16 the largest rows: a wave a row at a time.
+// delta, and for fp16 the largest rows: 16 lanes a row. Where few keys matter dP
+// and delta nearly cancel, so that delta is taken from the output before its
+// rounding: without what that lost, dq's and dk's errors over those of one rounding
+// (64 features, bf16, rows of 2 to 12 keys) are 1.8 instead of 1.1, of 1000 keys
+// 1.49 and 1.58 instead of 1.29 and 1.44.
 template <class T>
 __global__ __launch_bounds__(256) void k_delta(Args a, Backward b) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
@@ -455,6 +459,7 @@ __global__ __launch_bounds__(256) void k_delta(Args a, Backward b) {
       s += __shfl_xor(s, k);
       n += __shfl_xor(n, k);
     }
+    n = n < INFINITY ? n : 0.0f;  // a row that is not finite has no part in the others' scale
     if (i < rows) {
       if (sub == 0) {
         const int64_t t = i / a.heads;

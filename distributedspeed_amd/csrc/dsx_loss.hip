@@ -282,8 +282,8 @@ __global__ __launch_bounds__(1024) void k_weights(const float* __restrict__ d_lo
   }
   for (int r = threadIdx.x; r < rows; r += 1024)
     weight[r] = s.target[r] < 0 ? NAN : none ? d_loss[s.index[r]] * f : f;
-  if (threadIdx.x == 0)
-    scale[0] = (none ? 1.0f : reduction == DSX_REDUCE_MEAN ? *d_loss / (float)rows : *d_loss) / f;
+  if (threadIdx.x == 0)  // (the mean of no row is NaN, but there is nothing it could reach)
+    scale[0] = !rows ? 0.0f : (none ? 1.0f : reduction == DSX_REDUCE_MEAN ? *d_loss / (float)rows : *d_loss) / f;
 }
 
 // dz of a piece, [rows][ld] with zeros from the piece's end to ld.
