@@ -520,10 +520,10 @@ Sizes sizes_of(const DsxLoss& q) {
 
 Saved saved_of(const DsxLoss& q, int64_t* bytes) {
   Saved s{};
-  char* p = (char*)q.saved;
+  const uintptr_t p = (uintptr_t)q.saved;
   int64_t at = 0;
   auto take = [&](int64_t n) {
-    char* r = p + at;
+    char* r = (char*)(p + at);
     at += round_up(n, 256);
     return r;
   };
@@ -551,10 +551,10 @@ struct Work {
 };
 Work work_of(const DsxLoss& q, const Sizes& z, bool backward) {
   Work w{};
-  char* p = (char*)q.workspace;
+  const uintptr_t p = (uintptr_t)q.workspace;  // sizes are asked for with none
   int64_t at = 0;
   auto take = [&](int64_t n) {
-    char* r = p + at;
+    char* r = (char*)(p + at);
     at += round_up(n, 256);
     return r;
   };

@@ -2533,6 +2533,15 @@ int dsx_abi_version(void) { return DSX_ABI_VERSION; }
 
 const char* dsx_last_error(void) { return g_err; }
 
+int dsx_stream_capturing(void* stream) {
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(reinterpret_cast<hipStream_t>(stream), &status) != hipSuccess) {
+    (void)hipGetLastError();
+    return 0;
+  }
+  return status != hipStreamCaptureStatusNone;
+}
+
 int dsx_set_tuning(int k1_blocks_per_cu, int k2_blocks_per_cu, int k2_unroll, int nontemporal) {
   if (k1_blocks_per_cu < 1 || k1_blocks_per_cu > 32 || k2_blocks_per_cu < 0 || k2_blocks_per_cu > 64)
     return fail(DSX_EINVAL, "blocks per CU out of range");

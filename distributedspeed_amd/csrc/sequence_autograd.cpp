@@ -9,6 +9,7 @@ namespace {
 
 struct Entry {
   decltype(&dsx_last_error) last_error;
+  decltype(&dsx_stream_capturing) stream_capturing;
   decltype(&dsx_attention_forward) attention_forward;
   decltype(&dsx_attention_workspace_bytes) attention_workspace_bytes;
   decltype(&dsx_attention_backward) attention_backward;
@@ -22,6 +23,16 @@ struct Entry {
 void check(const char* name, int rc) { check_status(name, rc, entry.last_error); }
 Tensor scratch(int64_t bytes, const Tensor& like) { return scratch_of(bytes, like, entry.last_error); }
 void* stream_at(int64_t s) { return reinterpret_cast<void*>(s); }
+
+// The stream of a backward pass. One under capture is refused before autograd
+// gets to the leaves: where an eager graph of theirs lives, its accumulation nodes
+// belong to another stream, and the captured pass ends the process.
+void* backward_stream(const char* name, AutogradContext* ctx) {
+  void* s = stream_at(ctx->saved_data["stream"].toInt());
+  if (entry.stream_capturing(s))
+    throw std::runtime_error(std::string(name) + ": a backward pass cannot be captured into a graph (a forward can)");
+  return s;
+}
 
 // ---- attention ----------------------------------------------------------------
 
@@ -120,6 +131,7 @@ struct PackedAttention : torch::autograd::Function<PackedAttention> {
   // On the forward's stream, which autograd makes current here.
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto s = ctx->get_saved_variables();
+    void* stream = backward_stream("packed_attention", ctx);
     Tensor dq, dk, dv;
     if (grads[0].defined()) {
       const c10::DeviceGuard guard(s[0].device());
@@ -139,7 +151,7 @@ struct PackedAttention : torch::autograd::Function<PackedAttention> {
             entry.attention_backward(&a, at_of(s[3]), at_of(s[4]), static_cast<const float*>(at_of(s[5])), at_of(dout),
                                      dout.size(0) > 1 ? dout.stride(0) : dout.size(1) * dout.size(2),
                                      dout.size(1) > 1 ? dout.stride(1) : dout.size(2), at_of(dq), at_of(dk), at_of(dv),
-                                     at_of(work), work.numel(), stream_at(ctx->saved_data["stream"].toInt())));
+                                     at_of(work), work.numel(), stream));
       dq = first_features(dq, d);
       dk = ctx->needs_input_grad(1) ? first_features(dk, d) : Tensor();
       dv = ctx->needs_input_grad(2) ? first_features(dv, d) : Tensor();
@@ -212,6 +224,7 @@ struct Rotary : torch::autograd::Function<Rotary> {
     return rotary_run(q, k, {positions, base, dims, interleaved}, false, stream);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    (void)backward_stream("rotary", ctx);
     const Turn r{ctx->get_saved_variables()[0], ctx->saved_data["base"].toDouble(), ctx->saved_data["dims"].toInt(),
                  ctx->saved_data["interleaved"].toBool()};
     Tensor dq = ctx->needs_input_grad(0) ? grads[0] : Tensor(), dk = ctx->needs_input_grad(1) ? grads[1] : Tensor();
@@ -286,6 +299,7 @@ struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto s = ctx->get_saved_variables();
+    void* stream = backward_stream("linear_cross_entropy", ctx);
     Tensor dx, dw;
     if (grads[0].defined()) {
       const c10::DeviceGuard guard(s[0].device());
@@ -301,7 +315,7 @@ struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
         q.workspace = at_of(work);
         q.workspace_bytes = work.numel();
         check("dsx_loss_backward", entry.loss_backward(&q, static_cast<const float*>(at_of(d_loss)), at_of(dx), at_of(dw),
-                                                       stream_at(ctx->saved_data["stream"].toInt())));
+                                                       stream));
       }
     }
     return once({dx, dw, Tensor(), Tensor(), Tensor(), Tensor()});
@@ -322,6 +336,7 @@ Tensor linear_cross_entropy(const Tensor& x, const Tensor& w, const Tensor& targ
 PYBIND11_MODULE(_sequence_autograd, m) {
   m.def("bind", [](const pybind11::dict& d) {
     bind_one(entry.last_error, d, "dsx_last_error");
+    bind_one(entry.stream_capturing, d, "dsx_stream_capturing");
     bind_one(entry.attention_forward, d, "dsx_attention_forward");
     bind_one(entry.attention_workspace_bytes, d, "dsx_attention_workspace_bytes");
     bind_one(entry.attention_backward, d, "dsx_attention_backward");

@@ -3,7 +3,8 @@
     linear_cross_entropy(x, weight, targets)   cross entropy of x weight^T
 
 Both directions run the library's own kernels on the current stream, without a
-host synchronisation, and never hold the logits.
+host synchronisation, and never hold the logits. The forward can be captured into
+a graph; a backward under capture is refused.
 """
 from __future__ import annotations
 

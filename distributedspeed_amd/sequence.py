@@ -7,7 +7,8 @@
 
 Both directions run the library's own kernels on the current stream, without a
 host synchronisation; the gradients work with torch.autograd and so with the
-optimizers of this package.
+optimizers of this package. Forwards can be captured into a graph; a backward
+under capture is refused.
 """
 from __future__ import annotations
 
@@ -37,8 +38,8 @@ def _native():
         except ImportError as e:
             raise RuntimeError("the sequence operators' autograd nodes are not built or do not load: run `python -c "
                                "'import __graft_entry__ as g; g.build()'` at the repository root") from e
-        names = ("dsx_last_error", "dsx_attention_forward", "dsx_attention_workspace_bytes", "dsx_attention_backward",
-                 "dsx_rotary", "dsx_loss_saved_bytes", "dsx_loss_workspace_bytes", "dsx_loss_forward",
+        names = ("dsx_last_error", "dsx_stream_capturing", "dsx_attention_forward", "dsx_attention_workspace_bytes",
+                 "dsx_attention_backward", "dsx_rotary", "dsx_loss_saved_bytes", "dsx_loss_workspace_bytes", "dsx_loss_forward",
                  "dsx_loss_backward")
         nodes.bind({n: ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in names})
         _nodes = nodes

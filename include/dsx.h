@@ -189,6 +189,9 @@ typedef struct DsxChunk {
 int         dsx_abi_version(void);
 const char* dsx_last_error(void);
 
+/* 1 while `stream` records a graph, else 0. */
+int dsx_stream_capturing(void* stream);
+
 /* Launch-shape override for the current process (library tuning; no
  * counterpart in the reference): K1 blocks per CU (default 2), K2 blocks per
  * CU (0, the default, picks by n: below 3 * 2^27 elements one trip per block
