@@ -21,7 +21,7 @@ def main() -> int:
         from distributedspeed_amd import _lib
         _lib.load(path)  # cached: every test's _lib.load() returns this build
         files = ["test_abi_cpu.py", "test_host_logic.py", "test_block_refusals_cpu.py",
-                 "test_orthogonalize_cpu.py"]
+                 "test_orthogonalize_cpu.py", "test_sequence_refusals_cpu.py"]
     elif which == "oracle":
         from oracle import oracle as O
         O._LIB_PATH = path
