@@ -89,13 +89,15 @@ struct Args {
 
 // ---- tiles in shared memory --------------------------------------------------
 
-template <int HD>
+// Of D features, a multiple of 32, in rows of HD, a power of two.
+template <int D>
 struct Tile {
+  static constexpr int HD = D <= 64 ? 64 : D <= 128 ? 128 : 256;
   static constexpr int kChunks = HD / 8;               // of 16 bytes, in a row
   static constexpr int kBytes = kTile * HD * 2;
   static constexpr int kLoads = kTile * kChunks / kThreads;
-  static constexpr int kSteps = HD / 16;               // matrix instructions along a row
-  static constexpr int kBlocks = HD / 32;              // of 32 features
+  static constexpr int kSteps = D / 16;                // matrix instructions along a row
+  static constexpr int kBlocks = D / 32;               // of 32 features
 
   // Chunk c of row r lies at c ^ swizzle(r): the 16 rows of a fragment read, and
   // the 4 x 32 bytes that 16 lanes of a transposing read touch, then fall on
@@ -157,9 +159,10 @@ struct Tile {
 // kBytes apart.
 typedef __attribute__((address_space(3))) s8v LdsChunk;
 __device__ inline s8v read_chunk(LdsChunk* __restrict__ p) { return *p; }
-template <int HD>
+template <int D>
 struct Reader {
-  using L = Tile<HD>;
+  using L = Tile<D>;
+  static constexpr int HD = L::HD;
   uint32_t row, lo, hi;
   __device__ inline void init(const char* lds, int lane) {
     const uint32_t base = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)lds;
@@ -217,10 +220,11 @@ __device__ constexpr int row_of(int r, int half) { return 8 * (r >> 2) + 4 * hal
 
 // Writes a wave's 32 rows of o (one a lane, features as row_of has them) by way
 // of its part of shared memory. `rest`: what rounding to 16 bits loses instead.
-template <class T, int HD>
+template <class T, int D>
 __device__ inline void store_rows(char* strip, const f16v* o, float factor, bool rest, short* out, int64_t ld,
                                   int rows, int d, int lane) {
-  using L = Tile<HD>;
+  using L = Tile<D>;
+  constexpr int HD = L::HD;
   const int r = lane & 31, half = lane >> 5;
 #pragma unroll
   for (int i = 0; i < L::kBlocks; i++)
@@ -268,11 +272,10 @@ __device__ inline Place place_of(const Args& a, int heads) {
   return p;
 }
 
-// WAVES: a SIMD's, for 64 features; two for 128 and one for 256, which is what
-// their registers allow.
-#define DSX_ATTENTION_KERNEL(HD, WAVES)                                                       \
-  __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(HD == 64 ? WAVES : HD == 128 ? 2 : 1, \
-                                                                 HD == 64 ? WAVES : HD == 128 ? 2 : 1)))
+// A SIMD's waves: as many as the registers of a kernel of D features allow.
+constexpr int dsx_waves(int d, int at_64) { return d <= 32 ? 4 : d <= 64 ? at_64 : d <= 128 ? 2 : 1; }
+#define DSX_ATTENTION_KERNEL(D, WAVES)                                                        \
+  __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(dsx_waves(D, WAVES), dsx_waves(D, WAVES))))
 
 // v, as the compiler may not know it before this place: keeps what the masks of
 // the few tiles at a sequence's edges need out of every tile's way.
@@ -302,9 +305,10 @@ struct Forward {
   float* lse;     // [heads][tokens], base 2; NULL: not kept
 };
 
-template <class T, int HD>
-__global__ DSX_ATTENTION_KERNEL(HD, 4) void k_attend(Args a, Forward f) {
-  using L = Tile<HD>;
+template <class T, int D>
+__global__ DSX_ATTENTION_KERNEL(D, 4) void k_attend(Args a, Forward f) {
+  using L = Tile<D>;
+  constexpr int HD = L::HD;
   __shared__ __attribute__((aligned(1024))) char lds[2][2][L::kBytes];
   const Place p = place_of(a, a.heads);
   if (!p.good) return;
@@ -340,7 +344,7 @@ __global__ DSX_ATTENTION_KERNEL(HD, 4) void k_attend(Args a, Forward f) {
     for (int i = 0; i < L::kSteps; i++)
 #pragma unroll
       for (int b = 0; b < 2; b++) s[b] = T::mfma(L::rows(kt, b * 32, i, lane), qf[i], s[b]);
-    feed<2 * L::kSteps, 1, 6>();
+    feed<2 * L::kSteps, 1, D <= 32 ? 2 : 6>();
     __builtin_amdgcn_sched_barrier(0);
     if (j0 + kTile - 1 > (a.causal ? min(w0, p.end - 1) : p.end - 1)) {
       const int left = only_here(last) - j0 - 4 * half;
@@ -356,7 +360,8 @@ __global__ DSX_ATTENTION_KERNEL(HD, 4) void k_attend(Args a, Forward f) {
     // The maximum that P is taken against may lag behind by kLazy: the sums are
     // the same, and most tiles need no scaling of o.
     if (__any(top > m + kLazy || m == -INFINITY)) {
-      const float next = fmaxf(m, top), alpha = exp2f(m - next);
+      // (finite, so that a row whose scores have all been -inf so far stays at zero)
+      const float next = fmaxf(fmaxf(m, top), -0x1.fffffep127f), alpha = exp2f(m - next);
       l *= alpha;
 #pragma unroll
       for (int i = 0; i < L::kBlocks; i++) o[i] *= alpha;
@@ -378,7 +383,7 @@ __global__ DSX_ATTENTION_KERNEL(HD, 4) void k_attend(Args a, Forward f) {
     }
     // The first fragments are on their way while the vector unit works, and what
     // is left of its work goes between the matrix instructions.
-    constexpr int kAhead = 4, kFrags = 4 * L::kBlocks;
+    constexpr int kFrags = 4 * L::kBlocks, kAhead = kFrags > 4 ? 4 : 2;
     __builtin_amdgcn_sched_group_barrier(0x100, 2 * kAhead, 0);
     __builtin_amdgcn_sched_group_barrier(0x002, 40, 0);
 #pragma unroll
@@ -395,8 +400,8 @@ __global__ DSX_ATTENTION_KERNEL(HD, 4) void k_attend(Args a, Forward f) {
   if (rows <= 0) return;
   char* strip = (char*)lds + w * 32 * HD * 2;
   const int64_t ld = (int64_t)a.heads * a.d, at = w0 * ld + (int64_t)p.head * a.d;
-  store_rows<T, HD>(strip, o, 1.0f / l, false, f.out + at, ld, rows, a.d, lane);
-  if (f.out_lo) store_rows<T, HD>(strip, o, 1.0f / l, true, f.out_lo + at, ld, rows, a.d, lane);
+  store_rows<T, D>(strip, o, 1.0f / l, false, f.out + at, ld, rows, a.d, lane);
+  if (f.out_lo) store_rows<T, D>(strip, o, 1.0f / l, true, f.out_lo + at, ld, rows, a.d, lane);
   if (f.lse && half == 0 && row < p.end) f.lse[(int64_t)p.head * a.tokens + row] = m - T::kBias + log2f(l);
 }
 
@@ -527,9 +532,10 @@ __device__ inline float gradient_scale(const float* most, float* buf) {
 // dk with none 1.44; 60 keys, dq and dk: 1.65 with none, 1.07 with all. Time of dq
 // for 16384 rows, 16 heads of 64: 0.77 ms with none, 0.89 with every other 16, 1.02
 // with all.
-template <class T, int HD, bool FEW>
-__global__ DSX_ATTENTION_KERNEL(HD, 3) void k_query_grads(Args a, Backward b) {
-  using L = Tile<HD>;
+template <class T, int D, bool FEW>
+__global__ DSX_ATTENTION_KERNEL(D, 3) void k_query_grads(Args a, Backward b) {
+  using L = Tile<D>;
+  constexpr int HD = L::HD;
   __shared__ __attribute__((aligned(1024))) char lds[2][2][L::kBytes];
   const Place p = place_of(a, a.heads);
   if (!p.good) return;
@@ -602,16 +608,16 @@ __global__ DSX_ATTENTION_KERNEL(HD, 3) void k_query_grads(Args a, Backward b) {
   __syncthreads();
   if (rows <= 0) return;
   const int64_t ld = (int64_t)a.heads * a.d;
-  store_rows<T, HD>((char*)lds + w * 32 * HD * 2, dq, a.scale / ds_scale, false,
+  store_rows<T, D>((char*)lds + w * 32 * HD * 2, dq, a.scale / ds_scale, false,
                     b.dq + w0 * ld + (int64_t)p.head * a.d, ld, rows, a.d, lane);
 }
 
 // Rows of fp32 partial sums, one a lane.
-template <int HD>
+template <int D>
 __device__ inline void store_part(float* out, const f16v* o, float factor, bool there, int d, int half) {
   if (!there) return;
 #pragma unroll
-  for (int i = 0; i < HD / 32; i++)
+  for (int i = 0; i < D / 32; i++)
 #pragma unroll
     for (int c = 0; c < 4; c++) {
       const int f = i * 32 + c * 8 + half * 4;
@@ -619,9 +625,10 @@ __device__ inline void store_part(float* out, const f16v* o, float factor, bool 
     }
 }
 
-template <class T, int HD, bool FEW>
-__global__ DSX_ATTENTION_KERNEL(HD, 3) void k_key_grads(Args a, Backward b) {
-  using L = Tile<HD>;
+template <class T, int D, bool FEW>
+__global__ DSX_ATTENTION_KERNEL(D, 3) void k_key_grads(Args a, Backward b) {
+  using L = Tile<D>;
+  constexpr int HD = L::HD;
   // One array: with two, the compiler waits for all direct loads in flight before
   // each read. Two pairs of tiles, then lse and delta of their rows.
   __shared__ __attribute__((aligned(1024))) char lds[4 * L::kBytes + 4 * kTile * 4];
@@ -649,7 +656,7 @@ __global__ DSX_ATTENTION_KERNEL(HD, 3) void k_key_grads(Args a, Backward b) {
     L::load(lds + ((t & 1) * 2 + 1) * L::kBytes, b.dout.p + head * b.dout.head + i0 * b.dout.ld, b.dout.ld, left, a.d);
     if (w < 2) stat = (w ? b.delta : b.lse)[(int64_t)head * a.tokens + i0 + min(lane, left - 1)];
   };
-  Reader<HD> reader;
+  Reader<D> reader;
   reader.init((const char*)lds, lane);
   f16v dk[L::kBlocks], dv[L::kBlocks];
 #pragma unroll
@@ -671,7 +678,7 @@ __global__ DSX_ATTENTION_KERNEL(HD, 3) void k_key_grads(Args a, Backward b) {
     constexpr int kUnroll = HD == 64 ? 2 : 1;
 #pragma unroll kUnroll
     for (int c = 0; c < 2; c++) {
-      const Reader<HD> rd = reader.from((t & 1) * 2 * L::kBytes + c * 32 * HD * 2);
+      const Reader<D> rd = reader.from((t & 1) * 2 * L::kBytes + c * 32 * HD * 2);
       f16v s = {}, dp;  // dP's sums begin at -delta
 #pragma unroll
       for (int q = 0; q < 4; q++) {
@@ -685,7 +692,7 @@ __global__ DSX_ATTENTION_KERNEL(HD, 3) void k_key_grads(Args a, Backward b) {
         dp = T::mfma(rd.template rows<1>(i), vf[i], dp);
       }
       __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
-      feed<2 * L::kSteps, 1, 4>();
+      feed<2 * L::kSteps, 1, D <= 32 ? 2 : 4>();
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int q = 0; q < 4; q++) {
@@ -745,13 +752,13 @@ __global__ DSX_ATTENTION_KERNEL(HD, 3) void k_key_grads(Args a, Backward b) {
   if (b.parts > 1) {
     const int64_t plane = (int64_t)a.tokens * ld;
     float* out = b.part + part * plane + at + (lane & 31) * ld;
-    store_part<HD>(out, dk, fk, key < p.end, a.d, half);
-    store_part<HD>(out + b.parts * plane, dv, fv, key < p.end, a.d, half);
+    store_part<D>(out, dk, fk, key < p.end, a.d, half);
+    store_part<D>(out + b.parts * plane, dv, fv, key < p.end, a.d, half);
     return;
   }
   char* strip = (char*)lds + w * 32 * HD * 2;
-  store_rows<T, HD>(strip, dk, fk, false, b.dk + at, ld, rows, a.d, lane);
-  store_rows<T, HD>(strip, dv, fv, false, b.dv + at, ld, rows, a.d, lane);
+  store_rows<T, D>(strip, dk, fk, false, b.dk + at, ld, rows, a.d, lane);
+  store_rows<T, D>(strip, dv, fv, false, b.dv + at, ld, rows, a.d, lane);
 }
 
 // The parts' sums, added in order: eight values a thread.
@@ -776,7 +783,6 @@ __global__ __launch_bounds__(256) void k_join(const float* __restrict__ part, sh
 }
 
 // ---- host ------------------------------------------------------------------
-
 
 // Parts of k_key_grads' work on a tile: enough blocks for four rounds of two
 // blocks a CU, since a causal mask makes the blocks of a sequence as unequal as
@@ -827,26 +833,26 @@ Args args_of(const DsxAttention& q) {
   return a;
 }
 
-template <class T, int HD>
+template <class T, int D>
 void forward(const Args& a, const Forward& f, int64_t tiles, hipStream_t s) {
-  k_attend<T, HD><<<dim3((unsigned)(tiles * a.heads)), kThreads, 0, s>>>(a, f);
+  k_attend<T, D><<<dim3((unsigned)(tiles * a.heads)), kThreads, 0, s>>>(a, f);
 }
 
-template <class T, int HD, bool FEW>
+template <class T, int D, bool FEW>
 void gradients(Args a, const Backward& b, int64_t tiles, hipStream_t s) {
-  if (b.dq) k_query_grads<T, HD, FEW><<<dim3((unsigned)(tiles * a.heads)), kThreads, 0, s>>>(a, b);
+  if (b.dq) k_query_grads<T, D, FEW><<<dim3((unsigned)(tiles * a.heads)), kThreads, 0, s>>>(a, b);
   if (!b.dk) return;
   a.tiles += tiles;  // by keys
-  k_key_grads<T, HD, FEW><<<dim3((unsigned)(tiles * a.kv_heads * b.parts)), kThreads, 0, s>>>(a, b);
+  k_key_grads<T, D, FEW><<<dim3((unsigned)(tiles * a.kv_heads * b.parts)), kThreads, 0, s>>>(a, b);
   const int64_t n = (int64_t)a.tokens * a.kv_heads * a.d;
   if (b.parts > 1) k_join<T><<<dim3((unsigned)ceil_div(n, 2048), 2), 256, 0, s>>>(b.part, b.dk, b.dv, n, b.parts);
 }
 
-template <class T, int HD>
+template <class T, int D>
 void backward(const Args& a, const Backward& b, int64_t tiles, int64_t longest, hipStream_t s) {
   k_delta<T><<<kMost, 256, 0, s>>>(a, b);
-  if (longest <= 256 || a.d <= 32) gradients<T, HD, true>(a, b, tiles, s);
-  else gradients<T, HD, false>(a, b, tiles, s);
+  if (D <= 32 || longest <= 256) gradients<T, D, true>(a, b, tiles, s);
+  else gradients<T, D, D <= 32>(a, b, tiles, s);
 }
 
 bool off16(const void* p) { return ((uintptr_t)p & 15) != 0; }
@@ -862,7 +868,8 @@ int check(const char* what, const DsxAttention* q) {
     return fail(DSX_EINVAL, "%s: head_dim must be a multiple of 8 up to %d", what, DSX_ATTENTION_MAX_HEAD_DIM);
   if (q->tile_count < 0 || q->tile_count > q->tokens || (q->tokens && !q->tile_count))
     return fail(DSX_EINVAL, "%s: tile_count must lie in [1, tokens]", what);
-  if (q->tile_count * q->heads > INT32_MAX / 64) return fail(DSX_EINVAL, "%s: more than 2^25 tiles and heads", what);
+  if (q->tile_count * q->heads >= 1 << 24)  // a launch's threads are counted in 32 bits
+    return fail(DSX_EINVAL, "%s: tile_count times heads must be below 2^24", what);
   if (q->longest < 0 || q->longest > q->tokens) return fail(DSX_EINVAL, "%s: longest must lie in [0, tokens]", what);
   if (!(q->scale > 0.0f) || !(q->scale < INFINITY)) return fail(DSX_EINVAL, "%s: scale must be positive and finite", what);
   return DSX_OK;
@@ -883,10 +890,18 @@ int check_device(const char* what, const DsxAttention* q) {
   return DSX_OK;
 }
 
+// The sizes between powers of two keep the rows of the next one in shared memory
+// but leave its last products out. Forward and backward with them and in the next
+// size's kernels (bf16, causal): 24 features, 16 heads of 2 x 4096 rows 79 + 304
+// and 96 + 399 us; 96, 32 heads (8 of keys) of 4096 rows 139 + 454 and 161 + 534;
+// 160, 16 heads (8) of 2 x 2048 rows 89 + 337 and 118 + 453.
 #define DSX_BY_HEAD(CALL, T, ...)                                \
   do {                                                           \
-    if (args->head_dim <= 64) CALL<T, 64>(__VA_ARGS__);          \
+    if (args->head_dim <= 32) CALL<T, 32>(__VA_ARGS__);          \
+    else if (args->head_dim <= 64) CALL<T, 64>(__VA_ARGS__);     \
+    else if (args->head_dim <= 96) CALL<T, 96>(__VA_ARGS__);     \
     else if (args->head_dim <= 128) CALL<T, 128>(__VA_ARGS__);   \
+    else if (args->head_dim <= 192) CALL<T, 192>(__VA_ARGS__);   \
     else CALL<T, 256>(__VA_ARGS__);                              \
   } while (0)
 

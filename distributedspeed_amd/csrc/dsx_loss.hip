@@ -757,6 +757,8 @@ int dsx_loss_forward(const DsxLoss* args, float* loss, void* stream) {
   if (int rc = check(what, args)) return rc;
   if (int rc = check_device(what, args, false)) return rc;
   if (!loss || ((uintptr_t)loss & 3)) return fail(DSX_EINVAL, "%s: loss is NULL or misaligned", what);
+  if (args->tokens * args->vocab > (int64_t)1 << 38)  // a launch's threads are counted in 32 bits
+    return fail(DSX_EINVAL, "%s: tokens times vocab must be at most 2^38", what);
   if (args->tokens && (!args->x || ((uintptr_t)args->x & 1) || args->ld_x < args->width))
     return fail(DSX_EINVAL, "%s: x is NULL or misaligned, or its row stride below the row's length", what);
   if (args->tokens && (!args->targets || ((uintptr_t)args->targets & (args->target_bytes - 1))))

@@ -14,6 +14,7 @@ from . import ops, sequence
 
 REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 MAX_DIM = 1 << 20
+MAX_LOGITS = 1 << 38
 
 
 def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, *, ignore_index: int = -100,
@@ -31,7 +32,7 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, targets: torch.T
     backward computes them again, a piece of the vocabulary at a time, and
     rounds their gradients to the inputs' type for the two products. Rows of x
     and weight may be strided; a weight whose rows are not whole 16-byte chunks
-    is copied first. At most 2^20 rows, width and vocab.
+    is copied first. At most 2^20 rows, width and vocab, and 2^38 logits.
 
     Differentiable once in x and weight, backwards (a forward-mode tangent is
     refused); results do not depend on timing. The backward keeps a copy of the
@@ -57,6 +58,8 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, targets: torch.T
     d = x.shape[-1]
     if not (1 <= d <= MAX_DIM and 1 <= weight.shape[0] <= MAX_DIM and targets.numel() <= MAX_DIM):
         raise ValueError(f"width and vocab must lie in [1, {MAX_DIM}] and rows in [0, {MAX_DIM}]")
+    if targets.numel() * weight.shape[0] > MAX_LOGITS:
+        raise ValueError(f"rows * vocab must be at most 2^38, got {targets.numel()} * {weight.shape[0]}")
     ignore_index = int(ignore_index)
     if not -2 ** 63 <= ignore_index < 2 ** 63:
         raise ValueError(f"ignore_index must fit 64 bits, got {ignore_index}")

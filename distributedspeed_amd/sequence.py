@@ -14,6 +14,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import operator
 
 import numpy as np
 import torch
@@ -50,7 +51,8 @@ class PackedSequences:
     """Where the sequences of a batch lie: of the given lengths (host integers,
     zero allowed), one behind the other from row 0. Made once for a batch and
     used by all its layers, in both directions; it holds the kernels' tile table
-    on `device`, so that a captured graph needs it alive.
+    on `device`, so that a captured graph needs it alive. positions and offsets
+    are made at their first use, which belongs before a capture.
 
         lengths   as a tuple
         tokens    their sum
@@ -58,7 +60,7 @@ class PackedSequences:
         offsets   int32 [sequences + 1]: first rows, and the end"""
 
     def __init__(self, lengths, *, device=None):
-        lengths = [int(n) for n in (lengths.tolist() if isinstance(lengths, (torch.Tensor, np.ndarray)) else lengths)]
+        lengths = [operator.index(n) for n in (lengths.tolist() if isinstance(lengths, (torch.Tensor, np.ndarray)) else lengths)]
         if any(n < 0 for n in lengths) or sum(lengths) > MAX_TOKENS:
             raise ValueError(f"lengths must be at least 0 and add up to at most {MAX_TOKENS}")
         device = torch.device("cuda" if device is None else device)
@@ -156,8 +158,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, packing:
     if rows < packing.tokens:
         raise ValueError(f"q has {rows} rows, packing {packing.tokens} tokens")
     scale = 1 / math.sqrt(d) if scale is None else float(scale)
-    if not 0 < scale <= 3e38:
-        raise ValueError(f"scale must be positive and finite, got {scale}")
+    if not 0 < scale <= 1e38:
+        raise ValueError(f"scale must be positive and at most 1e38, got {scale}")
     return (_nodes or _native()).packed_attention(q, k, v, packing._tiles, packing.tokens, packing._longest, bool(causal), scale,
                                                   ops.stream_of(dev).value or 0)
 

@@ -799,8 +799,9 @@ int dsx_norm_backward(const DsxNorm* args /* host */, const void* d_hidden,
  * strides ld_* and head strides head_* in elements. Bases are 16-byte aligned,
  * strides and head_dim multiples of 8. heads is a multiple of kv_heads; query
  * head h reads key head h / (heads / kv_heads). `tiles` is a device copy of
- * what dsx_attention_tiles made, whose sequences cover rows [0, tokens); longest
- * is the longest sequence's length, by which the work is shared out. */
+ * what dsx_attention_tiles made, whose sequences cover rows [0, tokens);
+ * tile_count times heads is below 2^24. longest is the longest sequence's
+ * length, by which the work is shared out. */
 typedef struct DsxAttention {
   const void*    q;
   const void*    k;
@@ -903,7 +904,7 @@ int dsx_rotary(const DsxRotary* args /* host */, void* q_out, void* k_out,
  * lies outside [0, vocab) has a loss of NaN, as have its gradients. `saved`
  * (dsx_loss_saved_bytes) is written by the forward and read by the backward;
  * it and `workspace` are 256-byte aligned device memory. Sizes are at most
- * 2^20 each. */
+ * 2^20 each, tokens times vocab at most 2^38. */
 typedef struct DsxLoss {
   const void* x;
   const void* weight;

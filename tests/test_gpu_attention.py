@@ -133,6 +133,24 @@ def test_work_in_parts(gpu, d, causal):
     _compare([1500, 3, 700], 3, 1, d, "bfloat16", causal, seed=d)
 
 
+@pytest.mark.parametrize("d", [32, 96, 192])
+@pytest.mark.parametrize("causal", [True, False])
+def test_sizes_between_in_parts(gpu, d, causal):
+    _compare([700, 1, 555], 4, 2, d, "bfloat16", causal)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_scores_below_the_range_of_fp32(gpu, d):
+    """Keys whose scores are -inf in fp32 have no weight, also where a row's first
+    tiles hold no others."""
+    lengths = [150, 20]
+    q, k, v, do = _make(170, 4, 2, d, "bfloat16")
+    q[..., 0] = 2.0 ** 70
+    k[..., 0] = 0
+    k[:70, :, 0] = -2.0 ** 70
+    _check(_run(q, k, v, do, lengths, False), _exact(q, k, v, do, lengths, False, 1 / math.sqrt(d)), "bfloat16")
+
+
 def test_a_given_scale(gpu):
     args = _make(300, 2, 2, 64, "bfloat16", 3)
     _check(_run(*args, [300], True, 0.4), _exact(*args, [300], True, 0.4), "bfloat16")
