@@ -53,11 +53,24 @@ struct Saved {
 
 // ---- the rows that count ------------------------------------------------------
 
+// Row `from` to rows of whole 16-byte chunks, zeros past the end: chunk c.
+__device__ inline s8v chunk_of(const short* from, int c, int cols) {
+  if (c * 8 + 8 <= cols) return *(const s8u*)(from + c * 8);
+  s8v v = {0, 0, 0, 0, 0, 0, 0, 0};
+  for (int e = 0; e < 8; e++)
+    if (c * 8 + e < cols) v[e] = from[c * 8 + e];
+  return v;
+}
+
 // One block: runs of 4096 targets, four a thread, numbered by a scan. `each`
-// (may be NULL) gets the loss of the rows that do not count.
+// (may be NULL) gets the loss of the rows that do not count. Where x is given,
+// the block then copies the rows that count as well: kCopyHere bytes at most,
+// which take it less time than k_copy_rows takes to launch.
+constexpr int64_t kCopyHere = 32 << 10;
 template <class I>
 __global__ __launch_bounds__(1024) void k_select(const I* __restrict__ targets, int tokens, int64_t ignore, int vocab,
-                                                 Saved s, float* __restrict__ each) {
+                                                 Saved s, float* __restrict__ each, const short* __restrict__ x,
+                                                 int64_t ld, int cols) {
   __shared__ int sums[16];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   int base = 0;
@@ -100,6 +113,12 @@ __global__ __launch_bounds__(1024) void k_select(const I* __restrict__ targets, 
     __syncthreads();
   }
   if (threadIdx.x == 0) *s.count = base;
+  if (!x) return;
+  const int per = (int)(s.ld / 8);  // (the block's own writes to index are visible behind the last barrier)
+  for (int i = threadIdx.x; i < base * per; i += 1024) {
+    const int r = i / per, c = i - r * per;
+    *(s8v*)(s.x + r * s.ld + c * 8) = chunk_of(x + s.index[r] * ld, c, cols);
+  }
 }
 
 // Rows of any stride and alignment to rows of whole 16-byte chunks, zeros past
@@ -111,15 +130,8 @@ __global__ __launch_bounds__(256) void k_copy_rows(const short* __restrict__ fro
   const int per = (int)(ld_to / 8);
   for (int r = blockIdx.y; r < n; r += gridDim.y) {
     const short* p = from + (index ? index[r] : r) * ld;
-    for (int c = blockIdx.x * 256 + threadIdx.x; c < per; c += gridDim.x * 256) {
-      s8v v = {0, 0, 0, 0, 0, 0, 0, 0};
-      if (c * 8 + 8 <= cols)
-        v = *(const s8u*)(p + c * 8);
-      else
-        for (int e = 0; e < 8; e++)
-          if (c * 8 + e < cols) v[e] = p[c * 8 + e];
-      *(s8v*)(to + r * ld_to + c * 8) = v;
-    }
+    for (int c = blockIdx.x * 256 + threadIdx.x; c < per; c += gridDim.x * 256)
+      *(s8v*)(to + r * ld_to + c * 8) = chunk_of(p, c, cols);
   }
 }
 
@@ -208,12 +220,14 @@ __global__ DSX_TILE_KERNEL(G) void k_logits(Logits p, float2* __restrict__ part,
   }
 }
 
-// Joins a row's tiles: 32 rows a block, 32 runs of tiles each.
+// Joins a row's tiles: 32 rows a block, 32 runs of tiles each. `total` (where
+// one block has all rows; or NULL): their sum, with `mean` divided by their number.
 __global__ __launch_bounds__(1024) void k_rows(const float2* __restrict__ part, const float* __restrict__ hit, int m,
-                                               int nt, Saved s, float* __restrict__ loss) {
+                                               int nt, Saved s, float* __restrict__ loss, float* __restrict__ total,
+                                               int mean) {
   __shared__ float2 runs[32][33];
   const int rows = min(*s.count, m), i = threadIdx.x & 31, q = threadIdx.x >> 5, r = blockIdx.x * 32 + i;
-  if (blockIdx.x * 32 >= rows) return;
+  if (blockIdx.x * 32 >= rows && !total) return;
   float top = -INFINITY, sum = 0;
   auto join = [&](const float2& o) {
     const float next = fmaxf(top, o.x), base = next == -INFINITY ? 0.0f : next;
@@ -227,11 +241,20 @@ __global__ __launch_bounds__(1024) void k_rows(const float2* __restrict__ part, 
   }
   runs[q][i] = {top, sum};
   __syncthreads();
-  if (q || r >= rows) return;
-  for (int k = 1; k < 32; k++) join(runs[k][i]);
-  const float log = log2f(sum);
-  s.stat[r] = {top, log};
-  loss[s.index[r]] = s.target[r] < 0 ? NAN : fmaf(log, kLn2, top - hit[r]);
+  if (q) return;
+  float own = 0;
+  if (r < rows) {
+    for (int k = 1; k < 32; k++) join(runs[k][i]);
+    const float log = log2f(sum);
+    s.stat[r] = {top, log};
+    own = s.target[r] < 0 ? NAN : fmaf(log, kLn2, top - hit[r]);
+    loss[s.index[r]] = own;
+  }
+  if (!total) return;
+  double v = own;
+#pragma unroll
+  for (int d = 16; d; d >>= 1) v += __shfl_xor(v, d);
+  if (i == 0) *total = mean ? (float)(v / rows) : (float)v;
 }
 
 // The rows' sum, in an order of its own whatever the tokens; with `mean`
@@ -253,43 +276,52 @@ __global__ __launch_bounds__(1024) void k_total(const float* __restrict__ each, 
 
 // ---- backward -----------------------------------------------------------------
 
-// The factor of a row in dz, and in scale[0] what takes the products with dz to
-// the gradients. Where all rows weigh alike, as in a mean, that weight stays out
-// of dz: near a target dz is then close to -1, which 16 bits hold, where w times
-// it would be off by the same 2^-9 of bf16 in every row. fp16's power of two
-// goes by the largest factor.
-__global__ __launch_bounds__(1024) void k_weights(const float* __restrict__ d_loss, int reduction, int half, Saved s,
-                                                  float* __restrict__ weight, float* __restrict__ scale) {
+// The factor of a row in dz, and what takes the products with dz to the
+// gradients. Where all rows weigh alike, as in a mean, that weight stays out of
+// dz: near a target dz is then close to -1, which 16 bits hold, where w times it
+// would be off by the same 2^-9 of bf16 in every row. fp16's power of two goes by
+// the largest factor.
+struct Weights {
+  const float* d_loss;
+  const float* power;  // the power of two in device memory, or NULL: `one`
+  float one;
+  int reduction;
+  __device__ inline float times() const { return power ? *power : one; }
+  __device__ inline float of_row(const int* index, int r, int target) const {
+    return target < 0 ? NAN : reduction == DSX_REDUCE_NONE ? d_loss[index[r]] * times() : times();
+  }
+  // (The mean of no row is NaN, but there is nothing it could reach.)
+  __device__ inline float of_products(int rows) const {
+    const float w = reduction == DSX_REDUCE_NONE ? 1.0f : reduction == DSX_REDUCE_MEAN ? *d_loss / (float)rows : *d_loss;
+    return rows ? w / times() : 0.0f;
+  }
+};
+
+// Takes the largest finite of the rows' factors to [2^14, 2^15).
+__global__ __launch_bounds__(1024) void k_power(const float* __restrict__ d_loss, Saved s, float* __restrict__ power) {
   __shared__ float tops[16];
   const int rows = *s.count;
-  const bool none = reduction == DSX_REDUCE_NONE;
-  float f = 1.0f;
-  if (half) {
-    float top = none ? 0.0f : 1.0f;
-    if (none) {
-      for (int r = threadIdx.x; r < rows; r += 1024) top = fmaxf(top, fabsf(d_loss[s.index[r]]));
-#pragma unroll
-      for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
-      if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
-      __syncthreads();
-      for (int i = 0; i < 16; i++) top = fmaxf(top, tops[i]);
-    }
-    if (top > 0.0f && top < INFINITY) {
-      int e;
-      frexpf(top, &e);  // top < 2^e
-      f = ldexpf(1.0f, max(-100, min(100, 15 - e)));
-    }
+  float top = 0;
+  for (int r = threadIdx.x; r < rows; r += 1024) {
+    const float v = fabsf(d_loss[s.index[r]]);
+    top = fmaxf(top, v < INFINITY ? v : 0.0f);
   }
-  for (int r = threadIdx.x; r < rows; r += 1024)
-    weight[r] = s.target[r] < 0 ? NAN : none ? d_loss[s.index[r]] * f : f;
-  if (threadIdx.x == 0)  // (the mean of no row is NaN, but there is nothing it could reach)
-    scale[0] = !rows ? 0.0f : (none ? 1.0f : reduction == DSX_REDUCE_MEAN ? *d_loss / (float)rows : *d_loss) / f;
+#pragma unroll
+  for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+  if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
+  __syncthreads();
+  if (threadIdx.x) return;
+  for (int i = 1; i < 16; i++) top = fmaxf(top, tops[i]);
+  int e = 15;
+  if (top > 0.0f) frexpf(top, &e);  // top < 2^e
+  *power = ldexpf(1.0f, max(-100, min(100, 15 - e)));
 }
 
 // dz of a piece, [rows][ld] with zeros from the piece's end to ld.
 template <class G, class T>
 __global__ DSX_TILE_KERNEL(G) void k_dlogits(Logits p, const float2* __restrict__ stat,
-                                             const float* __restrict__ weight, short* __restrict__ dz, int64_t ld) {
+                                             Weights weights, const int* __restrict__ index,
+                                             short* __restrict__ dz, int64_t ld) {
   __shared__ __attribute__((aligned(1024))) char lds[G::kLds];
   int ti, tj, rows;
   if (!tile_of<G>(p, &ti, &tj, &rows)) return;
@@ -308,7 +340,8 @@ __global__ DSX_TILE_KERNEL(G) void k_dlogits(Logits p, const float2* __restrict_
       [&](int r, int) {
         if (m0 + r >= rows) return Row{};
         const float2 s = stat[m0 + r];
-        return Row{s.x, s.y, weight[m0 + r], p.target[m0 + r] - p.v0};
+        const int target = p.target[m0 + r];
+        return Row{s.x, s.y, weights.of_row(index, m0 + r, target), target - p.v0};
       },
       [&](int r, int c, float* v, float*, const Row& q) {
         const int n = n0 + c;
@@ -379,9 +412,9 @@ __global__ DSX_TILE_KERNEL(G) void k_input_grad(InputGrad p) {
 // The planes added in order and rounded; zeros in rows that do not count.
 template <class T>
 __global__ __launch_bounds__(256) void k_input_join(const float* __restrict__ planes, int splits, int m, int64_t ld,
-                                                    int n, Saved s, const float* __restrict__ scale,
+                                                    int n, Saved s, Weights weights,
                                                     short* __restrict__ dx) {
-  const float f = scale[0];
+  const float f = weights.of_products(*s.count);
   const int c = (blockIdx.x * 256 + threadIdx.x) * 8;
   if (c >= n) return;
   for (int t = blockIdx.y; t < m; t += gridDim.y) {
@@ -411,7 +444,7 @@ struct WeightGrad {
   Operand dz, x;
   int m, n, mt, nt;  // vocabulary rows of the piece, width
   const int* count;
-  const float* scale;
+  Weights weights;
   short* out;        // the piece's rows, contiguous
 };
 template <class G, class T>
@@ -422,7 +455,7 @@ __global__ DSX_TILE_KERNEL(G) void k_weight_grad(WeightGrad p) {
   G g;
   g.init();
   g.run(lds, p.dz, p.x, p.x, ti * G::TM, tj * G::TN, *p.count);
-  const float f = p.scale[0];
+  const float f = p.weights.of_products(*p.count);
   g.template emit<false>(
       lds, [](int, int) { return Nothing{}; },
       [&](int r, int c, float* v, float*, const Nothing&) {
@@ -543,8 +576,7 @@ struct Work {
   float2* part;           // forward: [nt][tokens]
   float* hit;
   float* each;
-  float* row_weight;      // backward
-  float* scale;
+  float* power;           // backward
   short* dz;
   float* planes;
   int64_t total;
@@ -564,8 +596,7 @@ Work work_of(const DsxLoss& q, const Sizes& z, bool backward) {
     w.hit = (float*)take(z.t * 4);
     w.each = (float*)take(z.t * 4);
   } else {
-    w.row_weight = (float*)take(z.t * 4);
-    w.scale = (float*)take(4);
+    w.power = (float*)take(4);
     w.dz = (short*)take(z.t * z.ld_piece * 2);
     w.planes = (float*)take(z.splits * z.t * z.ld * 4);
   }
@@ -616,16 +647,21 @@ int forward(const DsxLoss& q, float* loss, hipStream_t st) {
   const Work w = work_of(q, z, false);
   const bool none = q.reduction == DSX_REDUCE_NONE;
   float* each = none ? loss : w.each;
+  const bool here = z.t * z.ld * 2 <= kCopyHere;
+  const short* x = here ? (const short*)q.x : nullptr;
   if (q.target_bytes == 8)
-    k_select<<<1, 1024, 0, st>>>((const int64_t*)q.targets, (int)z.t, q.ignore_index, (int)z.v, s, none ? loss : nullptr);
+    k_select<<<1, 1024, 0, st>>>((const int64_t*)q.targets, (int)z.t, q.ignore_index, (int)z.v, s, none ? loss : nullptr, x,
+                                 q.ld_x, (int)z.d);
   else
-    k_select<<<1, 1024, 0, st>>>((const int32_t*)q.targets, (int)z.t, q.ignore_index, (int)z.v, s, none ? loss : nullptr);
+    k_select<<<1, 1024, 0, st>>>((const int32_t*)q.targets, (int)z.t, q.ignore_index, (int)z.v, s, none ? loss : nullptr, x,
+                                 q.ld_x, (int)z.d);
   if (!z.t) {
     if (!none) k_total<<<1, 1024, 0, st>>>(nullptr, s, q.reduction == DSX_REDUCE_MEAN, loss);
     return launch_status("dsx_loss_forward");
   }
-  k_copy_rows<<<dim3((unsigned)ceil_div(z.ld / 8, 256), (unsigned)(z.t < 65535 ? z.t : 65535)), 256, 0, st>>>(
-      (const short*)q.x, q.ld_x, (int)z.d, s.index, s.count, (int)z.t, s.x, s.ld);
+  if (!here)
+    k_copy_rows<<<dim3((unsigned)ceil_div(z.ld / 8, 256), (unsigned)(z.t < 65535 ? z.t : 65535)), 256, 0, st>>>(
+        (const short*)q.x, q.ld_x, (int)z.d, s.index, s.count, (int)z.t, s.x, s.ld);
   copy_weight(q, z, w, st);
   const Logits p = logits_of(q, z, s, w, 0, z.v, z.tile);
   const dim3 grid((unsigned)(p.mt * p.nt));
@@ -636,8 +672,10 @@ int forward(const DsxLoss& q, float* loss, hipStream_t st) {
   } while (0)
   DSX_BY_TILE(z.tile, (int64_t)p.mt * p.nt, RUN);
 #undef RUN
-  k_rows<<<dim3((unsigned)ceil_div(z.t, 32)), 1024, 0, st>>>(w.part, w.hit, (int)z.t, (int)z.nt, s, each);
-  if (!none) k_total<<<1, 1024, 0, st>>>(each, s, q.reduction == DSX_REDUCE_MEAN, loss);
+  const bool one = !none && z.t <= 32, mean = q.reduction == DSX_REDUCE_MEAN;
+  k_rows<<<dim3((unsigned)ceil_div(z.t, 32)), 1024, 0, st>>>(w.part, w.hit, (int)z.t, (int)z.nt, s, each,
+                                                             one ? loss : nullptr, mean);
+  if (!none && !one) k_total<<<1, 1024, 0, st>>>(each, s, mean, loss);
   return launch_status("dsx_loss_forward");
 }
 
@@ -646,7 +684,9 @@ int backward(const DsxLoss& q, const float* d_loss, short* dx, short* dw, hipStr
   const Sizes z = sizes_of(q);
   const Saved s = saved_of(q, nullptr);
   const Work w = work_of(q, z, true);
-  k_weights<<<1, 1024, 0, st>>>(d_loss, q.reduction, q.dtype == DSX_F16, s, w.row_weight, w.scale);
+  const bool half = q.dtype == DSX_F16, none = q.reduction == DSX_REDUCE_NONE;
+  const Weights weights{d_loss, half && none ? w.power : nullptr, half ? 0x1p14f : 1.0f, q.reduction};
+  if (weights.power) k_power<<<1, 1024, 0, st>>>(d_loss, s, w.power);
   copy_weight(q, z, w, st);
   for (int64_t v0 = 0; v0 < z.v; v0 += z.piece) {
     const int64_t n = z.v - v0 < z.piece ? z.v - v0 : z.piece, ld = round_up(n, 8);
@@ -656,7 +696,7 @@ int backward(const DsxLoss& q, const float* d_loss, short* dx, short* dw, hipStr
 #define RUN(TM, TN, WM, WN, STAGES)                                                              \
   do {                                                                                           \
     using G = Gemm<T, TM, TN, WM, WN, true, true, true, false, STAGES>;                          \
-    k_dlogits<G, T><<<grid, G::THREADS, 0, st>>>(p, s.stat, w.row_weight, w.dz, ld);             \
+    k_dlogits<G, T><<<grid, G::THREADS, 0, st>>>(p, s.stat, weights, s.index, w.dz, ld);         \
   } while (0)
     if (z.t) DSX_BY_TILE(tile, (int64_t)p.mt * p.nt, RUN);
 #undef RUN
@@ -692,7 +732,7 @@ int backward(const DsxLoss& q, const float* d_loss, short* dx, short* dw, hipStr
       g.m = (int)n;
       g.n = (int)z.d;
       g.count = s.count;
-      g.scale = w.scale;
+      g.weights = weights;
       g.out = dw + v0 * z.d;
       const int tile = square_tile(ceil_div(n, 256) * ceil_div(z.d, 256), ceil_div(n, 128) * ceil_div(z.d, 128));
       g.mt = (int)ceil_div(n, tile);
@@ -709,7 +749,7 @@ int backward(const DsxLoss& q, const float* d_loss, short* dx, short* dw, hipStr
   }
   if (dx && z.t)
     k_input_join<T><<<dim3((unsigned)ceil_div(z.d, 2048), (unsigned)(z.t < 65535 ? z.t : 65535)), 256, 0, st>>>(
-        w.planes, z.splits, (int)z.t, z.ld, (int)z.d, s, w.scale, dx);
+        w.planes, z.splits, (int)z.t, z.ld, (int)z.d, s, weights, dx);
   return launch_status("dsx_loss_backward");
 }
 
