@@ -111,7 +111,7 @@ class DsxAttention(_c.Structure):
                [(k, _c.c_int64) for k in ("ld_q", "ld_k", "ld_v", "head_q", "head_k", "head_v", "tokens")] + \
                [("tiles", _P), ("tile_count", _c.c_int64)] + \
                [(k, _c.c_int32) for k in ("heads", "kv_heads", "head_dim", "dtype", "causal")] + \
-               [("scale", _c.c_float), ("longest", _c.c_int64)]
+               [("scale", _c.c_float), ("longest", _c.c_int64), ("pairs", _c.c_int64)]
 
 
 class DsxRotary(_c.Structure):
@@ -131,7 +131,7 @@ class DsxLoss(_c.Structure):
 for _s, _n in ((DsxState, 64), (DsxScalerConfig, 32), (DsxAdamwHyper, 56), (DsxStepScalars, 64),
                (DsxTensorRef, 56), (DsxChunk, 24), (DsxGroupsDev, 1112), (DsxFlatPlan, 248),
                (DsxMatrix, 48), (DsxMuonParam, 64), (DsxMuonHyper, 32), (DsxFfn, 128), (DsxNorm, 104),
-               (DsxAttention, 128), (DsxRotary, 104), (DsxLoss, 112)):
+               (DsxAttention, 136), (DsxRotary, 104), (DsxLoss, 112)):
     assert _c.sizeof(_s) == _n, (_s.__name__, _c.sizeof(_s))
 
 # name -> (restype, argtypes); every symbol include/dsx.h declares.

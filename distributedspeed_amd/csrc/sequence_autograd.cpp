@@ -67,7 +67,7 @@ Tensor rows_for(const Tensor& like, int64_t tokens) {
 
 struct Sequences {
   Tensor tiles;  // int32 [2, count, 4] on the device
-  int64_t tokens, longest;
+  int64_t tokens, longest, pairs;
 };
 
 DsxAttention describe(const Tensor& q, const Tensor& k, const Tensor& v, const Sequences& s, bool causal,
@@ -94,6 +94,7 @@ DsxAttention describe(const Tensor& q, const Tensor& k, const Tensor& v, const S
   a.causal = causal;
   a.scale = static_cast<float>(scale);
   a.longest = s.longest;
+  a.pairs = s.pairs;
   return a;
 }
 
@@ -117,11 +118,12 @@ Kept attention_run(const Tensor& q, const Tensor& k, const Tensor& v, const Sequ
 
 struct PackedAttention : torch::autograd::Function<PackedAttention> {
   static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& tiles,
-                        int64_t tokens, int64_t longest, bool causal, double scale, int64_t stream) {
-    const Kept r = attention_run(q, k, v, {tiles, tokens, longest}, causal, scale, stream, true);
+                        int64_t tokens, int64_t longest, int64_t pairs, bool causal, double scale, int64_t stream) {
+    const Kept r = attention_run(q, k, v, {tiles, tokens, longest, pairs}, causal, scale, stream, true);
     ctx->save_for_backward({r.q, r.k, r.v, r.out, r.out_lo, r.lse, tiles});
     ctx->saved_data["tokens"] = tokens;
     ctx->saved_data["longest"] = longest;
+    ctx->saved_data["pairs"] = pairs;
     ctx->saved_data["causal"] = causal;
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["d"] = q.size(2);
@@ -135,7 +137,8 @@ struct PackedAttention : torch::autograd::Function<PackedAttention> {
     Tensor dq, dk, dv;
     if (grads[0].defined()) {
       const c10::DeviceGuard guard(s[0].device());
-      const Sequences seq{s[6], ctx->saved_data["tokens"].toInt(), ctx->saved_data["longest"].toInt()};
+      const Sequences seq{s[6], ctx->saved_data["tokens"].toInt(), ctx->saved_data["longest"].toInt(),
+                          ctx->saved_data["pairs"].toInt()};
       const int64_t d = ctx->saved_data["d"].toInt();
       const DsxAttention a = describe(s[0], s[1], s[2], seq, ctx->saved_data["causal"].toBool(),
                                       ctx->saved_data["scale"].toDouble());
@@ -156,16 +159,16 @@ struct PackedAttention : torch::autograd::Function<PackedAttention> {
       dk = ctx->needs_input_grad(1) ? first_features(dk, d) : Tensor();
       dv = ctx->needs_input_grad(2) ? first_features(dv, d) : Tensor();
     }
-    return once({dq, dk, dv, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()});
+    return once({dq, dk, dv, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()});
   }
 };
 
 Tensor packed_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& tiles, int64_t tokens,
-                        int64_t longest, bool causal, double scale, int64_t stream) {
+                        int64_t longest, int64_t pairs, bool causal, double scale, int64_t stream) {
   for (const Tensor* t : {&q, &k, &v}) refuse_tangent("packed_attention", *t);
   if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad()))
-    return PackedAttention::apply(q, k, v, tiles, tokens, longest, causal, scale, stream);
-  return first_features(attention_run(q, k, v, {tiles, tokens, longest}, causal, scale, stream, false).out, q.size(2));
+    return PackedAttention::apply(q, k, v, tiles, tokens, longest, pairs, causal, scale, stream);
+  return first_features(attention_run(q, k, v, {tiles, tokens, longest, pairs}, causal, scale, stream, false).out, q.size(2));
 }
 
 // ---- rotary --------------------------------------------------------------------

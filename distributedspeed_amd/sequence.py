@@ -68,7 +68,7 @@ class PackedSequences:
             raise ValueError(f"device must be a GPU, got {device}")
         self.lengths = tuple(lengths)
         self.tokens = sum(lengths)
-        self._longest = max(lengths, default=0)
+        self._longest, self._pairs = max(lengths, default=0), sum(n * n for n in lengths)
         self.device = torch.device("cuda", torch.cuda.current_device()) if device.index is None else device
         self._tiles = torch.from_numpy(_tile_table(lengths)).to(self.device)
         self._positions = self._offsets = None
@@ -160,8 +160,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, packing:
     scale = 1 / math.sqrt(d) if scale is None else float(scale)
     if not 0 < scale <= 1e38:
         raise ValueError(f"scale must be positive and at most 1e38, got {scale}")
-    return (_nodes or _native()).packed_attention(q, k, v, packing._tiles, packing.tokens, packing._longest, bool(causal), scale,
-                                                  ops.stream_of(dev).value or 0)
+    return (_nodes or _native()).packed_attention(q, k, v, packing._tiles, packing.tokens, packing._longest, packing._pairs,
+                                                  bool(causal), scale, ops.stream_of(dev).value or 0)
 
 
 def rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, *, base: float = 10000.0,

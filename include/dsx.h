@@ -801,7 +801,8 @@ int dsx_norm_backward(const DsxNorm* args /* host */, const void* d_hidden,
  * head h reads key head h / (heads / kv_heads). `tiles` is a device copy of
  * what dsx_attention_tiles made, whose sequences cover rows [0, tokens);
  * tile_count times heads is below 2^24. longest is the longest sequence's
- * length, by which the work is shared out. */
+ * length and pairs the sum of the squared lengths, by which the work is shared
+ * out. */
 typedef struct DsxAttention {
   const void*    q;
   const void*    k;
@@ -822,6 +823,7 @@ typedef struct DsxAttention {
   int32_t        causal;
   float          scale;
   int64_t        longest;
+  int64_t        pairs;
 } DsxAttention;
 
 /* The tile table of sequences of the given lengths (zero allowed), one behind

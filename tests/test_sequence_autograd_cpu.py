@@ -44,7 +44,7 @@ def nodes():
 
 def _attention(nodes, q, k, v):
     import torch
-    return nodes.packed_attention(q, k, v, torch.zeros(2, 1, 4, dtype=torch.int32), 10, 7, True, 0.5, 0)
+    return nodes.packed_attention(q, k, v, torch.zeros(2, 1, 4, dtype=torch.int32), 10, 7, 58, True, 0.5, 0)
 
 
 def _rotary(nodes, q, k):
@@ -112,7 +112,8 @@ def test_attention_hands_on_strides_and_copies_what_it_must(nodes):
     q, k, v = rows[:, :4], rows[:, 4:6], rows[:, 6:]
     out = _attention(nodes, q, k, v)
     a = nodes.seen["attention"][0]
-    assert (a.ld_q, a.head_q, a.ld_k, a.tokens, a.longest, a.heads, a.kv_heads, a.head_dim) == (128, 16, 128, 10, 7, 4, 2, 16)
+    assert (a.ld_q, a.head_q, a.ld_k, a.tokens, a.longest, a.pairs) == (128, 16, 128, 10, 7, 58)
+    assert (a.heads, a.kv_heads, a.head_dim) == (4, 2, 16)
     assert a.q == q.data_ptr() and a.k == k.data_ptr() and a.v == v.data_ptr()
     assert out.shape == (12, 4, 16) and not out[10:].any()  # rows behind the sequences
     for bad in (torch.ones(12, 4, 32).bfloat16()[..., ::2], torch.ones(12, 4, 15).bfloat16(),

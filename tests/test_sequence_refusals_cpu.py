@@ -65,7 +65,8 @@ BAD_SIZES = [dict(dtype=0), dict(dtype=9), dict(tokens=-1), dict(tokens=2 ** 27 
              dict(heads=5), dict(heads=1), dict(heads=2048, kv_heads=1), dict(head_dim=0), dict(head_dim=4),
              dict(head_dim=60), dict(head_dim=264), dict(tile_count=-1), dict(tile_count=0), dict(tile_count=301),
              dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")), dict(longest=-1),
-             dict(longest=301), dict(tokens=2 ** 27, tile_count=2 ** 27), dict(tokens=2 ** 23, tile_count=2 ** 22)]
+             dict(longest=301), dict(tokens=2 ** 27, tile_count=2 ** 27), dict(tokens=2 ** 23, tile_count=2 ** 22),
+             dict(pairs=-1), dict(pairs=60001)]
 BAD_ROWS = [dict(q=None), dict(k=None), dict(v=None), dict(q=4104), dict(k=4098), dict(tiles=None), dict(tiles=4100),
             dict(ld_q=60), dict(ld_q=257), dict(ld_k=8), dict(ld_v=2 ** 24 + 8), dict(head_q=4), dict(head_k=63),
             dict(head_v=8)]
