@@ -17,6 +17,15 @@
 // of the largest size and blocks without rows end at once). The copy also
 // gives the product's direct loads the aligned rows that they need.
 //
+// Bound by the matrix instructions, and where the products are large by the power
+// that they take: 8192 rows, 15% of them ignored, of 4096 against 128256, bf16, 25.4
+// ms; k_logits 1.14 PFLOP/s, k_dlogits 1.05, dx 1.17, dW 1.28, where one product of
+// 8192^3 reaches 1.42 in the library. A fourth of the backward's products computes
+// the logits again: kept, they would take 2.1 GB in bf16, and their gradients would
+// begin from rounded values. With 768 features (4096 rows against 50257, 1.41 ms) a
+// tile's sum is of 12 steps, whose start and epilogue show: k_logits 0.99 PFLOP/s,
+// k_dlogits, which writes 412 MB, 0.72, dx and dW 0.95.
+//
 // In fp16, dz is held times a power of two that takes the largest factor to
 // about 2^14, so that probabilities down to 2^-28 keep their digits.
 

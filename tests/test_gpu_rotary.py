@@ -149,3 +149,19 @@ def test_values_that_are_not_finite_and_no_rows(gpu):
     y, z = rotary(x, x, positions[:0])
     (y.sum() + z.sum()).backward()
     assert y.shape == (0, 2, 32) and x.grad.shape == (0, 2, 32)
+
+
+def test_as_many_rows_as_there_may_be(gpu):
+    """2^27: a block then takes several runs of rows."""
+    import torch
+    from distributedspeed_amd import rotary
+    n = 2 ** 27
+    gen = torch.Generator("cuda").manual_seed(0)
+    q = torch.randn(n, 1, 2, generator=gen, device="cuda", dtype=torch.float16)
+    k = q.view(n, 2, 1)[:, :1].expand(-1, 1, 2)
+    positions = torch.arange(n, dtype=torch.int32, device="cuda") % 1000
+    got = rotary(q, k, positions)
+    for first in (0, 2 ** 25 - 500, 2 ** 26 - 500, n - 1000):
+        at = slice(first, first + 1000)
+        for x, y in zip(got, (q, k)):
+            _check(x[at], y[at], positions[at], 10000.0, 2, False)
