@@ -122,7 +122,7 @@ struct Tile {
   // the last one again and a chunk past d the row's first (the products' other
   // operand holds zeros there).
   static __device__ inline void load(char* dst, const short* p, int64_t ld, int left, int d) {
-    const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int tid = threadIdx.x & (kThreads - 1), w = __builtin_amdgcn_readfirstlane(tid >> 6);
 #pragma unroll
     for (int j = 0; j < kLoads; j++) {
       const int at = j * kThreads + tid, r = at / kChunks;
@@ -284,12 +284,16 @@ __device__ inline Place place_of(const Args& a, int heads) {
   return p;
 }
 
-// A SIMD's waves: as many as the registers of a kernel of D features allow. (16384
+// A SIMD's waves: as many as the registers of a kernel of D features allow; of a
+// block of eight, two or four. (16384
 // rows, 16 heads of 64: k_attend with four 625 us, with three 635; both gradients
 // with three 2.08 ms, with two 2.14.)
-constexpr int dsx_waves(int d, int at_64) { return d <= 32 ? 4 : d <= 64 ? at_64 : d <= 128 ? 2 : 1; }
-#define DSX_ATTENTION_KERNEL(D, WAVES)                                                        \
-  __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(dsx_waves(D, WAVES), dsx_waves(D, WAVES))))
+constexpr int dsx_waves(int d, int at_64, int groups) {
+  return groups == 2 && at_64 == 3 ? 2 : d <= 32 ? 4 : d <= 64 ? at_64 : d <= 128 ? 2 : 1;
+}
+#define DSX_ATTENTION_KERNEL(D, WAVES, GROUPS)              \
+  __launch_bounds__(kThreads * GROUPS) __attribute__((       \
+      amdgpu_waves_per_eu(dsx_waves(D, WAVES, GROUPS), dsx_waves(D, WAVES, GROUPS))))
 
 // v, as the compiler may not know it before this place: keeps what the masks of
 // the few tiles at a sequence's edges need out of every tile's way.
@@ -319,14 +323,33 @@ struct Forward {
   float* lse;     // [heads][tokens], base 2; NULL: not kept
 };
 
-template <class T, int D>
-__global__ DSX_ATTENTION_KERNEL(D, 4) void k_attend(Args a, Forward f) {
+// Two groups of four waves share a block's rows where there are few blocks: a
+// group takes every other tile, and the second hands its sums to the first.
+template <int D>
+__device__ inline void hand_over(float* to, const f16v* o) {
+#pragma unroll
+  for (int i = 0; i < D / 32; i++)
+#pragma unroll
+    for (int r = 0; r < 16; r++) to[(i * 16 + r) * 64] = o[i][r];
+}
+template <int D>
+__device__ inline void take_over(const float* from, f16v* o, float mine, float theirs) {
+#pragma unroll
+  for (int i = 0; i < D / 32; i++)
+#pragma unroll
+    for (int r = 0; r < 16; r++) o[i][r] = o[i][r] * mine + from[(i * 16 + r) * 64] * theirs;
+}
+
+template <class T, int D, int GROUPS>
+__global__ DSX_ATTENTION_KERNEL(D, 4, GROUPS) void k_attend(Args a, Forward f) {
   using L = Tile<D>;
   constexpr int HD = L::HD;
-  __shared__ __attribute__((aligned(1024))) char lds[2][2][L::kBytes];
+  __shared__ __attribute__((aligned(1024))) char shared[GROUPS][2][2][L::kBytes];
   const Place p = place_of(a, a.heads);
   if (!p.good) return;
-  const int lane = threadIdx.x & 63, half = lane >> 5, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, half = lane >> 5, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 3;
+  const int group = GROUPS == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / kThreads);
+  auto& lds = shared[group];
   const int w0 = p.row0 + 32 * w, row = w0 + (lane & 31);
   s8v qf[L::kSteps];
   L::own(qf, a.q.p + p.head * a.q.head, a.q.ld, min(row, p.end - 1), a.d, lane);
@@ -339,20 +362,20 @@ __global__ DSX_ATTENTION_KERNEL(D, 4) void k_attend(Args a, Forward f) {
   L::arrived(qf);
   auto load = [&](int t) {
     const int left = p.end - p.start - t * kTile;
-    L::load(lds[t & 1][0], kp + (int64_t)t * kTile * a.k.ld, a.k.ld, left, a.d);
-    L::load(lds[t & 1][1], vp + (int64_t)t * kTile * a.v.ld, a.v.ld, left, a.d);
+    L::load(lds[(t / GROUPS) & 1][0], kp + (int64_t)t * kTile * a.k.ld, a.k.ld, left, a.d);
+    L::load(lds[(t / GROUPS) & 1][1], vp + (int64_t)t * kTile * a.v.ld, a.v.ld, left, a.d);
   };
   f16v o[L::kBlocks];
 #pragma unroll
   for (int i = 0; i < L::kBlocks; i++) o[i] = f16v{};
   float m = -INFINITY, l = 0;
-  load(0);
-  for (int t = 0; t < nt; t++) {
+  if (group < nt) load(group);
+  for (int t = group; t - group < nt; t += GROUPS) {
     sync_loads();
-    if (t + 1 < nt) load(t + 1);
+    if (t + GROUPS < nt) load(t + GROUPS);
     const int j0 = p.start + t * kTile;
     if (j0 >= wave_hi) continue;
-    const char *kt = lds[t & 1][0], *vt = lds[t & 1][1];
+    const char *kt = lds[(t / GROUPS) & 1][0], *vt = lds[(t / GROUPS) & 1][1];
     f16v s[2] = {};
 #pragma unroll
     for (int i = 0; i < L::kSteps; i++)
@@ -412,8 +435,25 @@ __global__ DSX_ATTENTION_KERNEL(D, 4) void k_attend(Args a, Forward f) {
   l += other_half(l);
   const int rows = min(32, p.end - w0);
   __syncthreads();  // the tiles' place is free
+  if (GROUPS == 2) {
+    float* there = (float*)shared + w * 64 * (L::kBlocks * 16 + 2) + lane;
+    if (group) {
+      hand_over<D>(there, o);
+      there[L::kBlocks * 16 * 64] = m;
+      there[(L::kBlocks * 16 + 1) * 64] = l;
+    }
+    __syncthreads();
+    if (!group) {
+      const float m2 = there[L::kBlocks * 16 * 64], top = fmaxf(m, m2), mine = exp2f(m - top), theirs = exp2f(m2 - top);
+      l = l * mine + there[(L::kBlocks * 16 + 1) * 64] * theirs;
+      m = top;
+      take_over<D>(there, o, mine, theirs);
+    }
+    __syncthreads();
+    if (group) return;
+  }
   if (rows <= 0) return;
-  char* strip = (char*)lds + w * 32 * HD * 2;
+  char* strip = (char*)shared + w * 32 * HD * 2;
   const int64_t ld = (int64_t)a.heads * a.d, at = w0 * ld + (int64_t)p.head * a.d;
   store_rows<T, D>(strip, o, 1.0f / l, false, f.out + at, ld, rows, a.d, lane);
   if (f.out_lo) store_rows<T, D>(strip, o, 1.0f / l, true, f.out_lo + at, ld, rows, a.d, lane);
@@ -547,15 +587,17 @@ __device__ inline float gradient_scale(const float* most, float* buf) {
 // dk with none 1.44; 60 keys, dq and dk: 1.65 with none, 1.07 with all. Time of dq
 // for 16384 rows, 16 heads of 64: 0.77 ms with none, 0.89 with every other 16, 1.02
 // with all.
-template <class T, int D, bool FEW>
-__global__ DSX_ATTENTION_KERNEL(D, 3) void k_query_grads(Args a, Backward b) {
+template <class T, int D, bool FEW, int GROUPS>
+__global__ DSX_ATTENTION_KERNEL(D, 3, GROUPS) void k_query_grads(Args a, Backward b) {
   using L = Tile<D>;
   constexpr int HD = L::HD;
-  __shared__ __attribute__((aligned(1024))) char lds[2][2][L::kBytes];
+  __shared__ __attribute__((aligned(1024))) char shared[GROUPS][2][2][L::kBytes];
   const Place p = place_of(a, a.heads);
   if (!p.good) return;
-  const float ds_scale = T::kScaled ? gradient_scale(b.most, (float*)lds) : 1.0f;
-  const int lane = threadIdx.x & 63, half = lane >> 5, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const float ds_scale = T::kScaled ? gradient_scale(b.most, (float*)shared) : 1.0f;
+  const int lane = threadIdx.x & 63, half = lane >> 5, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 3;
+  const int group = GROUPS == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / kThreads);
+  auto& lds = shared[group];
   const int w0 = p.row0 + 32 * w, row = w0 + (lane & 31), there = min(row, p.end - 1);
   s8v qf[L::kSteps], gf[L::kSteps];
   L::own(qf, a.q.p + p.head * a.q.head, a.q.ld, there, a.d, lane);
@@ -575,19 +617,19 @@ __global__ DSX_ATTENTION_KERNEL(D, 3) void k_query_grads(Args a, Backward b) {
   L::arrived(gf);
   auto load = [&](int t) {
     const int left = p.end - p.start - t * kTile;
-    L::load(lds[t & 1][0], kp + (int64_t)t * kTile * a.k.ld, a.k.ld, left, a.d);
-    L::load(lds[t & 1][1], vp + (int64_t)t * kTile * a.v.ld, a.v.ld, left, a.d);
+    L::load(lds[(t / GROUPS) & 1][0], kp + (int64_t)t * kTile * a.k.ld, a.k.ld, left, a.d);
+    L::load(lds[(t / GROUPS) & 1][1], vp + (int64_t)t * kTile * a.v.ld, a.v.ld, left, a.d);
   };
   f16v dq[L::kBlocks];
 #pragma unroll
   for (int i = 0; i < L::kBlocks; i++) dq[i] = f16v{};
-  load(0);
-  for (int t = 0; t < nt; t++) {
+  if (group < nt) load(group);
+  for (int t = group; t - group < nt; t += GROUPS) {
     sync_loads();
-    if (t + 1 < nt) load(t + 1);
+    if (t + GROUPS < nt) load(t + GROUPS);
     const int j0 = p.start + t * kTile;
     if (j0 >= wave_hi) continue;
-    const char *kt = lds[t & 1][0], *vt = lds[t & 1][1];
+    const char *kt = lds[(t / GROUPS) & 1][0], *vt = lds[(t / GROUPS) & 1][1];
     const bool edge = j0 + kTile - 1 > (a.causal ? min(w0, p.end - 1) : p.end - 1);
 #pragma unroll
     for (int c = 0; c < 2; c++) {
@@ -621,9 +663,17 @@ __global__ DSX_ATTENTION_KERNEL(D, 3) void k_query_grads(Args a, Backward b) {
   }
   const int rows = min(32, p.end - w0);
   __syncthreads();
+  if (GROUPS == 2) {
+    float* there = (float*)shared + w * 64 * L::kBlocks * 16 + lane;
+    if (group) hand_over<D>(there, dq);
+    __syncthreads();
+    if (!group) take_over<D>(there, dq, 1.0f, 1.0f);
+    __syncthreads();
+    if (group) return;
+  }
   if (rows <= 0) return;
   const int64_t ld = (int64_t)a.heads * a.d;
-  store_rows<T, D>((char*)lds + w * 32 * HD * 2, dq, a.scale / ds_scale, false,
+  store_rows<T, D>((char*)shared + w * 32 * HD * 2, dq, a.scale / ds_scale, false,
                     b.dq + w0 * ld + (int64_t)p.head * a.d, ld, rows, a.d, lane);
 }
 
@@ -641,7 +691,7 @@ __device__ inline void store_part(float* out, const f16v* o, float factor, bool 
 }
 
 template <class T, int D, bool FEW>
-__global__ DSX_ATTENTION_KERNEL(D, 3) void k_key_grads(Args a, Backward b) {
+__global__ DSX_ATTENTION_KERNEL(D, 3, 1) void k_key_grads(Args a, Backward b) {
   using L = Tile<D>;
   constexpr int HD = L::HD;
   // One array: with two, the compiler waits for all direct loads in flight before
@@ -859,14 +909,35 @@ Args args_of(const DsxAttention& q) {
   return a;
 }
 
+// Whether a block's tiles are shared by two groups of waves: where the blocks
+// leave CUs or half of them idle and have several tiles to share. k_attend (bf16,
+// causal) with one and two: 96 blocks of 1024 rows, 64 features, 19.7 and 16.0 us;
+// 512 of 4096 rows 69.1 and 55.9; 768 of 1024 rows 26.0 and 28.6; 512 of 256 rows 9.3
+// and 10.2; 128 features, 512 of 2048 rows 55.9 and 48.2, 1024 of 2048 rows 86.2 and
+// 97.2. k_delta and k_query_grads, 512 of 4096 rows of 64 features: 90.7 and 78.5.
+// (Heads above 128 features have no registers for eight waves.)
+bool two_groups(int64_t blocks, int64_t longest) { return blocks <= 2 * kCus && longest >= 8 * kTile; }
+
 template <class T, int D>
-void forward(const Args& a, const Forward& f, int64_t tiles, hipStream_t s) {
-  k_attend<T, D><<<dim3((unsigned)(tiles * a.heads)), kThreads, 0, s>>>(a, f);
+void forward(const Args& a, const Forward& f, int64_t tiles, int64_t longest, hipStream_t s) {
+  const dim3 grid((unsigned)(tiles * a.heads));
+  if constexpr (D <= 128)
+    if (two_groups(tiles * a.heads, longest)) {
+      k_attend<T, D, 2><<<grid, 2 * kThreads, 0, s>>>(a, f);
+      return;
+    }
+  k_attend<T, D, 1><<<grid, kThreads, 0, s>>>(a, f);
 }
 
 template <class T, int D, bool FEW>
-void gradients(Args a, const Backward& b, int64_t tiles, hipStream_t s) {
-  if (b.dq) k_query_grads<T, D, FEW><<<dim3((unsigned)(tiles * a.heads)), kThreads, 0, s>>>(a, b);
+void gradients(Args a, const Backward& b, int64_t tiles, int64_t longest, hipStream_t s) {
+  const dim3 grid((unsigned)(tiles * a.heads));
+  bool two = false;
+  if constexpr (D <= 128) {
+    two = two_groups(tiles * a.heads, longest);
+    if (b.dq && two) k_query_grads<T, D, FEW, 2><<<grid, 2 * kThreads, 0, s>>>(a, b);
+  }
+  if (b.dq && !two) k_query_grads<T, D, FEW, 1><<<grid, kThreads, 0, s>>>(a, b);
   if (!b.dk) return;
   a.tiles += tiles;  // by keys
   k_key_grads<T, D, FEW><<<dim3((unsigned)(tiles * a.kv_heads * b.parts)), kThreads, 0, s>>>(a, b);
@@ -877,8 +948,8 @@ void gradients(Args a, const Backward& b, int64_t tiles, hipStream_t s) {
 template <class T, int D>
 void backward(const Args& a, const Backward& b, int64_t tiles, int64_t longest, hipStream_t s) {
   k_delta<T><<<kMost, 256, 0, s>>>(a, b);
-  if (D <= 32 || longest <= 256) gradients<T, D, true>(a, b, tiles, s);
-  else gradients<T, D, D <= 32>(a, b, tiles, s);
+  if (D <= 32 || longest <= 256) gradients<T, D, true>(a, b, tiles, longest, s);
+  else gradients<T, D, D <= 32>(a, b, tiles, longest, s);
 }
 
 bool off16(const void* p) { return ((uintptr_t)p & 15) != 0; }
@@ -990,8 +1061,8 @@ int dsx_attention_forward(const DsxAttention* args, void* out, void* out_lo, flo
   const Args a = args_of(*args);
   const Forward f{(short*)out, (short*)out_lo, lse};
   hipStream_t s = as_stream(stream);
-  if (args->dtype == DSX_F16) DSX_BY_HEAD(forward, F16, a, f, args->tile_count, s);
-  else DSX_BY_HEAD(forward, BF16, a, f, args->tile_count, s);
+  if (args->dtype == DSX_F16) DSX_BY_HEAD(forward, F16, a, f, args->tile_count, args->longest, s);
+  else DSX_BY_HEAD(forward, BF16, a, f, args->tile_count, args->longest, s);
   return launch_status(what);
 }
 

@@ -131,7 +131,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, packing:
     where it may reach any row.
 
     Differentiable once in q, k and v, backwards (a forward-mode tangent is
-    refused); results do not depend on timing. The backward keeps the output
+    refused); results do not depend on timing, but in their last bits on how much
+    other work a batch holds, by which it is shared out. The backward keeps the output
     twice (its rounding errors too) and 4 bytes a row and head beside the
     inputs."""
     if not isinstance(q, torch.Tensor):
