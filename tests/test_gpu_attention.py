@@ -24,6 +24,7 @@ pytestmark = pytest.mark.gpu
 
 U = {"bfloat16": 2.0 ** -8, "float16": 2.0 ** -11}
 FP32 = 2.0 ** -13
+LEAST = {"bfloat16": 0.0, "float16": 2.0 ** -25}  # below 2^-14 fp16's step is 2^-24 whatever the value: half of it
 
 
 def _say(msg):
@@ -94,7 +95,7 @@ def _check(got, exact, dtype):
     for name, g in got.items():
         w = want[name]
         assert g.shape == w.shape and bool(g.isfinite().all()), name
-        bound = u * (1 + u) * (w.abs() + mags[name]) + FP32 * sums[name] + 2.0 ** -24 * w.abs().max()
+        bound = u * (1 + u) * (w.abs() + mags[name]) + FP32 * sums[name] + 2.0 ** -24 * w.abs().max() + LEAST[dtype]
         far = ((g.double() - w).abs() - bound).max().item() if w.numel() else 0
         assert far <= 0, (name, far)
 
@@ -149,6 +150,14 @@ def test_scores_below_the_range_of_fp32(gpu, d):
     k[..., 0] = 0
     k[:70, :, 0] = -2.0 ** 70
     _check(_run(q, k, v, do, lengths, False), _exact(q, k, v, do, lengths, False, 1 / math.sqrt(d)), "bfloat16")
+
+
+@pytest.mark.parametrize("d", [32, 64, 96, 128])
+@pytest.mark.parametrize("lengths", [[511], [512], [513, 1], [575], [576, 2], [577], [640, 0, 1000]])
+def test_few_blocks(gpu, lengths, d):
+    """From 512 rows on, where there are few blocks, two groups of waves share one's
+    tiles: even and odd numbers of them, and other sequences of one tile."""
+    _compare(lengths, 3, 1, d, "float16", len(lengths) != 2)
 
 
 def test_a_given_scale(gpu):
