@@ -477,7 +477,10 @@ struct Backward {
 };
 constexpr int kMost = 512;
 
-// delta, and for fp16 the largest rows: 16 lanes a row. Where few keys matter dP
+// delta, and for fp16 the largest rows: 16 lanes a row. In bf16 k_query_grads forms
+// delta itself, where it runs, beside the loads of other blocks (9 sequences of 53 to
+// 2048 rows, 32 heads of 128, all gradients: 518 us instead of 527; 8 x 1024 rows, 12
+// heads of 64: 81 instead of 89). Where few keys matter dP
 // and delta nearly cancel, so that delta is taken from the output before its
 // rounding: without what that lost, dq's and dk's errors over those of one rounding
 // (64 features, bf16, rows of 2 to 12 keys) are 1.8 instead of 1.1, of 1000 keys
@@ -498,12 +501,14 @@ __global__ __launch_bounds__(256) void k_delta(Args a, Backward b) {
       for (int c = sub * 8; c < a.d; c += 128) {
         const s8v x = *(const s8v*)(go + c), y = *(const s8v*)(b.out + i * a.d + c),
                   z = *(const s8v*)(b.out_lo + i * a.d + c);
+        float chunk = 0;
 #pragma unroll
         for (int e = 0; e < 8; e++) {
           const float v = T::widen(x[e]);
-          s = fmaf(v, T::widen(y[e]) + T::widen(z[e]), s);
+          chunk = fmaf(v, T::widen(y[e]) + T::widen(z[e]), chunk);
           n = fmaf(v, v, n);
         }
+        s += chunk;
       }
     } else {
       const int64_t t = (i - rows) / a.kv_heads;
@@ -606,7 +611,29 @@ __global__ DSX_ATTENTION_KERNEL(D, 3, GROUPS) void k_query_grads(Args a, Backwar
   // rounding errors of dP - delta.
   const bool one = a.causal ? row == p.start : p.end - p.start == 1;
   const float lse = one ? INFINITY : b.lse[(int64_t)p.head * a.tokens + there];
-  const float delta = b.delta[(int64_t)p.head * a.tokens + there];
+  float delta;
+  if (T::kScaled) {
+    delta = b.delta[(int64_t)p.head * a.tokens + there];
+  } else {  // k_delta is for fp16's scale, and for calls without dq
+    const int64_t at = ((int64_t)there * a.heads + p.head) * a.d;
+    s8v y[L::kSteps], z[L::kSteps];
+    L::own(y, b.out + at, 0, 0, a.d, lane);
+    L::own(z, b.out_lo + at, 0, 0, a.d, lane);
+    float sum[L::kSteps];  // a chunk's, added in k_delta's order
+#pragma unroll
+    for (int i = 0; i < L::kSteps; i++) {
+      sum[i] = 0;
+#pragma unroll
+      for (int e = 0; e < 8; e++) sum[i] = fmaf(T::widen(gf[i][e]), T::widen(y[i][e]) + T::widen(z[i][e]), sum[i]);
+    }
+#pragma unroll
+    for (int n = 8; n; n >>= 1)
+#pragma unroll
+      for (int i = 0; i < n; i++)
+        if (i + n < L::kSteps) sum[i] += sum[i + n];
+    delta = -(sum[0] + other_half(sum[0]));
+    if (group == 0 && half == 0 && row < p.end) b.delta[(int64_t)p.head * a.tokens + row] = delta;
+  }
   const short* kp = a.k.p + p.kv * a.k.head + p.start * a.k.ld;
   const short* vp = a.v.p + p.kv * a.v.head + p.start * a.v.ld;
   const int hi = a.causal ? min(p.row0 + kRows, p.end) : p.end;
@@ -947,7 +974,7 @@ void gradients(Args a, const Backward& b, int64_t tiles, int64_t longest, hipStr
 
 template <class T, int D>
 void backward(const Args& a, const Backward& b, int64_t tiles, int64_t longest, hipStream_t s) {
-  k_delta<T><<<kMost, 256, 0, s>>>(a, b);
+  if (T::kScaled || !b.dq) k_delta<T><<<kMost, 256, 0, s>>>(a, b);
   if (D <= 32 || longest <= 256) gradients<T, D, true>(a, b, tiles, longest, s);
   else gradients<T, D, D <= 32>(a, b, tiles, longest, s);
 }
