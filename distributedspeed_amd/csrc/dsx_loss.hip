@@ -137,9 +137,9 @@ __global__ __launch_bounds__(256) void k_copy_rows(const short* __restrict__ fro
                                                    int rows, short* __restrict__ to, int64_t ld_to) {
   const int n = count ? *count : rows;
   const int per = (int)(ld_to / 8);
-  for (int r = blockIdx.y; r < n; r += gridDim.y) {
+  for (int r = blockIdx.y * blockDim.y + threadIdx.y; r < n; r += gridDim.y * blockDim.y) {
     const short* p = from + (index ? index[r] : r) * ld;
-    for (int c = blockIdx.x * 256 + threadIdx.x; c < per; c += gridDim.x * 256)
+    for (int c = blockIdx.x * blockDim.x + threadIdx.x; c < per; c += gridDim.x * blockDim.x)
       *(s8v*)(to + r * ld_to + c * 8) = chunk_of(p, c, cols);
   }
 }
@@ -245,7 +245,7 @@ __global__ __launch_bounds__(1024) void k_rows(const float2* __restrict__ part, 
   };
   if (r < rows) {
     const int hi = (int)((int64_t)nt * (q + 1) / 32);
-#pragma unroll 4
+#pragma unroll 8
     for (int t = (int)((int64_t)nt * q / 32); t < hi; t++) join(part[(int64_t)t * m + r]);
   }
   runs[q][i] = {top, sum};
@@ -429,6 +429,7 @@ __global__ __launch_bounds__(256) void k_input_join(const float* __restrict__ pl
   for (int t = blockIdx.y; t < m; t += gridDim.y) {
     const int r = s.place[t];
     f4v a = {}, b = {};
+#pragma unroll 8
     for (int k = 0; k < (r < 0 ? 0 : splits); k++) {
       const float* q = planes + ((int64_t)k * m + r) * ld + c;
       a += *(const f4v*)q;
@@ -613,11 +614,19 @@ Work work_of(const DsxLoss& q, const Sizes& z, bool backward) {
   return w;
 }
 
+// As many threads for a row as it has chunks, rows for the others of a block of 256.
+void copy_rows(const short* from, int64_t ld, int64_t cols, const int* index, const int* count, int64_t rows, short* to,
+               int64_t ld_to, hipStream_t s) {
+  unsigned x = 1;
+  while (x < 256 && x < ld_to / 8) x *= 2;
+  const int64_t blocks = ceil_div(rows, 256 / x);
+  k_copy_rows<<<dim3((unsigned)ceil_div(ld_to / 8, x), (unsigned)(blocks < 65535 ? blocks : 65535)), dim3(x, 256 / x), 0,
+                s>>>(from, ld, (int)cols, index, count, (int)rows, to, ld_to);
+}
+
 void copy_weight(const DsxLoss& q, const Sizes& z, const Work& w, hipStream_t s) {
   if (!z.copied) return;
-  const unsigned x = (unsigned)ceil_div(z.ld / 8, 256);
-  k_copy_rows<<<dim3(x, (unsigned)(z.v < 65535 ? z.v : 65535)), 256, 0, s>>>((const short*)q.weight, q.ld_weight, (int)z.d,
-                                                                           nullptr, nullptr, (int)z.v, w.weight, z.ld);
+  copy_rows((const short*)q.weight, q.ld_weight, z.d, nullptr, nullptr, z.v, w.weight, z.ld, s);
 }
 
 Logits logits_of(const DsxLoss& q, const Sizes& z, const Saved& s, const Work& w, int64_t v0, int64_t n, int tile) {
@@ -668,9 +677,7 @@ int forward(const DsxLoss& q, float* loss, hipStream_t st) {
     if (!none) k_total<<<1, 1024, 0, st>>>(nullptr, s, q.reduction == DSX_REDUCE_MEAN, loss);
     return launch_status("dsx_loss_forward");
   }
-  if (!here)
-    k_copy_rows<<<dim3((unsigned)ceil_div(z.ld / 8, 256), (unsigned)(z.t < 65535 ? z.t : 65535)), 256, 0, st>>>(
-        (const short*)q.x, q.ld_x, (int)z.d, s.index, s.count, (int)z.t, s.x, s.ld);
+  if (!here) copy_rows((const short*)q.x, q.ld_x, z.d, s.index, s.count, z.t, s.x, s.ld, st);
   copy_weight(q, z, w, st);
   const Logits p = logits_of(q, z, s, w, 0, z.v, z.tile);
   const dim3 grid((unsigned)(p.mt * p.nt));
