@@ -553,7 +553,7 @@ __global__ __launch_bounds__(256) void k_delta(Args a, Backward b) {
 }
 
 // A power of two that takes dS to at most 2^15 in fp16: |dP - delta| is at most
-// 2 |do| |v|, whatever the rows. `buf`: 8 floats of shared memory.
+// 2 |do| |v|, whatever the rows. `buf`: two floats a wave of shared memory.
 __device__ inline float gradient_scale(const float* most, float* buf) {
   float mo = 0, mv = 0;
   for (int i = threadIdx.x; i < kMost; i += kThreads) {
