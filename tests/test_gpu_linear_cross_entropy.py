@@ -127,6 +127,14 @@ def test_a_vocabulary_in_pieces(gpu):
     _check(_run(x, w, targets, weights, "mean"), x, w, targets, weights, "mean", "bfloat16")
 
 
+@pytest.mark.parametrize("d", [512, 520])
+def test_the_largest_tiles(gpu, d):
+    """On both sides of the width up to which the logits' gradients have smaller ones."""
+    x, w, targets, weights = _make(2050, d, 20001, "float16", seed=d, ignored=0.2)
+    _say(f"2050 x {d} x 20001")
+    _check(_run(x, w, targets, weights, "sum"), x, w, targets, weights, "sum", "float16")
+
+
 @pytest.mark.parametrize("scale", [1e-6, 1.0, 3e4])
 def test_weights_of_any_scale_in_fp16(gpu, scale):
     """dz is held at a scale of its own; results below fp16's least step are zero."""
