@@ -468,117 +468,76 @@ struct Backward {
   const short* out_lo;
   const float* lse;     // [heads][tokens]
   float* delta;         // [heads][tokens]: -delta
-  float* most;          // [kMost][2]: the largest |do|^2 and |v|^2 of a block's rows (fp16)
   short* dq;            // [tokens][heads][d]
   short* dk;            // [tokens][kv_heads][d]
   short* dv;
   float* part;          // where there are several parts: fp32 [2][parts][tokens][kv_heads][d]
   int parts;            // of a tile's work in k_key_grads
 };
-constexpr int kMost = 512;
+constexpr int kDeltaBlocks = 512;
 
-// delta, and for fp16 the largest rows: 16 lanes a row. In bf16 k_query_grads forms
-// delta itself, where it runs, beside the loads of other blocks (9 sequences of 53 to
-// 2048 rows, 32 heads of 128, all gradients: 518 us instead of 527; 8 x 1024 rows, 12
-// heads of 64: 81 instead of 89). Where few keys matter dP
-// and delta nearly cancel, so that delta is taken from the output before its
-// rounding: without what that lost, dq's and dk's errors over those of one rounding
-// (64 features, bf16, rows of 2 to 12 keys) are 1.8 instead of 1.1, of 1000 keys
-// 1.49 and 1.58 instead of 1.29 and 1.44.
+// delta, 16 lanes a row, for calls without dq: k_query_grads forms it itself, beside
+// the loads of other blocks (bf16, 9 sequences of 53 to 2048 rows, 32 heads of 128, all
+// gradients: 518 us instead of 527; 8 x 1024 rows, 12 heads of 64: 81 instead of 89).
+// Where few keys matter dP and delta nearly cancel, so that delta is taken from the
+// output before its rounding: without what that lost, dq's and dk's errors over those
+// of one rounding (64 features, bf16, rows of 2 to 12 keys) are 1.8 instead of 1.1, of
+// 1000 keys 1.49 and 1.58 instead of 1.29 and 1.44.
 template <class T>
 __global__ __launch_bounds__(256) void k_delta(Args a, Backward b) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int64_t rows = (int64_t)a.tokens * a.heads, values = T::kScaled ? (int64_t)a.tokens * a.kv_heads : 0;
-  float mo = 0, mv = 0;
+  const int64_t rows = (int64_t)a.tokens * a.heads;
   const int per = 64 / 16;  // rows of a wave, 16 lanes each
   const int sub = lane & 15;
-  for (int64_t i = ((int64_t)blockIdx.x * 4 + w) * per + (lane >> 4); i < rows + values; i += (int64_t)gridDim.x * 4 * per) {
-    float s = 0, n = 0;
-    if (i < rows) {
-      const int64_t t = i / a.heads;
-      const int h = (int)(i - t * a.heads);
-      const short* go = b.dout.p + t * b.dout.ld + h * b.dout.head;
-      for (int c = sub * 8; c < a.d; c += 128) {
-        const s8v x = *(const s8v*)(go + c), y = *(const s8v*)(b.out + i * a.d + c),
-                  z = *(const s8v*)(b.out_lo + i * a.d + c);
-        float chunk = 0;
+  for (int64_t i = ((int64_t)blockIdx.x * 4 + w) * per + (lane >> 4); i < rows; i += (int64_t)gridDim.x * 4 * per) {
+    float s = 0;
+    const int64_t t = i / a.heads;
+    const int h = (int)(i - t * a.heads);
+    const short* go = b.dout.p + t * b.dout.ld + h * b.dout.head;
+    for (int c = sub * 8; c < a.d; c += 128) {
+      const s8v x = *(const s8v*)(go + c), y = *(const s8v*)(b.out + i * a.d + c),
+                z = *(const s8v*)(b.out_lo + i * a.d + c);
+      float chunk = 0;
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-          const float v = T::widen(x[e]);
-          chunk = fmaf(v, T::widen(y[e]) + T::widen(z[e]), chunk);
-          n = fmaf(v, v, n);
-        }
-        s += chunk;
-      }
-    } else {
-      const int64_t t = (i - rows) / a.kv_heads;
-      const short* v = a.v.p + t * a.v.ld + (i - rows - t * a.kv_heads) * a.v.head;
-      for (int c = sub * 8; c < a.d; c += 128) {
-        const s8v x = *(const s8v*)(v + c);
-#pragma unroll
-        for (int e = 0; e < 8; e++) n = fmaf(T::widen(x[e]), T::widen(x[e]), n);
-      }
+      for (int e = 0; e < 8; e++) chunk = fmaf(T::widen(x[e]), T::widen(y[e]) + T::widen(z[e]), chunk);
+      s += chunk;
     }
 #pragma unroll
-    for (int k = 8; k; k >>= 1) {
-      s += __shfl_xor(s, k);
-      n += __shfl_xor(n, k);
-    }
-    n = n < INFINITY ? n : 0.0f;  // a row that is not finite has no part in the others' scale
-    if (i < rows) {
-      if (sub == 0) {
-        const int64_t t = i / a.heads;
-        b.delta[(i - t * a.heads) * a.tokens + t] = -s;
-      }
-      mo = fmaxf(mo, n);
-    } else {
-      mv = fmaxf(mv, n);
-    }
+    for (int k = 8; k; k >>= 1) s += __shfl_xor(s, k);
+    if (sub == 0) b.delta[(int64_t)h * a.tokens + t] = -s;
   }
-  if (!T::kScaled) return;
-  __shared__ float buf[4][2];
-#pragma unroll
-  for (int k = 32; k >= 16; k >>= 1) {
-    mo = fmaxf(mo, __shfl_xor(mo, k));
-    mv = fmaxf(mv, __shfl_xor(mv, k));
-  }
-  if (lane == 0) {
-    buf[w][0] = mo;
-    buf[w][1] = mv;
-  }
-  __syncthreads();
-  if (threadIdx.x < 2)
-    b.most[blockIdx.x * 2 + threadIdx.x] = fmaxf(fmaxf(buf[0][threadIdx.x], buf[1][threadIdx.x]),
-                                                 fmaxf(buf[2][threadIdx.x], buf[3][threadIdx.x]));
 }
 
-// A power of two that takes dS to at most 2^15 in fp16: |dP - delta| is at most
-// 2 |do| |v|, whatever the rows. `buf`: two floats a wave of shared memory.
-__device__ inline float gradient_scale(const float* most, float* buf) {
-  float mo = 0, mv = 0;
-  for (int i = threadIdx.x; i < kMost; i += kThreads) {
-    mo = fmaxf(mo, most[2 * i]);
-    mv = fmaxf(mv, most[2 * i + 1]);
-  }
+// fp16 holds a row's dS (k_query_grads; a key's in k_key_grads) times a power of two
+// of its own, whose place is a lane: it begins at 2^kLift and goes by the largest dS
+// that the row has met, taken to [2^11, 2^12) where one passes 2^15, which scales the
+// row's sums as well (exactly). What is below 2^-25 of a row's largest dS loses
+// digits, to an error of 2^-36 of that one; a scale that rows share would lose those of
+// small rows beside large ones. |dS| is below 2^41 (of finite inputs), so that
+// nothing overflows at the start.
+constexpr int kLift = 60;
+template <class T, int N>
+__device__ inline void fit(f16v& ds, f16v* sums, int& lift) {
+  if constexpr (T::kScaled) {
+    float top = fabsf(ds[0]);
 #pragma unroll
-  for (int k = 32; k; k >>= 1) {
-    mo = fmaxf(mo, __shfl_xor(mo, k));
-    mv = fmaxf(mv, __shfl_xor(mv, k));
+    for (int r = 1; r < 16; r++) top = fmaxf(top, fabsf(ds[r]));
+    if (!__any(top > 0x1p15f)) return;
+    top = fmaxf(top, other_half(top));
+    const int by = top > 0x1p15f && top < INFINITY ? 12 - __builtin_amdgcn_frexp_expf(top) : 0;
+    const float down = ldexpf(1.0f, by);
+    lift += by;
+    ds *= down;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      // Above 128 features the sums live in the accumulation registers: said before and
+      // behind, or they are moved out of them in every round (k_key_grads, 2 x 2048
+      // rows, 16 heads of 256, both gradients: 722 us instead of 440).
+      if (N > 4) asm volatile("" : "+a"(sums[i]));
+      sums[i] *= down;
+      if (N > 4) asm volatile("" : "+a"(sums[i]));
+    }
   }
-  const int w = threadIdx.x >> 6;
-  if ((threadIdx.x & 63) == 0) {
-    buf[2 * w] = mo;
-    buf[2 * w + 1] = mv;
-  }
-  __syncthreads();
-  mo = fmaxf(fmaxf(buf[0], buf[2]), fmaxf(buf[4], buf[6]));
-  mv = fmaxf(fmaxf(buf[1], buf[3]), fmaxf(buf[5], buf[7]));
-  __syncthreads();
-  const float bound = 2.0f * sqrtf(mo) * sqrtf(mv);
-  if (!(bound > 0.0f) || !(bound < INFINITY)) return 1.0f;
-  int e;
-  frexpf(bound, &e);  // bound < 2^e
-  return ldexpf(1.0f, max(-100, min(100, 15 - e)));
 }
 
 // dS is rounded to the inputs' type for its products with k and q, which adds an
@@ -599,7 +558,6 @@ __global__ DSX_ATTENTION_KERNEL(D, 3, GROUPS) void k_query_grads(Args a, Backwar
   __shared__ __attribute__((aligned(1024))) char shared[GROUPS][2][2][L::kBytes];
   const Place p = place_of(a, a.heads);
   if (!p.good) return;
-  const float ds_scale = T::kScaled ? gradient_scale(b.most, (float*)shared) : 1.0f;
   const int lane = threadIdx.x & 63, half = lane >> 5, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 3;
   const int group = GROUPS == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / kThreads);
   auto& lds = shared[group];
@@ -612,9 +570,8 @@ __global__ DSX_ATTENTION_KERNEL(D, 3, GROUPS) void k_query_grads(Args a, Backwar
   const bool one = a.causal ? row == p.start : p.end - p.start == 1;
   const float lse = one ? INFINITY : b.lse[(int64_t)p.head * a.tokens + there];
   float delta;
-  if (T::kScaled) {
-    delta = b.delta[(int64_t)p.head * a.tokens + there];
-  } else {  // k_delta is for fp16's scale, and for calls without dq
+  int lift = T::kScaled ? kLift : 0;  // of the power of two in dS
+  {
     const int64_t at = ((int64_t)there * a.heads + p.head) * a.d;
     s8v y[L::kSteps], z[L::kSteps];
     L::own(y, b.out + at, 0, 0, a.d, lane);
@@ -660,6 +617,7 @@ __global__ DSX_ATTENTION_KERNEL(D, 3, GROUPS) void k_query_grads(Args a, Backwar
     const bool edge = j0 + kTile - 1 > (a.causal ? min(w0, p.end - 1) : p.end - 1);
 #pragma unroll
     for (int c = 0; c < 2; c++) {
+      const float shift = (float)lift - lse;
       f16v s = {}, dp = {};
 #pragma unroll
       for (int i = 0; i < L::kSteps; i++) {
@@ -668,14 +626,15 @@ __global__ DSX_ATTENTION_KERNEL(D, 3, GROUPS) void k_query_grads(Args a, Backwar
       }
 #pragma unroll
       for (int r = 0; r < 16; r++) {
-        const float e = __builtin_amdgcn_exp2f(fmaf(s[r], a.scale2, -lse));
-        s[r] = e * (dp[r] + delta) * ds_scale;
+        const float e = __builtin_amdgcn_exp2f(fmaf(s[r], a.scale2, shift));
+        s[r] = e * (dp[r] + delta);
       }
       if (edge) {
         const int left = only_here(last) - j0 - c * 32 - 4 * half;
 #pragma unroll
         for (int r = 0; r < 16; r++) s[r] = row_of(r, 0) <= left ? s[r] : 0.0f;
       }
+      fit<T, L::kBlocks>(s, dq, lift);
 #pragma unroll
       for (int g = 0; g < 2; g++) {
         const s8v sf = pack<T>(s, g), rest = pack_rest<T>(s, g, sf);
@@ -691,16 +650,23 @@ __global__ DSX_ATTENTION_KERNEL(D, 3, GROUPS) void k_query_grads(Args a, Backwar
   const int rows = min(32, p.end - w0);
   __syncthreads();
   if (GROUPS == 2) {
-    float* there = (float*)shared + w * 64 * L::kBlocks * 16 + lane;
-    if (group) hand_over<D>(there, dq);
+    float* there = (float*)shared + w * 64 * (L::kBlocks * 16 + 1) + lane;
+    if (group) {
+      hand_over<D>(there, dq);
+      there[L::kBlocks * 16 * 64] = (float)lift;
+    }
     __syncthreads();
-    if (!group) take_over<D>(there, dq, 1.0f, 1.0f);
+    if (!group) {  // to the smaller of the two powers of two
+      const int other = (int)there[L::kBlocks * 16 * 64], least = min(lift, other);
+      take_over<D>(there, dq, ldexpf(1.0f, least - lift), ldexpf(1.0f, least - other));
+      lift = least;
+    }
     __syncthreads();
     if (group) return;
   }
   if (rows <= 0) return;
   const int64_t ld = (int64_t)a.heads * a.d;
-  store_rows<T, D>((char*)shared + w * 32 * HD * 2, dq, a.scale / ds_scale, false,
+  store_rows<T, D>((char*)shared + w * 32 * HD * 2, dq, ldexpf(a.scale, -lift), false,
                     b.dq + w0 * ld + (int64_t)p.head * a.d, ld, rows, a.d, lane);
 }
 
@@ -727,7 +693,6 @@ __global__ DSX_ATTENTION_KERNEL(D, 3, 1) void k_key_grads(Args a, Backward b) {
   float* stats = (float*)(lds + 4 * L::kBytes);
   const Place p = place_of(a, a.kv_heads * b.parts);
   if (!p.good) return;
-  const float ds_scale = T::kScaled ? gradient_scale(b.most, (float*)lds) : 1.0f;
   const int lane = threadIdx.x & 63, half = lane >> 5, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int w0 = p.row0 + 32 * w, key = w0 + (lane & 31), there = min(key, p.end - 1);
   s8v kf[L::kSteps], vf[L::kSteps];
@@ -753,6 +718,7 @@ __global__ DSX_ATTENTION_KERNEL(D, 3, 1) void k_key_grads(Args a, Backward b) {
   f16v dk[L::kBlocks], dv[L::kBlocks];
 #pragma unroll
   for (int i = 0; i < L::kBlocks; i++) dk[i] = dv[i] = f16v{};
+  int lift = T::kScaled ? kLift : 0;
   int head = p.kv * a.group + step0 / per, i0 = first + step0 % per * kTile;
   if (nt > 0) load(0, head, i0);
   for (int t = 0; t < nt; t++) {
@@ -771,6 +737,7 @@ __global__ DSX_ATTENTION_KERNEL(D, 3, 1) void k_key_grads(Args a, Backward b) {
 #pragma unroll kUnroll
     for (int c = 0; c < 2; c++) {
       const Reader<D> rd = reader.from((t & 1) * 2 * L::kBytes + c * 32 * HD * 2);
+      const float ds_scale = ldexpf(1.0f, lift - (int)(2 * T::kBias));  // (P's 2^14 is taken off)
       f16v s = {}, dp;  // dP's sums begin at -delta
 #pragma unroll
       for (int q = 0; q < 4; q++) {
@@ -793,7 +760,7 @@ __global__ DSX_ATTENTION_KERNEL(D, 3, 1) void k_key_grads(Args a, Backward b) {
         for (int e = 0; e < 4; e++) {
           const int r = q * 4 + e;
           s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.scale2, 2.0f * T::kBias - lse[e]));
-          dp[r] = s[r] * dp[r] * (ds_scale * (T::kScaled ? 0x1p-14f : 1.0f));
+          dp[r] = s[r] * dp[r] * ds_scale;
         }
       }
       __builtin_amdgcn_sched_barrier(0);
@@ -809,6 +776,7 @@ __global__ DSX_ATTENTION_KERNEL(D, 3, 1) void k_key_grads(Args a, Backward b) {
           dp[r] = i >= more && i < hi ? dp[r] : 0.0f;
         }
       }
+      fit<T, L::kBlocks>(dp, dk, lift);
       s8v pf[2], sf[2];
 #pragma unroll
       for (int g = 0; g < 2; g++) {
@@ -839,7 +807,7 @@ __global__ DSX_ATTENTION_KERNEL(D, 3, 1) void k_key_grads(Args a, Backward b) {
   const int rows = min(32, p.end - w0);
   __syncthreads();
   if (rows <= 0) return;
-  const float fk = a.scale / ds_scale, fv = T::kScaled ? 0x1p-14f : 1.0f;
+  const float fk = ldexpf(a.scale, -lift), fv = T::kScaled ? 0x1p-14f : 1.0f;
   const int64_t ld = (int64_t)a.kv_heads * a.d, at = w0 * ld + (int64_t)p.kv * a.d;
   if (b.parts > 1) {
     const int64_t plane = (int64_t)a.tokens * ld;
@@ -908,12 +876,11 @@ int parts_of(const DsxAttention& q) {
 }
 
 struct Layout {
-  int64_t delta, most, part, total;
+  int64_t delta, part, total;
 };
 Layout layout_of(const DsxAttention& q) {
   Layout l{};
-  l.most = round_up(q.tokens * q.heads * 4, 256);
-  l.part = l.most + kMost * 2 * 4;
+  l.part = round_up(q.tokens * q.heads * 4, 256);
   const int parts = parts_of(q);
   l.total = l.part + (parts > 1 ? round_up(2 * parts * q.tokens * q.kv_heads * q.head_dim * 4, 256) : 0);
   return l;
@@ -974,7 +941,7 @@ void gradients(Args a, const Backward& b, int64_t tiles, int64_t longest, hipStr
 
 template <class T, int D>
 void backward(const Args& a, const Backward& b, int64_t tiles, int64_t longest, hipStream_t s) {
-  if (T::kScaled || !b.dq) k_delta<T><<<kMost, 256, 0, s>>>(a, b);
+  if (!b.dq) k_delta<T><<<kDeltaBlocks, 256, 0, s>>>(a, b);
   if (D <= 32 || longest <= 256) gradients<T, D, true>(a, b, tiles, longest, s);
   else gradients<T, D, D <= 32>(a, b, tiles, longest, s);
 }
@@ -1121,7 +1088,6 @@ int dsx_attention_backward(const DsxAttention* args, const void* out, const void
   b.out_lo = (const short*)out_lo;
   b.lse = lse;
   b.delta = (float*)(ws + l.delta);
-  b.most = (float*)(ws + l.most);
   b.part = (float*)(ws + l.part);
   b.dq = (short*)dq;
   b.dk = (short*)dk;

@@ -1,0 +1,62 @@
+"""What packed_attention's gradients lose in rounding, where a batch's rows differ:
+beside large values elsewhere, and in short sequences beside long ones."""
+from __future__ import annotations
+
+import math
+
+import pytest
+
+import test_gpu_attention as A
+
+pytestmark = pytest.mark.gpu
+
+
+def _compare_some(got, exact, dtype, rows, heads, kv_heads):
+    """test_gpu_attention's bound for some rows and heads; what is left out has no
+    part in it."""
+    parts = [{n: t[rows][:, heads if n in ("out", "dq") else kv_heads] for n, t in d.items()} for d in (got, *exact)]
+    A._check(parts[0], parts[1:], dtype)
+
+
+@pytest.mark.parametrize("large_do,large_v", [(1e4, 30.0), (1e5, 100.0), (1e5, 1.0), (1.0, 1000.0)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_large_values_elsewhere_in_fp16(gpu, causal, large_do, large_v):
+    """One sequence, or one key head, has output gradients and values far larger
+    than the others': their gradients are within the bound for their own values,
+    as they are without it."""
+    lengths, scale = [300, 200, 64, 5], 1 / math.sqrt(64)
+    q, k, v, do = A._make(569, 4, 2, 64, "float16", 21)
+    A._say(f"large values: do {large_do:g}, v {large_v:g}, causal {causal}")
+    bad_v, bad_do = v.clone(), do.clone()
+    bad_v[300:500] *= large_v  # up to 500, 30000 (finite in fp16)
+    bad_do[300:500] *= large_do
+    assert bad_v.isfinite().all()
+    bad_do.clamp_(-60000, 60000)
+    got = A._run(q, k, bad_v, bad_do, lengths, causal)
+    exact = A._exact(q, k, bad_v, bad_do, lengths, causal, scale)
+    for rows in (slice(0, 300), slice(500, 569)):
+        _compare_some(got, exact, "float16", rows, slice(0, 4), slice(0, 2))
+    bad_v, bad_do = v.clone(), do.clone()
+    bad_v[:, 1] *= large_v
+    bad_do[:, 2:] *= large_do
+    bad_do.clamp_(-60000, 60000)
+    got = A._run(q, k, bad_v, bad_do, lengths, causal)
+    exact = A._exact(q, k, bad_v, bad_do, lengths, causal, scale)
+    _compare_some(got, exact, "float16", slice(0, 569), slice(0, 2), slice(0, 1))
+
+
+@pytest.mark.parametrize("lengths", [[200], [1000], [700, 30]])
+def test_large_rows_in_the_same_sequence_in_fp16(gpu, lengths):
+    """A row with a large output gradient, and a last key with a large value, which
+    only the last row sees: the rows that see neither, and the keys that the large
+    row does not see, are within the bound for their own values."""
+    n, scale = lengths[0], 1 / math.sqrt(64)
+    q, k, v, do = A._make(sum(lengths), 2, 1, 64, "float16", 22)
+    do[20] = do[20].sign() * 30000
+    v[n - 1] = v[n - 1].sign() * 3000
+    A._say(f"large rows in {lengths}")
+    got = A._run(q, k, v, do, lengths)
+    exact = A._exact(q, k, v, do, lengths, True, scale)
+    for rows, names in ((slice(0, 20), ("out", "dq")), (slice(21, n - 1), ("out", "dq", "dk", "dv"))):
+        parts = [{m: d[m][rows] for m in names} for d in (got, *exact)]
+        A._check(parts[0], parts[1:], "float16")
