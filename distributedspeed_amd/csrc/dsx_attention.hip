@@ -544,20 +544,24 @@ __device__ inline void fit(f16v& ds, f16v* sums, int& lift) {
 // error to dq as large as that of dq's own rounding, and a larger one where the
 // keys that matter have a direction in common (unrounded, dS adds up to zero along
 // a row). What the rounding loses, in the same type, can go through the matrix
-// unit as another operand. FEW (short sequences and small heads, where that effect
-// is largest): all of it does, for dq and dk. Otherwise that of every other 16
+// unit as another operand. FEW (sequences of up to kFew rows, by a block's own, and
+// small heads, where that effect is largest): all of it does, for dq and dk. Otherwise that of every other 16
 // keys, for dq alone. The error of dq over that of one rounding (bf16, 64
 // features, 2500 keys): 1.53 with none, 1.32 with every other 16, 1.13 with all; of
 // dk with none 1.44; 60 keys, dq and dk: 1.65 with none, 1.07 with all. Time of dq
 // for 16384 rows, 16 heads of 64: 0.77 ms with none, 0.89 with every other 16, 1.02
 // with all.
+constexpr int kFew = 256;
+template <int D>
+__device__ inline bool few(const Place& p) {
+  return D <= 32 || p.end - p.start <= kFew;
+}
+
 template <class T, int D, bool FEW, int GROUPS>
-__global__ DSX_ATTENTION_KERNEL(D, 3, GROUPS) void k_query_grads(Args a, Backward b) {
+__device__ __forceinline__ void query_grads(const Args& a, const Backward& b, const Place& p,
+                                            char (&shared)[GROUPS][2][2][Tile<D>::kBytes]) {
   using L = Tile<D>;
   constexpr int HD = L::HD;
-  __shared__ __attribute__((aligned(1024))) char shared[GROUPS][2][2][L::kBytes];
-  const Place p = place_of(a, a.heads);
-  if (!p.good) return;
   const int lane = threadIdx.x & 63, half = lane >> 5, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 3;
   const int group = GROUPS == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / kThreads);
   auto& lds = shared[group];
@@ -670,6 +674,15 @@ __global__ DSX_ATTENTION_KERNEL(D, 3, GROUPS) void k_query_grads(Args a, Backwar
                     b.dq + w0 * ld + (int64_t)p.head * a.d, ld, rows, a.d, lane);
 }
 
+template <class T, int D, int GROUPS>
+__global__ DSX_ATTENTION_KERNEL(D, 3, GROUPS) void k_query_grads(Args a, Backward b) {
+  __shared__ __attribute__((aligned(1024))) char shared[GROUPS][2][2][Tile<D>::kBytes];
+  const Place p = place_of(a, a.heads);
+  if (!p.good) return;
+  if (few<D>(p)) query_grads<T, D, true, GROUPS>(a, b, p, shared);
+  else query_grads<T, D, false, GROUPS>(a, b, p, shared);
+}
+
 // Rows of fp32 partial sums, one a lane.
 template <int D>
 __device__ inline void store_part(float* out, const f16v* o, float factor, bool there, int d, int half) {
@@ -683,16 +696,16 @@ __device__ inline void store_part(float* out, const f16v* o, float factor, bool 
     }
 }
 
+// `lds`: two pairs of tiles, then lse and delta of their rows. (One array: with two,
+// the compiler waits for all direct loads in flight before each read.)
+template <int D>
+constexpr int kKeyGradsLds = 4 * Tile<D>::kBytes + 4 * kTile * 4;
 template <class T, int D, bool FEW>
-__global__ DSX_ATTENTION_KERNEL(D, 3, 1) void k_key_grads(Args a, Backward b) {
+__device__ __forceinline__ void key_grads(const Args& a, const Backward& b, const Place& p,
+                                          char (&lds)[kKeyGradsLds<D>]) {
   using L = Tile<D>;
   constexpr int HD = L::HD;
-  // One array: with two, the compiler waits for all direct loads in flight before
-  // each read. Two pairs of tiles, then lse and delta of their rows.
-  __shared__ __attribute__((aligned(1024))) char lds[4 * L::kBytes + 4 * kTile * 4];
   float* stats = (float*)(lds + 4 * L::kBytes);
-  const Place p = place_of(a, a.kv_heads * b.parts);
-  if (!p.good) return;
   const int lane = threadIdx.x & 63, half = lane >> 5, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int w0 = p.row0 + 32 * w, key = w0 + (lane & 31), there = min(key, p.end - 1);
   s8v kf[L::kSteps], vf[L::kSteps];
@@ -821,6 +834,15 @@ __global__ DSX_ATTENTION_KERNEL(D, 3, 1) void k_key_grads(Args a, Backward b) {
   store_rows<T, D>(strip, dv, fv, false, b.dv + at, ld, rows, a.d, lane);
 }
 
+template <class T, int D>
+__global__ DSX_ATTENTION_KERNEL(D, 3, 1) void k_key_grads(Args a, Backward b) {
+  __shared__ __attribute__((aligned(1024))) char lds[kKeyGradsLds<D>];
+  const Place p = place_of(a, a.kv_heads * b.parts);
+  if (!p.good) return;
+  if (few<D>(p)) key_grads<T, D, true>(a, b, p, lds);
+  else key_grads<T, D, false>(a, b, p, lds);
+}
+
 // The parts' sums, added in order: eight values a thread.
 template <class T>
 __global__ __launch_bounds__(256) void k_join(const float* __restrict__ part, short* __restrict__ dk,
@@ -923,27 +945,21 @@ void forward(const Args& a, const Forward& f, int64_t tiles, int64_t longest, hi
   k_attend<T, D, 1><<<grid, kThreads, 0, s>>>(a, f);
 }
 
-template <class T, int D, bool FEW>
-void gradients(Args a, const Backward& b, int64_t tiles, int64_t longest, hipStream_t s) {
+template <class T, int D>
+void backward(Args a, const Backward& b, int64_t tiles, int64_t longest, hipStream_t s) {
+  if (!b.dq) k_delta<T><<<kDeltaBlocks, 256, 0, s>>>(a, b);
   const dim3 grid((unsigned)(tiles * a.heads));
   bool two = false;
   if constexpr (D <= 128) {
     two = two_groups(tiles * a.heads, longest);
-    if (b.dq && two) k_query_grads<T, D, FEW, 2><<<grid, 2 * kThreads, 0, s>>>(a, b);
+    if (b.dq && two) k_query_grads<T, D, 2><<<grid, 2 * kThreads, 0, s>>>(a, b);
   }
-  if (b.dq && !two) k_query_grads<T, D, FEW, 1><<<grid, kThreads, 0, s>>>(a, b);
+  if (b.dq && !two) k_query_grads<T, D, 1><<<grid, kThreads, 0, s>>>(a, b);
   if (!b.dk) return;
   a.tiles += tiles;  // by keys
-  k_key_grads<T, D, FEW><<<dim3((unsigned)(tiles * a.kv_heads * b.parts)), kThreads, 0, s>>>(a, b);
+  k_key_grads<T, D><<<dim3((unsigned)(tiles * a.kv_heads * b.parts)), kThreads, 0, s>>>(a, b);
   const int64_t n = (int64_t)a.tokens * a.kv_heads * a.d;
   if (b.parts > 1) k_join<T><<<dim3((unsigned)ceil_div(n, 2048), 2), 256, 0, s>>>(b.part, b.dk, b.dv, n, b.parts);
-}
-
-template <class T, int D>
-void backward(const Args& a, const Backward& b, int64_t tiles, int64_t longest, hipStream_t s) {
-  if (!b.dq) k_delta<T><<<kDeltaBlocks, 256, 0, s>>>(a, b);
-  if (D <= 32 || longest <= 256) gradients<T, D, true>(a, b, tiles, longest, s);
-  else gradients<T, D, D <= 32>(a, b, tiles, longest, s);
 }
 
 bool off16(const void* p) { return ((uintptr_t)p & 15) != 0; }
