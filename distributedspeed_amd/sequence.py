@@ -50,9 +50,10 @@ def _native():
 class PackedSequences:
     """Where the sequences of a batch lie: of the given lengths (host integers,
     zero allowed), one behind the other from row 0. Made once for a batch and
-    used by all its layers, in both directions; it holds the kernels' tile table
-    on `device`, so that a captured graph needs it alive. positions and offsets
-    are made at their first use, which belongs before a capture.
+    used by all its layers, in both directions, on any stream of `device`; it may
+    be dropped as soon as the calls with it are made. It holds the kernels' tile
+    table, so that a captured graph needs it alive. positions and offsets are made
+    at their first use, which belongs before a capture.
 
         lengths   as a tuple
         tokens    their sum
@@ -70,25 +71,41 @@ class PackedSequences:
         self.tokens = sum(lengths)
         self._longest, self._pairs = max(lengths, default=0), sum(n * n for n in lengths)
         self.device = torch.device("cuda", torch.cuda.current_device()) if device.index is None else device
-        self._tiles = torch.from_numpy(_tile_table(lengths)).to(self.device)
+        self._seen = set()
+        self._tiles = self._made("tiles", _tile_table(lengths))
         self._positions = self._offsets = None
 
     def __repr__(self) -> str:
         return f"PackedSequences({len(self.lengths)} sequences, {self.tokens} tokens, {self.device})"
+
+    def _made(self, name: str, values: np.ndarray) -> torch.Tensor:
+        """On the device when this returns, for any stream of it."""
+        t = torch.from_numpy(values).to(self.device)
+        self._seen.add((name, ops.stream_of(self.device).value or 0))
+        return t
+
+    def _on_stream(self, name: str, t: torch.Tensor, stream: int) -> torch.Tensor:
+        """t for work on `stream`, the current one: where it was made on another, its
+        memory is not handed out again before what is queued by the time it is
+        dropped has run. (A graph's replays come later: it needs t alive.)"""
+        if (name, stream) not in self._seen:
+            t.record_stream(torch.cuda.current_stream(self.device))
+            self._seen.add((name, stream))
+        return t
 
     @property
     def positions(self) -> torch.Tensor:
         if self._positions is None:
             first = np.cumsum([0, *self.lengths], dtype=np.int64)[:-1]
             at = np.arange(self.tokens, dtype=np.int64) - np.repeat(first, self.lengths)
-            self._positions = torch.from_numpy(at.astype(np.int32)).to(self.device)
-        return self._positions
+            self._positions = self._made("positions", at.astype(np.int32))
+        return self._on_stream("positions", self._positions, ops.stream_of(self.device).value or 0)
 
     @property
     def offsets(self) -> torch.Tensor:
         if self._offsets is None:
-            self._offsets = torch.from_numpy(np.cumsum([0, *self.lengths]).astype(np.int32)).to(self.device)
-        return self._offsets
+            self._offsets = self._made("offsets", np.cumsum([0, *self.lengths]).astype(np.int32))
+        return self._on_stream("offsets", self._offsets, ops.stream_of(self.device).value or 0)
 
 
 def _tile_table(lengths) -> np.ndarray:
@@ -161,8 +178,10 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, packing:
     scale = 1 / math.sqrt(d) if scale is None else float(scale)
     if not 0 < scale <= 1e38:
         raise ValueError(f"scale must be positive and at most 1e38, got {scale}")
-    return (_nodes or _native()).packed_attention(q, k, v, packing._tiles, packing.tokens, packing._longest, packing._pairs,
-                                                  bool(causal), scale, ops.stream_of(dev).value or 0)
+    stream = ops.stream_of(dev).value or 0
+    tiles = packing._on_stream("tiles", packing._tiles, stream)
+    return (_nodes or _native()).packed_attention(q, k, v, tiles, packing.tokens, packing._longest, packing._pairs,
+                                                  bool(causal), scale, stream)
 
 
 def rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, *, base: float = 10000.0,
