@@ -23,6 +23,7 @@ from . import _lib, ops
 from .block import gated_residual_norm
 
 MAX_TOKENS, MAX_HEADS, MAX_HEAD_DIM, MAX_ROTARY_DIM = 1 << 27, 1024, 256, 1024
+MAX_TILES = 1 << 24  # of 128 rows, times heads
 
 _nodes = None
 
@@ -136,12 +137,14 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, packing:
     to the query's own where `causal`: q [rows, heads, head_dim], k and v [rows,
     kv_heads, head_dim], all fp16 or all bf16 on one GPU; heads is a multiple of
     kv_heads, and query head h reads key head h // (heads // kv_heads). head_dim
-    is at most 256, scale 1 / sqrt(head_dim) unless given. rows may be more than
+    is at most 256, scale 1 / sqrt(head_dim) unless given (2^-126 to 1e38), and the
+    sequences' tiles of 128 rows times heads below 2^24. rows may be more than
     packing.tokens: the rest hold anything, and zeros in the result and in the
     gradients.
 
     Scores, statistics and sums are fp32; the probabilities are rounded to the
-    inputs' type for the product with v. Rows and heads may be strided (the
+    inputs' type for the product with v. (Scaled scores of 2^24 and more, which fp32
+    does not tell apart by one, may give NaN.) Rows and heads may be strided (the
     parts of one projection's rows); tensors whose features are not adjacent,
     not a multiple of eight or not 16-byte aligned are copied first. Sequences
     do not see each other: a value that is not finite stays within its own,
@@ -176,8 +179,10 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, packing:
     if rows < packing.tokens:
         raise ValueError(f"q has {rows} rows, packing {packing.tokens} tokens")
     scale = 1 / math.sqrt(d) if scale is None else float(scale)
-    if not 0 < scale <= 1e38:
-        raise ValueError(f"scale must be positive and at most 1e38, got {scale}")
+    if not 2.0 ** -126 <= scale <= 1e38:
+        raise ValueError(f"scale must lie in [2^-126, 1e38], got {scale}")
+    if packing._tiles.shape[1] * heads >= MAX_TILES:
+        raise ValueError(f"tiles times heads must be below 2^24, got {packing._tiles.shape[1]} * {heads}")
     stream = ops.stream_of(dev).value or 0
     tiles = packing._on_stream("tiles", packing._tiles, stream)
     return (_nodes or _native()).packed_attention(q, k, v, tiles, packing.tokens, packing._longest, packing._pairs,

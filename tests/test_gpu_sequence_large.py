@@ -92,3 +92,19 @@ def test_a_step_of_the_example_changes_every_parameter(gpu):
     adamw.step()
     for n, p in model.named_parameters():
         assert p.isfinite().all() and not torch.equal(p, before[n]), n
+
+
+def test_attention_past_its_limits_is_refused(gpu):
+    """By the wrapper, as its other arguments: a scale that fp32 does not hold, and more
+    tiles and heads than a launch takes."""
+    import torch
+    from distributedspeed_amd import PackedSequences, packed_attention
+    q = torch.zeros(4, 2, 8, device="cuda").bfloat16()
+    for scale in (1e-50, 2.0 ** -127, 2e38, float("inf"), -1.0):
+        with pytest.raises(ValueError, match="scale"):
+            packed_attention(q, q, q, PackedSequences([4]), scale=scale)
+    assert packed_attention(q, q, q, PackedSequences([4]), scale=2.0 ** -126).isfinite().all()
+    one = torch.zeros(1, 1, 8, device="cuda").bfloat16()
+    n = 1 << 14
+    with pytest.raises(ValueError, match="tiles"):
+        packed_attention(one.expand(n, 1024, 8), one.expand(n, 1, 8), one.expand(n, 1, 8), PackedSequences([1] * n))
