@@ -30,10 +30,11 @@
 // us, 0.91 PFLOP/s of the visible pairs' products (a large product reaches 1.42);
 // without the softmax's arithmetic 139, without the loads 151, without both 126.
 // With 64 features there is twice the softmax for a product: 16384 rows, 16 heads
-// (2), k_attend 0.62 ms, 0.89 PFLOP/s; k_query_grads 0.90 ms, 0.92 (pack_rest's
-// products not counted); k_key_grads 1.08 ms, 1.02. Waves of 64 rows would halve the LDS reads, but their
-// registers leave one wave a SIMD, which was slower, as was computing the next
-// tile's scores beside a tile's softmax.
+// (2), k_attend 0.60 to 0.64 ms, 0.89 PFLOP/s; k_query_grads 0.90 to 0.95 ms, 0.92
+// (pack_rest's products not counted); k_key_grads 1.05 to 1.11 ms, 1.02. Waves of 64
+// rows would halve the LDS reads: with 128 features their registers leave one wave a
+// SIMD, which was slower; with 64 they would leave two, which has not been tried.
+// Computing the next tile's scores beside a tile's softmax was slower.
 
 #include <hip/hip_runtime.h>
 #include <math.h>
@@ -267,8 +268,9 @@ __device__ inline void store_rows(char* strip, const f16v* o, float factor, bool
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-// A block's tile and heads: tile by tile (the longest first), the heads of a
-// key head eight blocks apart so that one XCD's L2 serves them.
+// A block's tile and heads: tile by tile in the table's order (of causal calls: the
+// most work first), the heads of a key head eight blocks apart so that one XCD's L2
+// serves them.
 struct Place {
   int row0, start, end, head, kv;
   bool good;
@@ -1029,8 +1031,10 @@ int64_t dsx_attention_tiles(const int64_t* lengths, int64_t count, int32_t* tile
   }
   if (!tiles) return n;
   if (capacity < n) return fail(-1, "dsx_attention_tiles: %lld tiles do not fit", (long long)n);
-  // Most work first, by counting the tiles of each distance (in tiles) from the
-  // sequence's first row, or from its end.
+  // Most work first for causal calls, by counting the tiles of each distance (in
+  // tiles) from the sequence's first row, or from its end. Calls that are not causal
+  // use the same order, where a tile's work is its whole sequence's: the first tile
+  // of a long sequence behind many short ones then comes late.
   int64_t longest = 0;
   for (int64_t i = 0; i < count; i++)
     if (ceil_div(lengths[i], kRows) > longest) longest = ceil_div(lengths[i], kRows);

@@ -27,7 +27,9 @@
 // k_dlogits, which writes 412 MB, 0.72, dx and dW 0.95.
 //
 // In fp16, dz is held times a power of two that takes the largest factor to
-// about 2^14, so that probabilities down to 2^-28 keep their digits.
+// about 2^14, so that probabilities down to 2^-28 keep their digits. (Where the rows'
+// factors differ, those of a row 2^r below the largest: down to 2^(r-28). The results'
+// own least step is met before that, unless the largest factor is above 2^11.)
 
 #include <hip/hip_runtime.h>
 #include <math.h>
@@ -512,7 +514,8 @@ struct Sizes {
 
 // dz of a piece: at most this many bytes. (8192 x 4096 against 128256 rows, bf16,
 // dz and both products: 19.0 ms with 128 MiB, 18.8 with 256, 19.4 with 512, 19.3
-// with 1 GiB; 4096 x 768 against 50257: 1.17 ms with 256, 1.06 in one piece.)
+// with 1 GiB; 4096 x 768 against 50257: 1.17 ms with 256, 1.06 in one piece. One size
+// for all widths, 3% from the best for the wide one.)
 constexpr int64_t kPieceBytes = (int64_t)512 << 20;
 
 // Tile and splits of dx's sum over k vocabulary rows, which is long where its
