@@ -72,26 +72,27 @@ class PackedSequences:
         self.tokens = sum(lengths)
         self._longest, self._pairs = max(lengths, default=0), sum(n * n for n in lengths)
         self.device = torch.device("cuda", torch.cuda.current_device()) if device.index is None else device
-        self._seen = set()
-        self._tiles = self._made("tiles", _tile_table(lengths))
+        self._seen = set()  # (address, stream) of its tensors and the streams that the allocator knows of
+        self._tiles = self._made(_tile_table(lengths))
         self._positions = self._offsets = None
 
     def __repr__(self) -> str:
         return f"PackedSequences({len(self.lengths)} sequences, {self.tokens} tokens, {self.device})"
 
-    def _made(self, name: str, values: np.ndarray) -> torch.Tensor:
+    def _made(self, values: np.ndarray) -> torch.Tensor:
         """On the device when this returns, for any stream of it."""
         t = torch.from_numpy(values).to(self.device)
-        self._seen.add((name, ops.stream_of(self.device).value or 0))
+        self._seen.add((t.data_ptr(), ops.stream_of(self.device).value or 0))
         return t
 
-    def _on_stream(self, name: str, t: torch.Tensor, stream: int) -> torch.Tensor:
+    def _on_stream(self, t: torch.Tensor, stream: int) -> torch.Tensor:
         """t for work on `stream`, the current one: where it was made on another, its
         memory is not handed out again before what is queued by the time it is
         dropped has run. (A graph's replays come later: it needs t alive.)"""
-        if (name, stream) not in self._seen:
+        use = (t.data_ptr(), stream)
+        if use not in self._seen:
             t.record_stream(torch.cuda.current_stream(self.device))
-            self._seen.add((name, stream))
+            self._seen.add(use)
         return t
 
     @property
@@ -99,14 +100,14 @@ class PackedSequences:
         if self._positions is None:
             first = np.cumsum([0, *self.lengths], dtype=np.int64)[:-1]
             at = np.arange(self.tokens, dtype=np.int64) - np.repeat(first, self.lengths)
-            self._positions = self._made("positions", at.astype(np.int32))
-        return self._on_stream("positions", self._positions, ops.stream_of(self.device).value or 0)
+            self._positions = self._made(at.astype(np.int32))
+        return self._on_stream(self._positions, ops.stream_of(self.device).value or 0)
 
     @property
     def offsets(self) -> torch.Tensor:
         if self._offsets is None:
-            self._offsets = self._made("offsets", np.cumsum([0, *self.lengths]).astype(np.int32))
-        return self._on_stream("offsets", self._offsets, ops.stream_of(self.device).value or 0)
+            self._offsets = self._made(np.cumsum([0, *self.lengths]).astype(np.int32))
+        return self._on_stream(self._offsets, ops.stream_of(self.device).value or 0)
 
 
 def _tile_table(lengths) -> np.ndarray:
@@ -184,7 +185,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, packing:
     if packing._tiles.shape[1] * heads >= MAX_TILES:
         raise ValueError(f"tiles times heads must be below 2^24, got {packing._tiles.shape[1]} * {heads}")
     stream = ops.stream_of(dev).value or 0
-    tiles = packing._on_stream("tiles", packing._tiles, stream)
+    tiles = packing._on_stream(packing._tiles, stream)
     return (_nodes or _native()).packed_attention(q, k, v, tiles, packing.tokens, packing._longest, packing._pairs,
                                                   bool(causal), scale, stream)
 

@@ -1,6 +1,8 @@
 """A batch's plan on another stream than the one it was made on."""
 from __future__ import annotations
 
+import copy
+
 import pytest
 
 pytestmark = pytest.mark.gpu
@@ -10,8 +12,9 @@ def _overlaps(tensors, ranges):
     return [t for t in tensors if any(t.data_ptr() < hi and lo < t.data_ptr() + t.nbytes for lo, hi in ranges)]
 
 
-def test_a_plan_dropped_while_another_stream_reads_it(gpu):
-    """Made on a stream that prepares batches, used on the current one behind queued
+@pytest.mark.parametrize("copied", [False, True])
+def test_a_plan_dropped_while_another_stream_reads_it(gpu, copied):
+    """Made (or copied) on a stream that prepares batches, used on the current one behind queued
     work, and dropped: its memory is not handed out again on the first stream before
     that work has run, and the results are those of a plan that is kept."""
     import torch
@@ -26,11 +29,13 @@ def test_a_plan_dropped_while_another_stream_reads_it(gpu):
         out = packed_attention(a, b, v, packing)
         return out, *torch.autograd.grad(out, (q, k, v), dout)
 
-    want = run(PackedSequences(lengths))
+    kept = PackedSequences(lengths)
+    kept.offsets
+    want = run(kept)
     big = torch.randn(8192, 8192, device="cuda").bfloat16()
     prepare = torch.cuda.Stream()
     with torch.cuda.stream(prepare):
-        packing = PackedSequences(lengths)
+        packing = copy.deepcopy(kept) if copied else PackedSequences(lengths)
         made = [packing._tiles, packing.positions, packing.offsets]
         places = [(t.data_ptr(), t.data_ptr() + t.nbytes) for t in made]
         sizes = [t.nbytes for t in made]
